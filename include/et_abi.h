@@ -115,7 +115,7 @@ int et_graph_destroy(et_graph graph);
 
 /* ------------------------------------------------------------------------
  * Linear layers: Y[T x out] = act(X[T x in] * W^T + bias).
- * bias may be NULL (treated as zero).  T, in and out must be multiples of 16.
+ * bias may be NULL (treated as zero).  T, in and out must be multiples of 16 where a call does not say otherwise.
  * ------------------------------------------------------------------------ */
 
 /* 16x16 block-sparse weight (tile_mat): row_ptr[out/16 + 1], col_idx[ntile]
@@ -565,6 +565,26 @@ int et_linear_csr_f16(const int32_t *indptr, const int32_t *indices,
                       et_f16 *Y, int T, int in, int out, int act,
                       et_stream stream);
 
+/* Dense weight in 4 bits for the few rows of a decoding step, where a Linear
+ * costs what its weight costs to read.  `group` (32, 64 or 128) input features
+ * of an output feature share a scale and a lowest value, formed as those of
+ * et_kv_cache with L = 15; in is a multiple of group, out of 16.
+ *   codes  [out][in / 2] bytes, the even input feature in the low four bits
+ *   scales [in / group][out][2]: scale, low;   W = low + scale * code
+ * Both 16-byte aligned.  et_dense_to_w4_f16 makes them of W [out x in] (16-byte aligned),
+ * et_w4_to_dense_f16 writes what they stand for, rounded to binary16 (at most its largest number).
+ * et_linear_w4_f16: T any number of rows; X, Y, Y32 16-byte aligned, bias 8-byte; exactly one of Y and Y32 (the
+ * binary32 sum after bias and activation, unrounded) is non-NULL.  The codes
+ * enter the matrix products as they are, scale and low are applied to the binary32
+ * sums of their group.  No reference counterpart. */
+int et_dense_to_w4_f16(const et_f16 *W, uint8_t *codes, et_f16 *scales, int in,
+                       int out, int group, et_stream stream);
+int et_w4_to_dense_f16(const uint8_t *codes, const et_f16 *scales, et_f16 *W,
+                       int in, int out, int group, et_stream stream);
+int et_linear_w4_f16(const uint8_t *codes, const et_f16 *scales, int group,
+                     const et_f16 *bias, const et_f16 *X, et_f16 *Y, float *Y32,
+                     int T, int in, int out, int act, et_stream stream);
+
 /* C[r][c] = bias[c] (0 when bias is NULL) for a dense [rows x cols] matrix. */
 int et_fill_rows_bias_f16(et_f16 *C, const et_f16 *bias, int rows, int cols,
                           et_stream stream);
@@ -637,6 +657,78 @@ int et_mha_fuseo_f16(const et_f16 *Q, const et_f16 *K, const et_f16 *V,
                      const int32_t *o_row_ptr, const int32_t *o_col_idx,
                      const et_f16 *o_tiles, const et_f16 *o_bias, et_f16 *out,
                      int emdim, et_stream stream);
+
+/* ------------------------------------------------------------------------
+ * Keys and values kept from step to step (no reference counterpart: its
+ * attention sees whole sequences): a paged cache in 4 or 8 bits, written as
+ * tokens arrive, read back, and the attention that reads it.
+ *
+ * A page holds `page` tokens (a multiple of 16) of all nkv heads.  hd is a
+ * multiple of 32, at most 256; each 32 channels of a token's head share a scale
+ * and a lowest value.  L = 2^bits - 1:
+ *   low   = smallest of the 32 values,
+ *   scale = smallest binary16 number with L * scale >= largest - smallest,
+ *   code  = (value - low) / scale rounded to nearest, ties to even (scale 0: 0),
+ * and the code stands for low + scale * code.  The decisions are exact, not
+ * those of a rounded quotient.  A NaN or an infinity among the 32 makes all of
+ * them NaN.  Buffers (16-byte aligned):
+ *   k_codes  [npages][nkv][page][hd * bits / 8] bytes, channel 0 in the lowest bits
+ *   v_codes  [npages][nkv][page / 4][hd * bits / 16][4] units of 16 bits: the
+ *            codes of four tokens side by side, as the attention multiplies them
+ *   k_scales, v_scales  [npages][nkv][hd / 32][page][2]: scale, low
+ *
+ * table [B][max_pages]: page i of sequence b holds its positions [i * page,
+ * (i + 1) * page).  The calls below work on n rows for each of B sequences: row
+ * i of sequence b (row b * n + i of a matrix) is the token at position
+ * starts[b] + i, for i < counts[b].  starts NULL: 0; counts NULL: n; counts
+ * outside [0, n] are taken as the nearer end.  Rows from counts[b] on are
+ * neither read nor written.  A position below 0, behind max_pages, or on a page
+ * number outside [0, npages) has no place: it is not written, a row of et_kv_read_f16
+ * stays as it was, and attention does not see it.  Pages may be shared by
+ * sequences for reading; two rows of one call that go to one place leave a
+ * mixture of both there.  table, starts and counts are device memory.
+ * ------------------------------------------------------------------------ */
+typedef struct et_kv_cache {
+    void *k_codes;
+    et_f16 *k_scales;
+    void *v_codes;
+    et_f16 *v_scales;
+    int bits; /* 4 or 8 */
+    int nkv, hd, page, npages;
+} et_kv_cache;
+#define ET_KV_GROUP 32 /* channels of a token under one scale */
+
+/* K and V [B*n x nkv*hd] (row strides ldk, ldv in elements, multiples of 8; 16-byte aligned) into the cache. */
+int et_kv_write_f16(const et_kv_cache *cache, const int32_t *table,
+                    int max_pages, const int32_t *starts, const int32_t *counts,
+                    const et_f16 *K, const et_f16 *V, int ldk, int ldv, int B,
+                    int n, et_stream stream);
+/* The values that the cache stands for, rounded to binary16 (one that rounding the scale up carries beyond its largest
+ * number becomes that number), into K and V laid out as above.  K or V may be NULL. */
+int et_kv_read_f16(const et_kv_cache *cache, const int32_t *table, int max_pages,
+                   const int32_t *starts, const int32_t *counts, et_f16 *K,
+                   et_f16 *V, int ldk, int ldv, int B, int n, et_stream stream);
+
+/* Attention of n rows a sequence over the cache, which holds these rows' own keys and values already:
+ *   P = softmax(scale * Q_h K_g^T),  Z_h = P V_g,  g = h * nkv / nh
+ * over positions 0 .. starts[b] + counts[b] - 1 of sequence b; with
+ * ET_MHA_CAUSAL row i sees none behind its own, starts[b] + i.  nh is a
+ * multiple of nkv.  Q and Z [B*n x nh*hd] (row strides multiples of 8, 16-byte
+ * aligned).  A row that sees nothing becomes zero.  What lies in the cache
+ * behind a sequence's end may be anything, NaN included.  n = 1 is a decoding
+ * step, n > 1 several tokens at once (a piece of a prompt, guessed tokens).
+ * The codes enter the matrix products as they are; scores, softmax and sums are
+ * binary32, a probability times its value's scale is rounded once, to binary16.
+ * workspace: et_mha_kv_workspace bytes of device memory, 16-byte aligned (may be NULL where that
+ * says 0); launches that can overlap in time need one each.  The sums are
+ * taken in an order that only the sizes given to the call decide. */
+int et_mha_kv_workspace(const et_kv_cache *cache, int max_pages, int B, int n,
+                        int nh, size_t *bytes);
+int et_mha_kv_f16(const et_kv_cache *cache, const int32_t *table, int max_pages,
+                  const int32_t *starts, const int32_t *counts, const et_f16 *Q,
+                  int ldq, et_f16 *Z, int ldz, int B, int n, int nh, float scale,
+                  int flags, void *workspace, size_t workspace_bytes,
+                  et_stream stream);
 
 /* Attention-aware pruning: W_V is row-pruned, so V arrives compact,
  * Vc[T x nnz_col] (row stride ldvc), holding only the surviving V columns.

@@ -126,6 +126,13 @@ _SIGNATURES = {
                          _vp, _vp, _vp, _vp, _vp, _i, _vp),
     "et_mha_fuseo_f16_geom": (_vp, _vp, _vp, _i, _i, _i, _vp, _i, _vp, _vp, _i, _i, _i, _i, _f, _i,
                               _vp, _vp, _vp, _vp, _vp, _i, _i, _vp),
+    "et_kv_write_f16": (_vp, _vp, _i, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _vp),
+    "et_kv_read_f16": (_vp, _vp, _i, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _vp),
+    "et_mha_kv_workspace": (_vp, _i, _i, _i, _i, C.POINTER(_sz)),
+    "et_mha_kv_f16": (_vp, _vp, _i, _vp, _vp, _vp, _i, _vp, _i, _i, _i, _i, _f, _i, _vp, _sz, _vp),
+    "et_dense_to_w4_f16": (_vp, _vp, _vp, _i, _i, _i, _vp),
+    "et_w4_to_dense_f16": (_vp, _vp, _vp, _i, _i, _i, _vp),
+    "et_linear_w4_f16": (_vp, _vp, _i, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _vp),
     "et_skip_layernorm_f16": (_vp, _vp, _vp, _vp, _vp, _i, _i, _f, _vp),
     "et_layernorm_f16": (_vp, _vp, _vp, _vp, _i, _i, _f, _vp),
     "et_gelu_f16": (_vp, _vp, _sz, _vp),
@@ -216,6 +223,12 @@ class ChainDesc(C.Structure):
                 ("down", _vp), ("bias_down", _vp), ("V2", _vp), ("stats2", _vp),
                 ("qkv", _vp), ("bias_qkv", _vp), ("gamma2", _vp), ("beta2", _vp), ("eps2", _f), ("fin2", _vp), ("QKV", _vp),
                 ("T", _i), ("sync", _vp)]
+
+
+class KvCache(C.Structure):
+    """et_kv_cache of include/et_abi.h: the buffers of a paged cache of keys and values, which the caller owns"""
+    _fields_ = [("k_codes", _vp), ("k_scales", _vp), ("v_codes", _vp), ("v_scales", _vp),
+                ("bits", _i), ("nkv", _i), ("hd", _i), ("page", _i), ("npages", _i)]
 
 
 _RESTYPES = {"et_status_string": C.c_char_p, "et_last_error": C.c_char_p}
@@ -398,6 +411,40 @@ def skip_layernorm(out, src, skip, gamma, beta, rows, H, eps=1e-5, stream=None):
 
 def layernorm(out, src, gamma, beta, rows, H, eps=1e-5, stream=None):
     check(lib().et_layernorm_f16(_ptr(out), _ptr(src), _ptr(gamma), _ptr(beta), rows, H, eps, stream))
+
+
+# Decoding from a cache of keys and values (KvCache) and 4-bit weights.
+
+def kv_write(cache, table, max_pages, starts, counts, K, V, ldk, ldv, B, n, stream=None):
+    check(lib().et_kv_write_f16(C.byref(cache), _ptr(table), max_pages, _ptr(starts), _ptr(counts), _ptr(K), _ptr(V), ldk, ldv, B, n, stream))
+
+
+def kv_read(cache, table, max_pages, starts, counts, K, V, ldk, ldv, B, n, stream=None):
+    check(lib().et_kv_read_f16(C.byref(cache), _ptr(table), max_pages, _ptr(starts), _ptr(counts), _ptr(K), _ptr(V), ldk, ldv, B, n, stream))
+
+
+def mha_kv_workspace(cache, max_pages, B, n, nh) -> int:
+    """Bytes of device memory that mha_kv needs for these sizes."""
+    need = _sz()
+    check(lib().et_mha_kv_workspace(C.byref(cache), max_pages, B, n, nh, C.byref(need)))
+    return need.value
+
+
+def mha_kv(cache, table, max_pages, starts, counts, Q, ldq, Z, ldz, B, n, nh, scale, flags=0, workspace=None, workspace_bytes=0, stream=None):
+    check(lib().et_mha_kv_f16(C.byref(cache), _ptr(table), max_pages, _ptr(starts), _ptr(counts), _ptr(Q), ldq, _ptr(Z), ldz, B, n, nh, scale, flags,
+                              _ptr(workspace), workspace_bytes, stream))
+
+
+def dense_to_w4(W, codes, scales, n_in, n_out, group, stream=None):
+    check(lib().et_dense_to_w4_f16(_ptr(W), _ptr(codes), _ptr(scales), n_in, n_out, group, stream))
+
+
+def w4_to_dense(codes, scales, W, n_in, n_out, group, stream=None):
+    check(lib().et_w4_to_dense_f16(_ptr(codes), _ptr(scales), _ptr(W), n_in, n_out, group, stream))
+
+
+def linear_w4(codes, scales, group, bias, X, Y, Y32, T, n_in, n_out, act=ACT_NONE, stream=None):
+    check(lib().et_linear_w4_f16(_ptr(codes), _ptr(scales), group, _ptr(bias), _ptr(X), _ptr(Y), _ptr(Y32), T, n_in, n_out, act, stream))
 
 
 # ---------------------------------------------------------------------------
