@@ -33,7 +33,7 @@ DEVICE = [f"--offload-arch={ARCH}", "-Xclang", "-target-feature", "-Xclang", "-p
 # Leading scalar arguments of a kernel in its registers when a wave starts: for the sources whose kernels have those that the first requests
 # need in front.  (A launch that preloads them begins 0.1 us later, which the shortest kernels do not win back: a dense image of a 1x16 weight 2.20 -> 2.29 us.)
 PRELOAD = ["-mllvm", "-amdgpu-kernarg-preload-count=14"]
-PRELOADED = {"attention", "bsr_linear", "encoder_layer", "f32_path", "f32_sparse", "gemm", "gemm_dma", "norm"}
+PRELOADED = {"attention", "attention_kv", "bsr_linear", "encoder_layer", "f32_path", "f32_sparse", "gemm", "gemm_dma", "norm"}
 RESOURCES = LIBDIR / "kernel_resources.txt"
 _resource_lines: list[str] = []
 

@@ -1,6 +1,8 @@
 // Attention over a cache of keys and values in 4 or 8 bits (layout: et_abi.h).
 #include <math.h>
 
+#include <algorithm>
+
 #include "group_quant.hip.h"
 
 namespace et {
@@ -8,82 +10,744 @@ namespace et {
 int kv_check_cache(const char *fn, const et_kv_cache *c, const int32_t *table, int max_pages, int B, int n);
 
 struct KvMhaArgs {
-    const unsigned char *k_codes;
-    const unsigned short *v_codes;
-    const unsigned *k_scales, *v_scales;
-    const int32_t *table, *starts, *counts;
+    const char *k_codes, *v_codes;
+    const unsigned *k_scales, *v_scales;  // scale in the low half, low in the high one
+    const int32_t *counts;
     const _Float16 *Q;
     _Float16 *Z;
+    float *parts;         // of every (split, unit): stats [16][2], then values [rows of a block][hd]
     int ldq, ldz;
-    int nkv, hd, page, npages, max_pages;
-    int n, nh, causal;
+    int nkv, per, page, npages;
+    int n, causal;
+    int hd, cols, block_rows;  // columns of statistics a query row has, query rows of a workgroup
+    int units, splits;    // (sequence, key/value head) pairs; workgroups that share the keys of one
     float scale_log2e;
 };
 
-// One wave a (row, head): 64 keys at a time, one a lane; then the channels of Z one a lane.
-template <int BITS> __global__ __launch_bounds__(64) void mha_kv_plain_kernel(const KvMhaArgs a) {
-    const int lane = threadIdx.x;
-    const int h = blockIdx.x, row = blockIdx.y, b = blockIdx.z;
-    const long long start = a.starts ? a.starts[b] : 0;
-    const int count = a.counts ? min(max(a.counts[b], 0), a.n) : a.n;
-    if (row >= count) return;
-    const int kv = h / (a.nh / a.nkv), groups = a.hd / ET_KV_GROUP;
-    long long end = a.causal ? start + row + 1 : start + count;
-    end = min(end, (long long)a.max_pages * a.page);
-    const _Float16 *q = a.Q + ((size_t)b * a.n + row) * a.ldq + h * a.hd;
-    float m = -INFINITY, l = 0.0f, acc[4] = {0, 0, 0, 0};
-    for (long long k0 = 0; k0 < end; k0 += 64) {
-        const long long pos = k0 + lane;
-        int page = -1;
-        if (pos < end) page = a.table[(size_t)b * a.max_pages + (size_t)(pos / a.page)];
-        const bool seen = page >= 0 && page < a.npages;
-        const int off = (int)(pos % a.page);
-        const size_t ph = (size_t)(seen ? page : 0) * a.nkv + kv;
-        float score = -INFINITY;
-        if (seen) {
-            const unsigned char *c = a.k_codes + (ph * a.page + off) * (a.hd * BITS / 8);
-            score = 0.0f;
-            for (int g = 0; g < groups; g++) {
-                const unsigned sl = a.k_scales[(ph * groups + g) * a.page + off];
-                float dot = 0.0f, sum = 0.0f;
-                for (int d = 0; d < 32; d++) {
-                    const int ch = g * 32 + d;
-                    const float x = (float)q[ch];
-                    dot += x * (float)(BITS == 4 ? (c[ch / 2] >> (ch % 2 * 4)) & 15 : c[ch]);
-                    sum += x;
-                }
-                score += f16_bits_value(sl & 0xffffu) * dot + f16_bits_value(sl >> 16) * sum;
-            }
-            score *= a.scale_log2e;
-        }
-        const float top = fmaxf(m, wave_max(score));
-        if (top == -INFINITY) continue;
-        const float keep = exp2f(m - top), p = exp2f(score - top);
-        m = top;
-        l = l * keep + wave_sum(p);
-        for (int i = 0; i < 4; i++) acc[i] *= keep;
-        const int last = (int)min(64LL, end - k0);
-        for (int t = 0; t < last; t++) {
-            const float pt = lane_value(p, t);
-            const int tp = __builtin_amdgcn_readlane(seen ? page : -1, t), to = __builtin_amdgcn_readlane(off, t);
-            if (tp < 0) continue;
-            const size_t th = (size_t)tp * a.nkv + kv;
-            const unsigned short *units = a.v_codes + (th * a.page + (to & ~3)) * (a.hd * BITS / 16) + (to & 3);
-            for (int i = 0; i < 4; i++) {
-                const int d = lane + 64 * i;
-                if (d >= a.hd) break;
-                const unsigned sl = a.v_scales[(th * groups + d / 32) * a.page + to];
-                const unsigned u = units[(d * BITS / 16) * 4];
-                const float c = (float)((u >> (d * BITS % 16)) & (BITS == 4 ? 15u : 255u));
-                acc[i] += pt * __builtin_fmaf(f16_bits_value(sl & 0xffffu), c, f16_bits_value(sl >> 16));
-            }
+// What the first requests need stands in front, in registers when a wave starts (14 words are):
+//   splits   workgroups that share the keys of a (sequence, key/value head), units such pairs; per   query heads of one
+//   magic, shift   pieces of 16 keys to pages: piece / (page / 16) = piece * magic >> shift
+#define KV_LEADING const int32_t *table_at, const int32_t *starts_at, const int32_t *counts_at, int max_pages, int units, int splits, int per, unsigned magic, unsigned shift, \
+                   int page_pieces, int n
+
+// The places of the pieces of 16 keys of a tile, and their pages as the table has them (-1: behind it).
+template <int N> struct KvPages {
+    int page[N], off[N];
+    __device__ __forceinline__ void ask(const __attribute__((address_space(4))) int32_t *table, int tile, int max_pages, unsigned magic, unsigned shift, int page_pieces) {
+#pragma unroll
+        for (int s = 0; s < N; s++) {
+            const int piece = N * tile + s;
+            const int pidx = (int)(((unsigned long long)(unsigned)piece * magic) >> shift);
+            off[s] = (piece - pidx * page_pieces) << 4;
+            page[s] = pidx < max_pages ? table[pidx] : -1;
         }
     }
-    for (int i = 0; i < 4; i++) {
-        const int d = lane + 64 * i;
-        if (d < a.hd) a.Z[((size_t)b * a.n + row) * a.ldz + h * a.hd + d] = (_Float16)(l > 0.0f ? acc[i] / l : 0.0f);
+    // pieces that nobody sees or that have no page: -1
+    __device__ __forceinline__ void resolve(int tile, int lim_most, int npages) {
+#pragma unroll
+        for (int s = 0; s < N; s++) page[s] = (N * tile + s) * 16 < lim_most && page[s] >= 0 && page[s] < npages ? page[s] : -1;
+    }
+};
+
+typedef unsigned u1 __attribute__((ext_vector_type(1), aligned(4)));
+typedef unsigned u2 __attribute__((ext_vector_type(2), aligned(4)));
+typedef unsigned u3 __attribute__((ext_vector_type(3), aligned(4)));
+typedef unsigned u4 __attribute__((ext_vector_type(4), aligned(4)));
+
+// N consecutive words.
+template <int N> __device__ __forceinline__ void load_words(unsigned (&to)[N], const char *from) {
+    constexpr int kWhole = N / 4 * 4;
+#pragma unroll
+    for (int i = 0; i < kWhole; i += 4) {
+        const u4 v = *reinterpret_cast<const u4 *>(from + i * 4);
+        to[i] = v[0], to[i + 1] = v[1], to[i + 2] = v[2], to[i + 3] = v[3];
+    }
+    if constexpr (N % 4 == 3) {
+        const u3 v = *reinterpret_cast<const u3 *>(from + kWhole * 4);
+        to[kWhole] = v[0], to[kWhole + 1] = v[1], to[kWhole + 2] = v[2];
+    } else if constexpr (N % 4 == 2) {
+        const u2 v = *reinterpret_cast<const u2 *>(from + kWhole * 4);
+        to[kWhole] = v[0], to[kWhole + 1] = v[1];
+    } else if constexpr (N % 4 == 1) {
+        to[kWhole] = *reinterpret_cast<const unsigned *>(from + kWhole * 4);
     }
 }
+
+template <int BITS, int HD> struct KvShape {
+    static constexpr int kGroups = HD / 32;
+    static constexpr int kCols = kGroups == 1 ? 1 : kGroups == 2 ? 2 : kGroups <= 4 ? 4 : 8;  // columns of a query row
+    static constexpr int kRows = 16 / kCols;                                                   // query rows of a block
+    static constexpr int kTokenBytes = HD * BITS / 8;
+    static constexpr int kKeyWords = kTokenBytes / 16;  // of a lane: a quarter of a key
+    static constexpr int kPieces = HD / 32;             // of eight channels in that quarter
+    static constexpr int kUnits = HD * BITS / 16 / 16;  // whole units of 16 bits of a value that a lane has
+    static constexpr bool kHalfUnit = HD * BITS / 16 % 16 != 0;  // and two channels of one that two lanes share
+    static constexpr int kValueWords = 2 * kUnits + 2 * kHalfUnit;
+    static constexpr int kUnitChannels = 16 / BITS;
+    static constexpr int kAcc = HD / 16;
+    static constexpr int kPart = 32 + kRows * HD;  // floats that a workgroup leaves
+};
+
+constexpr float kNothing = -1e30f;
+
+#define ET_KV_CONST(T, p) ((const __attribute__((address_space(4))) T *)(p))
+
+__device__ __forceinline__ h8 as_h8(unsigned a, unsigned b, unsigned c, unsigned d) {
+    typedef unsigned w4 __attribute__((ext_vector_type(4)));
+    return __builtin_bit_cast(h8, w4{a, b, c, d});
+}
+__device__ __forceinline__ float low_half(unsigned w) { return (float)__builtin_bit_cast(h2, w)[0]; }
+__device__ __forceinline__ float high_half(unsigned w) { return (float)__builtin_bit_cast(h2, w)[1]; }
+
+// Codes of a value's unit, taken from both halves of a word, as subnormal binary16 numbers.  The products lose what lies some 2^-24 under the largest's place, and a code in the
+// lowest bits of a half, where it stands 2^10 under that place, cost results 3e-4 of themselves where the values' sum nearly cancels (131071 keys): the codes
+// are moved up.  4 bits: bits 3 to 6 (codes 0 and 1, code * 2^-21) and 7 to 10 (2 and 3, * 2^-17; bit 10 is the lowest of the exponent, where the numbers still are as far
+// apart), three shifts and four masks a word; 8 bits: bits 2 to 9 (* 2^-22).
+template <int BITS> constexpr float code_unit(int k) { return BITS == 8 ? 0x1p22f : k < 2 ? 0x1p21f : 0x1p17f; }
+template <int BITS> __device__ __forceinline__ unsigned raised(unsigned w, int k) {
+    if constexpr (BITS == 8) return (k == 0 ? w << 2 : w >> 6) & 0x03fc03fcu;
+    return k == 0 ? (w << 3) & 0x00780078u : k == 1 ? (w >> 1) & 0x00780078u : k == 2 ? (w >> 1) & 0x07800780u : (w >> 5) & 0x07800780u;
+}
+
+// Sum over the kCols neighbouring lanes of a query row.
+template <int COLS> __device__ __forceinline__ float cols_sum(float v) {
+    if constexpr (COLS >= 2) v += dpp_move<kDppQuadXor1>(v);
+    if constexpr (COLS >= 4) v += dpp_move<kDppQuadXor2>(v);
+    if constexpr (COLS >= 8) v += dpp_move<0x141>(v);  // row_half_mirror
+    return v;
+}
+
+// Eight channels of a key as subnormal numbers, code * 2^-24, every other one * 16 for 4 bits: channels 0 4 1 5 2 6 3 7, or 0 2 1 3 4 6 5 7.
+template <int BITS> __device__ __forceinline__ h8 key_codes(const unsigned *w) {
+    if constexpr (BITS == 4) {
+        const unsigned x = w[0] >> 8;
+        return as_h8(w[0] & 0x000f000fu, w[0] & 0x00f000f0u, x & 0x000f000fu, x & 0x00f000f0u);
+    } else {
+        return as_h8(w[0] & 0x00ff00ffu, (w[0] >> 8) & 0x00ff00ffu, w[1] & 0x00ff00ffu, (w[1] >> 8) & 0x00ff00ffu);
+    }
+}
+
+// The same eight channels of a query times `grow`, 1 / 16 of that where the code comes out 16-fold; their sum goes to `sum`.
+template <int BITS> __device__ __forceinline__ h8 query_order(h8 x, float grow, float &sum) {
+    float f[8];
+#pragma unroll
+    for (int k = 0; k < 8; k++) {
+        f[k] = grow != 0.0f ? (float)x[k] * grow : 0.0f;
+        sum += f[k];
+    }
+    if constexpr (BITS == 4)
+        return h8{(_Float16)f[0], (_Float16)f[4], (_Float16)(f[1] / 16), (_Float16)(f[5] / 16), (_Float16)f[2], (_Float16)f[6], (_Float16)(f[3] / 16), (_Float16)(f[7] / 16)};
+    else
+        return h8{(_Float16)f[0], (_Float16)f[2], (_Float16)f[1], (_Float16)f[3], (_Float16)f[4], (_Float16)f[6], (_Float16)f[5], (_Float16)f[7]};
+}
+
+// acc += (w + rest) * codes over 32 keys: 4 j .. 4 j + 3 of two pieces.
+template <int BITS, int HD> __device__ __forceinline__ void weigh_values(f4 *acc, h8 w, h8 rest, const unsigned *first, const unsigned *second, int c) {
+    using S = KvShape<BITS, HD>;
+    auto weigh = [&](int i, h8 codes) {
+        acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w, codes, acc[i], 0, 0, 0);
+        acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(rest, codes, acc[i], 0, 0, 0);
+    };
+#pragma unroll
+    for (int u = 0; u < S::kUnits; u++)
+#pragma unroll
+        for (int k = 0; k < S::kUnitChannels; k++)
+            weigh(S::kUnitChannels * u + k, as_h8(raised<BITS>(first[2 * u], k), raised<BITS>(first[2 * u + 1], k), raised<BITS>(second[2 * u], k), raised<BITS>(second[2 * u + 1], k)));
+    if constexpr (S::kHalfUnit) {
+        // codes 2 (c % 2) and the next, moved to the places of codes 0 and 1
+        const int shift = (c & 1) * 8;
+        const unsigned a0 = first[2 * S::kUnits] >> shift, a1 = first[2 * S::kUnits + 1] >> shift;
+        const unsigned b0 = second[2 * S::kUnits] >> shift, b1 = second[2 * S::kUnits + 1] >> shift;
+#pragma unroll
+        for (int k = 0; k < 2; k++) weigh(4 * S::kUnits + k, as_h8(raised<4>(a0, k), raised<4>(a1, k), raised<4>(b0, k), raised<4>(b1, k)));
+    }
+}
+
+// The channel that column c of product i stands for.
+template <int BITS, int HD> __device__ __forceinline__ int value_channel(int i, int c) {
+    using S = KvShape<BITS, HD>;
+    if (S::kHalfUnit && i >= S::kUnits * S::kUnitChannels) return 64 * S::kUnits + (c >> 1) * 4 + (c & 1) * 2 + i - S::kUnits * S::kUnitChannels;
+    return (c * S::kUnits + i / S::kUnitChannels) * S::kUnitChannels + i % S::kUnitChannels;
+}
+
+// What its products are to be multiplied with.
+template <int BITS, int HD> constexpr float value_unit(int i) {
+    using S = KvShape<BITS, HD>;
+    return code_unit<BITS>(i < S::kUnits * S::kUnitChannels ? i % S::kUnitChannels : 0);
+}
+
+// A lane's words of the values of 16 keys.
+template <int BITS, int HD> __device__ __forceinline__ void load_value(unsigned *to, const char *units, const char *half_units) {
+    using S = KvShape<BITS, HD>;
+    unsigned whole[S::kUnits > 0 ? 2 * S::kUnits : 1], half[2];
+    if constexpr (S::kUnits > 0) load_words<2 * S::kUnits>(whole, units);
+    if constexpr (S::kHalfUnit) load_words<2>(half, half_units);
+#pragma unroll
+    for (int i = 0; i < 2 * S::kUnits; i++) to[i] = whole[i];
+    if constexpr (S::kHalfUnit) to[2 * S::kUnits] = half[0], to[2 * S::kUnits + 1] = half[1];
+}
+
+template <int BITS, int HD> struct KvTile {
+    using S = KvShape<BITS, HD>;
+    unsigned k[2][S::kKeyWords], v[2][S::kValueWords];
+    u4 ks[2], vs[2];
+};
+
+// Waves that a SIMD is to hold: more of them hide the loads' way better than a tile fetched ahead did.
+template <int BITS, int HD, int NW> constexpr int kv_waves() {
+    return NW == 16 ? 4 : HD == 32 ? 6 : HD == 64 ? (BITS == 4 ? 6 : 5) : HD <= 128 ? 4 : 2;
+}
+
+template <int BITS, int HD, int NW> __global__ __launch_bounds__(NW * 64, (kv_waves<BITS, HD, NW>())) void mha_kv_kernel(KV_LEADING, const KvMhaArgs a) {
+    using S = KvShape<BITS, HD>;
+    constexpr int COLS = S::kCols, ROWS = S::kRows, G = S::kGroups, PIECES = 2;
+    __shared__ float lds_vals[NW][ROWS * HD];
+    __shared__ float lds_stats[NW][3][16];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int c = lane & 15, j = lane >> 4;
+    const int qh = c / COLS, gg = c % COLS;
+    const int kv = blockIdx.x, b = blockIdx.y, nkv = gridDim.x;
+    const int block = splits == 1 ? blockIdx.z : blockIdx.z / splits, split = blockIdx.z - block * splits;
+
+    // Tiles are dealt to the waves of all workgroups in turn, whatever the sequence's length: the first one's pages are asked for together with it.
+    const auto *table = ET_KV_CONST(int32_t, table_at) + (size_t)b * max_pages;
+    const int t_step = splits * NW;
+    int t = split * NW + wave;
+    KvPages<PIECES> pages;
+    pages.ask(table, t, max_pages, magic, shift, page_pieces);
+
+    // the rows of this block, and what they see
+    const int start = starts_at ? ET_KV_CONST(int32_t, starts_at)[b] : 0;
+    const int count = counts_at ? min(max(ET_KV_CONST(int32_t, counts_at)[b], 0), n) : n;
+    const int row0 = block * ROWS, rows = min(ROWS, count * per - row0);
+    if (rows <= 0) return;
+    const long long most = (long long)max_pages * a.page;
+    const int end = (int)min(max((long long)start + count, 0LL), most);
+    auto row_of = [&](int row) { return n == 1 ? 0 : row / per; };  // of the call's rows
+    const int i_first = row_of(row0), i_last = row_of(row0 + rows - 1);
+    const int my_row = row0 + min(qh, rows - 1), my_i = row_of(my_row), my_r = my_row - my_i * per;
+    auto limit = [&](int i) { return a.causal ? (int)min((long long)end, max((long long)start + i + 1, 0LL)) : end; };
+    const int lim = limit(my_i), lim_least = limit(i_first), lim_most = limit(i_last);
+    const int t_end = (lim_most + 31) >> 5;
+
+    // Q in the order that the keys' codes come out of their words: 0 4 1 5 2 6 3 7 (4 bits, where 1 5 3 7 come out 16-fold) or 0 2 1 3 4 6 5 7; times a power of two
+    // that brings a row's largest to 2^14 .. 2^15, so that the smaller ones keep their bits below 1 / 16; zero in the columns of the other groups
+    h8 q[S::kPieces];
+    const _Float16 *qrow = a.Q + ((size_t)b * n + my_i) * a.ldq + (size_t)(kv * per + my_r) * HD + j * (HD / 4);
+    float top = 0.0f;
+#pragma unroll
+    for (int i = 0; i < S::kPieces; i++) {
+        q[i] = *reinterpret_cast<const h8 *>(qrow + 8 * i);
+#pragma unroll
+        for (int k = 0; k < 8; k++) top = fmaxf(top, fabsf((float)q[i][k]));
+    }
+    top = rows_max(top);
+    const int up = top > 0.0f ? 15 - __builtin_amdgcn_frexp_expf(top) : 0;
+    const float grow = __builtin_ldexpf(a.scale_log2e < 0.0f ? -1.0f : 1.0f, up);
+    const float key_scale = __builtin_ldexpf(fabsf(a.scale_log2e), 24 - up);
+    float qsum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < S::kPieces; i++) q[i] = query_order<BITS>(q[i], (j * (HD / 4) + 8 * i) / 32 == gg ? grow : 0.0f, qsum);
+    qsum = rows_sum(qsum) * 0x1p-24f;
+
+    f4 acc[S::kAcc];
+#pragma unroll
+    for (int i = 0; i < S::kAcc; i++) acc[i] = f4{0.f, 0.f, 0.f, 0.f};
+    float ref = kNothing, l = 0.0f, z = 0.0f;
+
+    auto load = [&](KvTile<BITS, HD> &t, const int (&page)[2], const int (&off)[2]) {
+#pragma unroll
+        for (int s = 0; s < 2; s++) {
+            const size_t ph = (size_t)max(page[s], 0) * nkv + kv;
+            const size_t token = ph * a.page + off[s];
+            load_words<S::kKeyWords>(t.k[s], a.k_codes + token * S::kTokenBytes + c * S::kTokenBytes + j * (S::kTokenBytes / 4));
+            const char *v = a.v_codes + token * S::kTokenBytes + j * (4 * S::kTokenBytes);
+            load_value<BITS, HD>(t.v[s], v + c * (8 * S::kUnits), v + 128 * S::kUnits + (c >> 1) * 8);
+            const size_t at = (ph * G + min(gg, G - 1)) * a.page + off[s] + 4 * j;
+            t.ks[s] = *reinterpret_cast<const u4 *>(a.k_scales + at);
+            t.vs[s] = *reinterpret_cast<const u4 *>(a.v_scales + at);
+        }
+    };
+    auto use = [&](const KvTile<BITS, HD> &t, int tile, const int (&page)[2]) {
+        float y[8];
+#pragma unroll
+        for (int s = 0; s < 2; s++) {
+            f4 d = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int i = 0; i < S::kPieces; i++) {
+                const h8 codes = key_codes<BITS>(&t.k[s][i * BITS / 4]);
+                d = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes, q[i], d, 0, 0, 0);
+            }
+#pragma unroll
+            for (int r = 0; r < 4; r++) y[4 * s + r] = cols_sum<COLS>(__builtin_fmaf(low_half(t.ks[s][r]), d[r], high_half(t.ks[s][r]) * qsum)) * key_scale;
+        }
+        u4 vs[2] = {t.vs[0], t.vs[1]};
+        const bool whole = tile * 32 + 32 <= lim_least && page[0] >= 0 && page[1] >= 0;
+        bool seen[8];
+        if (!whole) {
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const int s = e >> 2, r = e & 3;
+                seen[e] = tile * 32 + 16 * s + 4 * j + r < lim && page[s] >= 0;
+                y[e] = seen[e] ? y[e] : kNothing;
+                vs[s][r] = seen[e] ? vs[s][r] : 0u;
+            }
+        }
+        float most_y = y[0], most_s = low_half(vs[0][0]);
+#pragma unroll
+        for (int e = 1; e < 8; e++) {
+            most_y = fmaxf(most_y, y[e]);
+            most_s = fmaxf(most_s, low_half(vs[e >> 2][e & 3]));
+        }
+        // a weight is at most 2^15: p * scale < 2^(y - ref + exponent of the scale)
+        const float reach = most_y + (float)__builtin_amdgcn_frexp_expf(most_s);
+        if (__any(reach > ref + 15.0f)) {
+            const float next = fmaxf(ref, rows_max(reach) - 11.0f);
+            const float f = __builtin_amdgcn_exp2f(ref - next);
+            ref = next;
+            l *= f;
+            z *= f;
+            float fr[4];
+#pragma unroll
+            for (int r = 0; r < 4; r++) fr[r] = __shfl(f, 4 * j + r);
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+#pragma unroll
+                for (int i = 0; i < S::kAcc; i++) acc[i][r] *= fr[r];
+            }
+        }
+        float p[8];
+        // p * scale as two binary16 numbers: rounded to one, whose error is relative to a value's height above the group's lowest, results were 2 to 3 times as
+        // far off as their own rounding (5.9e-4 against 2.1e-4, 2-norm, 131071 keys of random values); the products are no bound here
+        h8 w, rest;
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            p[e] = __builtin_amdgcn_exp2f(y[e] - ref);
+            if (!whole) p[e] = seen[e] ? p[e] : 0.0f;
+            l += p[e];
+            const float ps = p[e] * low_half(vs[e >> 2][e & 3]);
+            z = __builtin_fmaf(p[e], high_half(vs[e >> 2][e & 3]), z);
+            w[e] = (_Float16)ps;
+            rest[e] = (_Float16)(ps - (float)w[e]);
+        }
+        weigh_values<BITS, HD>(acc, w, rest, t.v[0], t.v[1], c);
+    };
+
+    for (; t < t_end; t += t_step) {
+        KvTile<BITS, HD> tile;
+        pages.resolve(t, lim_most, a.npages);
+        load(tile, pages.page, pages.off);
+        KvPages<PIECES> next;
+        next.ask(table, t + t_step, max_pages, magic, shift, page_pieces);
+        use(tile, t, pages.page);
+        pages = next;
+    }
+
+    // what the waves have, side by side
+    l = rows_sum(l);
+    z = rows_sum(z);
+    if (j == 0) {
+        lds_stats[wave][0][c] = ref;
+        lds_stats[wave][1][c] = l;
+        lds_stats[wave][2][c] = z;
+    }
+#pragma unroll
+    for (int i = 0; i < S::kAcc; i++) {
+        const int ch = value_channel<BITS, HD>(i, c);
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+            const int row = 4 * j + r;
+            if (row % COLS == ch >> 5) lds_vals[wave][row / COLS * HD + ch] = acc[i][r] * value_unit<BITS, HD>(i);
+        }
+    }
+    __syncthreads();
+    float *part = splits > 1 ? a.parts + ((size_t)blockIdx.z * units + (unsigned)(b * nkv + kv)) * S::kPart : nullptr;
+    for (int e = threadIdx.x; e < rows * HD; e += NW * 64) {
+        const int h = e / HD, ch = e - h * HD, col = h * COLS + (ch >> 5);
+        float m = lds_stats[0][0][col];
+#pragma unroll
+        for (int w = 1; w < NW; w++) m = fmaxf(m, lds_stats[w][0][col]);
+        float sum = 0.0f, ls = 0.0f;
+#pragma unroll
+        for (int w = 0; w < NW; w++) {
+            const float f = __builtin_amdgcn_exp2f(lds_stats[w][0][col] - m);
+            sum = __builtin_fmaf(f, lds_vals[w][e] + lds_stats[w][2][col], sum);
+            ls = __builtin_fmaf(f, lds_stats[w][1][col], ls);
+        }
+        if (part) {
+            part[32 + e] = sum;
+            if ((ch & 31) == 0) part[2 * col] = m, part[2 * col + 1] = ls;
+        } else {
+            const int row = row0 + h, i = row_of(row), r = row - i * per;
+            a.Z[((size_t)b * n + i) * a.ldz + (size_t)(kv * per + r) * HD + ch] = (_Float16)(ls == 0.0f ? 0.0f : sum / ls);
+        }
+    }
+}
+
+// Few rows a key/value head (R: 1, or the 4 / kCols that fill the products' rows): a tile of 64 keys whose scores end one a lane, so that the softmax costs a key once.
+//
+// Scores: rows of the products are the groups of the query rows, four times over, columns 16 keys; a lane keeps those of piece lane / 16 of the tile.  Group by group
+// they are scaled and added in the lane.  The weights go through 1 KB of LDS (one wave's own, no barrier) to become the rows of the products with the values.
+template <int BITS, int HD, int R> struct KvFew {
+    static constexpr int kCols = KvShape<BITS, HD>::kCols;  // 1, 2 or 4 groups of a head
+    static constexpr int kLdsRow = 72;                      // halfs: 64 keys, and 16 bytes on to other banks
+    static constexpr int kLdsWave = 4 * kLdsRow * 2 > R * HD * 2 ? 4 * kLdsRow * 2 : R * HD * 2;  // halfs of a wave: the weights and their rests; at the end its results
+    static constexpr int kPart = 32 + R * HD;
+};
+
+template <int BITS, int HD> constexpr int kv_few_waves() { return BITS == 8 && HD == 128 ? 3 : HD > 64 ? 4 : 5; }
+
+template <int BITS, int HD, int R, int NW> __global__ __launch_bounds__(NW * 64, (kv_few_waves<BITS, HD>())) void mha_kv_few_kernel(KV_LEADING, const KvMhaArgs a) {
+    using S = KvShape<BITS, HD>;
+    using F = KvFew<BITS, HD, R>;
+    constexpr int GP = F::kCols, G = S::kGroups, TB = S::kTokenBytes;
+    __shared__ __align__(16) _Float16 lds[NW][F::kLdsWave];
+    __shared__ float lds_stats[NW][R][2];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int c = lane & 15, j = lane >> 4;
+    const int kv = blockIdx.x, b = blockIdx.y, nkv = gridDim.x;
+    const int block = splits == 1 ? blockIdx.z : blockIdx.z / splits, split = blockIdx.z - block * splits;
+
+    // Tiles are dealt to the waves of all workgroups in turn, whatever the sequence's length: the first one's pages are asked for together with it.
+    const auto *table = ET_KV_CONST(int32_t, table_at) + (size_t)b * max_pages;
+    const int t_step = splits * NW;
+    int t = split * NW + wave;
+    const bool wide = (page_pieces & 3) == 0;  // a tile lies in one page
+    int page[4], off[4];
+    auto ask = [&](int tile) {
+        const int piece = 4 * tile;
+        int pidx = (int)(((unsigned long long)(unsigned)piece * magic) >> shift), at = piece - pidx * page_pieces;
+        off[0] = at << 4;
+        page[0] = pidx < max_pages ? table[pidx] : -1;
+        if (wide) return;
+#pragma unroll
+        for (int s = 1; s < 4; s++) {
+            const bool on = ++at == page_pieces;
+            at = on ? 0 : at;
+            pidx += on;
+            off[s] = at << 4;
+            page[s] = pidx < max_pages ? table[pidx] : -1;
+        }
+    };
+    ask(t);
+
+    // the rows of this block, and what they see
+    const int start = starts_at ? ET_KV_CONST(int32_t, starts_at)[b] : 0;
+    const int count = counts_at ? min(max(ET_KV_CONST(int32_t, counts_at)[b], 0), n) : n;
+    const int row0 = block * R, rows = min(R, count * per - row0);
+    if (rows <= 0) return;
+    const long long most = (long long)max_pages * a.page;
+    const int end = (int)min(max((long long)start + count, 0LL), most);
+    auto row_of = [&](int row) { return n == 1 ? 0 : row / per; };  // of the call's rows
+    auto limit = [&](int row) { return a.causal ? (int)min((long long)end, max((long long)start + row_of(row) + 1, 0LL)) : end; };
+    int lim[R];
+#pragma unroll
+    for (int h = 0; h < R; h++) lim[h] = limit(row0 + min(h, rows - 1));
+    const int lim_least = lim[0], lim_most = lim[R - 1];
+    const int t_end = (lim_most + 63) >> 6;
+
+    // Q as in mha_kv_kernel; row c of the products is group c % GP of query row c / GP % HP
+    const int h_own = (c & 3) / GP, g_own = c % GP;
+    h8 q[S::kPieces];
+    float key_scale[R], qsum[R][G];
+    {
+        const int row = row0 + min(h_own, rows - 1), i_row = row_of(row), r_row = row - i_row * per;
+        const _Float16 *qrow = a.Q + ((size_t)b * n + i_row) * a.ldq + (size_t)(kv * per + r_row) * HD + j * (HD / 4);
+        float top = 0.0f;
+#pragma unroll
+        for (int i = 0; i < S::kPieces; i++) {
+            q[i] = *reinterpret_cast<const h8 *>(qrow + 8 * i);
+#pragma unroll
+            for (int k = 0; k < 8; k++) top = fmaxf(top, fabsf((float)q[i][k]));
+        }
+        top = rows_max(top);
+        const int up = top > 0.0f ? 15 - __builtin_amdgcn_frexp_expf(top) : 0;
+        const float grow = __builtin_ldexpf(a.scale_log2e < 0.0f ? -1.0f : 1.0f, up);
+        const float back = __builtin_ldexpf(fabsf(a.scale_log2e), 24 - up);
+        float sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < S::kPieces; i++) q[i] = query_order<BITS>(q[i], (j * (HD / 4) + 8 * i) / 32 == g_own ? grow : 0.0f, sum);
+        sum = rows_sum(sum) * 0x1p-24f;
+#pragma unroll
+        for (int h = 0; h < R; h++) {
+            key_scale[h] = lane_value(back, h * GP);
+#pragma unroll
+            for (int g = 0; g < G; g++) qsum[h][g] = lane_value(sum, h * GP + g);
+        }
+    }
+
+    f4 acc[S::kAcc];
+#pragma unroll
+    for (int i = 0; i < S::kAcc; i++) acc[i] = f4{0.f, 0.f, 0.f, 0.f};
+    float ref[R], l[R], z[R][G];
+#pragma unroll
+    for (int h = 0; h < R; h++) {
+        ref[h] = kNothing, l[h] = 0.0f;
+#pragma unroll
+        for (int g = 0; g < G; g++) z[h][g] = 0.0f;
+    }
+
+    const unsigned key_at = c * TB + j * (TB / 4), value_at = j * (4 * TB) + c * (8 * S::kUnits), half_at = j * (4 * TB) + 128 * S::kUnits + (c >> 1) * 8;
+    const char *k_codes = a.k_codes + (size_t)kv * a.page * TB, *v_codes = a.v_codes + (size_t)kv * a.page * TB;
+    const unsigned *k_scales = a.k_scales + (size_t)kv * (G * a.page), *v_scales = a.v_scales + (size_t)kv * (G * a.page);
+    const unsigned page_bytes = (unsigned)nkv * a.page * TB, page_scales = (unsigned)nkv * G * a.page;
+    _Float16 *weights = lds[wave];
+    // key 16 s + c of a tile among the 64 of a row: so that the keys 4 j .. 4 j + 3 of two pieces, which a lane multiplies, lie together
+    const int key_place = (j >> 1) * 32 + (c >> 2) * 8 + (j & 1) * 4 + (c & 3);
+    const _Float16 *weights_at = weights + (c & 3) * F::kLdsRow + j * 8;
+
+    for (; t < t_end; t += t_step) {
+        // where the pieces lie; one that nobody sees, or without a page, is read from the place of the one before it
+        const int there = (lim_most - t * 64 + 15) >> 4;  // pieces that somebody sees, or more
+        size_t at[4], scale_at;
+        bool mine, all;  // this lane's piece has a page; all have
+        if (wide) {
+            mine = all = page[0] >= 0 && page[0] < a.npages;
+            const unsigned from = mine ? page[0] : 0, from_off = mine ? off[0] : 0;
+            at[0] = (size_t)from * page_bytes + from_off * TB;
+#pragma unroll
+            for (int s = 1; s < 4; s++) at[s] = at[0] + min(s, there - 1) * (16 * TB);
+            scale_at = (size_t)from * page_scales + (from_off + lane);
+        } else {
+            int from = 0, from_off = 0, from_own = 0, off_own = 0;
+            mine = false;
+            all = true;
+#pragma unroll
+            for (int s = 0; s < 4; s++) {
+                const bool ok = s < there && page[s] >= 0 && page[s] < a.npages;
+                from = ok ? page[s] : from;
+                from_off = ok ? off[s] : from_off;
+                at[s] = (size_t)(unsigned)from * page_bytes + (unsigned)from_off * TB;
+                from_own = j == s ? from : from_own;
+                off_own = j == s ? from_off : off_own;
+                mine = j == s ? ok : mine;
+                all &= ok;
+            }
+            scale_at = (size_t)(unsigned)from_own * page_scales + (unsigned)(off_own + c);
+        }
+        unsigned kw[4][S::kKeyWords], vw[4][S::kValueWords], ks[G], vs[G];
+#pragma unroll
+        for (int s = 0; s < 4; s++) load_words<S::kKeyWords>(kw[s], k_codes + at[s] + key_at);
+#pragma unroll
+        for (int g = 0; g < G; g++) ks[g] = k_scales[scale_at + (unsigned)(g * a.page)];
+#pragma unroll
+        for (int g = 0; g < G; g++) vs[g] = v_scales[scale_at + (unsigned)(g * a.page)];
+#pragma unroll
+        for (int s = 0; s < 4; s++) load_value<BITS, HD>(vw[s], v_codes + at[s] + value_at, v_codes + at[s] + half_at);
+        ask(t + t_step);
+
+        // scores: every piece's products give all lanes of a column the same; a lane keeps those of piece j
+        f4 d = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int s = 0; s < 4; s++) {
+            f4 e = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int i = 0; i < S::kPieces; i++) e = __builtin_amdgcn_mfma_f32_16x16x32_f16(q[i], key_codes<BITS>(&kw[s][i * BITS / 4]), e, 0, 0, 0);
+#pragma unroll
+            for (int x = 0; x < 4; x++)
+                if (x < R * GP && x % GP < G) d[x] = s == 0 || j == s ? e[x] : d[x];
+        }
+        const int pos = t * 64 + lane;
+        const bool whole = t * 64 + 64 <= lim_least && all;
+        if (!whole && (pos >= lim_most || !mine)) {
+#pragma unroll
+            for (int g = 0; g < G; g++) vs[g] = 0;
+        }
+        float most_s = low_half(vs[0]);
+#pragma unroll
+        for (int g = 1; g < G; g++) most_s = fmaxf(most_s, low_half(vs[g]));
+        const float most_e = (float)__builtin_amdgcn_frexp_expf(most_s);
+#pragma unroll
+        for (int h = 0; h < R; h++) {
+            float y = 0.0f;
+#pragma unroll
+            for (int g = 0; g < G; g++) y = __builtin_fmaf(low_half(ks[g]), d[h * GP + g], __builtin_fmaf(high_half(ks[g]), qsum[h][g], y));
+            y *= key_scale[h];
+            const bool seen = whole || (pos < lim[h] && mine);
+            y = seen ? y : kNothing;
+            // a weight is at most 2^15: p * scale < 2^(y - ref + exponent of the scale)
+            const float reach = y + most_e;
+            if (__any(reach > ref[h] + 15.0f)) {
+                const float next = fmaxf(ref[h], wave_max(reach) - 11.0f);
+                const float f = __builtin_amdgcn_exp2f(ref[h] - next);
+                ref[h] = next;
+                l[h] *= f;
+#pragma unroll
+                for (int g = 0; g < G; g++) {
+                    z[h][g] *= f;
+#pragma unroll
+                    for (int i = 0; i < S::kAcc; i++) acc[i][h * GP + g] *= f;
+                }
+            }
+            const float p = seen ? __builtin_amdgcn_exp2f(y - ref[h]) : 0.0f;
+            l[h] += p;
+#pragma unroll
+            for (int g = 0; g < G; g++) {
+                z[h][g] = __builtin_fmaf(p, high_half(vs[g]), z[h][g]);
+                const float ps = p * low_half(vs[g]);
+                const _Float16 w = (_Float16)ps;
+                weights[(h * GP + g) * F::kLdsRow + key_place] = w;
+                weights[(4 + h * GP + g) * F::kLdsRow + key_place] = (_Float16)(ps - (float)w);
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            const h8 w = *reinterpret_cast<const h8 *>(weights_at + u * 32), rest = *reinterpret_cast<const h8 *>(weights_at + 4 * F::kLdsRow + u * 32);
+            weigh_values<BITS, HD>(acc, w, rest, vw[2 * u], vw[2 * u + 1], c);
+        }
+    }
+
+    // what the waves have, side by side
+    float *vals = reinterpret_cast<float *>(lds[wave]);
+#pragma unroll
+    for (int h = 0; h < R; h++) {
+        const float sum = wave_sum(l[h]);
+        if (lane == 0) lds_stats[wave][h][0] = ref[h], lds_stats[wave][h][1] = sum;
+#pragma unroll
+        for (int g = 0; g < G; g++) z[h][g] = wave_sum(z[h][g]);
+    }
+    // (rows 4, 5, .. of these products are rows 0, 1, .. again: the first 16 lanes store)
+#pragma unroll
+    for (int i = 0; i < S::kAcc; i++) {
+        const int ch = value_channel<BITS, HD>(i, c);
+#pragma unroll
+        for (int h = 0; h < R; h++)
+#pragma unroll
+            for (int g = 0; g < G; g++)
+                if (j == 0 && g == ch >> 5) vals[h * HD + ch] = __builtin_fmaf(acc[i][h * GP + g], value_unit<BITS, HD>(i), z[h][g]);
+    }
+    __syncthreads();
+    float *part = splits > 1 ? a.parts + ((size_t)blockIdx.z * units + (unsigned)(b * nkv + kv)) * F::kPart : nullptr;
+    for (int e = threadIdx.x; e < rows * HD; e += NW * 64) {
+        const int h = e / HD, ch = e - h * HD;
+        float m = lds_stats[0][h][0];
+#pragma unroll
+        for (int w = 1; w < NW; w++) m = fmaxf(m, lds_stats[w][h][0]);
+        float sum = 0.0f, ls = 0.0f;
+#pragma unroll
+        for (int w = 0; w < NW; w++) {
+            const float f = __builtin_amdgcn_exp2f(lds_stats[w][h][0] - m);
+            sum = __builtin_fmaf(f, reinterpret_cast<const float *>(lds[w])[e], sum);
+            ls = __builtin_fmaf(f, lds_stats[w][h][1], ls);
+        }
+        if (part) {
+            part[32 + e] = sum;
+            if ((ch & 31) == 0) part[2 * (h * GP + (ch >> 5))] = m, part[2 * (h * GP + (ch >> 5)) + 1] = ls;
+        } else {
+            const int row = row0 + h, i = row_of(row), r = row - i * per;
+            a.Z[((size_t)b * n + i) * a.ldz + (size_t)(kv * per + r) * HD + ch] = (_Float16)(ls == 0.0f ? 0.0f : sum / ls);
+        }
+    }
+}
+
+// The parts of a unit's rows: one workgroup a (block of rows, unit, 32 channels of a row), 8 threads' worth of parts at a time a channel.
+__global__ __launch_bounds__(256) void mha_kv_join_kernel(const KvMhaArgs a) {
+    constexpr int kPer = 256 / 32;
+    __shared__ float lds[3][kPer][32];
+    const int groups = a.hd / ET_KV_GROUP, part_floats = 32 + a.block_rows * a.hd;
+    const int block = blockIdx.y, col_g = blockIdx.x % (a.block_rows * groups), unit = blockIdx.x / (a.block_rows * groups);
+    const int h = col_g / groups, g = col_g - h * groups;
+    const int b = unit / a.nkv, kv = unit - b * a.nkv;
+    const int count = a.counts ? min(max(a.counts[b], 0), a.n) : a.n;
+    const int row = block * a.block_rows + h;
+    if (row >= count * a.per) return;
+    const float *part = a.parts + ((size_t)block * a.splits * a.units + unit) * part_floats;
+    const size_t next = (size_t)a.units * part_floats;
+    const int ch = threadIdx.x & 31, lot = threadIdx.x >> 5, col = h * a.cols + g, at = 32 + h * a.hd + g * 32 + ch;
+    float m = kNothing, sum = 0.0f, ls = 0.0f;
+    for (int s0 = lot; s0 < a.splits; s0 += 4 * kPer) {  // four parts asked for at once
+        float pm[4], pl[4], pv[4];
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const int s = min(s0 + k * kPer, a.splits - 1);
+            const float *p = part + s * next;
+            pm[k] = s0 + k * kPer < a.splits ? p[2 * col] : kNothing;
+            pl[k] = s0 + k * kPer < a.splits ? p[2 * col + 1] : 0.0f;
+            pv[k] = s0 + k * kPer < a.splits ? p[at] : 0.0f;
+        }
+        const float most = fmaxf(fmaxf(fmaxf(pm[0], pm[1]), fmaxf(pm[2], pm[3])), m);
+        const float f = __builtin_amdgcn_exp2f(m - most);
+        m = most;
+        sum *= f;
+        ls *= f;
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const float fk = __builtin_amdgcn_exp2f(pm[k] - most);
+            sum = __builtin_fmaf(fk, pv[k], sum);
+            ls = __builtin_fmaf(fk, pl[k], ls);
+        }
+    }
+    lds[0][lot][ch] = m, lds[1][lot][ch] = sum, lds[2][lot][ch] = ls;
+    __syncthreads();
+    if (lot != 0) return;
+#pragma unroll
+    for (int w = 1; w < kPer; w++) {
+        const float mw = lds[0][w][ch], most = fmaxf(m, mw), f = __builtin_amdgcn_exp2f(m - most), fw = __builtin_amdgcn_exp2f(mw - most);
+        m = most;
+        sum = sum * f + lds[1][w][ch] * fw;
+        ls = ls * f + lds[2][w][ch] * fw;
+    }
+    const int i = row / a.per, r = row - i * a.per;
+    a.Z[((size_t)b * a.n + i) * a.ldz + (size_t)(kv * a.per + r) * a.hd + g * 32 + ch] = (_Float16)(ls == 0.0f ? 0.0f : sum / ls);
+}
+
+namespace {
+
+using KvKernel = void (*)(KV_LEADING, const KvMhaArgs);
+
+struct KvForm {
+    KvKernel few, many;  // of 4 waves; of many
+    int rows, cols, many_waves, tile;
+};
+
+// Rows: of a key/value head in the call.
+template <int BITS, int HD> KvForm form_of(long long rows) {
+    if constexpr (HD <= 128) {
+        constexpr int cols = KvShape<BITS, HD>::kCols, heads = 4 / cols;
+        if (rows == 1) return {mha_kv_few_kernel<BITS, HD, 1, 4>, mha_kv_few_kernel<BITS, HD, 1, 8>, 1, cols, 8, 64};
+        if (rows <= heads) return {mha_kv_few_kernel<BITS, HD, heads, 4>, mha_kv_few_kernel<BITS, HD, heads, 8>, heads, cols, 8, 64};
+    }
+    return {mha_kv_kernel<BITS, HD, 4>, mha_kv_kernel<BITS, HD, (HD <= 128 ? 16 : 8)>, KvShape<BITS, HD>::kRows, KvShape<BITS, HD>::kCols, HD <= 128 ? 16 : 8, 32};
+}
+
+template <int BITS> KvForm form_of(int hd, long long rows) {
+    switch (hd) {
+        case 32: return form_of<BITS, 32>(rows);
+        case 64: return form_of<BITS, 64>(rows);
+        case 96: return form_of<BITS, 96>(rows);
+        case 128: return form_of<BITS, 128>(rows);
+        case 160: return form_of<BITS, 160>(rows);
+        case 192: return form_of<BITS, 192>(rows);
+        case 224: return form_of<BITS, 224>(rows);
+        default: return form_of<BITS, 256>(rows);
+    }
+}
+
+struct KvPlan {
+    KvForm form;
+    int blocks, splits, waves;
+    size_t bytes;
+};
+
+// Waves of a workgroup and workgroups that share the keys of a (sequence, key/value head): 4096 waves, which fill the chip, but at least four tiles a wave if every
+// sequence were as long as its table; a second launch, which joins the parts, costs 3 to 6 us.
+int kv_plan(const char *fn, KvPlan &p, const et_kv_cache *c, int max_pages, int B, int n, int nh) {
+    ET_REQUIRE(nh > 0 && nh % c->nkv == 0, ET_ERR_INVALID_ARG, "%s: nh=%d must be a multiple of nkv=%d", fn, nh, c->nkv);
+    const int per = nh / c->nkv;
+    const long long rows = (long long)n * per;
+    p.form = c->bits == 4 ? form_of<4>(c->hd, rows) : form_of<8>(c->hd, rows);
+    const long long blocks = (rows + p.form.rows - 1) / p.form.rows, units = (long long)B * c->nkv;
+    ET_REQUIRE(rows <= 0x7fffffffLL && B <= 65535 && blocks <= 65535 && units * blocks <= (1LL << 24), ET_ERR_UNSUPPORTED, "%s: B=%d n=%d nh=%d", fn, B, n, nh);
+    p.blocks = (int)blocks;
+    const long long tiles = ((long long)max_pages * c->page + p.form.tile - 1) / p.form.tile, groups = units * blocks;
+    p.waves = groups >= 512 ? 4 : p.form.many_waves;
+    p.splits = groups == 0 ? 1 : (int)std::max(1LL, std::min({(4096 / p.waves + groups - 1) / groups, tiles / (4 * p.waves), 256LL}));
+    p.splits = std::min(p.splits, (int)(65535 / std::max(1LL, blocks)));
+    p.bytes = p.splits > 1 ? (size_t)(groups * p.splits) * (32 + p.form.rows * c->hd) * sizeof(float) : 0;
+    return ET_OK;
+}
+
+}  // namespace
 
 }  // namespace et
 
@@ -96,8 +760,10 @@ int et_mha_kv_workspace(const et_kv_cache *cache, int max_pages, int B, int n, i
     static const int32_t any = 0;
     const int st = kv_check_cache("et_mha_kv_workspace", cache, &any, max_pages, B, n);
     if (st != ET_OK) return st;
-    *bytes = 0;
-    return ET_OK;
+    KvPlan p;
+    const int sp = kv_plan("et_mha_kv_workspace", p, cache, max_pages, B, n, nh);
+    if (sp == ET_OK) *bytes = p.bytes;
+    return sp;
 }
 
 int et_mha_kv_f16(const et_kv_cache *cache, const int32_t *table, int max_pages, const int32_t *starts, const int32_t *counts, const et_f16 *Q, int ldq,
@@ -106,36 +772,50 @@ int et_mha_kv_f16(const et_kv_cache *cache, const int32_t *table, int max_pages,
     const int st = kv_check_cache("et_mha_kv_f16", cache, table, max_pages, B, n);
     if (st != ET_OK) return st;
     ET_REQUIRE((flags & ~ET_MHA_CAUSAL) == 0, ET_ERR_INVALID_ARG, "et_mha_kv_f16: flags=%d", flags);
-    ET_REQUIRE(nh > 0 && nh % cache->nkv == 0, ET_ERR_INVALID_ARG, "et_mha_kv_f16: nh=%d must be a multiple of nkv=%d", nh, cache->nkv);
+    KvPlan p;
+    const int sp = kv_plan("et_mha_kv_f16", p, cache, max_pages, B, n, nh);
+    if (sp != ET_OK) return sp;
     const long long width = (long long)nh * cache->hd;
     ET_REQUIRE(ldq >= width && ldz >= width, ET_ERR_INVALID_ARG, "et_mha_kv_f16: row strides %d, %d below nh * hd = %lld", ldq, ldz, width);
     ET_REQUIRE(ldq % 8 == 0 && ldz % 8 == 0, ET_ERR_UNSUPPORTED, "et_mha_kv_f16: row strides must be multiples of 8");
     ET_REQUIRE(((reinterpret_cast<uintptr_t>(Q) | reinterpret_cast<uintptr_t>(Z)) & 15) == 0, ET_ERR_UNSUPPORTED,
                "et_mha_kv_f16: Q and Z must be 16-byte aligned");
-    ET_REQUIRE(B <= 65535 && n <= 65535, ET_ERR_UNSUPPORTED, "et_mha_kv_f16: B=%d n=%d", B, n);
+    ET_REQUIRE(workspace_bytes >= p.bytes && (workspace || p.bytes == 0), ET_ERR_INVALID_ARG, "et_mha_kv_f16: a workspace of %zu bytes, %zu are needed",
+               workspace ? workspace_bytes : 0, p.bytes);
+    ET_REQUIRE(p.bytes == 0 || (reinterpret_cast<uintptr_t>(workspace) & 15) == 0, ET_ERR_UNSUPPORTED, "et_mha_kv_f16: the workspace must be 16-byte aligned");
     if (B == 0 || n == 0) return ET_OK;
     KvMhaArgs a;
-    a.k_codes = static_cast<const unsigned char *>(cache->k_codes);
-    a.v_codes = static_cast<const unsigned short *>(cache->v_codes);
+    a.k_codes = static_cast<const char *>(cache->k_codes);
+    a.v_codes = static_cast<const char *>(cache->v_codes);
     a.k_scales = reinterpret_cast<const unsigned *>(cache->k_scales);
     a.v_scales = reinterpret_cast<const unsigned *>(cache->v_scales);
-    a.table = table;
-    a.starts = starts;
     a.counts = counts;
     a.Q = reinterpret_cast<const _Float16 *>(Q);
     a.Z = reinterpret_cast<_Float16 *>(Z);
+    a.parts = static_cast<float *>(workspace);
     a.ldq = ldq;
     a.ldz = ldz;
     a.nkv = cache->nkv;
-    a.hd = cache->hd;
+    a.per = nh / cache->nkv;
     a.page = cache->page;
     a.npages = cache->npages;
-    a.max_pages = max_pages;
     a.n = n;
-    a.nh = nh;
     a.causal = flags & ET_MHA_CAUSAL;
+    a.hd = cache->hd;
+    a.cols = p.form.cols;
+    a.block_rows = p.form.rows;
+    a.units = B * cache->nkv;
+    a.splits = p.splits;
+    // pieces below 2^27 (and a few tiles on): piece / d = piece * ceil(2^s / d) >> s with s = 28 + ceil(log2 d)
+    const unsigned d = (unsigned)cache->page / 16;
+    unsigned shift = 28;
+    while ((1ull << (shift - 28)) < d) shift++;
+    const unsigned magic = (unsigned)(((1ull << shift) + d - 1) / d);
     a.scale_log2e = scale * 1.4426950408889634f;
-    return launch_kernel("mha_kv_plain_kernel", cache->bits == 4 ? mha_kv_plain_kernel<4> : mha_kv_plain_kernel<8>, dim3(nh, n, B), 64, 0, as_stream(stream), a);
+    const int sl = launch_kernel("mha_kv_kernel", p.waves == 4 ? p.form.few : p.form.many, dim3((unsigned)cache->nkv, (unsigned)B, (unsigned)(p.blocks * p.splits)), p.waves * 64, 0, as_stream(stream),
+                                 table, starts, counts, max_pages, a.units, a.splits, a.per, magic, shift, (int)d, n, a);
+    if (sl != ET_OK || p.splits == 1) return sl;
+    return launch_kernel("mha_kv_join_kernel", mha_kv_join_kernel, dim3((unsigned)(a.units * p.form.rows * (cache->hd / ET_KV_GROUP)), (unsigned)p.blocks), 256, 0, as_stream(stream), a);
 }
 
 }  // extern "C"

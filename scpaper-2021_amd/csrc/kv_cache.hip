@@ -193,7 +193,8 @@ int kv_check_cache(const char *fn, const et_kv_cache *c, const int32_t *table, i
                  reinterpret_cast<uintptr_t>(c->v_scales)) & 15) == 0, ET_ERR_UNSUPPORTED, "%s: the cache's buffers must be 16-byte aligned", fn);
     ET_REQUIRE((reinterpret_cast<uintptr_t>(table) & 3) == 0, ET_ERR_UNSUPPORTED, "%s: table must be 4-byte aligned", fn);
     ET_REQUIRE((long long)max_pages * c->page <= 0x7fffffffLL, ET_ERR_UNSUPPORTED, "%s: max_pages * page = %lld positions", fn, (long long)max_pages * c->page);
-    ET_REQUIRE((long long)c->nkv * c->hd <= (1 << 24), ET_ERR_UNSUPPORTED, "%s: nkv * hd = %lld", fn, (long long)c->nkv * c->hd);
+    ET_REQUIRE((long long)c->nkv * c->hd <= (1 << 24) && (long long)c->nkv * c->hd * c->page / 8 * c->bits < (1LL << 31), ET_ERR_UNSUPPORTED,
+               "%s: nkv * hd = %lld, %d tokens a page", fn, (long long)c->nkv * c->hd, c->page);
     return ET_OK;
 }
 

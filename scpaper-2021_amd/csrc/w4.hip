@@ -1,4 +1,6 @@
 // Linear with 4-bit weights, a scale and a lowest value for every 32, 64 or 128 input features of an output feature (layout: et_abi.h).
+#include <atomic>
+
 #include "group_quant.hip.h"
 
 namespace et {
@@ -54,31 +56,278 @@ __global__ __launch_bounds__(256) void w4_to_dense_kernel(const unsigned *codes,
 
 struct W4Args {
     const unsigned char *codes;
-    const unsigned *scales;
+    const unsigned *scales;  // scale in the low half, low in the high one
     const _Float16 *bias, *X;
     _Float16 *Y;
     float *Y32;
-    int T, in, out, group, act;
+    int T, in, out, act;
 };
 
-// One wave an output value.
-__global__ __launch_bounds__(256) void w4_linear_plain_kernel(const W4Args a) {
-    const int lane = threadIdx.x & 63, o = blockIdx.x * 4 + (threadIdx.x >> 6);
-    const size_t t = blockIdx.y;
-    const _Float16 *x = a.X + t * a.in;
-    float y = 0.0f;
-    for (int i = lane; i < a.in; i += 64) {
-        const unsigned sl = a.scales[(size_t)(i / a.group) * a.out + o];
-        const unsigned c = (a.codes[((size_t)o * a.in + i) / 2] >> (i % 2 * 4)) & 15u;
-        y += (float)x[i] * __builtin_fmaf(f16_bits_value(sl & 0xffffu), (float)c, f16_bits_value(sl >> 16));
+typedef unsigned w4u __attribute__((ext_vector_type(4)));
+
+constexpr int kW4Raw = 0x00020000;             // word 3 of a resource: raw, 32-bit data
+constexpr unsigned kW4Nothing = 0x80000000u;  // an offset behind every resource: reads as zero
+
+__device__ __forceinline__ w4u w4_load(__amdgpu_buffer_rsrc_t r, unsigned lane_at, int at) {
+    return __builtin_bit_cast(w4u, __builtin_amdgcn_raw_buffer_load_b128(r, (int)lane_at, at, 0));
+}
+
+__device__ __forceinline__ h8 w4_h8(unsigned a, unsigned b, unsigned c, unsigned d) { return __builtin_bit_cast(h8, w4u{a, b, c, d}); }
+
+// The eight codes of a word as binary16 numbers, code * 2^-17 (bits 7 to 10: up to 7 subnormal, as far apart from 8 on), in the order 0 4 1 5 2 6 3 7.
+__device__ __forceinline__ h8 w4_codes(unsigned w) {
+    constexpr unsigned m = 0x07800780u;
+    return w4_h8((w << 7) & m, (w << 3) & m, (w >> 1) & m, (w >> 5) & m);
+}
+// Eight activations in the same order.
+__device__ __forceinline__ h8 w4_order(w4u x) {
+    constexpr unsigned lows = 0x05040100u, highs = 0x07060302u;
+    return w4_h8(__builtin_amdgcn_perm(x[2], x[0], lows), __builtin_amdgcn_perm(x[2], x[0], highs), __builtin_amdgcn_perm(x[3], x[1], lows),
+                 __builtin_amdgcn_perm(x[3], x[1], highs));
+}
+// -> x0 x4 | x1 x5 | x2 x6 | x3 x7
+
+__device__ __forceinline__ float w4_scale(unsigned sl) { return (float)__builtin_bit_cast(h2, sl)[0]; }
+__device__ __forceinline__ float w4_low(unsigned sl) { return (float)__builtin_bit_cast(h2, sl)[1]; }
+
+// Y = act(X W^T + bias), W = low + scale * code.  Rows of the products are 16 output features, contraction is over the codes as they are, 128 input features ("a chunk") in
+// four products; scale and low come to a group's binary32 sums: y += scale * sum x code + low * sum x, the second sum from products with ones.
+//   SWAP 0: a lane's 16 bytes of a weight row are 32 input features, so the four lanes of a row hold the groups of a chunk side by side.  The products' columns are (row of
+//           X, group), zero outside the group: 16 / groups rows of X at a time.  GROUP 128: 16 rows.
+//   SWAP 1 (groups of 32 and 64, more rows): four (two) row swaps bring the words of one group into one register; columns are 16 rows of X.
+// A wave has RBK blocks of 16 output features, TBK blocks of columns of which TR rows of X are real, and takes U chunks at a time.  What it loads, 64 U bytes of a weight row and 256 U of X in a
+// piece, goes through LDS of its own to the lanes that multiply it: asked for by those, every 16 bytes were an access of the vector cache of their own, 52 an instruction, which bound
+// the kernel at 2.2 TB/s (16 rows, 8192 to 28672 features).  The next U chunks are in flight meanwhile.  The four or eight waves of a workgroup share the chunks of its
+// blocks and add up through LDS.
+template <int GROUP, int SWAP, int TBK, int TR, int RBK, int U> struct W4Shape {
+    static constexpr int NG = 128 / GROUP, COLS = SWAP ? 1 : NG, TPB = 16 / COLS;  // groups of a chunk; columns of a row of X; rows of X of a column block
+    static constexpr int SG = SWAP ? NG : 1;                                       // groups that a lane scales by itself
+    static constexpr int kWRow = 64 * U + 16, kXRow = 256 * U + 16;                // bytes of a row in LDS: the 16 lanes of a read on different banks
+    static constexpr int kW = RBK * 16 * kWRow, kX = TR * kXRow, kS = RBK * U * NG * 64;
+    static constexpr int kZero = 64;
+    static constexpr int kWave = kW + kX + kS + kZero;            // bytes of a wave
+    static constexpr int kSum = RBK * TBK * TPB * 4 * 16;         // what it leaves in the end, in the same place
+    static constexpr int kLds = kWave > kSum ? kWave : kSum;
+    static constexpr int kXLoads = (TR * U * 16 + 63) / 64, kSLoads = (RBK * U * NG * 4 + 63) / 64;
+};
+
+template <int GROUP, int SWAP, int TBK, int TR, int RBK, int U> __global__ __launch_bounds__(512) void w4_linear_kernel(const W4Args a) {
+    using S = W4Shape<GROUP, SWAP, TBK, TR, RBK, U>;
+    constexpr int NG = S::NG, COLS = S::COLS, TPB = S::TPB, SG = S::SG;
+    extern __shared__ __align__(16) char lds_all[];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int c = lane & 15, j = lane >> 4;
+    const int gg = c % COLS, tl = c / COLS;
+    const int nb = a.out >> 4, nc = (a.in + 127) >> 7;
+    const int rb0 = blockIdx.x * RBK, waves_log2 = blockDim.x == 512 ? 3 : 2;
+    const int t0 = blockIdx.y * (TPB * TBK);
+    char *lds_w = lds_all + wave * S::kLds, *lds_x = lds_w + S::kW, *lds_s = lds_x + S::kX, *lds_zero = lds_s + S::kS;
+
+    // what this lane loads: pieces of 16 bytes of rows of weights, of X, of scales
+    __amdgpu_buffer_rsrc_t w[RBK];
+#pragma unroll
+    for (int i = 0; i < RBK; i++)
+        w[i] = __builtin_amdgcn_make_buffer_rsrc(const_cast<unsigned char *>(a.codes) + (size_t)(min(rb0 + i, nb - 1) * 16) * (a.in / 2), 0, 8 * a.in, kW4Raw);
+    const int x_rows = min(a.T - t0, TPB * TBK);
+    const auto xr = __builtin_amdgcn_make_buffer_rsrc(const_cast<_Float16 *>(a.X) + (size_t)t0 * a.in, 0, x_rows * a.in * 2, kW4Raw);
+    w4u gw[RBK][U], gx[S::kXLoads], gs[S::kSLoads];
+    const int share = (nc + (1 << waves_log2) - 1) >> waves_log2, k_first = wave * share, in_end = min(a.in, (k_first + share) * 128);
+    auto load = [&](int k0) {
+        const int left = in_end - k0 * 128;  // input features from here on
+#pragma unroll
+        for (int i = 0; i < U; i++) {
+            const int row = (i * 64 + lane) / (4 * U), piece = lane % (4 * U);
+            const unsigned at = 32 * piece < left ? row * (a.in / 2) + 16 * piece : kW4Nothing;
+#pragma unroll
+            for (int r = 0; r < RBK; r++) gw[r][i] = w4_load(w[r], at, k0 * 64);
+        }
+#pragma unroll
+        for (int i = 0; i < S::kXLoads; i++) {
+            const int row = (i * 64 + lane) / (16 * U), piece = lane % (16 * U);
+            gx[i] = w4_load(xr, 8 * piece < left && row < x_rows ? row * a.in * 2 + 16 * piece : kW4Nothing, k0 * 256);
+        }
+#pragma unroll
+        for (int i = 0; i < S::kSLoads; i++) {
+            const int e = i * 64 + lane, quarter = e & 3, ug = (e >> 2) % (U * NG), r = min((e >> 2) / (U * NG), RBK - 1);
+            const int grp = min(k0 * NG + ug, a.in / GROUP - 1);
+            gs[i] = *reinterpret_cast<const w4u *>(a.scales + (size_t)grp * a.out + min(rb0 + r, nb - 1) * 16 + 4 * quarter);
+        }
+    };
+    auto keep = [&]() {
+#pragma unroll
+        for (int i = 0; i < U; i++) {
+            const int row = (i * 64 + lane) / (4 * U), piece = lane % (4 * U);
+#pragma unroll
+            for (int r = 0; r < RBK; r++) *reinterpret_cast<w4u *>(lds_w + (r * 16 + row) * S::kWRow + piece * 16) = gw[r][i];
+        }
+#pragma unroll
+        for (int i = 0; i < S::kXLoads; i++) {
+            const int row = (i * 64 + lane) / (16 * U), piece = lane % (16 * U);
+            if (S::kXLoads * 64 == TR * U * 16 || row < TR) *reinterpret_cast<h8 *>(lds_x + row * S::kXRow + piece * 16) = w4_order(gx[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < S::kSLoads; i++)
+            if (S::kSLoads * 64 == RBK * U * NG * 4 || i * 64 + lane < RBK * U * NG * 4) *reinterpret_cast<w4u *>(lds_s + (i * 64 + lane) * 16) = gs[i];
+    };
+
+    // what this lane multiplies: nothing in a column of another group, or of a row of X that is none
+    const char *w_from = lds_w + c * S::kWRow + 16 * j, *s_from = lds_s + (SWAP ? 0 : gg * 64) + 16 * j;
+    const char *x_from[TBK];
+    int x_step[TBK];  // of a chunk
+#pragma unroll
+    for (int b = 0; b < TBK; b++) {
+        const int t = b * TPB + tl;
+        const bool mine = t < TR && (SWAP || gg == j * 32 / GROUP);
+        x_from[b] = mine ? lds_x + t * S::kXRow + (!SWAP ? 64 * j : GROUP == 32 ? 16 * j : 64 * (j & 1) + 16 * (j >> 1)) : lds_zero;
+        x_step[b] = mine ? 1 : 0;
     }
-    y = apply_act(wave_sum(y) + (a.bias ? (float)a.bias[o] : 0.0f), a.act);
-    if (lane != 0) return;
-    if (a.Y) a.Y[t * a.out + o] = (_Float16)y;
-    else a.Y32[t * a.out + o] = y;
+    if (lane < 4) *reinterpret_cast<w4u *>(lds_zero + lane * 16) = w4u{0, 0, 0, 0};
+
+    f4 acc[RBK][TBK];
+#pragma unroll
+    for (int i = 0; i < RBK; i++)
+#pragma unroll
+        for (int b = 0; b < TBK; b++) acc[i][b] = f4{0.f, 0.f, 0.f, 0.f};
+
+    if (k_first * 128 < in_end) load(k_first);
+    for (int k0 = k_first; k0 * 128 < in_end; k0 += U) {
+        keep();
+        if ((k0 + U) * 128 < in_end) load(k0 + U);
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            h8 xo[TBK][4];
+            f4 sums[TBK][SG];  // of X, * 2^-17
+            const h8 ones = w4_h8(0x00800080u, 0x00800080u, 0x00800080u, 0x00800080u);
+#pragma unroll
+            for (int b = 0; b < TBK; b++) {
+#pragma unroll
+                for (int g = 0; g < SG; g++) sums[b][g] = f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    const int g = !SWAP ? 0 : GROUP == 32 ? r : r & 1;
+                    // the piece of a chunk that product r multiplies; the others' lanes stay at the zeros
+                    const int piece = !SWAP ? 16 * r : GROUP == 32 ? 64 * r : 128 * (r & 1) + 32 * (r >> 1);
+                    xo[b][r] = *reinterpret_cast<const h8 *>(x_from[b] + x_step[b] * (256 * u + piece));
+                    sums[b][g] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, xo[b][r], sums[b][g], 0, 0, 0);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < RBK; i++) {
+                const w4u raw = *reinterpret_cast<const w4u *>(w_from + i * 16 * S::kWRow + 64 * u);
+                unsigned v[4] = {raw[0], raw[1], raw[2], raw[3]};
+                if constexpr (SWAP) {
+                    auto swap32 = [](unsigned &p, unsigned &q) {
+                        auto r = __builtin_amdgcn_permlane32_swap(p, q, false, false);
+                        p = r[0], q = r[1];
+                    };
+                    auto swap16 = [](unsigned &p, unsigned &q) {
+                        auto r = __builtin_amdgcn_permlane16_swap(p, q, false, false);
+                        p = r[0], q = r[1];
+                    };
+                    if constexpr (GROUP == 32) {
+                        swap32(v[0], v[2]);
+                        swap32(v[1], v[3]);
+                        swap16(v[0], v[1]);
+                        swap16(v[2], v[3]);
+                    } else {
+                        swap32(v[0], v[1]);
+                        swap32(v[2], v[3]);
+                    }
+                }
+                h8 cd[4];
+#pragma unroll
+                for (int r = 0; r < 4; r++) cd[r] = w4_codes(v[r]);
+                w4u sl[SG];
+#pragma unroll
+                for (int g = 0; g < SG; g++) sl[g] = *reinterpret_cast<const w4u *>(s_from + ((i * U + u) * NG + g) * 64);
+#pragma unroll
+                for (int b = 0; b < TBK; b++) {
+                    f4 d[SG];
+#pragma unroll
+                    for (int g = 0; g < SG; g++) d[g] = f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int r = 0; r < 4; r++) {
+                        const int g = !SWAP ? 0 : GROUP == 32 ? r : r & 1;
+                        d[g] = __builtin_amdgcn_mfma_f32_16x16x32_f16(cd[r], xo[b][r], d[g], 0, 0, 0);
+                    }
+#pragma unroll
+                    for (int g = 0; g < SG; g++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++)
+                            acc[i][b][e] = __builtin_fmaf(w4_scale(sl[g][e]), d[g][e], __builtin_fmaf(w4_low(sl[g][e]), sums[b][g][0], acc[i][b][e]));
+                }
+            }
+        }
+    }
+
+    // a row of X over its columns, then over the waves
+#pragma unroll
+    for (int i = 0; i < RBK; i++)
+#pragma unroll
+        for (int b = 0; b < TBK; b++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                if constexpr (COLS >= 2) acc[i][b][e] += dpp_move<kDppQuadXor1>(acc[i][b][e]);
+                if constexpr (COLS >= 4) acc[i][b][e] += dpp_move<kDppQuadXor2>(acc[i][b][e]);
+            }
+    auto store = [&](int i, int b, int t_in, int quarter, f4 y) {  // four output features of a row of X
+        const int t = t0 + b * TPB + t_in, o = (rb0 + i) * 16 + 4 * quarter;
+        if (t >= a.T || rb0 + i >= nb) return;
+        h4 bias = {0, 0, 0, 0};
+        if (a.bias) bias = *reinterpret_cast<const h4 *>(a.bias + o);
+        h4 out16;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            y[e] = apply_act(__builtin_fmaf(y[e], 0x1p17f, (float)bias[e]), a.act);
+            out16[e] = (_Float16)y[e];
+        }
+        if (a.Y) *reinterpret_cast<h4 *>(a.Y + (size_t)t * a.out + o) = out16;
+        else *reinterpret_cast<f4 *>(a.Y32 + (size_t)t * a.out + o) = y;
+    };
+    if (gg == 0) {
+#pragma unroll
+        for (int i = 0; i < RBK; i++)
+#pragma unroll
+            for (int b = 0; b < TBK; b++) reinterpret_cast<f4 *>(lds_w)[(i * TBK + b) * (TPB * 4) + tl * 4 + j] = acc[i][b];
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < RBK * TBK * TPB * 4; e += blockDim.x) {
+        const int ib = e / (TPB * 4), q = e - ib * (TPB * 4);
+        auto of = [&](int w) { return reinterpret_cast<const f4 *>(lds_all + w * S::kLds)[e]; };
+        f4 y = (of(0) + of(1)) + (of(2) + of(3));
+        if (waves_log2 == 3) y += (of(4) + of(5)) + (of(6) + of(7));
+        store(ib / TBK, ib % TBK, q >> 2, q & 3, y);
+    }
 }
 
 namespace {
+
+struct W4Form {
+    void (*kernel)(W4Args);
+    int rows_x, blocks, kw, lds;             // rows of X and blocks of output features of a workgroup; its waves; bytes of LDS
+    std::atomic<unsigned long long> *large;  // devices where the kernel may have that much, a bit each
+};
+
+template <int GROUP, int SWAP, int TBK, int TR, int RBK, int U> W4Form w4_form_of(int kw) {
+    using S = W4Shape<GROUP, SWAP, TBK, TR, RBK, U>;
+    static std::atomic<unsigned long long> large{0};
+    return {w4_linear_kernel<GROUP, SWAP, TBK, TR, RBK, U>, S::TPB * TBK, RBK, kw, S::kLds * kw, &large};
+}
+
+// Blocks of output features (nb of them) a wave and waves that share a block, by what fills the chip: measured at 1024 -> 4096 (nb 256), 4096 -> 4096 (256), 800 -> 28800 (1800)
+// and 8192 -> 28672 (1792 blocks), in us for 1, 2 and 4 blocks a wave of four (of eight waves):
+//   1 row, 256 blocks 3.5 3.8 (3.8 4.3), 1800 blocks 6.9 6.1 (10.9 8.8); 16 rows, groups of 128, 1792 blocks 45 37 36 (55 43 36);
+//   45 rows, groups of 32, 256 blocks 12.8 15.8 (11.5 13.1), 1792 blocks 105 83 (116 89).
+template <int GROUP> W4Form w4_form(int T, int nb) {
+    constexpr int few = GROUP / 8;  // rows of X whose columns fill a product
+    if (T == 1) return nb <= 1024 ? w4_form_of<GROUP, 0, 1, 1, 1, 2>(4) : w4_form_of<GROUP, 0, 1, 1, 2, 2>(4);
+    if (T <= few) return nb <= 512 ? w4_form_of<GROUP, 0, 1, few, 1, 2>(4) : nb <= 1024 ? w4_form_of<GROUP, 0, 1, few, 2, 2>(4) : w4_form_of<GROUP, 0, 1, few, 4, 1>(4);
+    constexpr int swap = GROUP < 128;
+    if constexpr (swap)
+        if (T <= 16) return nb <= 512 ? w4_form_of<GROUP, 1, 1, 16, 1, 1>(8) : w4_form_of<GROUP, 1, 1, 16, 2, 1>(4);
+    if (T > 32 && T <= 48) return nb <= 512 ? w4_form_of<GROUP, swap, 3, 48, 1, 1>(8) : w4_form_of<GROUP, swap, 3, 48, 2, 1>(4);
+    return nb <= 512 ? w4_form_of<GROUP, swap, 2, 32, 1, 1>(8) : w4_form_of<GROUP, swap, 2, 32, 2, 1>(4);
+}
 
 int w4_check(const char *fn, const void *codes, const void *scales, const void *dense, int in, int out, int group) {
     ET_REQUIRE(codes && scales && dense, ET_ERR_INVALID_ARG, "%s: NULL pointer", fn);
@@ -125,11 +374,23 @@ int et_linear_w4_f16(const uint8_t *codes, const et_f16 *scales, int group, cons
     ET_REQUIRE(act == ET_ACT_NONE || act == ET_ACT_RELU || act == ET_ACT_GELU, ET_ERR_INVALID_ARG, "et_linear_w4_f16: act=%d", act);
     ET_REQUIRE(((reinterpret_cast<uintptr_t>(Y) | reinterpret_cast<uintptr_t>(Y32)) & 15) == 0 && (reinterpret_cast<uintptr_t>(bias) & 7) == 0,
                ET_ERR_UNSUPPORTED, "et_linear_w4_f16: the result must be 16-byte and the bias 8-byte aligned");
-    ET_REQUIRE(T <= 65535, ET_ERR_UNSUPPORTED, "et_linear_w4_f16: T=%d", T);
+    ET_REQUIRE(in <= (1 << 23) && T <= 65535 * 4, ET_ERR_UNSUPPORTED, "et_linear_w4_f16: T=%d in=%d", T, in);
     if (T == 0) return ET_OK;
-    W4Args a{codes, reinterpret_cast<const unsigned *>(scales), reinterpret_cast<const _Float16 *>(bias), reinterpret_cast<const _Float16 *>(X),
-             reinterpret_cast<_Float16 *>(Y), Y32, T, in, out, group, act};
-    return launch_kernel("w4_linear_plain_kernel", w4_linear_plain_kernel, dim3(out / 4, T), 256, 0, as_stream(stream), a);
+    const int nb = out / 16;
+    const W4Form f = group == 32 ? w4_form<32>(T, nb) : group == 64 ? w4_form<64>(T, nb) : w4_form<128>(T, nb);
+    if (f.lds > 64 * 1024) {
+        int dev = 0;
+        ET_HIP(hipGetDevice(&dev));
+        const unsigned long long bit = 1ull << (dev & 63);
+        if (!(f.large->load(std::memory_order_relaxed) & bit)) {
+            ET_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(f.kernel), hipFuncAttributeMaxDynamicSharedMemorySize, f.lds));
+            f.large->fetch_or(bit, std::memory_order_relaxed);
+        }
+    }
+    const W4Args a{codes, reinterpret_cast<const unsigned *>(scales), reinterpret_cast<const _Float16 *>(bias), reinterpret_cast<const _Float16 *>(X),
+                   reinterpret_cast<_Float16 *>(Y), Y32, T, in, out, act};
+    return launch_kernel("w4_linear_kernel", f.kernel, dim3((unsigned)((nb + f.blocks - 1) / f.blocks), (unsigned)((T + f.rows_x - 1) / f.rows_x)), f.kw * 64u, (size_t)f.lds,
+                         as_stream(stream), a);
 }
 
 }  // extern "C"

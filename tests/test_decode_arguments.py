@@ -64,6 +64,17 @@ def test_other_arguments(et):
     assert lib.et_kv_write_f16(None, P, 4, None, None, P, P, 128, 128, 1, 1, None) == -1
 
 
+def test_workspace_is_asked_for(et):
+    """One sequence of a million tokens on one head is shared out: what the parts leave needs memory, and a call without it is refused."""
+    c = cache(et, nkv=1, npages=1 << 16)
+    pages = 1 << 16
+    need = et.mha_kv_workspace(c, pages, 1, 1, 1)
+    assert need > 0
+    for ws, have in ((None, need), (P, need - 1), (P + 8, need)):
+        assert calls(et, c, max_pages=pages, nh=1, ws=ws, ws_bytes=have)["mha"] == (-2 if ws == P + 8 else -1), (ws, have)
+        assert b"workspace" in et.lib().et_last_error()
+
+
 def linear(et, codes=P, scales=P, group=32, bias=P, X=P, Y=P, Y32=None, T=1, n_in=64, out=16, act=0):
     return et.lib().et_linear_w4_f16(codes, scales, group, bias, X, Y, Y32, T, n_in, out, act, None)
 

@@ -144,11 +144,11 @@ def allowed(Z, stepped, lows, reach, hd, keys):
     """How far a row of et_mha_kv_f16 may be from binary64.  Half a step of binary16 (2^-11, relative) for the result and for every
     probability times scale; scores off by d, from hd + 16 roundings of 2^-24 in sums of magnitude `reach` and 2^-20 for exp2, move every p by
     d, and the sum of p by d; sums over the keys are in binary32 (keys + 16 roundings of 2^-24).  A product of probability and scale that is a
-    subnormal binary16 number is off by half a step of those instead, 2^-25, where the largest stands between 2^14 and 2^15 and the values
-    reach over at most 8 (they lie within 4 of zero): 2^-39 * 8 a key.  A subnormal result: 2^-25."""
+    subnormal binary16 number is off by half a step of those instead, 2^-25, where the largest stands between 2^10 and 2^15 and the values
+    reach over at most 8 (they lie within 4 of zero): 2^-35 * 8 a key.  A subnormal result: 2^-25."""
     d = (hd + 16) * 2.0 ** -24 * reach + 2.0 ** -20
     a = stepped + lows
-    return 2.0 ** -11 * np.abs(Z) + 2.0 ** -11 * stepped * (1 + 2.0 ** -10) + (2 * np.expm1(2 * d) + (keys + 16) * 2.0 ** -24) * a + keys * 2.0 ** -36 + 2.0 ** -25
+    return 2.0 ** -11 * np.abs(Z) + 2.0 ** -11 * stepped * (1 + 2.0 ** -10) + (2 * np.expm1(2 * d) + (keys + 16) * 2.0 ** -24) * a + keys * 2.0 ** -32 + 2.0 ** -25
 
 
 def filled(bits, nkv, hd, page, table, lengths, seed, npages):
