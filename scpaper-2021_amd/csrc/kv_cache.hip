@@ -1,12 +1,22 @@
 // A paged cache of keys and values in 4 or 8 bits: written as tokens arrive, read back (layout: et_abi.h).
 //
-// Sixteen lanes take one group of 32 channels of four tokens whose positions are 4q .. 4q + 3: lane % 4 the token, lane / 4 eight of the
-// channels.  A group's extremes are then two rotations inside the 16 lanes, and the four tokens' codes of V, which the cache holds side by
-// side, change places inside four neighbouring lanes.  Where a call does not hold all four tokens, the units of 16 bits of those it
-// holds are stored one by one: the bytes of the others are not touched.
+// Eight lanes take one group of 32 channels of four tokens whose positions are 4q .. 4q + 3, bits of the lane: 0 and 1 the token, 3 the eights of channels 0 and 2 or 1 and
+// 3 (bit 2: the next group).  A group's extremes are then one rotation inside the 16 lanes, and the four tokens' codes of V, which the cache holds side by side, change places
+// inside four neighbouring lanes.  Where a call does not hold all four tokens, the units of 16 bits of those it holds are stored one by one: the bytes of the others are not
+// touched.  Writing is bound by its arithmetic next to memory: 16 channels a lane share a group's scale (8 did not: 27 us for 16 x 1000 tokens of 8 heads of 128).
 #include "group_quant.hip.h"
 
 namespace et {
+
+// n / d of 31-bit n as a product: ceil(2^(31 + l) / d), l = ceil(log2 d), is off by less than 2^l / 2^(31 + l) of it.
+struct Divisor {
+    unsigned d, magic, shift;
+    explicit Divisor(unsigned by = 1) : d(by), shift(0) {
+        while ((1ull << shift) < by) shift++;
+        magic = (unsigned)((((1ull << (31 + shift)) + by - 1) / by) - 1);  // (- 1: of 1 it would not fit)
+    }
+    __device__ __forceinline__ unsigned of(unsigned n) const { return (unsigned)(((unsigned long long)n * magic + n) >> (31 + shift)); }
+};
 
 struct KvArgs {
     char *k_codes, *v_codes;
@@ -16,137 +26,108 @@ struct KvArgs {
     _Float16 *Kout, *Vout;
     int ldk, ldv;
     int nkv, hd, page, npages, max_pages;
-    int n, quads;         // rows of a sequence; groups of four positions that they can touch
-    unsigned nkvg, total; // groups of a token; units of work
+    int n;
+    unsigned total;            // units of work of a sequence: groups of a token times groups of four positions that n rows can touch
+    Divisor nkvg, groups, page_quads;  // groups of a token, of a head; groups of four positions of a page
 };
-
-template <int CTRL> __device__ __forceinline__ unsigned dpp_bits(unsigned v) {
-    return (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, false);
-}
 
 // Where a unit's tokens lie.
 struct KvUnit {
-    int group, head;   // of the head's groups; of the heads
-    long long row;     // row of this lane's token in the call's matrices
-    bool mine, all;    // this lane's token is one of the call's and has a place; all four are
-    size_t token, quad;  // token's index [pages][nkv][page] with page/head resolved, and that of the first of the four
-    size_t scale;      // index of the scale of (group, first token of the four)
+    int group, head;     // of the head's groups; of the heads
+    size_t row;          // of this lane's token in the call's matrices, or the nearest that is one
+    int count;           // rows of the sequence
+    bool mine, all;      // this lane's token is one of the call's and has a place; all four are
+    size_t token, quad;  // this lane's token and the first of the four, counted [pages][nkv][page]
+    size_t scale;        // the scale of (group, first token of the four)
     int tq, sub;
 };
 
 __device__ __forceinline__ KvUnit kv_unit(const KvArgs &a, unsigned unit) {
     KvUnit u;
-    const int lane = threadIdx.x & 15;
-    u.tq = lane & 3;
-    u.sub = lane >> 2;
-    const unsigned g = unit % a.nkvg, rest = unit / a.nkvg;
-    const int quad = (int)(rest % (unsigned)a.quads), b = (int)(rest / (unsigned)a.quads);
-    const int groups = a.hd / ET_KV_GROUP;
-    u.head = (int)g / groups;
-    u.group = (int)g - u.head * groups;
-    const long long start = a.starts ? a.starts[b] : 0;
-    const int count = a.counts ? min(max(a.counts[b], 0), a.n) : a.n;
-    // floor(start / 4) also below zero
-    const long long pos0 = ((start >> 2) + quad) * 4;
-    const long long i = pos0 + u.tq - start;
-    const long long pidx = pos0 / a.page;
+    const int b = blockIdx.y;
+    u.tq = threadIdx.x & 3;
+    u.sub = threadIdx.x >> 3 & 1;
+    const bool none = unit >= a.total;  // (of the pair of units that 16 lanes take, the second may be none: its lanes stay for the rotations, on the last unit)
+    if (none) unit = a.total - 1;
+    const unsigned q = a.nkvg.of(unit), g = unit - q * a.nkvg.d;
+    u.head = (int)a.groups.of(g);
+    u.group = (int)(g - u.head * a.groups.d);
+    const int start = a.starts ? a.starts[b] : 0, count = a.counts ? min(max(a.counts[b], 0), a.n) : a.n;
+    // floor(start / 4) + q also below zero; as 64-bit numbers where start + count pass 2^31
+    const long long quad = (start >> 2) + (long long)q;
+    const long long i0 = quad * 4 - start;  // row of the first of the four
+    const long long i = i0 + u.tq;
+    const bool reach = quad >= 0 && quad < (1ll << 29);
+    const unsigned page_at = a.page_quads.of(reach ? (unsigned)quad : 0u), off = ((reach ? (unsigned)quad : 0u) - page_at * a.page_quads.d) * 4;
     int page = -1;
-    if (pos0 >= 0 && pidx < a.max_pages) page = a.table[(size_t)b * a.max_pages + (size_t)pidx];
+    if (reach && page_at < (unsigned)a.max_pages) page = a.table[(size_t)b * a.max_pages + page_at];
     const bool placed = page >= 0 && page < a.npages;
-    const bool inside = i >= 0 && i < count;
-    u.mine = placed && inside;
-    const long long i0 = pos0 - start;
-    u.all = placed && i0 >= 0 && i0 + 3 < count;
-    const int off = placed ? (int)(pos0 - pidx * a.page) : 0;
+    u.mine = !none && placed && i >= 0 && i < count;
+    u.all = !none && placed && i0 >= 0 && i0 + 3 < count;
     const size_t ph = (size_t)(placed ? page : 0) * a.nkv + u.head;
-    u.quad = ph * a.page + off;
+    u.quad = ph * a.page + (placed ? off : 0u);
     u.token = u.quad + u.tq;
-    u.scale = (ph * groups + u.group) * a.page + off;
-    u.row = (long long)b * a.n + i;
+    u.scale = (ph * a.groups.d + u.group) * a.page + (placed ? off : 0u);
+    u.row = (size_t)b * a.n + (size_t)min(max(i, 0LL), (long long)max(count - 1, 0));
+    u.count = count;
     return u;
 }
 
-__device__ __forceinline__ float row16_min(float v) {
-    v = fminf(v, dpp_move<kRowRor4>(v));
-    return fminf(v, dpp_move<kRowRor8>(v));
-}
-__device__ __forceinline__ float row16_max(float v) {
-    v = fmaxf(v, dpp_move<kRowRor4>(v));
-    return fmaxf(v, dpp_move<kRowRor8>(v));
+template <int CTRL> __device__ __forceinline__ unsigned dpp_bits(unsigned v) {
+    return (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, false);
 }
 
-// Codes of eight values, and the group's (scale, low).
-template <int BITS> __device__ __forceinline__ void kv_quantise(const h8 x, unsigned (&codes)[BITS / 4], unsigned &scale_low) {
-    float lo = (float)x[0], hi = lo, bad = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 8; i++) {
-        const float v = (float)x[i];
-        lo = fminf(lo, v);
-        hi = fmaxf(hi, v);
-        bad = __builtin_fmaf(v, 0.0f, bad);  // NaN from the first NaN or infinity on
-    }
-    lo = row16_min(lo);
-    hi = row16_max(hi);
-    bad += dpp_move<kRowRor4>(bad);
-    bad += dpp_move<kRowRor8>(bad);
-    const bool finite = bad == 0.0f;
-    lo = finite ? lo : 0.0f;
-    hi = finite ? hi : 0.0f;
-    const unsigned sb = group_scale_bits(lo, hi, BITS == 4 ? 15.0f : 255.0f);
-    const float s = f16_bits_value(sb), inv = s > 0.0f ? 1.0f / s : 0.0f;
-#pragma unroll
-    for (int w = 0; w < BITS / 4; w++) codes[w] = 0;
-#pragma unroll
-    for (int i = 0; i < 8; i++) {
-        const unsigned c = finite ? (unsigned)(int)nearest_step((float)x[i], lo, s, inv) : 0u;
-        codes[i * BITS / 32] |= c << (i * BITS % 32);
-    }
-    const unsigned short low_bits = finite ? __builtin_bit_cast(unsigned short, (_Float16)lo) : (unsigned short)0x7E00;
-    scale_low = sb | (unsigned)low_bits << 16;
+template <int BITS> __device__ __forceinline__ void kv_quantise(const h8 (&x)[2], unsigned (&codes)[BITS / 2], unsigned &scale_low) {
+    unsigned magnitude, more, tiny, tiny_more;
+    h2 e = extremes(x[0], magnitude, tiny);
+    const h2 f = extremes(x[1], more, tiny_more);
+    extremes_of(e, magnitude, f, more);
+    extremes_across<kDppRowRor8>(e, magnitude);
+    quantise<BITS, 2>(codes, scale_low, x, e, magnitude, least_of(tiny, tiny_more));
 }
 
 template <int BITS> __global__ __launch_bounds__(256) void kv_write_kernel(const KvArgs a) {
-    const unsigned unit = blockIdx.x * 16 + (threadIdx.x >> 4);
-    if (unit >= a.total) return;
+    const unsigned unit = blockIdx.x * 32 + (threadIdx.x >> 4) * 2 + (threadIdx.x >> 2 & 1);
     const KvUnit u = kv_unit(a, unit);
     const int col = u.head * a.hd + u.group * ET_KV_GROUP + u.sub * 8;
-    h8 k = {0, 0, 0, 0, 0, 0, 0, 0}, v = k;
-    if (u.mine) {
-        k = *reinterpret_cast<const h8 *>(a.K + (size_t)u.row * a.ldk + col);
-        v = *reinterpret_cast<const h8 *>(a.V + (size_t)u.row * a.ldv + col);
-    }
-    constexpr int W = BITS / 4;  // words of a lane's eight codes
-    unsigned c[W], sl;
+    if (u.count <= 0) return;  // (of the whole workgroup's sequence)
+    // (lanes whose token is none of the call's take the nearest row that is)
+    const _Float16 *from_k = a.K + u.row * a.ldk + col, *from_v = a.V + u.row * a.ldv + col;
+    const h8 k[2] = {*reinterpret_cast<const h8 *>(from_k), *reinterpret_cast<const h8 *>(from_k + 16)};
+    const h8 v[2] = {*reinterpret_cast<const h8 *>(from_v), *reinterpret_cast<const h8 *>(from_v + 16)};
+    constexpr int W = BITS / 4;  // words of eight codes
+    unsigned c[2 * W], sl;
     const int token_bytes = a.hd * BITS / 8, at = (u.group * ET_KV_GROUP + u.sub * 8) * BITS / 8;
     kv_quantise<BITS>(k, c, sl);
     if (u.mine) {
-        unsigned *to = reinterpret_cast<unsigned *>(a.k_codes + u.token * token_bytes + at);
+        char *to = a.k_codes + u.token * token_bytes + at;
 #pragma unroll
-        for (int w = 0; w < W; w++) to[w] = c[w];
+        for (int e = 0; e < 2; e++)
+#pragma unroll
+            for (int w = 0; w < W; w++) *reinterpret_cast<unsigned *>(to + e * 2 * BITS + w * 4) = c[e * W + w];
         if (u.sub == 0) a.k_scales[u.scale + u.tq] = sl;
     }
     kv_quantise<BITS>(v, c, sl);
     // the four tokens' units from at / 2 on, [unit][token]
     char *to = a.v_codes + u.quad * token_bytes + (size_t)at * 4;
-    if (u.all) {
+#pragma unroll
+    for (int e = 0; e < 2; e++)
 #pragma unroll
         for (int w = 0; w < W; w++) {
             // lane m of four stores unit m / 2 of tokens 2 (m % 2) and the next
-            const unsigned first = dpp_bits<0x88>(c[w]), second = dpp_bits<0xDD>(c[w]);  // quad_perm [0,2,0,2] and [1,3,1,3]
-            const unsigned word = u.tq & 2 ? (first >> 16) | (second & 0xffff0000u) : (first & 0xffffu) | second << 16;
-            *reinterpret_cast<unsigned *>(to + w * 16 + u.tq * 4) = word;
+            const unsigned word = c[e * W + w], first = dpp_bits<0x88>(word), second = dpp_bits<0xDD>(word);  // quad_perm [0,2,0,2] and [1,3,1,3]
+            char *here = to + e * 8 * BITS + w * 16;
+            if (u.all) {
+                *reinterpret_cast<unsigned *>(here + u.tq * 4) = u.tq & 2 ? (first >> 16) | (second & 0xffff0000u) : (first & 0xffffu) | second << 16;
+            } else if (u.mine) {
+                *reinterpret_cast<unsigned short *>(here + u.tq * 2) = (unsigned short)word;
+                *reinterpret_cast<unsigned short *>(here + 8 + u.tq * 2) = (unsigned short)(word >> 16);
+            }
         }
-    } else if (u.mine) {
-#pragma unroll
-        for (int w = 0; w < W; w++) {
-            *reinterpret_cast<unsigned short *>(to + w * 16 + u.tq * 2) = (unsigned short)c[w];
-            *reinterpret_cast<unsigned short *>(to + w * 16 + 8 + u.tq * 2) = (unsigned short)(c[w] >> 16);
-        }
-    }
     if (u.mine && u.sub == 0) a.v_scales[u.scale + u.tq] = sl;
 }
 
-template <int BITS> __device__ __forceinline__ h8 kv_values(const unsigned (&c)[BITS / 4], unsigned scale_low) {
+template <int BITS> __device__ __forceinline__ h8 kv_values(const unsigned *c, unsigned scale_low) {
     const float s = f16_bits_value(scale_low & 0xffffu), lo = f16_bits_value(scale_low >> 16);
     h8 x;
 #pragma unroll
@@ -155,31 +136,46 @@ template <int BITS> __device__ __forceinline__ h8 kv_values(const unsigned (&c)[
 }
 
 template <int BITS> __global__ __launch_bounds__(256) void kv_read_kernel(const KvArgs a) {
-    const unsigned unit = blockIdx.x * 16 + (threadIdx.x >> 4);
-    if (unit >= a.total) return;
+    const unsigned unit = blockIdx.x * 32 + (threadIdx.x >> 4) * 2 + (threadIdx.x >> 2 & 1);
     const KvUnit u = kv_unit(a, unit);
     const int col = u.head * a.hd + u.group * ET_KV_GROUP + u.sub * 8;
     constexpr int W = BITS / 4;
-    unsigned c[W] = {}, d[W] = {};
+    unsigned c[2 * W] = {}, d[2 * W] = {};
+    unsigned k_sl = 0, v_sl = 0;
     const int token_bytes = a.hd * BITS / 8, at = (u.group * ET_KV_GROUP + u.sub * 8) * BITS / 8;
     if (a.Kout && u.mine) {
-        const unsigned *from = reinterpret_cast<const unsigned *>(a.k_codes + u.token * token_bytes + at);
+        const char *from = a.k_codes + u.token * token_bytes + at;
 #pragma unroll
-        for (int w = 0; w < W; w++) c[w] = from[w];
-        *reinterpret_cast<h8 *>(a.Kout + (size_t)u.row * a.ldk + col) = kv_values<BITS>(c, a.k_scales[u.scale + u.tq]);
+        for (int e = 0; e < 2; e++)
+#pragma unroll
+            for (int w = 0; w < W; w++) c[e * W + w] = *reinterpret_cast<const unsigned *>(from + e * 2 * BITS + w * 4);
+        k_sl = a.k_scales[u.scale + u.tq];
+    }
+    if (a.Vout) {
+        // (the page of a token of this call holds all four: lanes whose token is not the call's read too, for their neighbours, or read page 0 and store nothing)
+        const char *from = a.v_codes + u.quad * token_bytes + (size_t)at * 4;
+#pragma unroll
+        for (int e = 0; e < 2; e++)
+#pragma unroll
+            for (int w = 0; w < W; w++) d[e * W + w] = *reinterpret_cast<const unsigned *>(from + e * 8 * BITS + w * 16 + u.tq * 4);
+        v_sl = a.v_scales[u.scale + u.tq];
+    }
+    if (a.Kout && u.mine) {
+        _Float16 *to = a.Kout + u.row * a.ldk + col;
+        *reinterpret_cast<h8 *>(to) = kv_values<BITS>(c, k_sl);
+        *reinterpret_cast<h8 *>(to + 16) = kv_values<BITS>(c + W, k_sl);
     }
     if (!a.Vout) return;
-    // (the page of a token of this call holds all four: lanes whose token is not the call's read too, for their neighbours, or read page 0 and store nothing)
-    const char *from = a.v_codes + u.quad * token_bytes + (size_t)at * 4;
 #pragma unroll
-    for (int w = 0; w < W; w++) d[w] = *reinterpret_cast<const unsigned *>(from + w * 16 + u.tq * 4);
-    const unsigned sl = a.v_scales[u.scale + u.tq];
-#pragma unroll
-    for (int w = 0; w < W; w++) {
+    for (int w = 0; w < 2 * W; w++) {
         const unsigned first = dpp_bits<0x50>(d[w]), second = dpp_bits<0xFA>(d[w]);  // quad_perm [0,0,1,1] and [2,2,3,3]
         c[w] = u.tq & 1 ? (first >> 16) | (second & 0xffff0000u) : (first & 0xffffu) | second << 16;
     }
-    if (u.mine) *reinterpret_cast<h8 *>(a.Vout + (size_t)u.row * a.ldv + col) = kv_values<BITS>(c, sl);
+    if (u.mine) {
+        _Float16 *to = a.Vout + u.row * a.ldv + col;
+        *reinterpret_cast<h8 *>(to) = kv_values<BITS>(c, v_sl);
+        *reinterpret_cast<h8 *>(to + 16) = kv_values<BITS>(c + W, v_sl);
+    }
 }
 
 int kv_check_cache(const char *fn, const et_kv_cache *c, const int32_t *table, int max_pages, int B, int n) {
@@ -225,11 +221,12 @@ int kv_args(const char *fn, KvArgs &a, const et_kv_cache *cache, const int32_t *
     a.npages = cache->npages;
     a.max_pages = max_pages;
     a.n = n;
+    a.nkvg = Divisor((unsigned)(width / ET_KV_GROUP));
+    a.groups = Divisor((unsigned)(cache->hd / ET_KV_GROUP));
+    a.page_quads = Divisor((unsigned)(cache->page / 4));
     // n positions from any start touch at most this many groups of four
-    a.quads = starts ? (int)((n + 2LL) / 4) + 1 : (int)((n + 3LL) / 4);
-    a.nkvg = (unsigned)(width / ET_KV_GROUP);
-    const long long total = (long long)B * a.quads * a.nkvg;
-    ET_REQUIRE(total <= 0x7fffffffLL, ET_ERR_UNSUPPORTED, "%s: %lld groups in one call", fn, total * 4);
+    const long long quads = starts ? (n + 2LL) / 4 + 1 : (n + 3LL) / 4, total = n == 0 ? 0 : quads * a.nkvg.d;
+    ET_REQUIRE(B <= 65535 && total <= 0x7fffffffLL && total * B <= 0x7fffffffLL * 16, ET_ERR_UNSUPPORTED, "%s: B=%d n=%d", fn, B, n);
     a.total = (unsigned)total;
     return ET_OK;
 }
@@ -247,20 +244,20 @@ int et_kv_write_f16(const et_kv_cache *cache, const int32_t *table, int max_page
     ET_REQUIRE(K && V, ET_ERR_INVALID_ARG, "et_kv_write_f16: NULL pointer");
     KvArgs a;
     const int st = kv_args("et_kv_write_f16", a, cache, table, max_pages, starts, counts, K, V, ldk, ldv, B, n);
-    if (st != ET_OK || a.total == 0 || n == 0) return st;
+    if (st != ET_OK || a.total == 0 || B == 0) return st;
     a.K = reinterpret_cast<const _Float16 *>(K);
     a.V = reinterpret_cast<const _Float16 *>(V);
-    return launch_kernel("kv_write_kernel", cache->bits == 4 ? kv_write_kernel<4> : kv_write_kernel<8>, dim3((a.total + 15) / 16), 256, 0, as_stream(stream), a);
+    return launch_kernel("kv_write_kernel", cache->bits == 4 ? kv_write_kernel<4> : kv_write_kernel<8>, dim3((a.total + 31) / 32, (unsigned)B), 256, 0, as_stream(stream), a);
 }
 
 int et_kv_read_f16(const et_kv_cache *cache, const int32_t *table, int max_pages, const int32_t *starts, const int32_t *counts, et_f16 *K, et_f16 *V,
                    int ldk, int ldv, int B, int n, et_stream stream) {
     KvArgs a;
     const int st = kv_args("et_kv_read_f16", a, cache, table, max_pages, starts, counts, K, V, ldk, ldv, B, n);
-    if (st != ET_OK || a.total == 0 || n == 0 || (!K && !V)) return st;
+    if (st != ET_OK || a.total == 0 || B == 0 || (!K && !V)) return st;
     a.Kout = reinterpret_cast<_Float16 *>(K);
     a.Vout = reinterpret_cast<_Float16 *>(V);
-    return launch_kernel("kv_read_kernel", cache->bits == 4 ? kv_read_kernel<4> : kv_read_kernel<8>, dim3((a.total + 15) / 16), 256, 0, as_stream(stream), a);
+    return launch_kernel("kv_read_kernel", cache->bits == 4 ? kv_read_kernel<4> : kv_read_kernel<8>, dim3((a.total + 31) / 32, (unsigned)B), 256, 0, as_stream(stream), a);
 }
 
 }  // extern "C"

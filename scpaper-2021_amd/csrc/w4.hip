@@ -5,41 +5,22 @@
 
 namespace et {
 
-// Sixteen lanes a group of an output feature: group / 16 values each, as words of codes where there are eight of them.
 template <int GROUP> __global__ __launch_bounds__(256) void dense_to_w4_kernel(const _Float16 *W, unsigned *codes, unsigned *scales, int in, int out, unsigned total) {
     // a lane holds eight values; GROUP / 8 neighbouring lanes (4, 8 or 16) a group
     const unsigned i = blockIdx.x * 256u + threadIdx.x;
     if (i >= total) return;  // (total is a multiple of GROUP / 8, and so are a wave's first and last)
     const h8 x = reinterpret_cast<const h8 *>(W)[i];
-    float lo = (float)x[0], hi = lo, bad = 0.0f;
-#pragma unroll
-    for (int k = 0; k < 8; k++) {
-        const float v = (float)x[k];
-        lo = fminf(lo, v);
-        hi = fmaxf(hi, v);
-        bad = __builtin_fmaf(v, 0.0f, bad);
-    }
-    auto across = [&](auto move) {
-        lo = fminf(lo, move(lo));
-        hi = fmaxf(hi, move(hi));
-        bad += move(bad);
-    };
-    across(dpp_move<kDppQuadXor1>);
-    across(dpp_move<kDppQuadXor2>);
-    if constexpr (GROUP >= 64) across(dpp_move<0x141>);   // row_half_mirror: the other four of eight
-    if constexpr (GROUP >= 128) across(dpp_move<0x128>);  // row_ror:8
-    const bool finite = bad == 0.0f;
-    lo = finite ? lo : 0.0f;
-    hi = finite ? hi : 0.0f;
-    const unsigned sb = group_scale_bits(lo, hi, 15.0f);
-    const float s = f16_bits_value(sb), inv = s > 0.0f ? 1.0f / s : 0.0f;
-    unsigned word = 0;
-#pragma unroll
-    for (int k = 0; k < 8; k++) word |= (finite ? (unsigned)(int)nearest_step((float)x[k], lo, s, inv) : 0u) << (4 * k);
-    codes[i] = word;
+    unsigned magnitude, tiny, word[1], scale_low;
+    h2 e = extremes(x, magnitude, tiny);
+    extremes_across<kDppQuadXor1>(e, magnitude);
+    extremes_across<kDppQuadXor2>(e, magnitude);
+    if constexpr (GROUP >= 64) extremes_across<0x141>(e, magnitude);          // row_half_mirror: the other four of eight
+    if constexpr (GROUP >= 128) extremes_across<kDppRowRor8>(e, magnitude);
+    const h8 all[1] = {x};
+    quantise<4, 1>(word, scale_low, all, e, magnitude, tiny);
+    codes[i] = word[0];
     const unsigned per_row = (unsigned)in / 8, o = i / per_row, at = i - o * per_row;
-    const unsigned low_bits = finite ? __builtin_bit_cast(unsigned short, (_Float16)lo) : (unsigned short)0x7E00;
-    if (at % (GROUP / 8) == 0) scales[(size_t)(at / (GROUP / 8)) * out + o] = sb | low_bits << 16;
+    if (at % (GROUP / 8) == 0) scales[(size_t)(at / (GROUP / 8)) * out + o] = scale_low;
 }
 
 __global__ __launch_bounds__(256) void w4_to_dense_kernel(const unsigned *codes, const unsigned *scales, _Float16 *W, int in, int out, int group, unsigned total) {
