@@ -30,26 +30,6 @@ struct KvMhaArgs {
 #define KV_LEADING const int32_t *table_at, const int32_t *starts_at, const int32_t *counts_at, int max_pages, int units, int splits, int per, unsigned magic, unsigned shift, \
                    int page_pieces, int n
 
-// The places of the pieces of 16 keys of a tile, and their pages as the table has them (-1: behind it).
-template <int N> struct KvPages {
-    int page[N], off[N];
-    __device__ __forceinline__ void ask(const __attribute__((address_space(4))) int32_t *table, int tile, int max_pages, unsigned magic, unsigned shift, int page_pieces) {
-#pragma unroll
-        for (int s = 0; s < N; s++) {
-            const int piece = N * tile + s;
-            const int pidx = (int)(((unsigned long long)(unsigned)piece * magic) >> shift);
-            off[s] = (piece - pidx * page_pieces) << 4;
-            page[s] = pidx < max_pages ? table[pidx] : -1;
-        }
-    }
-    // pieces that nobody sees or that have no page: -1
-    __device__ __forceinline__ void resolve(int tile, int lim_most, int npages) {
-#pragma unroll
-        for (int s = 0; s < N; s++) page[s] = (N * tile + s) * 16 < lim_most && page[s] >= 0 && page[s] < npages ? page[s] : -1;
-    }
-};
-
-typedef unsigned u1 __attribute__((ext_vector_type(1), aligned(4)));
 typedef unsigned u2 __attribute__((ext_vector_type(2), aligned(4)));
 typedef unsigned u3 __attribute__((ext_vector_type(3), aligned(4)));
 typedef unsigned u4 __attribute__((ext_vector_type(4), aligned(4)));
@@ -141,7 +121,7 @@ template <int BITS> __device__ __forceinline__ h8 query_order(h8 x, float grow, 
         return h8{(_Float16)f[0], (_Float16)f[2], (_Float16)f[1], (_Float16)f[3], (_Float16)f[4], (_Float16)f[6], (_Float16)f[5], (_Float16)f[7]};
 }
 
-// acc += (w + rest) * codes over 32 keys: 4 j .. 4 j + 3 of two pieces.
+// acc += (w + rest) * codes over 32 keys, 4 j .. 4 j + 3 of two pieces.
 template <int BITS, int HD> __device__ __forceinline__ void weigh_values(f4 *acc, h8 w, h8 rest, const unsigned *first, const unsigned *second, int c) {
     using S = KvShape<BITS, HD>;
     auto weigh = [&](int i, h8 codes) {
@@ -187,20 +167,15 @@ template <int BITS, int HD> __device__ __forceinline__ void load_value(unsigned 
     if constexpr (S::kHalfUnit) to[2 * S::kUnits] = half[0], to[2 * S::kUnits + 1] = half[1];
 }
 
-template <int BITS, int HD> struct KvTile {
-    using S = KvShape<BITS, HD>;
-    unsigned k[2][S::kKeyWords], v[2][S::kValueWords];
-    u4 ks[2], vs[2];
-};
+// More rows a key/value head: blocks of 16 / kCols query rows, whose (row, group) pairs fill the 16 columns of the products of a tile of 32 keys.
+//
+// Scores: keys are the rows of the products, so a lane ends with keys 4 j .. 4 j + 3 of both pieces for its column, and these are the very keys that it weighs as a row of the
+// products with the values: nothing moves between lanes but the sum of a row's groups, and a maximum when the reference moves.
+template <int BITS, int HD> constexpr int kv_rows_waves() { return HD == 32 ? 6 : HD == 64 ? (BITS == 4 ? 6 : 5) : HD <= 128 ? 4 : 2; }
 
-// Waves that a SIMD is to hold: more of them hide the loads' way better than a tile fetched ahead did.
-template <int BITS, int HD, int NW> constexpr int kv_waves() {
-    return NW == 16 ? 4 : HD == 32 ? 6 : HD == 64 ? (BITS == 4 ? 6 : 5) : HD <= 128 ? 4 : 2;
-}
-
-template <int BITS, int HD, int NW> __global__ __launch_bounds__(NW * 64, (kv_waves<BITS, HD, NW>())) void mha_kv_kernel(KV_LEADING, const KvMhaArgs a) {
+template <int BITS, int HD, int NW> __global__ __launch_bounds__(NW * 64, (kv_rows_waves<BITS, HD>())) void mha_kv_kernel(KV_LEADING, const KvMhaArgs a) {
     using S = KvShape<BITS, HD>;
-    constexpr int COLS = S::kCols, ROWS = S::kRows, G = S::kGroups, PIECES = 2;
+    constexpr int COLS = S::kCols, ROWS = S::kRows, G = S::kGroups, TB = S::kTokenBytes;
     __shared__ float lds_vals[NW][ROWS * HD];
     __shared__ float lds_stats[NW][3][16];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -209,12 +184,24 @@ template <int BITS, int HD, int NW> __global__ __launch_bounds__(NW * 64, (kv_wa
     const int kv = blockIdx.x, b = blockIdx.y, nkv = gridDim.x;
     const int block = splits == 1 ? blockIdx.z : blockIdx.z / splits, split = blockIdx.z - block * splits;
 
-    // Tiles are dealt to the waves of all workgroups in turn, whatever the sequence's length: the first one's pages are asked for together with it.
+    // as in mha_kv_few_kernel
     const auto *table = ET_KV_CONST(int32_t, table_at) + (size_t)b * max_pages;
     const int t_step = splits * NW;
     int t = split * NW + wave;
-    KvPages<PIECES> pages;
-    pages.ask(table, t, max_pages, magic, shift, page_pieces);
+    const bool wide = (page_pieces & 1) == 0;
+    int page[2], off[2];
+    auto ask = [&](int tile) {
+        const int piece = 2 * tile;
+        int pidx = (int)(((unsigned long long)(unsigned)piece * magic) >> shift), at = piece - pidx * page_pieces;
+        off[0] = at << 4;
+        page[0] = pidx < max_pages ? table[pidx] : -1;
+        if (wide) return;
+        const bool on = ++at == page_pieces;
+        off[1] = (on ? 0 : at) << 4;
+        pidx += on;
+        page[1] = pidx < max_pages ? table[pidx] : -1;
+    };
+    ask(t);
 
     // the rows of this block, and what they see
     const int start = starts_at ? ET_KV_CONST(int32_t, starts_at)[b] : 0;
@@ -224,132 +211,143 @@ template <int BITS, int HD, int NW> __global__ __launch_bounds__(NW * 64, (kv_wa
     const long long most = (long long)max_pages * a.page;
     const int end = (int)min(max((long long)start + count, 0LL), most);
     auto row_of = [&](int row) { return n == 1 ? 0 : row / per; };  // of the call's rows
-    const int i_first = row_of(row0), i_last = row_of(row0 + rows - 1);
-    const int my_row = row0 + min(qh, rows - 1), my_i = row_of(my_row), my_r = my_row - my_i * per;
     auto limit = [&](int i) { return a.causal ? (int)min((long long)end, max((long long)start + i + 1, 0LL)) : end; };
-    const int lim = limit(my_i), lim_least = limit(i_first), lim_most = limit(i_last);
+    const int lim_least = limit(row_of(row0)), lim_most = limit(row_of(row0 + rows - 1));
     const int t_end = (lim_most + 31) >> 5;
 
     // Q in the order that the keys' codes come out of their words: 0 4 1 5 2 6 3 7 (4 bits, where 1 5 3 7 come out 16-fold) or 0 2 1 3 4 6 5 7; times a power of two
     // that brings a row's largest to 2^14 .. 2^15, so that the smaller ones keep their bits below 1 / 16; zero in the columns of the other groups
     h8 q[S::kPieces];
-    const _Float16 *qrow = a.Q + ((size_t)b * n + my_i) * a.ldq + (size_t)(kv * per + my_r) * HD + j * (HD / 4);
-    float top = 0.0f;
+    const int row = row0 + min(qh, rows - 1), i_row = row_of(row), r_row = row - i_row * per;
+    const int lim = limit(i_row);
+    const _Float16 *qrow = a.Q + ((size_t)b * n + i_row) * a.ldq + (size_t)(kv * per + r_row) * HD + j * (HD / 4);
+    float top = 0.0f, sum = 0.0f;
 #pragma unroll
     for (int i = 0; i < S::kPieces; i++) {
         q[i] = *reinterpret_cast<const h8 *>(qrow + 8 * i);
 #pragma unroll
-        for (int k = 0; k < 8; k++) top = fmaxf(top, fabsf((float)q[i][k]));
+        for (int e = 0; e < 8; e++) top = fmaxf(top, fabsf((float)q[i][e]));
     }
     top = rows_max(top);
     const int up = top > 0.0f ? 15 - __builtin_amdgcn_frexp_expf(top) : 0;
     const float grow = __builtin_ldexpf(a.scale_log2e < 0.0f ? -1.0f : 1.0f, up);
     const float key_scale = __builtin_ldexpf(fabsf(a.scale_log2e), 24 - up);
-    float qsum = 0.0f;
 #pragma unroll
-    for (int i = 0; i < S::kPieces; i++) q[i] = query_order<BITS>(q[i], (j * (HD / 4) + 8 * i) / 32 == gg ? grow : 0.0f, qsum);
-    qsum = rows_sum(qsum) * 0x1p-24f;
+    for (int i = 0; i < S::kPieces; i++) q[i] = query_order<BITS>(q[i], (j * (HD / 4) + 8 * i) / 32 == gg ? grow : 0.0f, sum);
+    const float qsum = rows_sum(sum) * 0x1p-24f;
 
+    float ref = kNothing, l = 0.0f, z = 0.0f;
     f4 acc[S::kAcc];
 #pragma unroll
     for (int i = 0; i < S::kAcc; i++) acc[i] = f4{0.f, 0.f, 0.f, 0.f};
-    float ref = kNothing, l = 0.0f, z = 0.0f;
 
-    auto load = [&](KvTile<BITS, HD> &t, const int (&page)[2], const int (&off)[2]) {
+    const unsigned key_at = c * TB + j * (TB / 4), value_at = j * (4 * TB) + c * (8 * S::kUnits), half_at = j * (4 * TB) + 128 * S::kUnits + (c >> 1) * 8;
+    const char *k_codes = a.k_codes + (size_t)kv * a.page * TB, *v_codes = a.v_codes + (size_t)kv * a.page * TB;
+    const unsigned *k_scales = a.k_scales + (size_t)kv * (G * a.page), *v_scales = a.v_scales + (size_t)kv * (G * a.page);
+    const unsigned page_bytes = (unsigned)nkv * a.page * TB, page_scales = (unsigned)nkv * G * a.page, scales_at = (unsigned)(min(gg, G - 1) * a.page + 4 * j);
+
+    for (; t < t_end; t += t_step) {
+        // where the pieces lie; one that nobody sees, or without a page, is read from the place of the one before it
+        size_t at[2], scale_at[2];
+        bool ok[2];
+        ok[0] = page[0] >= 0 && page[0] < a.npages;
+        const unsigned from = ok[0] ? page[0] : 0, from_off = ok[0] ? off[0] : 0;
+        at[0] = (size_t)from * page_bytes + from_off * TB;
+        scale_at[0] = (size_t)from * page_scales + from_off + scales_at;
+        if (wide) {
+            ok[1] = ok[0];
+            const bool second = t * 32 + 16 < lim_most;
+            at[1] = at[0] + (second ? 16 * TB : 0);
+            scale_at[1] = scale_at[0] + (second ? 16 : 0);
+        } else {
+            ok[1] = t * 32 + 16 < lim_most && page[1] >= 0 && page[1] < a.npages;
+            const unsigned from1 = ok[1] ? page[1] : from, off1 = ok[1] ? off[1] : from_off;
+            at[1] = (size_t)from1 * page_bytes + off1 * TB;
+            scale_at[1] = (size_t)from1 * page_scales + off1 + scales_at;
+        }
+        unsigned kw[2][S::kKeyWords], vw[2][S::kValueWords];
+        u4 ks[2], vs[2];
 #pragma unroll
         for (int s = 0; s < 2; s++) {
-            const size_t ph = (size_t)max(page[s], 0) * nkv + kv;
-            const size_t token = ph * a.page + off[s];
-            load_words<S::kKeyWords>(t.k[s], a.k_codes + token * S::kTokenBytes + c * S::kTokenBytes + j * (S::kTokenBytes / 4));
-            const char *v = a.v_codes + token * S::kTokenBytes + j * (4 * S::kTokenBytes);
-            load_value<BITS, HD>(t.v[s], v + c * (8 * S::kUnits), v + 128 * S::kUnits + (c >> 1) * 8);
-            const size_t at = (ph * G + min(gg, G - 1)) * a.page + off[s] + 4 * j;
-            t.ks[s] = *reinterpret_cast<const u4 *>(a.k_scales + at);
-            t.vs[s] = *reinterpret_cast<const u4 *>(a.v_scales + at);
+            load_words<S::kKeyWords>(kw[s], k_codes + at[s] + key_at);
+            ks[s] = *reinterpret_cast<const u4 *>(k_scales + scale_at[s]);
         }
-    };
-    auto use = [&](const KvTile<BITS, HD> &t, int tile, const int (&page)[2]) {
+#pragma unroll
+        for (int s = 0; s < 2; s++) {
+            vs[s] = *reinterpret_cast<const u4 *>(v_scales + scale_at[s]);
+            load_value<BITS, HD>(vw[s], v_codes + at[s] + value_at, v_codes + at[s] + half_at);
+        }
+        const int tile = t * 32;
+        const bool whole = tile + 32 <= lim_least && ok[0] && ok[1];
+        const bool ok0 = ok[0], ok1 = ok[1];
+        ask(t + t_step);
+
         float y[8];
 #pragma unroll
         for (int s = 0; s < 2; s++) {
             f4 d = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int i = 0; i < S::kPieces; i++) {
-                const h8 codes = key_codes<BITS>(&t.k[s][i * BITS / 4]);
+                const h8 codes = key_codes<BITS>(&kw[s][i * BITS / 4]);
                 d = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes, q[i], d, 0, 0, 0);
             }
 #pragma unroll
-            for (int r = 0; r < 4; r++) y[4 * s + r] = cols_sum<COLS>(__builtin_fmaf(low_half(t.ks[s][r]), d[r], high_half(t.ks[s][r]) * qsum)) * key_scale;
+            for (int r = 0; r < 4; r++)
+                y[4 * s + r] = cols_sum<COLS>(__builtin_fmaf(low_half(ks[s][r]), d[r], high_half(ks[s][r]) * qsum)) * key_scale;
         }
-        u4 vs[2] = {t.vs[0], t.vs[1]};
-        const bool whole = tile * 32 + 32 <= lim_least && page[0] >= 0 && page[1] >= 0;
-        bool seen[8];
         if (!whole) {
+            // (what no row sees must not come into the sums, whatever it is; what some rows see is weighed with zero by the others)
 #pragma unroll
             for (int e = 0; e < 8; e++) {
-                const int s = e >> 2, r = e & 3;
-                seen[e] = tile * 32 + 16 * s + 4 * j + r < lim && page[s] >= 0;
-                y[e] = seen[e] ? y[e] : kNothing;
-                vs[s][r] = seen[e] ? vs[s][r] : 0u;
+                const int s = e >> 2, pos = tile + 16 * s + 4 * j + (e & 3);
+                const bool there = s == 0 ? ok0 : ok1;
+                vs[s][e & 3] = there && pos < lim_most ? vs[s][e & 3] : 0u;
+                y[e] = there && pos < lim ? y[e] : kNothing;
             }
         }
-        float most_y = y[0], most_s = low_half(vs[0][0]);
+        float most_s = low_half(vs[0][0]);
 #pragma unroll
-        for (int e = 1; e < 8; e++) {
-            most_y = fmaxf(most_y, y[e]);
-            most_s = fmaxf(most_s, low_half(vs[e >> 2][e & 3]));
-        }
+        for (int e = 1; e < 8; e++) most_s = fmaxf(most_s, low_half(vs[e >> 2][e & 3]));
+        const float most_e = (float)__builtin_amdgcn_frexp_expf(most_s);
+        h8 w, rest;
+        float most_y = y[0];
+#pragma unroll
+        for (int e = 1; e < 8; e++) most_y = fmaxf(most_y, y[e]);
         // a weight is at most 2^15: p * scale < 2^(y - ref + exponent of the scale)
-        const float reach = most_y + (float)__builtin_amdgcn_frexp_expf(most_s);
+        const float reach = most_y + most_e;
         if (__any(reach > ref + 15.0f)) {
             const float next = fmaxf(ref, rows_max(reach) - 11.0f);
             const float f = __builtin_amdgcn_exp2f(ref - next);
             ref = next;
             l *= f;
             z *= f;
-            float fr[4];
-#pragma unroll
-            for (int r = 0; r < 4; r++) fr[r] = __shfl(f, 4 * j + r);
 #pragma unroll
             for (int r = 0; r < 4; r++) {
+                const float fr = __shfl(f, 4 * j + r);
 #pragma unroll
-                for (int i = 0; i < S::kAcc; i++) acc[i][r] *= fr[r];
+                for (int i = 0; i < S::kAcc; i++) acc[i][r] *= fr;
             }
         }
-        float p[8];
         // p * scale as two binary16 numbers: rounded to one, whose error is relative to a value's height above the group's lowest, results were 2 to 3 times as
         // far off as their own rounding (5.9e-4 against 2.1e-4, 2-norm, 131071 keys of random values); the products are no bound here
-        h8 w, rest;
 #pragma unroll
         for (int e = 0; e < 8; e++) {
-            p[e] = __builtin_amdgcn_exp2f(y[e] - ref);
-            if (!whole) p[e] = seen[e] ? p[e] : 0.0f;
-            l += p[e];
-            const float ps = p[e] * low_half(vs[e >> 2][e & 3]);
-            z = __builtin_fmaf(p[e], high_half(vs[e >> 2][e & 3]), z);
+            const float p = y[e] == kNothing ? 0.0f : __builtin_amdgcn_exp2f(y[e] - ref);
+            l += p;
+            const float ps = p * low_half(vs[e >> 2][e & 3]);
+            z = __builtin_fmaf(p, high_half(vs[e >> 2][e & 3]), z);
             w[e] = (_Float16)ps;
             rest[e] = (_Float16)(ps - (float)w[e]);
         }
-        weigh_values<BITS, HD>(acc, w, rest, t.v[0], t.v[1], c);
-    };
-
-    for (; t < t_end; t += t_step) {
-        KvTile<BITS, HD> tile;
-        pages.resolve(t, lim_most, a.npages);
-        load(tile, pages.page, pages.off);
-        KvPages<PIECES> next;
-        next.ask(table, t + t_step, max_pages, magic, shift, page_pieces);
-        use(tile, t, pages.page);
-        pages = next;
+        weigh_values<BITS, HD>(acc, w, rest, vw[0], vw[1], c);
     }
 
     // what the waves have, side by side
-    l = rows_sum(l);
-    z = rows_sum(z);
+    const float ls = rows_sum(l), zs = rows_sum(z);
     if (j == 0) {
         lds_stats[wave][0][c] = ref;
-        lds_stats[wave][1][c] = l;
-        lds_stats[wave][2][c] = z;
+        lds_stats[wave][1][c] = ls;
+        lds_stats[wave][2][c] = zs;
     }
 #pragma unroll
     for (int i = 0; i < S::kAcc; i++) {
@@ -696,18 +694,18 @@ namespace {
 using KvKernel = void (*)(KV_LEADING, const KvMhaArgs);
 
 struct KvForm {
-    KvKernel few, many;  // of 4 waves; of many
-    int rows, cols, many_waves, tile;
+    KvKernel four, eight;  // waves
+    int rows, cols, tile;
 };
 
 // Rows: of a key/value head in the call.
 template <int BITS, int HD> KvForm form_of(long long rows) {
     if constexpr (HD <= 128) {
         constexpr int cols = KvShape<BITS, HD>::kCols, heads = 4 / cols;
-        if (rows == 1) return {mha_kv_few_kernel<BITS, HD, 1, 4>, mha_kv_few_kernel<BITS, HD, 1, 8>, 1, cols, 8, 64};
-        if (rows <= heads) return {mha_kv_few_kernel<BITS, HD, heads, 4>, mha_kv_few_kernel<BITS, HD, heads, 8>, heads, cols, 8, 64};
+        if (rows == 1) return {mha_kv_few_kernel<BITS, HD, 1, 4>, mha_kv_few_kernel<BITS, HD, 1, 8>, 1, cols, 64};
+        if (rows <= heads) return {mha_kv_few_kernel<BITS, HD, heads, 4>, mha_kv_few_kernel<BITS, HD, heads, 8>, heads, cols, 64};
     }
-    return {mha_kv_kernel<BITS, HD, 4>, mha_kv_kernel<BITS, HD, (HD <= 128 ? 16 : 8)>, KvShape<BITS, HD>::kRows, KvShape<BITS, HD>::kCols, HD <= 128 ? 16 : 8, 32};
+    return {mha_kv_kernel<BITS, HD, 4>, mha_kv_kernel<BITS, HD, 8>, KvShape<BITS, HD>::kRows, KvShape<BITS, HD>::kCols, 32};
 }
 
 template <int BITS> KvForm form_of(int hd, long long rows) {
@@ -740,7 +738,7 @@ int kv_plan(const char *fn, KvPlan &p, const et_kv_cache *c, int max_pages, int 
     ET_REQUIRE(rows <= 0x7fffffffLL && B <= 65535 && blocks <= 65535 && units * blocks <= (1LL << 24), ET_ERR_UNSUPPORTED, "%s: B=%d n=%d nh=%d", fn, B, n, nh);
     p.blocks = (int)blocks;
     const long long tiles = ((long long)max_pages * c->page + p.form.tile - 1) / p.form.tile, groups = units * blocks;
-    p.waves = groups >= 512 ? 4 : p.form.many_waves;
+    p.waves = groups >= 512 ? 4 : 8;
     p.splits = groups == 0 ? 1 : (int)std::max(1LL, std::min({(4096 / p.waves + groups - 1) / groups, tiles / (4 * p.waves), 256LL}));
     p.splits = std::min(p.splits, (int)(65535 / std::max(1LL, blocks)));
     p.bytes = p.splits > 1 ? (size_t)(groups * p.splits) * (32 + p.form.rows * c->hd) * sizeof(float) : 0;
@@ -812,7 +810,7 @@ int et_mha_kv_f16(const et_kv_cache *cache, const int32_t *table, int max_pages,
     while ((1ull << (shift - 28)) < d) shift++;
     const unsigned magic = (unsigned)(((1ull << shift) + d - 1) / d);
     a.scale_log2e = scale * 1.4426950408889634f;
-    const int sl = launch_kernel("mha_kv_kernel", p.waves == 4 ? p.form.few : p.form.many, dim3((unsigned)cache->nkv, (unsigned)B, (unsigned)(p.blocks * p.splits)), p.waves * 64, 0, as_stream(stream),
+    const int sl = launch_kernel("mha_kv_kernel", p.waves == 4 ? p.form.four : p.form.eight, dim3((unsigned)cache->nkv, (unsigned)B, (unsigned)(p.blocks * p.splits)), p.waves * 64, 0, as_stream(stream),
                                  table, starts, counts, max_pages, a.units, a.splits, a.per, magic, shift, (int)d, n, a);
     if (sl != ET_OK || p.splits == 1) return sl;
     return launch_kernel("mha_kv_join_kernel", mha_kv_join_kernel, dim3((unsigned)(a.units * p.form.rows * (cache->hd / ET_KV_GROUP)), (unsigned)p.blocks), 256, 0, as_stream(stream), a);
