@@ -617,6 +617,44 @@ template <> class Linear<mat1x16> {
     }
 };
 
+// Dense weight in 4 bits: any number of rows, made for the few of a decoding step.
+template <> class Linear<w4_mat> {
+  public:
+    const int in_size;
+    const int out_size;
+    const int size;
+    w4_mat weight;
+    et::DeviceBuffer<half> bias;
+
+    Linear(int _in_size, int _out_size, const w4_mat &w, const half *b, int _size)
+        : in_size(_in_size), out_size(_out_size), size(_size), weight(w), bias(b, (std::size_t)_out_size) {
+        check();
+    }
+    Linear(int _in_size, int _out_size, w4_mat &&w, const half *b, int _size)
+        : in_size(_in_size), out_size(_out_size), size(_size), weight(std::move(w)), bias(b, (std::size_t)_out_size) {
+        check();
+    }
+    void forward(half *output, const half *input, et::stream_t stream = nullptr) const {
+        forward_act(output, input, ET_ACT_NONE, stream);
+    }
+    void forward_act(half *output, const half *input, int act, et::stream_t stream = nullptr) const {
+        run(output, nullptr, input, act, stream);
+    }
+    // binary32 output: the sum after the bias, unrounded
+    void forward_f32(float *output, const half *input, et::stream_t stream = nullptr) const {
+        run(nullptr, output, input, ET_ACT_NONE, stream);
+    }
+
+  private:
+    void check() const {
+        et::require(weight.nrow == out_size && weight.ncol == in_size, "Linear<w4_mat>: weight shape does not match in/out sizes");
+    }
+    void run(half *y, float *y32, const half *x, int act, et::stream_t stream) const {
+        etChk(et_linear_w4_f16(weight.codes.get(), et::f16(weight.scales.get()), weight.group, et::f16(bias.get()), et::f16(x), y ? et::f16(y) : nullptr, y32, size,
+                               in_size, out_size, act, stream));
+    }
+};
+
 #include "gen_linear.hpp"
 
 namespace et {
