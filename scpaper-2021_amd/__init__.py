@@ -289,6 +289,11 @@ class DeviceBuffer:
         self.dtype = None
         self.shape = None
 
+    @property
+    def _as_parameter_(self):
+        """What ctypes passes for a buffer."""
+        return self.ptr
+
     @classmethod
     def from_numpy(cls, arr: np.ndarray) -> "DeviceBuffer":
         arr = np.ascontiguousarray(arr)
@@ -413,14 +418,15 @@ def layernorm(out, src, gamma, beta, rows, H, eps=1e-5, stream=None):
     check(lib().et_layernorm_f16(_ptr(out), _ptr(src), _ptr(gamma), _ptr(beta), rows, H, eps, stream))
 
 
-# Decoding from a cache of keys and values (KvCache) and 4-bit weights.
+# Decoding from a cache of keys and values (KvCache) and 4-bit weights.  Pointers are integers, DeviceBuffers or None, which ctypes takes by itself: these calls are
+# a few microseconds on the device, and what the host spends on one counts.
 
 def kv_write(cache, table, max_pages, starts, counts, K, V, ldk, ldv, B, n, stream=None):
-    check(lib().et_kv_write_f16(C.byref(cache), _ptr(table), max_pages, _ptr(starts), _ptr(counts), _ptr(K), _ptr(V), ldk, ldv, B, n, stream))
+    check(lib().et_kv_write_f16(C.byref(cache), table, max_pages, starts, counts, K, V, ldk, ldv, B, n, stream))
 
 
 def kv_read(cache, table, max_pages, starts, counts, K, V, ldk, ldv, B, n, stream=None):
-    check(lib().et_kv_read_f16(C.byref(cache), _ptr(table), max_pages, _ptr(starts), _ptr(counts), _ptr(K), _ptr(V), ldk, ldv, B, n, stream))
+    check(lib().et_kv_read_f16(C.byref(cache), table, max_pages, starts, counts, K, V, ldk, ldv, B, n, stream))
 
 
 def mha_kv_workspace(cache, max_pages, B, n, nh) -> int:
@@ -431,20 +437,20 @@ def mha_kv_workspace(cache, max_pages, B, n, nh) -> int:
 
 
 def mha_kv(cache, table, max_pages, starts, counts, Q, ldq, Z, ldz, B, n, nh, scale, flags=0, workspace=None, workspace_bytes=0, stream=None):
-    check(lib().et_mha_kv_f16(C.byref(cache), _ptr(table), max_pages, _ptr(starts), _ptr(counts), _ptr(Q), ldq, _ptr(Z), ldz, B, n, nh, scale, flags,
-                              _ptr(workspace), workspace_bytes, stream))
+    check(lib().et_mha_kv_f16(C.byref(cache), table, max_pages, starts, counts, Q, ldq, Z, ldz, B, n, nh, scale, flags,
+                              workspace, workspace_bytes, stream))
 
 
 def dense_to_w4(W, codes, scales, n_in, n_out, group, stream=None):
-    check(lib().et_dense_to_w4_f16(_ptr(W), _ptr(codes), _ptr(scales), n_in, n_out, group, stream))
+    check(lib().et_dense_to_w4_f16(W, codes, scales, n_in, n_out, group, stream))
 
 
 def w4_to_dense(codes, scales, W, n_in, n_out, group, stream=None):
-    check(lib().et_w4_to_dense_f16(_ptr(codes), _ptr(scales), _ptr(W), n_in, n_out, group, stream))
+    check(lib().et_w4_to_dense_f16(codes, scales, W, n_in, n_out, group, stream))
 
 
 def linear_w4(codes, scales, group, bias, X, Y, Y32, T, n_in, n_out, act=ACT_NONE, stream=None):
-    check(lib().et_linear_w4_f16(_ptr(codes), _ptr(scales), group, _ptr(bias), _ptr(X), _ptr(Y), _ptr(Y32), T, n_in, n_out, act, stream))
+    check(lib().et_linear_w4_f16(codes, scales, group, bias, X, Y, Y32, T, n_in, n_out, act, stream))
 
 
 # ---------------------------------------------------------------------------
