@@ -588,11 +588,13 @@ template <int BITS, int HD, int R, int NW> __global__ __launch_bounds__(NW * 64,
                 weights[(4 + h * GP + g) * F::kLdsRow + key_place] = (_Float16)(ps - (float)w);
             }
         }
+        wave_lds_order();
 #pragma unroll
         for (int u = 0; u < 2; u++) {
             const h8 w = *reinterpret_cast<const h8 *>(weights_at + u * 32), rest = *reinterpret_cast<const h8 *>(weights_at + 4 * F::kLdsRow + u * 32);
             weigh_values<BITS, HD>(acc, w, rest, vw[2 * u], vw[2 * u + 1], c);
         }
+        wave_lds_order();
     }
 
     // what the waves have, side by side

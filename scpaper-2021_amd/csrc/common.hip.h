@@ -64,6 +64,13 @@ constexpr int kDppQuadXor2 = 0x4E;  // quad_perm:[2,3,0,1]
 constexpr int kDppRowRor4 = 0x124;  // row_ror:4
 constexpr int kDppRowRor8 = 0x128;  // row_ror:8
 
+// Between LDS stores of a wave and loads by its other lanes of what they stored (and the other way round): a wave's LDS accesses are done in the order they
+// are issued in, so it is the compiler alone that must not move one over the other.
+__device__ __forceinline__ void wave_lds_order() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local");
+    __builtin_amdgcn_wave_barrier();
+}
+
 __device__ __forceinline__ float lane_value(float v, int lane) {
     return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), lane));
 }

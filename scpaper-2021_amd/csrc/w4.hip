@@ -66,7 +66,6 @@ __device__ __forceinline__ h8 w4_order(w4u x) {
     return w4_h8(__builtin_amdgcn_perm(x[2], x[0], lows), __builtin_amdgcn_perm(x[2], x[0], highs), __builtin_amdgcn_perm(x[3], x[1], lows),
                  __builtin_amdgcn_perm(x[3], x[1], highs));
 }
-// -> x0 x4 | x1 x5 | x2 x6 | x3 x7
 
 __device__ __forceinline__ float w4_scale(unsigned sl) { return (float)__builtin_bit_cast(h2, sl)[0]; }
 __device__ __forceinline__ float w4_low(unsigned sl) { return (float)__builtin_bit_cast(h2, sl)[1]; }
@@ -172,7 +171,9 @@ template <int GROUP, int SWAP, int TBK, int TR, int RBK, int U> __global__ __lau
 
     if (k_first * 128 < in_end) load(k_first);
     for (int k0 = k_first; k0 * 128 < in_end; k0 += U) {
+        wave_lds_order();
         keep();
+        wave_lds_order();
         if ((k0 + U) * 128 < in_end) load(k0 + U);
 #pragma unroll
         for (int u = 0; u < U; u++) {
@@ -265,6 +266,7 @@ template <int GROUP, int SWAP, int TBK, int TR, int RBK, int U> __global__ __lau
         if (a.Y) *reinterpret_cast<h4 *>(a.Y + (size_t)t * a.out + o) = out16;
         else *reinterpret_cast<f4 *>(a.Y32 + (size_t)t * a.out + o) = y;
     };
+    wave_lds_order();
     if (gg == 0) {
 #pragma unroll
         for (int i = 0; i < RBK; i++)
@@ -302,7 +304,7 @@ template <int GROUP, int SWAP, int TBK, int TR, int RBK, int U> W4Form w4_form_o
 template <int GROUP> W4Form w4_form(int T, int nb) {
     constexpr int few = GROUP / 8;  // rows of X whose columns fill a product
     if (T == 1) return nb <= 1024 ? w4_form_of<GROUP, 0, 1, 1, 1, 2>(4) : w4_form_of<GROUP, 0, 1, 1, 2, 2>(4);
-    if (T <= few) return nb <= 512 ? w4_form_of<GROUP, 0, 1, few, 1, 2>(4) : nb <= 1024 ? w4_form_of<GROUP, 0, 1, few, 2, 2>(4) : w4_form_of<GROUP, 0, 1, few, 4, 1>(4);
+    if (T <= few) return nb <= 512 ? w4_form_of<GROUP, 0, 1, few, 1, 2>(4) : nb <= 1024 ? w4_form_of<GROUP, 0, 1, few, 2, 2>(4) : w4_form_of<GROUP, 0, 1, few, 4, 2>(4);
     constexpr int swap = GROUP < 128;
     if constexpr (swap)
         if (T <= 16) return nb <= 512 ? w4_form_of<GROUP, 1, 1, 16, 1, 1>(8) : w4_form_of<GROUP, 1, 1, 16, 2, 1>(4);
