@@ -296,12 +296,12 @@ template <int BITS, int HD, int NW> __global__ __launch_bounds__(NW * 64, (kv_ro
                 y[4 * s + r] = cols_sum<COLS>(__builtin_fmaf(low_half(ks[s][r]), d[r], high_half(ks[s][r]) * qsum)) * key_scale;
         }
         if (!whole) {
-            // (what no row sees must not come into the sums, whatever it is; what some rows see is weighed with zero by the others)
+            // (what a row does not see must not come into its sums, whatever it is: the lowest value of another row's key may be NaN, and 0 * NaN is)
 #pragma unroll
             for (int e = 0; e < 8; e++) {
                 const int s = e >> 2, pos = tile + 16 * s + 4 * j + (e & 3);
                 const bool there = s == 0 ? ok0 : ok1;
-                vs[s][e & 3] = there && pos < lim_most ? vs[s][e & 3] : 0u;
+                vs[s][e & 3] = there && pos < lim ? vs[s][e & 3] : 0u;
                 y[e] = there && pos < lim ? y[e] : kNothing;
             }
         }
@@ -581,7 +581,7 @@ template <int BITS, int HD, int R, int NW> __global__ __launch_bounds__(NW * 64,
             l[h] += p;
 #pragma unroll
             for (int g = 0; g < G; g++) {
-                z[h][g] = __builtin_fmaf(p, high_half(vs[g]), z[h][g]);
+                z[h][g] = __builtin_fmaf(p, R == 1 || seen ? high_half(vs[g]) : 0.0f, z[h][g]);  // (what others see may be NaN, and 0 * NaN is)
                 const float ps = p * low_half(vs[g]);
                 const _Float16 w = (_Float16)ps;
                 weights[(h * GP + g) * F::kLdsRow + key_place] = w;

@@ -242,6 +242,26 @@ def test_attention_rows_that_see_nothing(et):
     assert (Z[1] == 0).all()
 
 
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("hd,per,n", [(64, 1, 2), (32, 1, 4), (32, 1, 3), (64, 3, 5), (128, 1, 2), (256, 2, 3)])
+@pytest.mark.parametrize("bad", [np.nan, np.inf])
+def test_attention_not_a_number_of_a_later_token(et, bits, hd, per, n, bad):
+    """The last token's key and value are NaN, which with causal attention only its own row sees: the other rows are what they are without it."""
+    nkv, lengths = 2, [40, n, 64 + n]
+    B, nh = len(lengths), nkv * per
+    table = tables(1, B, 5, 15)
+    host = filled(bits, nkv, hd, 16, table, lengths, 4, 15)
+    starts = [l - n for l in lengths]
+    Q = Hn.randn((B * n, nh * hd), 5)
+    want = run_attention(et, DeviceCache(et, host), table, starts, None, Q, B, n, nh, 0.125, True)
+    row = np.full((B, nkv * hd), bad, np.float16)
+    for K, V in ((row, row), (np.ones_like(row), row)):
+        host.write(table, [l - 1 for l in lengths], [1] * B, K, V, 1)
+        got = run_attention(et, DeviceCache(et, host), table, starts, None, Q, B, n, nh, 0.125, True).reshape(B, n, -1)
+        assert np.array_equal(got[:, :-1], want.reshape(B, n, -1)[:, :-1])
+        assert np.isnan(got[:, -1]).all()
+
+
 def test_attention_strides(et):
     check_attention(et, 4, 2, 2, 96, 16, [40, 25], 3, True, seed=8, ldq=3 * 384 + 8, ldz=384 + 8)
 
