@@ -62,7 +62,8 @@ class KvCache {
     DeviceBuffer<half> k_scales, v_scales;
 };
 
-// Device memory that the attention of steps up to these sizes needs (0: none).
+// Device memory that the attention of steps of these sizes, or with fewer pages, needs (0: none).
+// Other batches or rows may need more, smaller ones too.
 inline std::size_t cached_attention_workspace(const KvCache &cache, int max_pages, int batch, int n, int nhead) {
     const et_kv_cache c = cache.view();
     std::size_t bytes = 0;

@@ -573,7 +573,8 @@ int et_linear_csr_f16(const int32_t *indptr, const int32_t *indices,
  *   scales [in / group][out][2]: scale, low;   W = low + scale * code
  * Both 16-byte aligned.  et_dense_to_w4_f16 makes them of W [out x in] (16-byte aligned),
  * et_w4_to_dense_f16 writes what they stand for, rounded to binary16 (at most its largest number).
- * et_linear_w4_f16: T any number of rows; X, Y, Y32 16-byte aligned, bias 8-byte; exactly one of Y and Y32 (the
+ * et_linear_w4_f16: T from 0 to 2097120 rows, in up to 2^23; an infinity or a NaN in X stays in its row of
+ * the result, where it becomes infinities or NaN.  X, Y, Y32 16-byte aligned, bias 8-byte; exactly one of Y and Y32 (the
  * binary32 sum after bias and activation, unrounded) is non-NULL.  The codes
  * enter the matrix products as they are, scale and low are applied to the binary32
  * sums of their group.  No reference counterpart. */
@@ -718,7 +719,8 @@ int et_kv_read_f16(const et_kv_cache *cache, const int32_t *table, int max_pages
  * behind a sequence's end may be anything, NaN included.  n = 1 is a decoding
  * step, n > 1 several tokens at once (a piece of a prompt, guessed tokens).
  * The codes enter the matrix products as they are; scores, softmax and sums are
- * binary32, a probability times its value's scale is rounded once, to binary16.
+ * binary32, a probability times its value's scale is two binary16 numbers, the
+ * rounded one and what it leaves.  |scale| is at most 1e15.
  * workspace: et_mha_kv_workspace bytes of device memory, 16-byte aligned (may be NULL where that
  * says 0); launches that can overlap in time need one each.  The sums are
  * taken in an order that only the sizes given to the call decide. */

@@ -772,6 +772,8 @@ int et_mha_kv_f16(const et_kv_cache *cache, const int32_t *table, int max_pages,
     const int st = kv_check_cache("et_mha_kv_f16", cache, table, max_pages, B, n);
     if (st != ET_OK) return st;
     ET_REQUIRE((flags & ~ET_MHA_CAUSAL) == 0, ET_ERR_INVALID_ARG, "et_mha_kv_f16: flags=%d", flags);
+    // (scores stay below 1e30 in magnitude, which stands for minus infinity; 256 products of binary16 numbers reach 1.1e12)
+    ET_REQUIRE(fabsf(scale) <= 1e15f, ET_ERR_INVALID_ARG, "et_mha_kv_f16: scale=%g", (double)scale);
     KvPlan p;
     const int sp = kv_plan("et_mha_kv_f16", p, cache, max_pages, B, n, nh);
     if (sp != ET_OK) return sp;

@@ -188,7 +188,8 @@ int kv_check_cache(const char *fn, const et_kv_cache *c, const int32_t *table, i
     ET_REQUIRE(((reinterpret_cast<uintptr_t>(c->k_codes) | reinterpret_cast<uintptr_t>(c->k_scales) | reinterpret_cast<uintptr_t>(c->v_codes) |
                  reinterpret_cast<uintptr_t>(c->v_scales)) & 15) == 0, ET_ERR_UNSUPPORTED, "%s: the cache's buffers must be 16-byte aligned", fn);
     ET_REQUIRE((reinterpret_cast<uintptr_t>(table) & 3) == 0, ET_ERR_UNSUPPORTED, "%s: table must be 4-byte aligned", fn);
-    ET_REQUIRE((long long)max_pages * c->page <= 0x7fffffffLL, ET_ERR_UNSUPPORTED, "%s: max_pages * page = %lld positions", fn, (long long)max_pages * c->page);
+    // (a tile of keys may reach 64 positions beyond: positions stay 32-bit numbers)
+    ET_REQUIRE((long long)max_pages * c->page <= 0x7fffff80LL, ET_ERR_UNSUPPORTED, "%s: max_pages * page = %lld positions", fn, (long long)max_pages * c->page);
     ET_REQUIRE((long long)c->nkv * c->hd <= (1 << 24) && (long long)c->nkv * c->hd * c->page / 8 * c->bits < (1LL << 31), ET_ERR_UNSUPPORTED,
                "%s: nkv * hd = %lld, %d tokens a page", fn, (long long)c->nkv * c->hd, c->page);
     return ET_OK;
@@ -224,9 +225,9 @@ int kv_args(const char *fn, KvArgs &a, const et_kv_cache *cache, const int32_t *
     a.nkvg = Divisor((unsigned)(width / ET_KV_GROUP));
     a.groups = Divisor((unsigned)(cache->hd / ET_KV_GROUP));
     a.page_quads = Divisor((unsigned)(cache->page / 4));
-    // n positions from any start touch at most this many groups of four
+    // n positions from any start touch at most this many groups of four; eight threads a unit, and a launch counts its threads in 32 bits
     const long long quads = starts ? (n + 2LL) / 4 + 1 : (n + 3LL) / 4, total = n == 0 ? 0 : quads * a.nkvg.d;
-    ET_REQUIRE(B <= 65535 && total <= 0x7fffffffLL && total * B <= 0x7fffffffLL * 16, ET_ERR_UNSUPPORTED, "%s: B=%d n=%d", fn, B, n);
+    ET_REQUIRE(B <= 65535 && total <= (1LL << 29) - 32, ET_ERR_UNSUPPORTED, "%s: B=%d n=%d", fn, B, n);
     a.total = (unsigned)total;
     return ET_OK;
 }

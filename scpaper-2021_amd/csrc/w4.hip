@@ -357,7 +357,7 @@ int et_linear_w4_f16(const uint8_t *codes, const et_f16 *scales, int group, cons
     ET_REQUIRE(act == ET_ACT_NONE || act == ET_ACT_RELU || act == ET_ACT_GELU, ET_ERR_INVALID_ARG, "et_linear_w4_f16: act=%d", act);
     ET_REQUIRE(((reinterpret_cast<uintptr_t>(Y) | reinterpret_cast<uintptr_t>(Y32)) & 15) == 0 && (reinterpret_cast<uintptr_t>(bias) & 7) == 0,
                ET_ERR_UNSUPPORTED, "et_linear_w4_f16: the result must be 16-byte and the bias 8-byte aligned");
-    ET_REQUIRE(in <= (1 << 23) && T <= 65535 * 4, ET_ERR_UNSUPPORTED, "et_linear_w4_f16: T=%d in=%d", T, in);
+    ET_REQUIRE(in <= (1 << 23) && T <= 65535 * 32, ET_ERR_UNSUPPORTED, "et_linear_w4_f16: T=%d in=%d", T, in);
     if (T == 0) return ET_OK;
     const int nb = out / 16;
     const W4Form f = group == 32 ? w4_form<32>(T, nb) : group == 64 ? w4_form<64>(T, nb) : w4_form<128>(T, nb);

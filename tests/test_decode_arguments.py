@@ -1,5 +1,6 @@
 """What et_kv_*, et_mha_kv_* and et_*w4* refuse, before anything is launched, and the formats' own bounds."""
 import ctypes as C
+import math
 
 import numpy as np
 import pytest
@@ -62,6 +63,33 @@ def test_other_arguments(et):
     assert lib.et_mha_kv_workspace(None, 4, 1, 1, 4, C.byref(need)) == -1
     assert lib.et_mha_kv_workspace(C.byref(c), 4, 1, 1, 4, None) == -1
     assert lib.et_kv_write_f16(None, P, 4, None, None, P, P, 128, 128, 1, 1, None) == -1
+
+
+def test_the_largest_sizes(et):
+    """Positions, threads of a launch and scores that 32 bits would not hold."""
+    c = cache(et, page=1 << 20, npages=1, nkv=1, hd=32)
+    n = C.c_size_t()
+    for pages, status in ((2047, 0), (2048, -2)):
+        assert et.lib().et_mha_kv_workspace(C.byref(c), pages, 1, 1, 1, C.byref(n)) == status, pages
+    c = cache(et, page=16, npages=1, nkv=1, hd=32)
+    for pages, status in ((134217720, 0), (134217721, -2)):  # 2^31 - 128
+        assert et.lib().et_mha_kv_workspace(C.byref(c), pages, 1, 1, 1, C.byref(n)) == status, pages
+    c = cache(et)
+    many = calls(et, c, n=(1 << 29) + 64)  # rows of four groups
+    assert many["write"] == many["read"] == -2
+    assert linear(et, T=65535 * 32 + 1) == -2 and linear(et, T=0, n_in=(1 << 23) + 32) == -2
+    for scale in (math.nan, math.inf, -math.inf, 1.1e15):
+        assert et.lib().et_mha_kv_f16(C.byref(c), P, 4, None, None, P, 256, P, 256, 1, 0, 4, scale, 0, P, 1 << 30, None) == -1, scale
+    for scale in (1e15, -1e15, 0.0):
+        assert et.lib().et_mha_kv_f16(C.byref(c), P, 4, None, None, P, 256, P, 256, 1, 0, 4, scale, 0, P, 1 << 30, None) == 0, scale
+
+
+def test_workspace_does_not_grow_with_fewer_pages(et):
+    """A call with fewer pages than the workspace was made for fits."""
+    for nkv, hd, bits, B, n, nh in ((1, 64, 4, 1, 1, 1), (8, 128, 4, 1, 1, 32), (8, 96, 8, 3, 7, 8), (16, 64, 4, 40, 1, 16), (2, 256, 8, 2, 40, 16)):
+        c = cache(et, nkv=nkv, hd=hd, bits=bits, npages=1 << 14)
+        need = [et.mha_kv_workspace(c, pages, B, n, nh) for pages in range(1, 9000, 37)]
+        assert need == sorted(need)
 
 
 def test_workspace_is_asked_for(et):
