@@ -297,19 +297,27 @@ template <int GROUP, int SWAP, int TBK, int TR, int RBK, int U> W4Form w4_form_o
     return {w4_linear_kernel<GROUP, SWAP, TBK, TR, RBK, U>, S::TPB * TBK, RBK, kw, S::kLds * kw, &large};
 }
 
-// Blocks of output features (nb of them) a wave and waves that share a block, by what fills the chip: measured at 1024 -> 4096 (nb 256), 4096 -> 4096 (256), 800 -> 28800 (1800)
-// and 8192 -> 28672 (1792 blocks), in us for 1, 2 and 4 blocks a wave of four (of eight waves):
-//   1 row, 256 blocks 3.5 3.8 (3.8 4.3), 1800 blocks 6.9 6.1 (10.9 8.8); 16 rows, groups of 128, 1792 blocks 45 37 36 (55 43 36);
-//   45 rows, groups of 32, 256 blocks 12.8 15.8 (11.5 13.1), 1792 blocks 105 83 (116 89).
+// Blocks of output features (nb of them) a wave, and waves that share a block: fewer blocks fill the chip, more of them take what is loaded and ordered of X further.
+// Measured, in us (nb 256 is 1024 -> 4096 and 4096 -> 4096, 512 is 4096 -> 8192, 1024 is 8192 -> 16384 and 4096 -> 16384, 1792 is 8192 -> 28672, 1800 is 800 -> 28800), for
+// 1 block of eight waves, and 1, 2 and 4 blocks of four:
+//   1 row             nb 256: 3.8 3.5 3.8  -    nb 1800: 10.9 6.9 6.1  -
+//   16 rows, 128s     nb 1024:  -  21.6 18.0 19.5   nb 1792: 55 44.9 36.5 33.5
+//   16 rows, 32s      nb 512:  9.6  -  10.6 13.3    nb 1024: 16.1  -  13.3 14.5   nb 1792: 54.8  -  44.6 40.1
+//   32 rows, 32s      nb 256:  9.1 11.0 12.1  -     nb 512: 15.4  -  13.3 17.6
+//   32 rows, 128s     nb 1792:  76  71  53.6 42.3
+//   45 rows, 32s      nb 256: 11.5 12.8 15.8  -     nb 1792: 116 105 83  -
+//   64 rows, 32s      nb 256: 15.3 13.6 12.5 17.9   nb 512: 27.9  -  18.2 18.4    nb 1792:  -   -  105  99
+//   256 rows, 128s    nb 256: 42.7 33.1 23.3 19.7   nb 1792: 500 448 304 243
 template <int GROUP> W4Form w4_form(int T, int nb) {
     constexpr int few = GROUP / 8;  // rows of X whose columns fill a product
+    constexpr int swap = GROUP < 128;
     if (T == 1) return nb <= 1024 ? w4_form_of<GROUP, 0, 1, 1, 1, 2>(4) : w4_form_of<GROUP, 0, 1, 1, 2, 2>(4);
     if (T <= few) return nb <= 512 ? w4_form_of<GROUP, 0, 1, few, 1, 2>(4) : nb <= 1024 ? w4_form_of<GROUP, 0, 1, few, 2, 2>(4) : w4_form_of<GROUP, 0, 1, few, 4, 2>(4);
-    constexpr int swap = GROUP < 128;
     if constexpr (swap)
-        if (T <= 16) return nb <= 512 ? w4_form_of<GROUP, 1, 1, 16, 1, 1>(8) : w4_form_of<GROUP, 1, 1, 16, 2, 1>(4);
-    if (T > 32 && T <= 48) return nb <= 512 ? w4_form_of<GROUP, swap, 3, 48, 1, 1>(8) : w4_form_of<GROUP, swap, 3, 48, 2, 1>(4);
-    return nb <= 512 ? w4_form_of<GROUP, swap, 2, 32, 1, 1>(8) : w4_form_of<GROUP, swap, 2, 32, 2, 1>(4);
+        if (T <= 16) return nb <= 512 ? w4_form_of<GROUP, 1, 1, 16, 1, 1>(8) : nb <= 1024 ? w4_form_of<GROUP, 1, 1, 16, 2, 1>(4) : w4_form_of<GROUP, 1, 1, 16, 4, 1>(4);
+    if (T > 32 && T <= 48) return nb < 512 ? w4_form_of<GROUP, swap, 3, 48, 1, 1>(8) : w4_form_of<GROUP, swap, 3, 48, 2, 1>(4);
+    const long long blocks = (long long)nb * ((T + 31) / 32);
+    return blocks < 512 ? w4_form_of<GROUP, swap, 2, 32, 1, 1>(8) : blocks < 1024 ? w4_form_of<GROUP, swap, 2, 32, 2, 1>(4) : w4_form_of<GROUP, swap, 2, 32, 4, 1>(4);
 }
 
 int w4_check(const char *fn, const void *codes, const void *scales, const void *dense, int in, int out, int group) {

@@ -91,6 +91,13 @@ def test_sizes(et, T, n_in, out, group):
     check(et, T, n_in, out, group, T % 3, False, with_bias=out != 64)
 
 
+@pytest.mark.parametrize("T,out", [(1, 16400), (4, 8208), (4, 16416), (16, 8208), (16, 16416), (32, 8192), (45, 8208), (64, 4080), (64, 8224), (600, 1072), (70001, 16)])
+@pytest.mark.parametrize("group", [32, 64, 128])
+def test_many_output_features_or_rows(et, T, out, group):
+    """Waves that take several blocks of 16 output features, the last of them none; more rows than a grid's second dimension has numbers."""
+    check(et, T, 384, out, group, 0, False)
+
+
 @pytest.mark.parametrize("act", [0, 1, 2])
 @pytest.mark.parametrize("f32", [False, True])
 @pytest.mark.parametrize("with_bias", [False, True])
