@@ -121,6 +121,19 @@ template <int BITS> __device__ __forceinline__ h8 query_order(h8 x, float grow, 
         return h8{(_Float16)f[0], (_Float16)f[2], (_Float16)f[1], (_Float16)f[3], (_Float16)f[4], (_Float16)f[6], (_Float16)f[5], (_Float16)f[7]};
 }
 
+// p * scale as two binary16 numbers: rounded to one, whose error is relative to a value's height above the group's lowest, results were 2 to 3 times as far off as their own
+// rounding (5.9e-4 against 2.1e-4, 2-norm, 131071 keys of random values).  With a zero that the compiler does not know each is one instruction, which widens, multiplies,
+// adds and rounds.
+__device__ __forceinline__ float hidden_zero() {
+    float zero = 0.0f;
+    asm("" : "+v"(zero));
+    return zero;
+}
+__device__ __forceinline__ void weight_of(_Float16 &w, _Float16 &rest, float p, unsigned scale_low, float zero) {
+    w = (_Float16)__builtin_fmaf(p, low_half(scale_low), zero);
+    rest = (_Float16)__builtin_fmaf(p, low_half(scale_low), -(float)w);
+}
+
 // acc += (w + rest) * codes over 32 keys, 4 j .. 4 j + 3 of two pieces.
 template <int BITS, int HD> __device__ __forceinline__ void weigh_values(f4 *acc, h8 w, h8 rest, const unsigned *first, const unsigned *second, int c) {
     using S = KvShape<BITS, HD>;
@@ -167,7 +180,7 @@ template <int BITS, int HD> __device__ __forceinline__ void load_value(unsigned 
     if constexpr (S::kHalfUnit) to[2 * S::kUnits] = half[0], to[2 * S::kUnits + 1] = half[1];
 }
 
-// More rows a key/value head: blocks of 16 / kCols query rows, whose (row, group) pairs fill the 16 columns of the products of a tile of 32 keys.
+// Several rows a key/value head: blocks of 16 / kCols query rows, whose (row, group) pairs fill the 16 columns of the products of a tile of 32 keys.
 //
 // Scores: keys are the rows of the products, so a lane ends with keys 4 j .. 4 j + 3 of both pieces for its column, and these are the very keys that it weighs as a row of the
 // products with the values: nothing moves between lanes but the sum of a row's groups, and a maximum when the reference moves.
@@ -246,6 +259,7 @@ template <int BITS, int HD, int NW> __global__ __launch_bounds__(NW * 64, (kv_ro
     const unsigned *k_scales = a.k_scales + (size_t)kv * (G * a.page), *v_scales = a.v_scales + (size_t)kv * (G * a.page);
     const unsigned page_bytes = (unsigned)nkv * a.page * TB, page_scales = (unsigned)nkv * G * a.page, scales_at = (unsigned)(min(gg, G - 1) * a.page + 4 * j);
 
+    const float zero = hidden_zero();
     for (; t < t_end; t += t_step) {
         // where the pieces lie; one that nobody sees, or without a page, is read from the place of the one before it
         size_t at[2], scale_at[2];
@@ -328,16 +342,14 @@ template <int BITS, int HD, int NW> __global__ __launch_bounds__(NW * 64, (kv_ro
                 for (int i = 0; i < S::kAcc; i++) acc[i][r] *= fr;
             }
         }
-        // p * scale as two binary16 numbers: rounded to one, whose error is relative to a value's height above the group's lowest, results were 2 to 3 times as
-        // far off as their own rounding (5.9e-4 against 2.1e-4, 2-norm, 131071 keys of random values); the products are no bound here
 #pragma unroll
         for (int e = 0; e < 8; e++) {
             const float p = y[e] == kNothing ? 0.0f : __builtin_amdgcn_exp2f(y[e] - ref);
             l += p;
-            const float ps = p * low_half(vs[e >> 2][e & 3]);
             z = __builtin_fmaf(p, high_half(vs[e >> 2][e & 3]), z);
-            w[e] = (_Float16)ps;
-            rest[e] = (_Float16)(ps - (float)w[e]);
+            _Float16 we, re;
+            weight_of(we, re, p, vs[e >> 2][e & 3], zero);
+            w[e] = we, rest[e] = re;
         }
         weigh_values<BITS, HD>(acc, w, rest, vw[0], vw[1], c);
     }
@@ -375,6 +387,316 @@ template <int BITS, int HD, int NW> __global__ __launch_bounds__(NW * 64, (kv_ro
         if (part) {
             part[32 + e] = sum;
             if ((ch & 31) == 0) part[2 * col] = m, part[2 * col + 1] = ls;
+        } else {
+            const int row = row0 + h, i = row_of(row), r = row - i * per;
+            a.Z[((size_t)b * n + i) * a.ldz + (size_t)(kv * per + r) * HD + ch] = (_Float16)(ls == 0.0f ? 0.0f : sum / ls);
+        }
+    }
+}
+
+// Many rows: 16 query rows are the columns of the products, and the contraction is over one group at a time.
+//
+// Scores: lane (c, j) needs eight channels of every group of key c, so the words of a key, loaded 16 bytes a lane, change places between the four rows of lanes (KvWords).
+// Values: the 16 columns of a product are channels of one group, whose scale is in the rows' weights.
+//
+// Bound by its vector instructions, some 500 a tile of 16 rows and 32 keys of 128 channels (five a score and group, the rest the codes), next to 24 products: 64 sequences of
+// 1000 tokens, 16 heads of 128, 16 rows 50.7 us (88 in blocks of 4), 8 of 4000, 4 heads, 256 rows 117 (178).  A spilled register a lane costs more than a wave a SIMD: at three
+// of those, with spills, 109 us.
+template <int BITS> struct KvWords {
+    // Groups in fours, a two and a one: lane j loads what lies at j of a four's (two's, one's) bytes, group j of the four.
+    static constexpr int W = BITS / 4;  // words of eight channels
+    template <int G> static __device__ __forceinline__ void load(unsigned (&to)[G * W], const char *key, int j) {
+        each<G>([&](auto n, int g) {
+            constexpr int N = decltype(n)::value;
+            unsigned v[N * W];
+            load_words<N * W>(v, key + (g * 4 + j * N) * W * 4);
+#pragma unroll
+            for (int i = 0; i < N * W; i++) to[g * W + i] = v[i];
+        });
+    }
+    // -> word w of group g at g * W + w, of the group's eights that of(G, g, j) names
+    template <int G> static __device__ __forceinline__ void part(unsigned (&v)[G * W]) {
+        auto swap32 = [](unsigned &p, unsigned &q) {
+            auto r = __builtin_amdgcn_permlane32_swap(p, q, false, false);
+            p = r[0], q = r[1];
+        };
+        auto swap16 = [](unsigned &p, unsigned &q) {
+            auto r = __builtin_amdgcn_permlane16_swap(p, q, false, false);
+            p = r[0], q = r[1];
+        };
+        each<G>([&](auto n, int g) {
+#pragma unroll
+            for (int w = 0; w < W; w++) {
+                unsigned *x = v + g * W + w;
+                if constexpr (decltype(n)::value == 4) {
+                    swap32(x[0], x[2 * W]);
+                    swap32(x[W], x[3 * W]);
+                    swap16(x[0], x[W]);
+                    swap16(x[2 * W], x[3 * W]);
+                } else if constexpr (decltype(n)::value == 2) {
+                    swap32(x[0], x[W]);
+                }
+            }
+        });
+    }
+    // The eight channels (of four in a group) that lane j has of group g.
+    static constexpr __device__ __forceinline__ int of(int G, int g, int j) { return g < G / 4 * 4 || G % 2 == 1 && g == G - 1 ? j : (j & 1) * 2 + (j >> 1); }
+
+  private:
+    template <int N> struct Number { static constexpr int value = N; };
+    template <int G, typename F> static __device__ __forceinline__ void each(F f) {
+#pragma unroll
+        for (int g = 0; g + 4 <= G; g += 4) f(Number<4>(), g);
+        if constexpr (G % 4 >= 2) f(Number<2>(), G / 4 * 4);
+        if constexpr (G % 2 == 1) f(Number<1>(), G - 1);
+    }
+};
+
+template <int BITS, int HD> __global__ __launch_bounds__(256, (HD <= 64 ? 4 : 2)) void mha_kv_rows_kernel(KV_LEADING, const KvMhaArgs a) {
+    constexpr int NW = 4, ROWS = 16, G = HD / 32, TB = HD * BITS / 8, W = BITS / 4;
+    __shared__ float lds_vals[NW][ROWS * HD];
+    __shared__ float lds_stats[NW][2 + G][ROWS];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int c = lane & 15, j = lane >> 4;
+    const int kv = blockIdx.x, b = blockIdx.y, nkv = gridDim.x;
+    const int block = splits == 1 ? blockIdx.z : blockIdx.z / splits, split = blockIdx.z - block * splits;
+
+    // as in mha_kv_kernel
+    const auto *table = ET_KV_CONST(int32_t, table_at) + (size_t)b * max_pages;
+    const int t_step = splits * NW;
+    int t = split * NW + wave;
+    int page[2], off[2];
+    auto ask = [&](int tile) {
+        const int piece = 2 * tile;
+        int pidx = (int)(((unsigned long long)(unsigned)piece * magic) >> shift), at = piece - pidx * page_pieces;
+        off[0] = at << 4;
+        page[0] = pidx < max_pages ? table[pidx] : -1;
+        const bool on = ++at == page_pieces;
+        off[1] = (on ? 0 : at) << 4;
+        pidx += on;
+        page[1] = pidx < max_pages ? table[pidx] : -1;
+    };
+    ask(t);
+
+    const int start = starts_at ? ET_KV_CONST(int32_t, starts_at)[b] : 0;
+    const int count = counts_at ? min(max(ET_KV_CONST(int32_t, counts_at)[b], 0), n) : n;
+    const int row0 = block * ROWS, rows = min(ROWS, count * per - row0);
+    if (rows <= 0) return;
+    const long long most = (long long)max_pages * a.page;
+    const int end = (int)min(max((long long)start + count, 0LL), most);
+    auto row_of = [&](int row) { return n == 1 ? 0 : row / per; };  // of the call's rows
+    auto limit = [&](int i) { return a.causal ? (int)min((long long)end, max((long long)start + i + 1, 0LL)) : end; };
+    const int lim_least = limit(row_of(row0)), lim_most = limit(row_of(row0 + rows - 1));
+    const int t_end = (lim_most + 31) >> 5;
+
+    h8 q[G];
+    float qsum[G];
+    const int row = row0 + min(c, rows - 1), i_row = row_of(row), r_row = row - i_row * per;
+    const int lim = limit(i_row);
+    const _Float16 *qrow = a.Q + ((size_t)b * n + i_row) * a.ldq + (size_t)(kv * per + r_row) * HD;
+    float top = 0.0f;
+#pragma unroll
+    for (int g = 0; g < G; g++) {
+        q[g] = *reinterpret_cast<const h8 *>(qrow + g * 32 + KvWords<BITS>::of(G, g, j) * 8);
+#pragma unroll
+        for (int e = 0; e < 8; e++) top = fmaxf(top, fabsf((float)q[g][e]));
+    }
+    top = rows_max(top);
+    const int up = top > 0.0f ? 15 - __builtin_amdgcn_frexp_expf(top) : 0;
+    const float grow = __builtin_ldexpf(a.scale_log2e < 0.0f ? -1.0f : 1.0f, up);
+    const float key_scale = __builtin_ldexpf(fabsf(a.scale_log2e), 24 - up);
+#pragma unroll
+    for (int g = 0; g < G; g++) {
+        float sum = 0.0f;
+        q[g] = query_order<BITS>(q[g], grow, sum);
+        qsum[g] = rows_sum(sum) * 0x1p-24f;
+    }
+
+    float ref = kNothing, l = 0.0f, z[G];
+    f4 acc[G][2];
+#pragma unroll
+    for (int g = 0; g < G; g++) {
+        z[g] = 0.0f;
+        acc[g][0] = acc[g][1] = f4{0.f, 0.f, 0.f, 0.f};
+    }
+
+    // units of 16 bits of a value: 8 a group with 4 bits, of which two lanes take one, codes 0 and 1 or 2 and 3; 16 with 8 bits
+    const unsigned key_at = c * TB, value_at = j * (4 * TB) + (BITS == 4 ? c & 7 : c) * 8;
+    const int code_at = BITS == 4 ? c & 8 : 0;
+    const char *k_codes = a.k_codes + (size_t)kv * a.page * TB, *v_codes = a.v_codes + (size_t)kv * a.page * TB;
+    const unsigned *k_scales = a.k_scales + (size_t)kv * (G * a.page), *v_scales = a.v_scales + (size_t)kv * (G * a.page);
+    const unsigned page_bytes = (unsigned)nkv * a.page * TB, page_scales = (unsigned)nkv * G * a.page;
+
+    constexpr int kFirst = HD <= 192 ? G : 4;  // groups of the values that are asked for at once
+    const float zero = hidden_zero();
+    for (; t < t_end; t += t_step) {
+        // where the pieces lie; one that nobody sees, or without a page, is read from the place of the one before it
+        size_t at[2], scale_at[2];
+        const bool ok0 = page[0] >= 0 && page[0] < a.npages, ok1 = t * 32 + 16 < lim_most && page[1] >= 0 && page[1] < a.npages;
+        const unsigned from = ok0 ? page[0] : 0, from_off = ok0 ? off[0] : 0, from1 = ok1 ? page[1] : from, off1 = ok1 ? off[1] : from_off;
+        at[0] = (size_t)from * page_bytes + from_off * TB;
+        at[1] = (size_t)from1 * page_bytes + off1 * TB;
+        scale_at[0] = (size_t)from * page_scales + from_off + 4 * j;
+        scale_at[1] = (size_t)from1 * page_scales + off1 + 4 * j;
+        unsigned kw[2][G * W], vw[2][G][2];
+        u4 ks[2][G], vs[2][G];
+        auto load_keys = [&](int s) {
+            KvWords<BITS>::template load<G>(kw[s], k_codes + at[s] + key_at, j);
+#pragma unroll
+            for (int g = 0; g < G; g++) ks[s][g] = *reinterpret_cast<const u4 *>(k_scales + scale_at[s] + (unsigned)(g * a.page));
+        };
+        load_keys(0);
+        if constexpr (HD <= 192) load_keys(1);
+        auto load_value_scales = [&]() {
+#pragma unroll
+            for (int s = 0; s < 2; s++)
+#pragma unroll
+                for (int g = 0; g < G; g++) vs[s][g] = *reinterpret_cast<const u4 *>(v_scales + scale_at[s] + (unsigned)(g * a.page));
+        };
+        auto load_values = [&](int g) {
+#pragma unroll
+            for (int s = 0; s < 2; s++) load_words<2>(vw[s][g], v_codes + at[s] + value_at + g * (BITS == 4 ? 64 : 128));
+        };
+        if constexpr (HD <= 128) {  // (beyond, the registers do not hold keys and values at once)
+            load_value_scales();
+#pragma unroll
+            for (int g = 0; g < G; g++) load_values(g);
+        }
+        const int tile = t * 32;
+        const bool whole = tile + 32 <= lim_least && ok0 && ok1;
+        ask(t + t_step);
+
+        float y[8];
+#pragma unroll
+        for (int s = 0; s < 2; s++) {
+            if constexpr (HD > 192)
+                if (s == 1) {
+                    __builtin_amdgcn_sched_barrier(0);
+                    load_keys(1);
+                }
+            KvWords<BITS>::template part<G>(kw[s]);
+            f4 sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int g = 0; g < G; g++) {
+                const f4 d = __builtin_amdgcn_mfma_f32_16x16x32_f16(key_codes<BITS>(&kw[s][g * W]), q[g], f4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+#pragma unroll
+                for (int r = 0; r < 4; r++) sum[r] = __builtin_fmaf(low_half(ks[s][g][r]), d[r], __builtin_fmaf(high_half(ks[s][g][r]), qsum[g], sum[r]));
+            }
+#pragma unroll
+            for (int r = 0; r < 4; r++) y[4 * s + r] = sum[r] * key_scale;
+        }
+        if constexpr (HD > 128) {
+            __builtin_amdgcn_sched_barrier(0);
+            load_value_scales();
+#pragma unroll
+            for (int g = 0; g < kFirst; g++) load_values(g);
+        }
+        // (as in mha_kv_kernel; masks, since two values of every scale would take as many registers again)
+        unsigned seen[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++) seen[e] = ~0u;
+        if (!whole) {
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const int s = e >> 2, pos = tile + 16 * s + 4 * j + (e & 3);
+                const bool is = (s == 0 ? ok0 : ok1) && pos < lim;
+                seen[e] = is ? ~0u : 0u;
+                y[e] = is ? y[e] : kNothing;
+            }
+        }
+#pragma unroll
+        for (int g = 0; g < G; g++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) vs[e >> 2][g][e & 3] &= seen[e];
+        // the largest scale: they are not negative, and their bits in the low halves of the words go up with them
+        typedef unsigned short s2 __attribute__((ext_vector_type(2)));
+        s2 most_s = __builtin_bit_cast(s2, vs[0][0][0]);
+#pragma unroll
+        for (int i = 1; i < 8 * G; i++) most_s = __builtin_elementwise_max(most_s, __builtin_bit_cast(s2, vs[i / (4 * G)][i / 4 % G][i & 3]));
+        const float most_e = (float)__builtin_amdgcn_frexp_expf(low_half(__builtin_bit_cast(unsigned, most_s)));
+        float most_y = y[0];
+#pragma unroll
+        for (int e = 1; e < 8; e++) most_y = fmaxf(most_y, y[e]);
+        const float reach = most_y + most_e;
+        if (__any(reach > ref + 15.0f)) {
+            const float next = fmaxf(ref, rows_max(reach) - 11.0f);
+            const float f = __builtin_amdgcn_exp2f(ref - next);
+            ref = next;
+            l *= f;
+            float fr[4];
+#pragma unroll
+            for (int r = 0; r < 4; r++) fr[r] = __shfl(f, 4 * j + r);
+#pragma unroll
+            for (int g = 0; g < G; g++) {
+                z[g] *= f;
+#pragma unroll
+                for (int r = 0; r < 4; r++) acc[g][0][r] *= fr[r], acc[g][1][r] *= fr[r];
+            }
+        }
+        float p[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            p[e] = y[e] == kNothing ? 0.0f : __builtin_amdgcn_exp2f(y[e] - ref);
+            l += p[e];
+        }
+#pragma unroll
+        for (int g = 0; g < G; g++) {
+            if (g + kFirst < G) {
+                __builtin_amdgcn_sched_barrier(0);
+                load_values(g + kFirst);
+            }
+            h8 w, rest;
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const unsigned sl = vs[e >> 2][g][e & 3];
+                _Float16 we, re;
+                weight_of(we, re, p[e], sl, zero);
+                w[e] = we, rest[e] = re;
+                z[g] = __builtin_fmaf(p[e], high_half(sl), z[g]);
+            }
+#pragma unroll
+            for (int k = 0; k < 2; k++) {
+                unsigned x[4];
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const unsigned word = vw[i >> 1][g][i & 1] >> code_at;
+                    x[i] = BITS == 8 ? raised<8>(word, k) : (k == 0 ? word << 7 : word << 3) & 0x07800780u;
+                }
+                const h8 codes = as_h8(x[0], x[1], x[2], x[3]);
+                acc[g][k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w, codes, acc[g][k], 0, 0, 0);
+                acc[g][k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(rest, codes, acc[g][k], 0, 0, 0);
+            }
+        }
+    }
+
+    // what the waves have, side by side
+    const float ls = rows_sum(l);
+    if (j == 0) lds_stats[wave][0][c] = ref, lds_stats[wave][1][c] = ls;
+    constexpr float unit = BITS == 8 ? code_unit<8>(0) : 0x1p17f;
+#pragma unroll
+    for (int g = 0; g < G; g++) {
+        const float zs = rows_sum(z[g]);
+        if (j == 0) lds_stats[wave][2 + g][c] = zs;
+        const int ch = g * 32 + (BITS == 4 ? 4 * (c & 7) + 2 * (c >> 3) : 2 * c);
+#pragma unroll
+        for (int r = 0; r < 4; r++)
+            *reinterpret_cast<float2 *>(&lds_vals[wave][(4 * j + r) * HD + ch]) = float2{acc[g][0][r] * unit, acc[g][1][r] * unit};
+    }
+    __syncthreads();
+    float *part = splits > 1 ? a.parts + ((size_t)blockIdx.z * units + (unsigned)(b * nkv + kv)) * (32 + ROWS * HD) : nullptr;
+    for (int e = threadIdx.x; e < rows * HD; e += NW * 64) {
+        const int h = e / HD, ch = e - h * HD, g = ch >> 5;
+        const float m = fmaxf(fmaxf(lds_stats[0][0][h], lds_stats[1][0][h]), fmaxf(lds_stats[2][0][h], lds_stats[3][0][h]));
+        float sum = 0.0f, ls = 0.0f;
+#pragma unroll
+        for (int w = 0; w < NW; w++) {
+            const float f = __builtin_amdgcn_exp2f(lds_stats[w][0][h] - m);
+            sum = __builtin_fmaf(f, lds_vals[w][e] + lds_stats[w][2 + g][h], sum);
+            ls = __builtin_fmaf(f, lds_stats[w][1][h], ls);
+        }
+        if (part) {
+            part[32 + e] = sum;
+            if (ch == 0) part[2 * h] = m, part[2 * h + 1] = ls;
         } else {
             const int row = row0 + h, i = row_of(row), r = row - i * per;
             a.Z[((size_t)b * n + i) * a.ldz + (size_t)(kv * per + r) * HD + ch] = (_Float16)(ls == 0.0f ? 0.0f : sum / ls);
@@ -494,6 +816,7 @@ template <int BITS, int HD, int R, int NW> __global__ __launch_bounds__(NW * 64,
     const int key_place = (j >> 1) * 32 + (c >> 2) * 8 + (j & 1) * 4 + (c & 3);
     const _Float16 *weights_at = weights + (c & 3) * F::kLdsRow + j * 8;
 
+    const float zero = hidden_zero();
     for (; t < t_end; t += t_step) {
         // where the pieces lie; one that nobody sees, or without a page, is read from the place of the one before it
         const int there = (lim_most - t * 64 + 15) >> 4;  // pieces that somebody sees, or more
@@ -582,10 +905,10 @@ template <int BITS, int HD, int R, int NW> __global__ __launch_bounds__(NW * 64,
 #pragma unroll
             for (int g = 0; g < G; g++) {
                 z[h][g] = __builtin_fmaf(p, R == 1 || seen ? high_half(vs[g]) : 0.0f, z[h][g]);  // (what others see may be NaN, and 0 * NaN is)
-                const float ps = p * low_half(vs[g]);
-                const _Float16 w = (_Float16)ps;
+                _Float16 w, rest;
+                weight_of(w, rest, p, vs[g], zero);
                 weights[(h * GP + g) * F::kLdsRow + key_place] = w;
-                weights[(4 + h * GP + g) * F::kLdsRow + key_place] = (_Float16)(ps - (float)w);
+                weights[(4 + h * GP + g) * F::kLdsRow + key_place] = rest;
             }
         }
         wave_lds_order();
@@ -653,7 +976,7 @@ __global__ __launch_bounds__(256) void mha_kv_join_kernel(const KvMhaArgs a) {
     if (row >= count * a.per) return;
     const float *part = a.parts + ((size_t)block * a.splits * a.units + unit) * part_floats;
     const size_t next = (size_t)a.units * part_floats;
-    const int ch = threadIdx.x & 31, lot = threadIdx.x >> 5, col = h * a.cols + g, at = 32 + h * a.hd + g * 32 + ch;
+    const int ch = threadIdx.x & 31, lot = threadIdx.x >> 5, col = a.cols == 1 ? h : h * a.cols + g, at = 32 + h * a.hd + g * 32 + ch;
     float m = kNothing, sum = 0.0f, ls = 0.0f;
     for (int s0 = lot; s0 < a.splits; s0 += 4 * kPer) {  // four parts asked for at once
         float pm[4], pl[4], pv[4];
@@ -700,13 +1023,16 @@ struct KvForm {
     int rows, cols, tile;
 };
 
-// Rows: of a key/value head in the call.
+// Rows: of a key/value head in the call.  Blocks of 16 / kCols rows or of 16, measured in us with 16 sequences of 4096 tokens, 8 heads (of 128: 8 rows 34.3 | 37.7, 9 rows
+// 50.4 | 40.4, 16 rows 82 | 46; of 64, 10 rows 27.3 | 24.6, 8 rows 22.5 | 26.9) and 4 sequences (of 192: 5 rows 32.3 | 22.0; of 256: 6 rows 34.7 | 27.2, 32 rows 91 | 45).
 template <int BITS, int HD> KvForm form_of(long long rows) {
     if constexpr (HD <= 128) {
         constexpr int cols = KvShape<BITS, HD>::kCols, heads = 4 / cols;
         if (rows == 1) return {mha_kv_few_kernel<BITS, HD, 1, 4>, mha_kv_few_kernel<BITS, HD, 1, 8>, 1, cols, 64};
         if (rows <= heads) return {mha_kv_few_kernel<BITS, HD, heads, 4>, mha_kv_few_kernel<BITS, HD, heads, 8>, heads, cols, 64};
     }
+    if constexpr (HD > 32)
+        if (rows > (HD <= 128 ? 8 : 4)) return {mha_kv_rows_kernel<BITS, HD>, mha_kv_rows_kernel<BITS, HD>, 16, 1, 32};
     return {mha_kv_kernel<BITS, HD, 4>, mha_kv_kernel<BITS, HD, 8>, KvShape<BITS, HD>::kRows, KvShape<BITS, HD>::kCols, 32};
 }
 
@@ -740,7 +1066,7 @@ int kv_plan(const char *fn, KvPlan &p, const et_kv_cache *c, int max_pages, int 
     ET_REQUIRE(rows <= 0x7fffffffLL && B <= 65535 && blocks <= 65535 && units * blocks <= (1LL << 24), ET_ERR_UNSUPPORTED, "%s: B=%d n=%d nh=%d", fn, B, n, nh);
     p.blocks = (int)blocks;
     const long long tiles = ((long long)max_pages * c->page + p.form.tile - 1) / p.form.tile, groups = units * blocks;
-    p.waves = groups >= 512 ? 4 : 8;
+    p.waves = groups >= 512 || p.form.four == p.form.eight ? 4 : 8;
     p.splits = groups == 0 ? 1 : (int)std::max(1LL, std::min({(4096 / p.waves + groups - 1) / groups, tiles / (4 * p.waves), 256LL}));
     p.splits = std::min(p.splits, (int)(65535 / std::max(1LL, blocks)));
     p.bytes = p.splits > 1 ? (size_t)(groups * p.splits) * (32 + p.form.rows * c->hd) * sizeof(float) : 0;

@@ -223,6 +223,13 @@ def test_attention_long(et, bits):
     check_attention(et, bits, 2, 1, 64, 16, [3333], 2, True, seed=6)
 
 
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("hd", [64, 96, 256])
+def test_attention_long_of_many_rows(et, bits, hd):
+    """Many rows a key/value head over keys that are shared out: the last block of rows is not full, one sequence has no key for most workgroups."""
+    check_attention(et, bits, 1, 7, hd, 48, [4000, 9], 3, True, seed=15)
+
+
 @pytest.mark.parametrize("qscale", [2.0 ** -13, 30.0])
 def test_attention_of_very_even_and_very_uneven_probabilities(et, qscale):
     check_attention(et, 4, 2, 2, 64, 16, [300, 81], 1, False, seed=9, qscale=qscale)
