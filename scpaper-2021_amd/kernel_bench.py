@@ -1,7 +1,7 @@
 #!/usr/bin/env python3
 """Per-kernel throughput against the roofline that bounds it, through the C ABI.
 
-    python scpaper-2021_amd/kernel_bench.py [--set configs|scale|vo|mha|qkv|fuseo|plan|machine|all] [--json FILE]
+    python scpaper-2021_amd/kernel_bench.py [--set configs|scale|vo|mha|qkv|fuseo|plan|machine|decode|all] [--json FILE]
 
 `configs` are the shapes of the benchmark configurations (attention block at batch
 1/4/16, the tile/row/column-pruned Linears at 2048 token rows, the BERT-large-shaped
@@ -382,6 +382,57 @@ class Bench:
                 self.rows.append({"kernel": "probe_read", "shape": f"{per_wg // 1024} KB/CU {threads} thr shared={shared}",
                                   "us": round(us, 2), "gb_s_per_cu": round(gbs, 1)})
 
+    def decode_cache(self, bits, B, length, nkv, hd, page, n, launches):
+        """A cache of B sequences, `length` tokens of which are written (n at a time if n > 0) and read: what a call of n tokens each takes."""
+        et = self.et
+        pages, width = -(-length // page), nkv * hd
+        size = B * pages * nkv * page * (hd * bits // 8)
+        bufs = [et.DeviceBuffer(b) for b in (size, size // hd * 8 // bits * hd // 32 * 4) * 2]
+        cache = et.KvCache(*(buf.ptr for buf in bufs), bits, nkv, hd, page, B * pages)
+        table = self.dev(self.rng.permutation(B * pages).astype(np.int32).reshape(B, pages))
+        rows = self.dev(self.rnd((min(B * length, 65536), width)))
+        for b in range(B):  # (rows of other sequences again, where there are more tokens than rows)
+            for at in range(0, length, 4096):
+                m = min(4096, length - at)
+                start = self.dev(np.array([at], np.int32))
+                et.kv_write(cache, table.offset(b * pages * 4), pages, start, None, rows, rows, width, width, 1, min(m, rows.shape[0]), self.stream)
+        et.check(self.lib.et_stream_sync(self.stream))
+        shape = f"{bits} bits B{B} n{n} {nkv} heads of {hd} page {page}"
+        token = width * bits // 8 + width // 32 * 4
+        if n:
+            starts = self.dev(np.full(B, length - n, np.int32))
+            k, v = self.dev(self.rnd((B * n, width))), self.dev(self.rnd((B * n, width)))
+            work = 2 * B * n * (width * 2 + token)
+            self.record("kv_write", shape, self.time_us(lambda: et.kv_write(cache, table, pages, starts, None, k, v, width, width, B, n, self.stream), launches), work, "hbm")
+            self.record("kv_read", shape, self.time_us(lambda: et.kv_read(cache, table, pages, starts, None, k, v, width, width, B, n, self.stream), launches), work, "hbm")
+        return cache, table, pages, bufs
+
+    def decode_attention(self, bits, B, length, nh, nkv, hd, page, n, launches):
+        et = self.et
+        cache, table, pages, bufs = self.decode_cache(bits, B, length, nkv, hd, page, 0, 1)
+        starts, width = self.dev(np.full(B, length - n, np.int32)), nh * hd
+        q, z = self.dev(self.rnd((B * n, width))), self.empty((B * n, width))
+        need = et.mha_kv_workspace(cache, pages, B, n, nh)
+        ws = et.DeviceBuffer(max(need, 16))
+        us = self.time_us(lambda: et.mha_kv(cache, table, pages, starts, None, q, width, z, width, B, n, nh, hd ** -0.5, et.MHA_CAUSAL, ws, need, self.stream), launches)
+        self.record("mha_kv", f"{bits} bits B{B} L{length} n{n} {nh}/{nkv} heads of {hd}", us, 2 * B * length * (nkv * hd * bits // 8 + nkv * hd // 32 * 4), "hbm")
+
+    def linear_w4(self, T, n_in, n_out, group, launches, nset=4):
+        et = self.et
+        w = self.dev(self.rnd((n_out, n_in), 0.02))
+        sets = [(et.DeviceBuffer(n_out * n_in // 2), et.DeviceBuffer(n_in // group * n_out * 4)) for _ in range(nset)]
+        for codes, scales in sets:
+            et.dense_to_w4(w, codes, scales, n_in, n_out, group, self.stream)
+        bias, x, y = self.dev(np.zeros(n_out, np.float16)), self.dev(self.rnd((T, n_in))), self.empty((T, n_out))
+        turn = {"n": 0}
+
+        def fn():
+            codes, scales = sets[turn["n"] % nset]
+            turn["n"] += 1
+            et.linear_w4(codes, scales, group, bias, x, y, None, T, n_in, n_out, 0, self.stream)
+        work = n_in * n_out // 2 + n_in // group * n_out * 4 + 2 * T * (n_in + n_out)
+        self.record("linear_w4", f"T{T} in{n_in} out{n_out} groups of {group}", self.time_us(fn, launches * nset), work, "hbm")
+
     def rowcol(self, T, n_in, n_out, sparsity, launches):
         et, lib = self.et, self.lib
         row_id = self.ids(lib.et_fmt_row_ids, n_out, sparsity, 7)
@@ -599,7 +650,7 @@ def run_scale(b: Bench):
 
 def main():
     ap = argparse.ArgumentParser()
-    ap.add_argument("--set", choices=("configs", "scale", "vo", "mha", "qkv", "fuseo", "local", "depth", "plan", "machine", "all"), default="all")
+    ap.add_argument("--set", choices=("configs", "scale", "vo", "mha", "qkv", "fuseo", "local", "depth", "plan", "machine", "decode", "all"), default="all")
     ap.add_argument("--json", default=None, help="also write the rows as JSON to this file")
     args = ap.parse_args()
     b = Bench()
@@ -659,6 +710,16 @@ def main():
                 if entry == "pack" and T > 4096:
                     continue
                 b.bsr(T, n_in, n_out, 0.8, 10 if T >= 16384 else 30, entry=entry)
+    if args.set == "decode":
+        print("# generating token by token: a cache of keys and values in 4 and 8 bits, attention over it, 4-bit Linears")
+        for bits, B, length, nkv, hd, n in ((4, 8, 512, 12, 64, 1), (4, 16, 1000, 8, 128, 1000), (8, 4, 8192, 16, 64, 8192)):
+            b.decode_cache(bits, B, length, nkv, hd, 64, n, 20)
+        for bits, B, length, nh, nkv, hd, n in ((4, 1, 128, 12, 12, 64, 1), (4, 8, 2048, 12, 12, 64, 1), (4, 64, 4096, 16, 16, 64, 1), (4, 16, 4096, 32, 8, 128, 1),
+                                                (4, 1, 131071, 32, 8, 128, 1), (8, 16, 1500, 8, 8, 96, 7), (4, 64, 1000, 16, 16, 128, 16), (4, 8, 4000, 64, 4, 128, 16)):
+            b.decode_attention(bits, B, length, nh, nkv, hd, 64, n, 10)
+        for T, n_in, n_out, group in ((1, 1024, 4096, 64), (1, 800, 28800, 32), (1, 8192, 28672, 128), (4, 8192, 28672, 128), (16, 8192, 28672, 128), (45, 4096, 4096, 32),
+                                      (64, 4096, 16384, 64), (256, 4096, 4096, 128)):
+            b.linear_w4(T, n_in, n_out, group, 10)
     if args.set == "machine":
         print("# machine probes")
         b.machine()
