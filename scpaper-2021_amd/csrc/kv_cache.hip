@@ -3,7 +3,8 @@
 // Eight lanes take one group of 32 channels of four tokens whose positions are 4q .. 4q + 3, bits of the lane: 0 and 1 the token, 3 the eights of channels 0 and 2 or 1 and
 // 3 (bit 2: the next group).  A group's extremes are then one rotation inside the 16 lanes, and the four tokens' codes of V, which the cache holds side by side, change places
 // inside four neighbouring lanes.  Where a call does not hold all four tokens, the units of 16 bits of those it holds are stored one by one: the bytes of the others are not
-// touched.  Writing is bound by its arithmetic next to memory: 16 channels a lane share a group's scale (8 did not: 27 us for 16 x 1000 tokens of 8 heads of 128).
+// touched.  Writing is bound by its arithmetic next to memory, 19 vector instructions a value: 16 channels a lane share a group's scale (8 did not: 27 us for 16 x 1000 tokens of
+// 8 heads of 128, of which it writes and reads 86 MB in 22.2 us; reading back is memory, 86 MB in 17.0).  8 bits, 4 x 8192 tokens of 16 heads of 64, 209 MB: 54.6 and 37.6 us.
 #include "group_quant.hip.h"
 
 namespace et {
@@ -86,6 +87,13 @@ template <int BITS> __device__ __forceinline__ void kv_quantise(const h8 (&x)[2]
     quantise<BITS, 2>(codes, scale_low, x, e, magnitude, least_of(tiny, tiny_more));
 }
 
+// Between pairs of lanes: the first of a pair ends with `first` of both, the second with `second` of both, in the lanes' order.
+template <int CTRL> __device__ __forceinline__ void trade(unsigned &mine, unsigned &other, unsigned first, unsigned second, bool is_second) {
+    const unsigned got = dpp_bits<CTRL>(is_second ? first : second);
+    mine = is_second ? got : first;
+    other = is_second ? second : got;
+}
+
 template <int BITS> __global__ __launch_bounds__(256) void kv_write_kernel(const KvArgs a) {
     const unsigned unit = blockIdx.x * 32 + (threadIdx.x >> 4) * 2 + (threadIdx.x >> 2 & 1);
     const KvUnit u = kv_unit(a, unit);
@@ -108,22 +116,36 @@ template <int BITS> __global__ __launch_bounds__(256) void kv_write_kernel(const
         if (u.sub == 0) a.k_scales[u.scale + u.tq] = sl;
     }
     kv_quantise<BITS>(v, c, sl);
-    // the four tokens' units from at / 2 on, [unit][token]
+    // The four tokens' units from at / 2 on, [unit][token]: words of two units change places between the four lanes, which each store 16 bytes (8 with 4 bits) in one
+    // piece.  Word by word, 4 bytes a lane, the stores were four times as many requests: 8 bits, 4 x 8192 tokens of 16 heads of 64 60.6 us instead of 54.6.
     char *to = a.v_codes + u.quad * token_bytes + (size_t)at * 4;
+    const bool odd = u.tq & 1, high = u.tq & 2;
+    unsigned x[2 * W];
 #pragma unroll
-    for (int e = 0; e < 2; e++)
+    for (int i = 0; i < 2 * W; i += 2) trade<kDppQuadXor1>(x[i], x[i + 1], c[i], c[i + 1], odd);  // -> word i, of odd lanes i + 1, of this lane and its neighbour, by token
+    constexpr unsigned lows = 0x05040100u, highs = 0x07060302u;
+    if constexpr (BITS == 8) {
+        unsigned y[4];
+        trade<kDppQuadXor2>(y[0], y[2], x[0], x[2], high);
+        trade<kDppQuadXor2>(y[1], y[3], x[1], x[3], high);
+        if (u.all)
+            *reinterpret_cast<uint4 *>(to + (u.tq >> 1) * 64 + odd * 16) = uint4{__builtin_amdgcn_perm(y[1], y[0], lows), __builtin_amdgcn_perm(y[3], y[2], lows),
+                                                                                 __builtin_amdgcn_perm(y[1], y[0], highs), __builtin_amdgcn_perm(y[3], y[2], highs)};
+    } else {
+        unsigned y[2];
+        trade<kDppQuadXor2>(y[0], y[1], __builtin_amdgcn_perm(x[1], x[0], lows), __builtin_amdgcn_perm(x[1], x[0], highs), high);
+        if (u.all) *reinterpret_cast<uint2 *>(to + odd * 32 + (u.tq >> 1) * 8) = uint2{y[0], y[1]};
+    }
+    if (!u.all && u.mine) {
 #pragma unroll
-        for (int w = 0; w < W; w++) {
-            // lane m of four stores unit m / 2 of tokens 2 (m % 2) and the next
-            const unsigned word = c[e * W + w], first = dpp_bits<0x88>(word), second = dpp_bits<0xDD>(word);  // quad_perm [0,2,0,2] and [1,3,1,3]
-            char *here = to + e * 8 * BITS + w * 16;
-            if (u.all) {
-                *reinterpret_cast<unsigned *>(here + u.tq * 4) = u.tq & 2 ? (first >> 16) | (second & 0xffff0000u) : (first & 0xffffu) | second << 16;
-            } else if (u.mine) {
-                *reinterpret_cast<unsigned short *>(here + u.tq * 2) = (unsigned short)word;
-                *reinterpret_cast<unsigned short *>(here + 8 + u.tq * 2) = (unsigned short)(word >> 16);
+        for (int e = 0; e < 2; e++)
+#pragma unroll
+            for (int w = 0; w < W; w++) {
+                char *here = to + e * 8 * BITS + w * 16 + u.tq * 2;
+                *reinterpret_cast<unsigned short *>(here) = (unsigned short)c[e * W + w];
+                *reinterpret_cast<unsigned short *>(here + 8) = (unsigned short)(c[e * W + w] >> 16);
             }
-        }
+    }
     if (u.mine && u.sub == 0) a.v_scales[u.scale + u.tq] = sl;
 }
 
