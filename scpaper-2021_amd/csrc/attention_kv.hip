@@ -452,8 +452,8 @@ template <int BITS> struct KvWords {
     }
 };
 
-template <int BITS, int HD> __global__ __launch_bounds__(256, (HD <= 64 ? 4 : 2)) void mha_kv_rows_kernel(KV_LEADING, const KvMhaArgs a) {
-    constexpr int NW = 4, ROWS = 16, G = HD / 32, TB = HD * BITS / 8, W = BITS / 4;
+template <int BITS, int HD, int NW> __global__ __launch_bounds__(NW * 64, (HD <= 64 ? 4 : 2)) void mha_kv_rows_kernel(KV_LEADING, const KvMhaArgs a) {
+    constexpr int ROWS = 16, G = HD / 32, TB = HD * BITS / 8, W = BITS / 4;
     __shared__ float lds_vals[NW][ROWS * HD];
     __shared__ float lds_stats[NW][2 + G][ROWS];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -686,7 +686,9 @@ template <int BITS, int HD> __global__ __launch_bounds__(256, (HD <= 64 ? 4 : 2)
     float *part = splits > 1 ? a.parts + ((size_t)blockIdx.z * units + (unsigned)(b * nkv + kv)) * (32 + ROWS * HD) : nullptr;
     for (int e = threadIdx.x; e < rows * HD; e += NW * 64) {
         const int h = e / HD, ch = e - h * HD, g = ch >> 5;
-        const float m = fmaxf(fmaxf(lds_stats[0][0][h], lds_stats[1][0][h]), fmaxf(lds_stats[2][0][h], lds_stats[3][0][h]));
+        float m = lds_stats[0][0][h];
+#pragma unroll
+        for (int w = 1; w < NW; w++) m = fmaxf(m, lds_stats[w][0][h]);
         float sum = 0.0f, ls = 0.0f;
 #pragma unroll
         for (int w = 0; w < NW; w++) {
@@ -1021,6 +1023,7 @@ using KvKernel = void (*)(KV_LEADING, const KvMhaArgs);
 struct KvForm {
     KvKernel four, eight;  // waves
     int rows, cols, tile;
+    bool eight_if_whole;   // eight only where one workgroup has all the keys
 };
 
 // Rows: of a key/value head in the call.  Blocks of 16 / kCols rows or of 16, measured in us with 16 sequences of 4096 tokens, 8 heads (of 128: 8 rows 34.3 | 37.7, 9 rows
@@ -1028,12 +1031,12 @@ struct KvForm {
 template <int BITS, int HD> KvForm form_of(long long rows) {
     if constexpr (HD <= 128) {
         constexpr int cols = KvShape<BITS, HD>::kCols, heads = 4 / cols;
-        if (rows == 1) return {mha_kv_few_kernel<BITS, HD, 1, 4>, mha_kv_few_kernel<BITS, HD, 1, 8>, 1, cols, 64};
-        if (rows <= heads) return {mha_kv_few_kernel<BITS, HD, heads, 4>, mha_kv_few_kernel<BITS, HD, heads, 8>, heads, cols, 64};
+        if (rows == 1) return {mha_kv_few_kernel<BITS, HD, 1, 4>, mha_kv_few_kernel<BITS, HD, 1, 8>, 1, cols, 64, false};
+        if (rows <= heads) return {mha_kv_few_kernel<BITS, HD, heads, 4>, mha_kv_few_kernel<BITS, HD, heads, 8>, heads, cols, 64, false};
     }
     if constexpr (HD > 32)
-        if (rows > (HD <= 128 ? 8 : 4)) return {mha_kv_rows_kernel<BITS, HD>, mha_kv_rows_kernel<BITS, HD>, 16, 1, 32};
-    return {mha_kv_kernel<BITS, HD, 4>, mha_kv_kernel<BITS, HD, 8>, KvShape<BITS, HD>::kRows, KvShape<BITS, HD>::kCols, 32};
+        if (rows > (HD <= 128 ? 8 : 4)) return {mha_kv_rows_kernel<BITS, HD, 4>, mha_kv_rows_kernel<BITS, HD, HD <= 128 ? 8 : 4>, 16, 1, 32, HD > 64};
+    return {mha_kv_kernel<BITS, HD, 4>, mha_kv_kernel<BITS, HD, 8>, KvShape<BITS, HD>::kRows, KvShape<BITS, HD>::kCols, 32, false};
 }
 
 template <int BITS> KvForm form_of(int hd, long long rows) {
@@ -1056,7 +1059,9 @@ struct KvPlan {
 };
 
 // Waves of a workgroup and workgroups that share the keys of a (sequence, key/value head): 4096 waves, which fill the chip, but at least four tiles a wave if every
-// sequence were as long as its table; a second launch, which joins the parts, costs 3 to 6 us.
+// sequence were as long as its table; a second launch, which joins the parts, costs 3 to 6 us.  Eight waves a workgroup where there are few: 16 rows, 8 heads of 128, 1000
+// tokens, 16 sequences 25.0 us with four, 16.3 with eight, 32 sequences 34.2 and 17.7; but only two of them a SIMD fit so (of 96 three with four waves): where keys are shared
+// out anyway, four (16 x 10937 tokens, 5 heads of 96, 80 rows 147 and 170 us).
 int kv_plan(const char *fn, KvPlan &p, const et_kv_cache *c, int max_pages, int B, int n, int nh) {
     ET_REQUIRE(nh > 0 && nh % c->nkv == 0, ET_ERR_INVALID_ARG, "%s: nh=%d must be a multiple of nkv=%d", fn, nh, c->nkv);
     const int per = nh / c->nkv;
@@ -1066,7 +1071,7 @@ int kv_plan(const char *fn, KvPlan &p, const et_kv_cache *c, int max_pages, int 
     ET_REQUIRE(rows <= 0x7fffffffLL && B <= 65535 && blocks <= 65535 && units * blocks <= (1LL << 24), ET_ERR_UNSUPPORTED, "%s: B=%d n=%d nh=%d", fn, B, n, nh);
     p.blocks = (int)blocks;
     const long long tiles = ((long long)max_pages * c->page + p.form.tile - 1) / p.form.tile, groups = units * blocks;
-    p.waves = groups >= 512 || p.form.four == p.form.eight ? 4 : 8;
+    p.waves = groups >= 512 || p.form.four == p.form.eight || (p.form.eight_if_whole && tiles >= 64) ? 4 : 8;
     p.splits = groups == 0 ? 1 : (int)std::max(1LL, std::min({(4096 / p.waves + groups - 1) / groups, tiles / (4 * p.waves), 256LL}));
     p.splits = std::min(p.splits, (int)(65535 / std::max(1LL, blocks)));
     p.bytes = p.splits > 1 ? (size_t)(groups * p.splits) * (32 + p.form.rows * c->hd) * sizeof(float) : 0;
