@@ -965,53 +965,59 @@ template <int BITS, int HD, int R, int NW> __global__ __launch_bounds__(NW * 64,
     }
 }
 
-// The parts of a unit's rows: one workgroup a (block of rows, unit, 32 channels of a row), 8 threads' worth of parts at a time a channel.
-__global__ __launch_bounds__(256) void mha_kv_join_kernel(const KvMhaArgs a) {
-    constexpr int kPer = 256 / 32;
-    __shared__ float lds[3][kPer][32];
-    const int groups = a.hd / ET_KV_GROUP, part_floats = 32 + a.block_rows * a.hd;
-    const int block = blockIdx.y, col_g = blockIdx.x % (a.block_rows * groups), unit = blockIdx.x / (a.block_rows * groups);
+// The parts of a unit's rows: 32 threads a channel group of a row, or 2, 4, 8 times that many where there are many parts, which a workgroup then adds up (lots: how many).
+// (One workgroup of eight for each, whatever the parts, was 8192 waves to start for 16 sequences of 32 heads over 8 of 128, 4096 tokens in four parts: 24.0 us with
+// the attention, 22.9 so.)
+__global__ __launch_bounds__(256) void mha_kv_join_kernel(const KvMhaArgs a, int lots_log2) {
+    __shared__ float lds[3][8][32];
+    const int groups = a.hd / ET_KV_GROUP, part_floats = 32 + a.block_rows * a.hd, lots = 1 << lots_log2;
+    const int ch = threadIdx.x & 31, at_once = threadIdx.x >> 5, lot = at_once & (lots - 1);
+    const int mine = (int)blockIdx.x * (8 >> lots_log2) + (at_once >> lots_log2);
+    const int block = blockIdx.y, unit = mine / (a.block_rows * groups), col_g = mine - unit * (a.block_rows * groups);
     const int h = col_g / groups, g = col_g - h * groups;
     const int b = unit / a.nkv, kv = unit - b * a.nkv;
-    const int count = a.counts ? min(max(a.counts[b], 0), a.n) : a.n;
     const int row = block * a.block_rows + h;
-    if (row >= count * a.per) return;
-    const float *part = a.parts + ((size_t)block * a.splits * a.units + unit) * part_floats;
-    const size_t next = (size_t)a.units * part_floats;
-    const int ch = threadIdx.x & 31, lot = threadIdx.x >> 5, col = a.cols == 1 ? h : h * a.cols + g, at = 32 + h * a.hd + g * 32 + ch;
+    const bool there = unit < a.units && row < (a.counts ? min(max(a.counts[b], 0), a.n) : a.n) * a.per;
     float m = kNothing, sum = 0.0f, ls = 0.0f;
-    for (int s0 = lot; s0 < a.splits; s0 += 4 * kPer) {  // four parts asked for at once
-        float pm[4], pl[4], pv[4];
+    if (there) {
+        const float *part = a.parts + ((size_t)block * a.splits * a.units + unit) * part_floats;
+        const size_t next = (size_t)a.units * part_floats;
+        const int col = a.cols == 1 ? h : h * a.cols + g, at = 32 + h * a.hd + g * 32 + ch;
+        for (int s0 = lot; s0 < a.splits; s0 += 4 * lots) {  // four parts asked for at once
+            float pm[4], pl[4], pv[4];
 #pragma unroll
-        for (int k = 0; k < 4; k++) {
-            const int s = min(s0 + k * kPer, a.splits - 1);
-            const float *p = part + s * next;
-            pm[k] = s0 + k * kPer < a.splits ? p[2 * col] : kNothing;
-            pl[k] = s0 + k * kPer < a.splits ? p[2 * col + 1] : 0.0f;
-            pv[k] = s0 + k * kPer < a.splits ? p[at] : 0.0f;
-        }
-        const float most = fmaxf(fmaxf(fmaxf(pm[0], pm[1]), fmaxf(pm[2], pm[3])), m);
-        const float f = __builtin_amdgcn_exp2f(m - most);
-        m = most;
-        sum *= f;
-        ls *= f;
+            for (int k = 0; k < 4; k++) {
+                const bool is = s0 + k * lots < a.splits;
+                const float *p = part + (is ? s0 + k * lots : s0) * next;
+                pm[k] = is ? p[2 * col] : kNothing;
+                pl[k] = is ? p[2 * col + 1] : 0.0f;
+                pv[k] = is ? p[at] : 0.0f;
+            }
+            const float most = fmaxf(fmaxf(fmaxf(pm[0], pm[1]), fmaxf(pm[2], pm[3])), m);
+            const float f = __builtin_amdgcn_exp2f(m - most);
+            m = most;
+            sum *= f;
+            ls *= f;
 #pragma unroll
-        for (int k = 0; k < 4; k++) {
-            const float fk = __builtin_amdgcn_exp2f(pm[k] - most);
-            sum = __builtin_fmaf(fk, pv[k], sum);
-            ls = __builtin_fmaf(fk, pl[k], ls);
+            for (int k = 0; k < 4; k++) {
+                const float fk = __builtin_amdgcn_exp2f(pm[k] - most);
+                sum = __builtin_fmaf(fk, pv[k], sum);
+                ls = __builtin_fmaf(fk, pl[k], ls);
+            }
         }
     }
-    lds[0][lot][ch] = m, lds[1][lot][ch] = sum, lds[2][lot][ch] = ls;
-    __syncthreads();
-    if (lot != 0) return;
-#pragma unroll
-    for (int w = 1; w < kPer; w++) {
-        const float mw = lds[0][w][ch], most = fmaxf(m, mw), f = __builtin_amdgcn_exp2f(m - most), fw = __builtin_amdgcn_exp2f(mw - most);
-        m = most;
-        sum = sum * f + lds[1][w][ch] * fw;
-        ls = ls * f + lds[2][w][ch] * fw;
+    if (lots > 1) {
+        lds[0][at_once][ch] = m, lds[1][at_once][ch] = sum, lds[2][at_once][ch] = ls;
+        __syncthreads();
+        if (lot != 0) return;
+        for (int w = at_once + 1; w < at_once + lots; w++) {
+            const float mw = lds[0][w][ch], most = fmaxf(m, mw), f = __builtin_amdgcn_exp2f(m - most), fw = __builtin_amdgcn_exp2f(mw - most);
+            m = most;
+            sum = sum * f + lds[1][w][ch] * fw;
+            ls = ls * f + lds[2][w][ch] * fw;
+        }
     }
+    if (!there) return;
     const int i = row / a.per, r = row - i * a.per;
     a.Z[((size_t)b * a.n + i) * a.ldz + (size_t)(kv * a.per + r) * a.hd + g * 32 + ch] = (_Float16)(ls == 0.0f ? 0.0f : sum / ls);
 }
@@ -1148,7 +1154,10 @@ int et_mha_kv_f16(const et_kv_cache *cache, const int32_t *table, int max_pages,
     const int sl = launch_kernel("mha_kv_kernel", p.waves == 4 ? p.form.four : p.form.eight, dim3((unsigned)cache->nkv, (unsigned)B, (unsigned)(p.blocks * p.splits)), p.waves * 64, 0, as_stream(stream),
                                  table, starts, counts, max_pages, a.units, a.splits, a.per, magic, shift, (int)d, n, a);
     if (sl != ET_OK || p.splits == 1) return sl;
-    return launch_kernel("mha_kv_join_kernel", mha_kv_join_kernel, dim3((unsigned)(a.units * p.form.rows * (cache->hd / ET_KV_GROUP)), (unsigned)p.blocks), 256, 0, as_stream(stream), a);
+    const int lots_log2 = p.splits <= 4 ? 0 : p.splits <= 8 ? 1 : p.splits <= 16 ? 2 : 3;
+    const int channels = a.units * p.form.rows * (cache->hd / ET_KV_GROUP), of_workgroup = 8 >> lots_log2;
+    return launch_kernel("mha_kv_join_kernel", mha_kv_join_kernel, dim3((unsigned)((channels + of_workgroup - 1) / of_workgroup), (unsigned)p.blocks), 256, 0, as_stream(stream), a,
+                         lots_log2);
 }
 
 }  // extern "C"

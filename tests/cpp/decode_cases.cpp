@@ -1,6 +1,6 @@
 // Generating token by token through the C++ class layer: a CachedAttention block with 4-bit
 // projections over a paged cache, driven as a server drives it (a piece of every prompt, then
-// single tokens), and the results written as .npy files for the pytest side to judge.
+// single tokens), and the results written as .npy files for the Python side to compare.
 // Usage: decode_cases <dir>
 #include <cstdio>
 #include <string>
