@@ -394,7 +394,8 @@ template <int BITS, int HD, int NW> __global__ __launch_bounds__(NW * 64, (kv_ro
     }
 }
 
-// Many rows: 16 query rows are the columns of the products, and the contraction is over one group at a time.
+// Many rows: 16 query rows are the columns of the products, and the contraction is over one group at a time (P = 1).  P = 2: 8 rows, each in two columns, one for either of a
+// pair of groups, half of each contraction's lanes with either; a row's weights are computed twice instead of, in mha_kv_kernel, four times.
 //
 // Scores: lane (c, j) needs eight channels of every group of key c, so the words of a key, loaded 16 bytes a lane, change places between the four rows of lanes (KvWords).
 // Values: the 16 columns of a product are channels of one group, whose scale is in the rows' weights.
@@ -452,12 +453,13 @@ template <int BITS> struct KvWords {
     }
 };
 
-template <int BITS, int HD, int NW> __global__ __launch_bounds__(NW * 64, (HD <= 64 ? 4 : 2)) void mha_kv_rows_kernel(KV_LEADING, const KvMhaArgs a) {
-    constexpr int ROWS = 16, G = HD / 32, TB = HD * BITS / 8, W = BITS / 4;
+template <int BITS, int HD, int NW, int P> __global__ __launch_bounds__(NW * 64, (HD <= 64 ? 4 : 2)) void mha_kv_rows_kernel(KV_LEADING, const KvMhaArgs a) {
+    constexpr int ROWS = 16 / P, G = HD / 32, SETS = G / P, PRODUCTS = 2 * P, VW = BITS == 8 ? 2 * P : 2, TB = HD * BITS / 8, W = BITS / 4;
     __shared__ float lds_vals[NW][ROWS * HD];
-    __shared__ float lds_stats[NW][2 + G][ROWS];
+    __shared__ float lds_stats[NW][2 + SETS][16];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int c = lane & 15, j = lane >> 4;
+    const int side = P == 2 ? c & 1 : 0;  // of a pair of groups
     const int kv = blockIdx.x, b = blockIdx.y, nkv = gridDim.x;
     const int block = splits == 1 ? blockIdx.z : blockIdx.z / splits, split = blockIdx.z - block * splits;
 
@@ -490,14 +492,14 @@ template <int BITS, int HD, int NW> __global__ __launch_bounds__(NW * 64, (HD <=
     const int t_end = (lim_most + 31) >> 5;
 
     h8 q[G];
-    float qsum[G];
-    const int row = row0 + min(c, rows - 1), i_row = row_of(row), r_row = row - i_row * per;
+    float qsum[SETS];
+    const int row = row0 + min(c / P, rows - 1), i_row = row_of(row), r_row = row - i_row * per;
     const int lim = limit(i_row);
     const _Float16 *qrow = a.Q + ((size_t)b * n + i_row) * a.ldq + (size_t)(kv * per + r_row) * HD;
     float top = 0.0f;
 #pragma unroll
     for (int g = 0; g < G; g++) {
-        q[g] = *reinterpret_cast<const h8 *>(qrow + g * 32 + KvWords<BITS>::of(G, g, j) * 8);
+        q[g] = *reinterpret_cast<const h8 *>(qrow + (P == 2 ? ((g & ~1) + (j & 1)) * 32 + ((j >> 1) * 2 + (g & 1)) * 8 : g * 32 + KvWords<BITS>::of(G, g, j) * 8));
 #pragma unroll
         for (int e = 0; e < 8; e++) top = fmaxf(top, fabsf((float)q[g][e]));
     }
@@ -506,28 +508,31 @@ template <int BITS, int HD, int NW> __global__ __launch_bounds__(NW * 64, (HD <=
     const float grow = __builtin_ldexpf(a.scale_log2e < 0.0f ? -1.0f : 1.0f, up);
     const float key_scale = __builtin_ldexpf(fabsf(a.scale_log2e), 24 - up);
 #pragma unroll
-    for (int g = 0; g < G; g++) {
+    for (int g = 0; g < SETS; g++) {
         float sum = 0.0f;
-        q[g] = query_order<BITS>(q[g], grow, sum);
+#pragma unroll
+        for (int i = 0; i < P; i++) q[P * g + i] = query_order<BITS>(q[P * g + i], P == 1 || (j & 1) == side ? grow : 0.0f, sum);
         qsum[g] = rows_sum(sum) * 0x1p-24f;
     }
 
-    float ref = kNothing, l = 0.0f, z[G];
-    f4 acc[G][2];
+    float ref = kNothing, l = 0.0f, z[SETS];
+    f4 acc[SETS][PRODUCTS];
 #pragma unroll
-    for (int g = 0; g < G; g++) {
+    for (int g = 0; g < SETS; g++) {
         z[g] = 0.0f;
-        acc[g][0] = acc[g][1] = f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int k = 0; k < PRODUCTS; k++) acc[g][k] = f4{0.f, 0.f, 0.f, 0.f};
     }
 
-    // units of 16 bits of a value: 8 a group with 4 bits, of which two lanes take one, codes 0 and 1 or 2 and 3; 16 with 8 bits
-    const unsigned key_at = c * TB, value_at = j * (4 * TB) + (BITS == 4 ? c & 7 : c) * 8;
-    const int code_at = BITS == 4 ? c & 8 : 0;
+    // units of 16 bits of a value: 8 a group with 4 bits, of which two lanes take one, codes 0 and 1 or 2 and 3; 16 with 8 bits; of a pair of groups one or two a lane
+    const unsigned key_at = c * TB + (P == 2 ? ((j & 1) * 4 + (j >> 1) * 2) * W * 4 : 0), value_at = j * (4 * TB) + (P == 2 ? c * (4 * VW) : (BITS == 4 ? c & 7 : c) * 8);
+    const int code_at = P == 1 && BITS == 4 ? c & 8 : 0;
     const char *k_codes = a.k_codes + (size_t)kv * a.page * TB, *v_codes = a.v_codes + (size_t)kv * a.page * TB;
     const unsigned *k_scales = a.k_scales + (size_t)kv * (G * a.page), *v_scales = a.v_scales + (size_t)kv * (G * a.page);
-    const unsigned page_bytes = (unsigned)nkv * a.page * TB, page_scales = (unsigned)nkv * G * a.page;
+    const unsigned page_bytes = (unsigned)nkv * a.page * TB, page_scales = (unsigned)nkv * G * a.page, scales_at = (unsigned)(side * a.page + 4 * j);
 
-    constexpr int kFirst = HD <= 192 ? G : 4;  // groups of the values that are asked for at once
+    constexpr bool kAtOnce = HD <= 128, kKeysAtOnce = HD <= 192;  // (the registers do not hold keys and values, or all keys, of wider heads)
+    constexpr int kFirst = kKeysAtOnce ? SETS : 3;  // groups of the values that are asked for at once
     const float zero = hidden_zero();
     for (; t < t_end; t += t_step) {
         // where the pieces lie; one that nobody sees, or without a page, is read from the place of the one before it
@@ -536,31 +541,41 @@ template <int BITS, int HD, int NW> __global__ __launch_bounds__(NW * 64, (HD <=
         const unsigned from = ok0 ? page[0] : 0, from_off = ok0 ? off[0] : 0, from1 = ok1 ? page[1] : from, off1 = ok1 ? off[1] : from_off;
         at[0] = (size_t)from * page_bytes + from_off * TB;
         at[1] = (size_t)from1 * page_bytes + off1 * TB;
-        scale_at[0] = (size_t)from * page_scales + from_off + 4 * j;
-        scale_at[1] = (size_t)from1 * page_scales + off1 + 4 * j;
-        unsigned kw[2][G * W], vw[2][G][2];
-        u4 ks[2][G], vs[2][G];
+        scale_at[0] = (size_t)from * page_scales + from_off + scales_at;
+        scale_at[1] = (size_t)from1 * page_scales + off1 + scales_at;
+        unsigned kw[2][G * W], vw[2][SETS][VW];
+        u4 ks[2][SETS], vs[2][SETS];
         auto load_keys = [&](int s) {
-            KvWords<BITS>::template load<G>(kw[s], k_codes + at[s] + key_at, j);
+            if constexpr (P == 1) {
+                KvWords<BITS>::template load<G>(kw[s], k_codes + at[s] + key_at, j);
+            } else {
 #pragma unroll
-            for (int g = 0; g < G; g++) ks[s][g] = *reinterpret_cast<const u4 *>(k_scales + scale_at[s] + (unsigned)(g * a.page));
+                for (int g = 0; g < SETS; g++) {
+                    unsigned v[2 * W];
+                    load_words<2 * W>(v, k_codes + at[s] + key_at + g * (8 * W * 4));
+#pragma unroll
+                    for (int i = 0; i < 2 * W; i++) kw[s][2 * W * g + i] = v[i];
+                }
+            }
+#pragma unroll
+            for (int g = 0; g < SETS; g++) ks[s][g] = *reinterpret_cast<const u4 *>(k_scales + scale_at[s] + (unsigned)(P * g * a.page));
         };
         load_keys(0);
-        if constexpr (HD <= 192) load_keys(1);
+        if constexpr (kKeysAtOnce) load_keys(1);
         auto load_value_scales = [&]() {
 #pragma unroll
             for (int s = 0; s < 2; s++)
 #pragma unroll
-                for (int g = 0; g < G; g++) vs[s][g] = *reinterpret_cast<const u4 *>(v_scales + scale_at[s] + (unsigned)(g * a.page));
+                for (int g = 0; g < SETS; g++) vs[s][g] = *reinterpret_cast<const u4 *>(v_scales + scale_at[s] + (unsigned)(P * g * a.page));
         };
         auto load_values = [&](int g) {
 #pragma unroll
-            for (int s = 0; s < 2; s++) load_words<2>(vw[s][g], v_codes + at[s] + value_at + g * (BITS == 4 ? 64 : 128));
+            for (int s = 0; s < 2; s++) load_words<VW>(vw[s][g], v_codes + at[s] + value_at + g * (P * (BITS == 4 ? 64 : 128)));
         };
-        if constexpr (HD <= 128) {  // (beyond, the registers do not hold keys and values at once)
+        if constexpr (kAtOnce) {
             load_value_scales();
 #pragma unroll
-            for (int g = 0; g < G; g++) load_values(g);
+            for (int g = 0; g < SETS; g++) load_values(g);
         }
         const int tile = t * 32;
         const bool whole = tile + 32 <= lim_least && ok0 && ok1;
@@ -569,23 +584,25 @@ template <int BITS, int HD, int NW> __global__ __launch_bounds__(NW * 64, (HD <=
         float y[8];
 #pragma unroll
         for (int s = 0; s < 2; s++) {
-            if constexpr (HD > 192)
+            if constexpr (!kKeysAtOnce)
                 if (s == 1) {
                     __builtin_amdgcn_sched_barrier(0);
                     load_keys(1);
                 }
-            KvWords<BITS>::template part<G>(kw[s]);
+            if constexpr (P == 1) KvWords<BITS>::template part<G>(kw[s]);
             f4 sum = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int g = 0; g < G; g++) {
-                const f4 d = __builtin_amdgcn_mfma_f32_16x16x32_f16(key_codes<BITS>(&kw[s][g * W]), q[g], f4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+            for (int g = 0; g < SETS; g++) {
+                f4 d = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int i = 0; i < P; i++) d = __builtin_amdgcn_mfma_f32_16x16x32_f16(key_codes<BITS>(&kw[s][(P * g + i) * W]), q[P * g + i], d, 0, 0, 0);
 #pragma unroll
                 for (int r = 0; r < 4; r++) sum[r] = __builtin_fmaf(low_half(ks[s][g][r]), d[r], __builtin_fmaf(high_half(ks[s][g][r]), qsum[g], sum[r]));
             }
 #pragma unroll
-            for (int r = 0; r < 4; r++) y[4 * s + r] = sum[r] * key_scale;
+            for (int r = 0; r < 4; r++) y[4 * s + r] = cols_sum<P>(sum[r]) * key_scale;
         }
-        if constexpr (HD > 128) {
+        if constexpr (!kAtOnce) {
             __builtin_amdgcn_sched_barrier(0);
             load_value_scales();
 #pragma unroll
@@ -605,14 +622,14 @@ template <int BITS, int HD, int NW> __global__ __launch_bounds__(NW * 64, (HD <=
             }
         }
 #pragma unroll
-        for (int g = 0; g < G; g++)
+        for (int g = 0; g < SETS; g++)
 #pragma unroll
             for (int e = 0; e < 8; e++) vs[e >> 2][g][e & 3] &= seen[e];
         // the largest scale: they are not negative, and their bits in the low halves of the words go up with them
         typedef unsigned short s2 __attribute__((ext_vector_type(2)));
         s2 most_s = __builtin_bit_cast(s2, vs[0][0][0]);
 #pragma unroll
-        for (int i = 1; i < 8 * G; i++) most_s = __builtin_elementwise_max(most_s, __builtin_bit_cast(s2, vs[i / (4 * G)][i / 4 % G][i & 3]));
+        for (int i = 1; i < 8 * SETS; i++) most_s = __builtin_elementwise_max(most_s, __builtin_bit_cast(s2, vs[i / (4 * SETS)][i / 4 % SETS][i & 3]));
         const float most_e = (float)__builtin_amdgcn_frexp_expf(low_half(__builtin_bit_cast(unsigned, most_s)));
         float most_y = y[0];
 #pragma unroll
@@ -627,10 +644,12 @@ template <int BITS, int HD, int NW> __global__ __launch_bounds__(NW * 64, (HD <=
 #pragma unroll
             for (int r = 0; r < 4; r++) fr[r] = __shfl(f, 4 * j + r);
 #pragma unroll
-            for (int g = 0; g < G; g++) {
+            for (int g = 0; g < SETS; g++) {
                 z[g] *= f;
 #pragma unroll
-                for (int r = 0; r < 4; r++) acc[g][0][r] *= fr[r], acc[g][1][r] *= fr[r];
+                for (int k = 0; k < PRODUCTS; k++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++) acc[g][k][r] *= fr[r];
             }
         }
         float p[8];
@@ -640,8 +659,8 @@ template <int BITS, int HD, int NW> __global__ __launch_bounds__(NW * 64, (HD <=
             l += p[e];
         }
 #pragma unroll
-        for (int g = 0; g < G; g++) {
-            if (g + kFirst < G) {
+        for (int g = 0; g < SETS; g++) {
+            if (g + kFirst < SETS) {
                 __builtin_amdgcn_sched_barrier(0);
                 load_values(g + kFirst);
             }
@@ -655,12 +674,13 @@ template <int BITS, int HD, int NW> __global__ __launch_bounds__(NW * 64, (HD <=
                 z[g] = __builtin_fmaf(p[e], high_half(sl), z[g]);
             }
 #pragma unroll
-            for (int k = 0; k < 2; k++) {
+            for (int k = 0; k < PRODUCTS; k++) {
                 unsigned x[4];
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
-                    const unsigned word = vw[i >> 1][g][i & 1] >> code_at;
-                    x[i] = BITS == 8 ? raised<8>(word, k) : (k == 0 ? word << 7 : word << 3) & 0x07800780u;
+                    if constexpr (BITS == 8) x[i] = raised<8>(vw[i >> 1][g][(k >> 1) * 2 + (i & 1)], k & 1);
+                    else if constexpr (P == 2) x[i] = raised<4>(vw[i >> 1][g][i & 1], k);
+                    else x[i] = (k == 0 ? vw[i >> 1][g][i & 1] >> code_at << 7 : vw[i >> 1][g][i & 1] >> code_at << 3) & 0x07800780u;
                 }
                 const h8 codes = as_h8(x[0], x[1], x[2], x[3]);
                 acc[g][k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w, codes, acc[g][k], 0, 0, 0);
@@ -672,33 +692,34 @@ template <int BITS, int HD, int NW> __global__ __launch_bounds__(NW * 64, (HD <=
     // what the waves have, side by side
     const float ls = rows_sum(l);
     if (j == 0) lds_stats[wave][0][c] = ref, lds_stats[wave][1][c] = ls;
-    constexpr float unit = BITS == 8 ? code_unit<8>(0) : 0x1p17f;
 #pragma unroll
-    for (int g = 0; g < G; g++) {
+    for (int g = 0; g < SETS; g++) {
         const float zs = rows_sum(z[g]);
         if (j == 0) lds_stats[wave][2 + g][c] = zs;
-        const int ch = g * 32 + (BITS == 4 ? 4 * (c & 7) + 2 * (c >> 3) : 2 * c);
+        const int ch = P == 2 ? g * 64 + 4 * c : g * 32 + (BITS == 4 ? 4 * (c & 7) + 2 * (c >> 3) : 2 * c);
 #pragma unroll
         for (int r = 0; r < 4; r++)
-            *reinterpret_cast<float2 *>(&lds_vals[wave][(4 * j + r) * HD + ch]) = float2{acc[g][0][r] * unit, acc[g][1][r] * unit};
+#pragma unroll
+            for (int k = 0; k < PRODUCTS; k++)
+                if (P == 1 || (r & 1) == c >> 3) lds_vals[wave][(4 * j + r) / P * HD + ch + k] = acc[g][k][r] * (P == 1 && BITS == 4 ? 0x1p17f : code_unit<BITS>(k));
     }
     __syncthreads();
     float *part = splits > 1 ? a.parts + ((size_t)blockIdx.z * units + (unsigned)(b * nkv + kv)) * (32 + ROWS * HD) : nullptr;
     for (int e = threadIdx.x; e < rows * HD; e += NW * 64) {
-        const int h = e / HD, ch = e - h * HD, g = ch >> 5;
-        float m = lds_stats[0][0][h];
+        const int h = e / HD, ch = e - h * HD, g = ch >> 5, col = h * P + g % P;
+        float m = lds_stats[0][0][col];
 #pragma unroll
-        for (int w = 1; w < NW; w++) m = fmaxf(m, lds_stats[w][0][h]);
+        for (int w = 1; w < NW; w++) m = fmaxf(m, lds_stats[w][0][col]);
         float sum = 0.0f, ls = 0.0f;
 #pragma unroll
         for (int w = 0; w < NW; w++) {
-            const float f = __builtin_amdgcn_exp2f(lds_stats[w][0][h] - m);
-            sum = __builtin_fmaf(f, lds_vals[w][e] + lds_stats[w][2 + g][h], sum);
-            ls = __builtin_fmaf(f, lds_stats[w][1][h], ls);
+            const float f = __builtin_amdgcn_exp2f(lds_stats[w][0][col] - m);
+            sum = __builtin_fmaf(f, lds_vals[w][e] + lds_stats[w][2 + g / P][col], sum);
+            ls = __builtin_fmaf(f, lds_stats[w][1][col], ls);
         }
         if (part) {
             part[32 + e] = sum;
-            if (ch == 0) part[2 * h] = m, part[2 * h + 1] = ls;
+            if (g < P && (ch & 31) == 0) part[2 * col] = m, part[2 * col + 1] = ls;
         } else {
             const int row = row0 + h, i = row_of(row), r = row - i * per;
             a.Z[((size_t)b * n + i) * a.ldz + (size_t)(kv * per + r) * HD + ch] = (_Float16)(ls == 0.0f ? 0.0f : sum / ls);
@@ -982,7 +1003,7 @@ __global__ __launch_bounds__(256) void mha_kv_join_kernel(const KvMhaArgs a, int
     if (there) {
         const float *part = a.parts + ((size_t)block * a.splits * a.units + unit) * part_floats;
         const size_t next = (size_t)a.units * part_floats;
-        const int col = a.cols == 1 ? h : h * a.cols + g, at = 32 + h * a.hd + g * 32 + ch;
+        const int col = h * a.cols + (g & (a.cols - 1)), at = 32 + h * a.hd + g * 32 + ch;
         for (int s0 = lot; s0 < a.splits; s0 += 4 * lots) {  // four parts asked for at once
             float pm[4], pl[4], pv[4];
 #pragma unroll
@@ -1032,29 +1053,33 @@ struct KvForm {
     bool eight_if_whole;   // eight only where one workgroup has all the keys
 };
 
-// Rows: of a key/value head in the call.  Blocks of 16 / kCols rows or of 16, measured in us with 16 sequences of 4096 tokens, 8 heads (of 128: 8 rows 34.3 | 37.7, 9 rows
-// 50.4 | 40.4, 16 rows 82 | 46; of 64, 10 rows 27.3 | 24.6, 8 rows 22.5 | 26.9) and 4 sequences (of 192: 5 rows 32.3 | 22.0; of 256: 6 rows 34.7 | 27.2, 32 rows 91 | 45).
-template <int BITS, int HD> KvForm form_of(long long rows) {
+// Rows: of a key/value head in the call.  fills: one block of rows for each (sequence, key/value head) is enough work for the chip, there being many, or keys to share out.
+// Blocks of 16 / kCols rows or of 16, measured in us with 16 sequences of 4096 tokens, 8 heads (of 128: 8 rows 34.3 | 37.7, 9 rows
+// 50.4 | 40.4, 16 rows 82 | 46; of 64, 10 rows 27.3 | 24.6, 8 rows 22.5 | 26.9) and 4 sequences (of 192: 5 rows 32.3 | 22.0; of 256: 6 rows 34.7 | 27.2, 32 rows 91 | 45).  Heads of 128, 5 to 8 rows, blocks of 4 and of 8 over pairs of groups: 8 rows 32.7 | 27.8 (8 bits 45.4 | 30.6), one sequence of
+// 100000 47.6 | 38.7, but 16 sequences of 1500, 7 rows, 15.1 | 18.1.  Wider heads: pairs are no better than 16 rows.
+template <int BITS, int HD> KvForm form_of(long long rows, bool fills) {
     if constexpr (HD <= 128) {
         constexpr int cols = KvShape<BITS, HD>::kCols, heads = 4 / cols;
         if (rows == 1) return {mha_kv_few_kernel<BITS, HD, 1, 4>, mha_kv_few_kernel<BITS, HD, 1, 8>, 1, cols, 64, false};
         if (rows <= heads) return {mha_kv_few_kernel<BITS, HD, heads, 4>, mha_kv_few_kernel<BITS, HD, heads, 8>, heads, cols, 64, false};
     }
     if constexpr (HD > 32)
-        if (rows > (HD <= 128 ? 8 : 4)) return {mha_kv_rows_kernel<BITS, HD, 4>, mha_kv_rows_kernel<BITS, HD, HD <= 128 ? 8 : 4>, 16, 1, 32, HD > 64};
+        if (rows > (HD <= 128 ? 8 : 4)) return {mha_kv_rows_kernel<BITS, HD, 4, 1>, mha_kv_rows_kernel<BITS, HD, HD <= 128 ? 8 : 4, 1>, 16, 1, 32, HD > 64};
+    if constexpr (HD == 128)
+        if (rows > 4 && fills) return {mha_kv_rows_kernel<BITS, HD, 4, 2>, mha_kv_rows_kernel<BITS, HD, 8, 2>, 8, 2, 32, false};
     return {mha_kv_kernel<BITS, HD, 4>, mha_kv_kernel<BITS, HD, 8>, KvShape<BITS, HD>::kRows, KvShape<BITS, HD>::kCols, 32, false};
 }
 
-template <int BITS> KvForm form_of(int hd, long long rows) {
+template <int BITS> KvForm form_of(int hd, long long rows, bool fills) {
     switch (hd) {
-        case 32: return form_of<BITS, 32>(rows);
-        case 64: return form_of<BITS, 64>(rows);
-        case 96: return form_of<BITS, 96>(rows);
-        case 128: return form_of<BITS, 128>(rows);
-        case 160: return form_of<BITS, 160>(rows);
-        case 192: return form_of<BITS, 192>(rows);
-        case 224: return form_of<BITS, 224>(rows);
-        default: return form_of<BITS, 256>(rows);
+        case 32: return form_of<BITS, 32>(rows, fills);
+        case 64: return form_of<BITS, 64>(rows, fills);
+        case 96: return form_of<BITS, 96>(rows, fills);
+        case 128: return form_of<BITS, 128>(rows, fills);
+        case 160: return form_of<BITS, 160>(rows, fills);
+        case 192: return form_of<BITS, 192>(rows, fills);
+        case 224: return form_of<BITS, 224>(rows, fills);
+        default: return form_of<BITS, 256>(rows, fills);
     }
 }
 
@@ -1072,8 +1097,10 @@ int kv_plan(const char *fn, KvPlan &p, const et_kv_cache *c, int max_pages, int 
     ET_REQUIRE(nh > 0 && nh % c->nkv == 0, ET_ERR_INVALID_ARG, "%s: nh=%d must be a multiple of nkv=%d", fn, nh, c->nkv);
     const int per = nh / c->nkv;
     const long long rows = (long long)n * per;
-    p.form = c->bits == 4 ? form_of<4>(c->hd, rows) : form_of<8>(c->hd, rows);
-    const long long blocks = (rows + p.form.rows - 1) / p.form.rows, units = (long long)B * c->nkv;
+    const long long units = (long long)B * c->nkv;
+    const bool fills = units >= 256 || (long long)max_pages * c->page >= 2048;
+    p.form = c->bits == 4 ? form_of<4>(c->hd, rows, fills) : form_of<8>(c->hd, rows, fills);
+    const long long blocks = (rows + p.form.rows - 1) / p.form.rows;
     ET_REQUIRE(rows <= 0x7fffffffLL && B <= 65535 && blocks <= 65535 && units * blocks <= (1LL << 24), ET_ERR_UNSUPPORTED, "%s: B=%d n=%d nh=%d", fn, B, n, nh);
     p.blocks = (int)blocks;
     const long long tiles = ((long long)max_pages * c->page + p.form.tile - 1) / p.form.tile, groups = units * blocks;

@@ -86,7 +86,7 @@ def test_the_largest_sizes(et):
 
 def test_workspace_does_not_grow_with_fewer_pages(et):
     """A call with fewer pages than the workspace was made for fits."""
-    for nkv, hd, bits, B, n, nh in ((1, 64, 4, 1, 1, 1), (8, 128, 4, 1, 1, 32), (8, 96, 8, 3, 7, 8), (16, 64, 4, 40, 1, 16), (2, 256, 8, 2, 40, 16)):
+    for nkv, hd, bits, B, n, nh in ((1, 64, 4, 1, 1, 1), (8, 128, 4, 1, 1, 32), (8, 96, 8, 3, 7, 8), (16, 64, 4, 40, 1, 16), (2, 256, 8, 2, 40, 16), (8, 128, 4, 2, 1, 64), (8, 128, 8, 33, 7, 8)):
         c = cache(et, nkv=nkv, hd=hd, bits=bits, npages=1 << 14)
         need = [et.mha_kv_workspace(c, pages, B, n, nh) for pages in range(1, 9000, 37)]
         assert need == sorted(need)

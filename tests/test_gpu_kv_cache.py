@@ -230,6 +230,27 @@ def test_attention_long_of_many_rows(et, bits, hd):
     check_attention(et, bits, 1, 7, hd, 48, [4000, 9], 3, True, seed=15)
 
 
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("lengths,nkv,per,n", [([2100, 40], 3, 8, 1), ([2049, 9], 1, 1, 7), ([40] * 86, 3, 5, 1), ([33] * 64, 4, 2, 3), ([5000], 1, 3, 2)])
+def test_attention_five_to_eight_rows(et, bits, lengths, nkv, per, n):
+    """Heads of 128: blocks of 8 rows where there are many heads, or long sequences."""
+    check_attention(et, bits, nkv, per, 128, 64, lengths, n, True, seed=21)
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+def test_attention_not_a_number_of_a_later_token_in_blocks_of_eight(et, bits):
+    lengths, n, nkv = [2060, 30], 5, 2
+    table = tables(1, 2, 33, 66)
+    host = filled(bits, nkv, 128, 64, table, lengths, 4, 66)
+    starts = [l - n for l in lengths]
+    Q = Hn.randn((2 * n, nkv * 128), 5)
+    want = run_attention(et, DeviceCache(et, host), table, starts, None, Q, 2, n, nkv, 0.125, True).reshape(2, n, -1)
+    row = np.full((2, nkv * 128), np.nan, np.float16)
+    host.write(table, [l - 1 for l in lengths], [1] * 2, np.ones_like(row), row, 1)
+    got = run_attention(et, DeviceCache(et, host), table, starts, None, Q, 2, n, nkv, 0.125, True).reshape(2, n, -1)
+    assert np.array_equal(got[:, :-1], want[:, :-1]) and np.isnan(got[:, -1]).all()
+
+
 @pytest.mark.parametrize("qscale", [2.0 ** -13, 30.0])
 def test_attention_of_very_even_and_very_uneven_probabilities(et, qscale):
     check_attention(et, 4, 2, 2, 64, 16, [300, 81], 1, False, seed=9, qscale=qscale)
