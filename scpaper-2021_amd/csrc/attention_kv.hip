@@ -184,6 +184,9 @@ template <int BITS, int HD> __device__ __forceinline__ void load_value(unsigned 
 //
 // Scores: keys are the rows of the products, so a lane ends with keys 4 j .. 4 j + 3 of both pieces for its column, and these are the very keys that it weighs as a row of the
 // products with the values: nothing moves between lanes but the sum of a row's groups, and a maximum when the reference moves.
+//
+// One sequence of 131071 tokens, 32 heads over 8 of 128: 36.4 us, 4.6 TB/s, and 5 us to join 64 parts.  16 sequences of 1500, 8 heads of 96, 7 rows, 8 bits: 15 us, bound by 236
+// vector instructions a tile on two waves a SIMD (a tile ahead in registers: 16.3, and 43 us in the first).
 template <int BITS, int HD> constexpr int kv_rows_waves() { return HD == 32 ? 6 : HD == 64 ? (BITS == 4 ? 6 : 5) : HD <= 128 ? 4 : 2; }
 
 template <int BITS, int HD, int NW> __global__ __launch_bounds__(NW * 64, (kv_rows_waves<BITS, HD>())) void mha_kv_kernel(KV_LEADING, const KvMhaArgs a) {
@@ -731,6 +734,8 @@ template <int BITS, int HD, int NW, int P> __global__ __launch_bounds__(NW * 64,
 //
 // Scores: rows of the products are the groups of the query rows, four times over, columns 16 keys; a lane keeps those of piece lane / 16 of the tile.  Group by group
 // they are scaled and added in the lane.  The weights go through 1 KB of LDS (one wave's own, no barrier) to become the rows of the products with the values.
+//
+// Bound by memory: 64 sequences of 4096 tokens, 16 heads of 64, 4 bits 49.5 us, 5.1 TB/s (64.6 in tiles of 32 keys, whose softmax every group of a row repeats).
 template <int BITS, int HD, int R> struct KvFew {
     static constexpr int kCols = KvShape<BITS, HD>::kCols;  // 1, 2 or 4 groups of a head
     static constexpr int kLdsRow = 72;                      // halfs: 64 keys, and 16 bytes on to other banks
