@@ -341,14 +341,14 @@ def test_attention_takes_large_offsets(et):
     assert (np.abs(got - Z) <= allowed(Z, stepped, lows, reach, hd, n)).all()
 
 
-def test_attention_in_a_graph(et):
+@pytest.mark.parametrize("max_pages", [50, 300])  # (300: keys are shared out, and the parts joined)
+def test_attention_in_a_graph(et, max_pages):
     """A decoding step, written and attended, recorded once and replayed with the position on the device moving on between replays: every
     replay equals the eager calls on a second cache."""
     lib = et.lib()
     nkv, hd, page, B = 2, 64, 16, 3
     nh, width = 4, 128
     first = [30, 700, 15]
-    max_pages = 50
     table = tables(3, B, max_pages, B * max_pages)
     host = filled(4, nkv, hd, page, table, first, 1, B * max_pages)
     dev, dev2 = DeviceCache(et, host), DeviceCache(et, host)
@@ -383,6 +383,32 @@ def test_attention_in_a_graph(et):
         assert np.array_equal(dev.bufs[k].numpy().view(np.uint8), dev2.bufs[k].numpy().view(np.uint8))
     et.check(lib.et_graph_destroy(graph))
     et.check(lib.et_stream_destroy(stream))
+
+
+def test_attention_on_two_streams_at_once(et):
+    """Two batches over one cache, keys shared out over workgroups, each with its stream and workspace: what each gives alone."""
+    lib = et.lib()
+    table = tables(2, 2, 300, 600)
+    host = filled(4, 2, 64, 16, table, [4600, 900], 7, 600)
+    dev, dt, ds = DeviceCache(et, host), up(et, table), up(et, np.array([4599, 899], np.int32))
+    Q = [Hn.randn((2, 256), 5), Hn.randn((2, 256), 6)]
+    want = [run_attention(et, dev, table, [4599, 899], None, q, 2, 1, 4, 0.125, False) for q in Q]
+    need = et.mha_kv_workspace(dev.c, 300, 2, 1, 4)
+    assert need > 0
+    streams, q, z, ws = [], [up(et, x) for x in Q], [], []
+    for _ in Q:
+        s = C.c_void_p()
+        et.check(lib.et_stream_create(C.byref(s)))
+        streams.append(s)
+        z.append(up(et, np.zeros((20, 2, 256), np.float16)))
+        ws.append(up(et, np.full(need, 0xFF, np.uint8)))
+    for i in range(20):
+        for k, s in enumerate(streams):
+            et.mha_kv(dev.c, dt, 300, ds, None, q[k], 256, z[k].offset(i * 2 * 256 * 2), 256, 2, 1, 4, 0.125, 0, ws[k], need, s)
+    for k, s in enumerate(streams):
+        et.check(lib.et_stream_sync(s))
+        assert (z[k].numpy() == want[k]).all()
+        et.check(lib.et_stream_destroy(s))
 
 
 def test_attention_gives_the_same_bits_again(et):
