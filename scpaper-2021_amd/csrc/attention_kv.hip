@@ -1103,7 +1103,8 @@ int kv_plan(const char *fn, KvPlan &p, const et_kv_cache *c, int max_pages, int 
     const int per = nh / c->nkv;
     const long long rows = (long long)n * per;
     const long long units = (long long)B * c->nkv;
-    const bool fills = units >= 256 || (long long)max_pages * c->page >= 2048;
+    // (in tiles, which the shares below count too: were the two rounded differently, the form of fewer rows a block could need more for the last pages under the border)
+    const bool fills = units >= 256 || ((long long)max_pages * c->page + 31) / 32 >= 64;
     p.form = c->bits == 4 ? form_of<4>(c->hd, rows, fills) : form_of<8>(c->hd, rows, fills);
     const long long blocks = (rows + p.form.rows - 1) / p.form.rows;
     ET_REQUIRE(rows <= 0x7fffffffLL && B <= 65535 && blocks <= 65535 && units * blocks <= (1LL << 24), ET_ERR_UNSUPPORTED, "%s: B=%d n=%d nh=%d", fn, B, n, nh);

@@ -92,6 +92,17 @@ def test_workspace_does_not_grow_with_fewer_pages(et):
         assert need == sorted(need)
 
 
+@pytest.mark.parametrize("page", [16, 48, 64])
+@pytest.mark.parametrize("nkv,per,B,n", [(8, 8, 4, 1), (1, 1, 1, 7), (2, 5, 3, 1), (3, 3, 2, 2), (4, 7, 63, 1), (8, 4, 4, 1), (2, 9, 1, 1)])
+@pytest.mark.parametrize("hd", [64, 96, 128, 256])
+def test_workspace_grows_with_every_page(et, hd, nkv, per, B, n, page):
+    """Also by one page at a time around the sizes at which another kernel is chosen."""
+    for bits in (4, 8):
+        c = cache(et, nkv=nkv, hd=hd, bits=bits, page=page, npages=1 << 14)
+        need = [et.mha_kv_workspace(c, pages, B, n, nkv * per) for pages in range(1, 6400 // page)]
+        assert need == sorted(need), [i + 1 for i in range(len(need) - 1) if need[i] > need[i + 1]]
+
+
 def test_workspace_is_asked_for(et):
     """One sequence of a million tokens on one head is shared out: what the parts leave needs memory, and a call without it is refused."""
     c = cache(et, nkv=1, npages=1 << 16)
