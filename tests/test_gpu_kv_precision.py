@@ -1,0 +1,61 @@
+"""How near et_mha_kv_f16 is to binary64 by the 2-norm, in every kernel that it may run: the roundings of single weights, which a
+bound for each value has to grant one by one, show here where they add up."""
+import math
+
+import numpy as np
+import pytest
+
+from oracle import decode as D
+from tests.test_gpu_kv_cache import DeviceCache, run_attention, tables
+
+pytestmark = pytest.mark.gpu
+
+# A result is rounded to binary16 once: off by at most half a step, 2^-11 of it at the lower end of a binade and less above, evenly
+# spread, which is 2^-11 / sqrt(3) = 2.82e-4 of the 2-norm at most.  The rest is for what is kept in more bits: weights in two binary16 numbers (2^-22; values that
+# cancel in a sum of 5000 make 3e-5 of that if all of them err to one side), binary32 sums and scores.
+NEAR = 3e-4
+
+# (hd, key/value heads, query heads to each, rows, lengths): a key a lane (1, 2 and 4 rows), blocks of 16 / groups, of 16, of 8 over pairs of groups; keys of one
+# workgroup and keys shared out.
+FORMS = [(32, 4, 1, 1, [300, 290]), (64, 4, 1, 1, [300, 290]), (96, 4, 1, 1, [300, 290]), (128, 4, 1, 1, [300, 290]), (64, 4, 2, 1, [300, 290]), (32, 4, 4, 1, [300, 290]),
+         (64, 4, 4, 1, [300, 290]), (128, 2, 4, 1, [300, 290]), (160, 2, 4, 1, [300, 290]), (256, 2, 2, 1, [300, 290]), (64, 2, 5, 2, [300, 290]), (96, 2, 16, 1, [300, 290]),
+         (128, 2, 3, 4, [300, 290]), (192, 2, 8, 1, [300, 290]), (224, 2, 5, 1, [300, 290]), (256, 2, 8, 1, [300, 290]), (128, 2, 8, 1, [2100, 700]), (64, 2, 1, 1, [5000, 4000]),
+         (128, 1, 4, 1, [5000]), (128, 1, 8, 1, [5000]), (128, 1, 16, 1, [5000])]
+
+
+def rows_of(form, seed, values=lambda r, tokens, width: r.standard_normal((tokens, width)) * 0.5):
+    """Keys, values and queries of a form, and where its rows stand."""
+    hd, nkv, per, n, lengths = form
+    r = np.random.default_rng(seed)
+    tokens, width = len(lengths) * max(lengths), nkv * hd
+    K = (r.standard_normal((tokens, width)) + 1.5 * r.standard_normal(width)).astype(np.float16)
+    V = values(r, tokens, width).astype(np.float16)
+    Q = r.standard_normal((len(lengths) * n, nkv * per * hd))
+    return K, V, Q, [l - n for l in lengths], [n] * len(lengths)
+
+
+def attended(et, bits, form, seed, qscale=1.0, **kw):
+    """(result, the same in binary64), [rows][heads][hd]."""
+    hd, nkv, per, n, lengths = form
+    K, V, Q, starts, counts = rows_of(form, seed, **kw)
+    Q = (Q * qscale).astype(np.float16)
+    B, page = len(lengths), 64
+    max_pages = -(-max(lengths) // page)
+    table = tables(seed, B, max_pages, B * max_pages)
+    host = D.Cache(bits, nkv, hd, page, B * max_pages, fill=0xFF)
+    host.write(table, [0] * B, lengths, K, V, max(lengths))
+    nh = nkv * per
+    got = run_attention(et, DeviceCache(et, host), table, starts, counts, Q, B, n, nh, 1 / math.sqrt(hd), True)
+    Z = D.attention(host, table, starts, counts, Q, n, nh, 1 / math.sqrt(hd), True)[0]
+    return got.astype(np.float64).reshape(-1, nh, hd), Z.reshape(-1, nh, hd)
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("qscale", [1.0, 2.0 ** -13])
+@pytest.mark.parametrize("form", FORMS, ids=str)
+def test_attention_is_as_near_as_its_result_is_rounded(et, bits, form, qscale):
+    """With even probabilities (queries of 2^-13) equal weights are rounded alike and add up: with one binary16 number a weight this is 4e-4 to 9e-4
+    (tests/test_decode_precision.py)."""
+    got, Z = attended(et, bits, form, 11, qscale)
+    e = np.linalg.norm(got - Z) / np.linalg.norm(Z)
+    assert e <= NEAR, e
