@@ -89,6 +89,12 @@ template <int BITS> __device__ __forceinline__ unsigned raised(unsigned w, int k
     return k == 0 ? (w << 3) & 0x00780078u : k == 1 ? (w >> 1) & 0x00780078u : k == 2 ? (w >> 1) & 0x07800780u : (w >> 5) & 0x07800780u;
 }
 
+// A row's result: zero where it sees nothing; at most binary16's largest number, since it is the rounding up of a group's scale alone that can carry it beyond (as in step_value).
+__device__ __forceinline__ _Float16 result_value(float sum, float l) {
+    const float v = l == 0.0f ? 0.0f : sum / l;
+    return (_Float16)(v > 65504.0f ? 65504.0f : v);  // (a NaN passes)
+}
+
 // Sum over the kCols neighbouring lanes of a query row.
 template <int COLS> __device__ __forceinline__ float cols_sum(float v) {
     if constexpr (COLS >= 2) v += dpp_move<kDppQuadXor1>(v);
@@ -392,7 +398,7 @@ template <int BITS, int HD, int NW> __global__ __launch_bounds__(NW * 64, (kv_ro
             if ((ch & 31) == 0) part[2 * col] = m, part[2 * col + 1] = ls;
         } else {
             const int row = row0 + h, i = row_of(row), r = row - i * per;
-            a.Z[((size_t)b * n + i) * a.ldz + (size_t)(kv * per + r) * HD + ch] = (_Float16)(ls == 0.0f ? 0.0f : sum / ls);
+            a.Z[((size_t)b * n + i) * a.ldz + (size_t)(kv * per + r) * HD + ch] = result_value(sum, ls);
         }
     }
 }
@@ -725,7 +731,7 @@ template <int BITS, int HD, int NW, int P> __global__ __launch_bounds__(NW * 64,
             if (g < P && (ch & 31) == 0) part[2 * col] = m, part[2 * col + 1] = ls;
         } else {
             const int row = row0 + h, i = row_of(row), r = row - i * per;
-            a.Z[((size_t)b * n + i) * a.ldz + (size_t)(kv * per + r) * HD + ch] = (_Float16)(ls == 0.0f ? 0.0f : sum / ls);
+            a.Z[((size_t)b * n + i) * a.ldz + (size_t)(kv * per + r) * HD + ch] = result_value(sum, ls);
         }
     }
 }
@@ -986,7 +992,7 @@ template <int BITS, int HD, int R, int NW> __global__ __launch_bounds__(NW * 64,
             if ((ch & 31) == 0) part[2 * (h * GP + (ch >> 5))] = m, part[2 * (h * GP + (ch >> 5)) + 1] = ls;
         } else {
             const int row = row0 + h, i = row_of(row), r = row - i * per;
-            a.Z[((size_t)b * n + i) * a.ldz + (size_t)(kv * per + r) * HD + ch] = (_Float16)(ls == 0.0f ? 0.0f : sum / ls);
+            a.Z[((size_t)b * n + i) * a.ldz + (size_t)(kv * per + r) * HD + ch] = result_value(sum, ls);
         }
     }
 }
@@ -1045,7 +1051,7 @@ __global__ __launch_bounds__(256) void mha_kv_join_kernel(const KvMhaArgs a, int
     }
     if (!there) return;
     const int i = row / a.per, r = row - i * a.per;
-    a.Z[((size_t)b * a.n + i) * a.ldz + (size_t)(kv * a.per + r) * a.hd + g * 32 + ch] = (_Float16)(ls == 0.0f ? 0.0f : sum / ls);
+    a.Z[((size_t)b * a.n + i) * a.ldz + (size_t)(kv * a.per + r) * a.hd + g * 32 + ch] = result_value(sum, ls);
 }
 
 namespace {

@@ -59,3 +59,15 @@ def test_attention_is_as_near_as_its_result_is_rounded(et, bits, form, qscale):
     got, Z = attended(et, bits, form, 11, qscale)
     e = np.linalg.norm(got - Z) / np.linalg.norm(Z)
     assert e <= NEAR, e
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("form", FORMS, ids=str)
+def test_values_at_the_end_of_the_range(et, bits, form):
+    """A group from -65504 to 65504 gets a scale whose last steps lie beyond: what is read back is the largest number, and so is what attention gives."""
+    def values(r, tokens, width):
+        return np.tile(np.where(np.arange(width) % 3, 65504.0, -65504.0), (tokens, 1))
+    got, Z = attended(et, bits, form, 13, values=values)
+    assert np.abs(Z).max() > 65520
+    want = np.clip(Z, -65504, 65504)
+    assert np.isfinite(got).all() and (np.abs(got - want) <= 2.0 ** -10 * np.abs(want)).all()
