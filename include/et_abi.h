@@ -717,7 +717,8 @@ int et_kv_read_f16(const et_kv_cache *cache, const int32_t *table, int max_pages
  * multiple of nkv.  Q and Z [B*n x nh*hd] (row strides multiples of 8, 16-byte
  * aligned).  A row that sees nothing becomes zero; a result that rounding a
  * scale up carries beyond binary16's largest number becomes that number, as in
- * et_kv_read_f16.  What lies in the cache
+ * et_kv_read_f16.  A NaN or an infinity in a head's row of Q makes its result
+ * NaN, if it sees anything.  What lies in the cache
  * behind a sequence's end may be anything, NaN included.  n = 1 is a decoding
  * step, n > 1 several tokens at once (a piece of a prompt, guessed tokens).
  * The codes enter the matrix products as they are; scores, softmax and sums are

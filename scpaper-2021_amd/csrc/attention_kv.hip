@@ -127,6 +127,12 @@ template <int BITS> __device__ __forceinline__ h8 query_order(h8 x, float grow, 
         return h8{(_Float16)f[0], (_Float16)f[2], (_Float16)f[1], (_Float16)f[3], (_Float16)f[4], (_Float16)f[6], (_Float16)f[5], (_Float16)f[7]};
 }
 
+// What a row of Q is multiplied by.  Scores of a row with an infinity are infinite of either sign or NaN, and have no softmax: it becomes NaN here, or the weights of
+// scores that are all minus infinity would add up to nothing, as where a row sees no key.
+__device__ __forceinline__ float query_growth(float top, int up, float scale) {
+    return top <= 65504.0f ? __builtin_ldexpf(scale < 0.0f ? -1.0f : 1.0f, up) : __builtin_nanf("");
+}
+
 // p * scale as two binary16 numbers: rounded to one, whose error is relative to a value's height above the group's lowest, results were 2 to 3 times as far off as their own
 // rounding (5.9e-4 against 2.1e-4, 2-norm, 131071 keys of random values).  With a zero that the compiler does not know each is one instruction, which widens, multiplies,
 // adds and rounds.
@@ -252,7 +258,7 @@ template <int BITS, int HD, int NW> __global__ __launch_bounds__(NW * 64, (kv_ro
     }
     top = rows_max(top);
     const int up = top > 0.0f ? 15 - __builtin_amdgcn_frexp_expf(top) : 0;
-    const float grow = __builtin_ldexpf(a.scale_log2e < 0.0f ? -1.0f : 1.0f, up);
+    const float grow = query_growth(top, up, a.scale_log2e);
     const float key_scale = __builtin_ldexpf(fabsf(a.scale_log2e), 24 - up);
 #pragma unroll
     for (int i = 0; i < S::kPieces; i++) q[i] = query_order<BITS>(q[i], (j * (HD / 4) + 8 * i) / 32 == gg ? grow : 0.0f, sum);
@@ -514,7 +520,7 @@ template <int BITS, int HD, int NW, int P> __global__ __launch_bounds__(NW * 64,
     }
     top = rows_max(top);
     const int up = top > 0.0f ? 15 - __builtin_amdgcn_frexp_expf(top) : 0;
-    const float grow = __builtin_ldexpf(a.scale_log2e < 0.0f ? -1.0f : 1.0f, up);
+    const float grow = query_growth(top, up, a.scale_log2e);
     const float key_scale = __builtin_ldexpf(fabsf(a.scale_log2e), 24 - up);
 #pragma unroll
     for (int g = 0; g < SETS; g++) {
@@ -816,7 +822,7 @@ template <int BITS, int HD, int R, int NW> __global__ __launch_bounds__(NW * 64,
         }
         top = rows_max(top);
         const int up = top > 0.0f ? 15 - __builtin_amdgcn_frexp_expf(top) : 0;
-        const float grow = __builtin_ldexpf(a.scale_log2e < 0.0f ? -1.0f : 1.0f, up);
+        const float grow = query_growth(top, up, a.scale_log2e);
         const float back = __builtin_ldexpf(fabsf(a.scale_log2e), 24 - up);
         float sum = 0.0f;
 #pragma unroll

@@ -71,3 +71,43 @@ def test_values_at_the_end_of_the_range(et, bits, form):
     assert np.abs(Z).max() > 65520
     want = np.clip(Z, -65504, 65504)
     assert np.isfinite(got).all() and (np.abs(got - want) <= 2.0 ** -10 * np.abs(want)).all()
+
+
+@pytest.mark.parametrize("form", FORMS, ids=str)
+@pytest.mark.parametrize("bad", [np.inf, -np.inf, np.nan])
+def test_infinite_queries_make_their_row_not_a_number(et, form, bad):
+    """Scores of plus or minus infinity have no softmax, whatever the keys' signs; other rows and heads are what they are without them."""
+    hd, nkv, per, n, lengths = form
+    K, V, Q, starts, counts = rows_of(form, 14)
+    B, nh = len(lengths), nkv * per
+    max_pages = -(-max(lengths) // 64)
+    table = tables(14, B, max_pages, B * max_pages)
+    Q = Q.astype(np.float16)
+    host = D.Cache(4, nkv, hd, 64, B * max_pages, fill=0xFF)
+    host.write(table, [0] * B, lengths, np.abs(K) + np.float16(1), V, max(lengths))
+    dev = DeviceCache(et, host)
+    want = run_attention(et, dev, table, starts, counts, Q, B, n, nh, 0.1, True).reshape(-1, nh, hd)
+    Q[0, 5] = bad
+    got = run_attention(et, dev, table, starts, counts, Q, B, n, nh, 0.1, True).reshape(-1, nh, hd)
+    assert np.isnan(got[0, 0]).all()
+    got[0, 0] = want[0, 0]
+    assert np.array_equal(got, want)
+
+
+@pytest.mark.parametrize("form", FORMS, ids=str)
+@pytest.mark.parametrize("bad", [np.inf, -np.inf])
+def test_infinite_queries_over_keys_of_one_sign(et, form, bad):
+    """Every score is plus infinity, or every score is minus infinity: no key's code is 0 where the query is infinite."""
+    hd, nkv, per, n, _ = form
+    form = (hd, nkv, per, n, [5, 4])
+    K, V, Q, starts, counts = rows_of(form, 16)
+    nh = nkv * per
+    K = np.abs(K) + np.float16(1)
+    K[:, 5::hd] = 12
+    table = np.array([[1], [0]], np.int32)
+    host = D.Cache(4, nkv, hd, 64, 2, fill=0xFF)
+    host.write(table, [0, 0], [5, 4], K, V, 5)
+    Q = Q.astype(np.float16)
+    Q[0, 5] = bad
+    got = run_attention(et, DeviceCache(et, host), table, starts, counts, Q, 2, n, nh, 0.1, True).reshape(-1, nh, hd)
+    assert np.isnan(got[0, 0]).all() and np.isnan(got).sum() == hd
