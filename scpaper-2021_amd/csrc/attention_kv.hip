@@ -642,9 +642,10 @@ template <int BITS, int HD, int NW, int P> __global__ __launch_bounds__(NW * 64,
             for (int e = 0; e < 8; e++) vs[e >> 2][g][e & 3] &= seen[e];
         // the largest scale: they are not negative, and their bits in the low halves of the words go up with them
         typedef unsigned short s2 __attribute__((ext_vector_type(2)));
-        s2 most_s = __builtin_bit_cast(s2, vs[0][0][0]);
+        auto halves = [](unsigned w) { return __builtin_bit_cast(s2, w); };  // (of an element of a vector, __builtin_bit_cast takes the vector's first)
+        s2 most_s = halves(vs[0][0][0]);
 #pragma unroll
-        for (int i = 1; i < 8 * SETS; i++) most_s = __builtin_elementwise_max(most_s, __builtin_bit_cast(s2, vs[i / (4 * SETS)][i / 4 % SETS][i & 3]));
+        for (int i = 1; i < 8 * SETS; i++) most_s = __builtin_elementwise_max(most_s, halves(vs[i / (4 * SETS)][i / 4 % SETS][i & 3]));
         const float most_e = (float)__builtin_amdgcn_frexp_expf(low_half(__builtin_bit_cast(unsigned, most_s)));
         float most_y = y[0];
 #pragma unroll

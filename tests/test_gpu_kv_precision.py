@@ -62,6 +62,17 @@ def test_attention_is_as_near_as_its_result_is_rounded(et, bits, form, qscale):
 
 
 @pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("qscale", [1.0, 2.0 ** -13])
+@pytest.mark.parametrize("every", [2, 4, 7])
+@pytest.mark.parametrize("form", FORMS, ids=str)
+def test_values_of_single_tokens_far_larger(et, bits, form, every, qscale):
+    """Tokens of ordinary values beside tokens whose values are 256 times as large, at any place of four: weights are kept in range by the largest scale of all."""
+    got, Z = attended(et, bits, form, 17, qscale, values=lambda r, tokens, width: r.standard_normal((tokens, width)) * np.where(np.arange(tokens) % every == every - 1, 128.0, 0.5)[:, None])
+    e = np.linalg.norm(got - Z) / np.linalg.norm(Z)
+    assert e <= NEAR, e
+
+
+@pytest.mark.parametrize("bits", [4, 8])
 @pytest.mark.parametrize("form", FORMS, ids=str)
 def test_values_at_the_end_of_the_range(et, bits, form):
     """A group from -65504 to 65504 gets a scale whose last steps lie beyond: what is read back is the largest number, and so is what attention gives."""
