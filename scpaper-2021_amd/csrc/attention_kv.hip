@@ -70,6 +70,16 @@ template <int BITS, int HD> struct KvShape {
 
 constexpr float kNothing = -1e30f;
 
+// Weights of channel groups that share a reference: a group whose scales are far smaller than another's would have its weights among the subnormal binary16
+// numbers, where the second number of a weight holds nothing (300 keys, scales 2^20 apart: 3.5e-4 of the group's 2-norm instead of 2.1e-4, 2^22: 9e-4).  Where scales are more than 2^kLeastLift
+// apart, a group's weights, and with them its products, are times 2^lift: 15 is enough, since scales reach from 2^-24 to 2^13 and weights keep their bits 2^16 below the largest.
+constexpr float kMostLift = 15.0f, kLeastLift = 8.0f;
+
+// The lift of a group, at most 15, whose largest p * scale is below 2^reach: to 2^11 where lifts are chosen, else no more than keeps it at 2^15.
+__device__ __forceinline__ float next_lift(float lift, float reach, float most, bool choose) {
+    return fmaxf(fminf(choose ? floorf(11.0f - reach) : fminf(lift, floorf(15.0f - reach)), most), 0.0f);
+}
+
 #define ET_KV_CONST(T, p) ((const __attribute__((address_space(4))) T *)(p))
 
 __device__ __forceinline__ h8 as_h8(unsigned a, unsigned b, unsigned c, unsigned d) {
@@ -141,9 +151,15 @@ __device__ __forceinline__ float hidden_zero() {
     asm("" : "+v"(zero));
     return zero;
 }
-__device__ __forceinline__ void weight_of(_Float16 &w, _Float16 &rest, float p, unsigned scale_low, float zero) {
-    w = (_Float16)__builtin_fmaf(p, low_half(scale_low), zero);
-    rest = (_Float16)__builtin_fmaf(p, low_half(scale_low), -(float)w);
+// PAIRS: two weights are rounded in one instruction, from binary32, instead of each with its product (16 rows of heads of 128: 59.8 us instead of 60.7; four rows of
+// 131071 keys the other way, 37.0 and 36.1).
+template <bool PAIRS = false> __device__ __forceinline__ void weight_of(_Float16 &w, _Float16 &rest, float p, unsigned scale_low, float zero) {
+    float whole = __builtin_fmaf(p, low_half(scale_low), zero);
+    if constexpr (PAIRS) asm("" : "+v"(whole));
+    w = (_Float16)whole;
+    float part = __builtin_fmaf(p, low_half(scale_low), -(float)w);
+    if constexpr (PAIRS) asm("" : "+v"(part));
+    rest = (_Float16)part;
 }
 
 // acc += (w + rest) * codes over 32 keys, 4 j .. 4 j + 3 of two pieces.
@@ -532,6 +548,9 @@ template <int BITS, int HD, int NW, int P> __global__ __launch_bounds__(NW * 64,
 
     float ref = kNothing, l = 0.0f, z[SETS];
     f4 acc[SETS][PRODUCTS];
+    unsigned lift = 0;    // of the sets, four bits each: what acc is times 2^ of
+    bool lifted = false;  // any of any row
+    auto lift_of = [](unsigned lifts, int g) { return (int)(lifts >> (4 * g) & 15u); };
 #pragma unroll
     for (int g = 0; g < SETS; g++) {
         z[g] = 0.0f;
@@ -643,29 +662,78 @@ template <int BITS, int HD, int NW, int P> __global__ __launch_bounds__(NW * 64,
         // the largest scale: they are not negative, and their bits in the low halves of the words go up with them
         typedef unsigned short s2 __attribute__((ext_vector_type(2)));
         auto halves = [](unsigned w) { return __builtin_bit_cast(s2, w); };  // (of an element of a vector, __builtin_bit_cast takes the vector's first)
-        s2 most_s = halves(vs[0][0][0]);
+        auto scale_of = [&](int g) {
+            s2 m = halves(vs[0][g][0]);
 #pragma unroll
-        for (int i = 1; i < 8 * SETS; i++) most_s = __builtin_elementwise_max(most_s, halves(vs[i / (4 * SETS)][i / 4 % SETS][i & 3]));
-        const float most_e = (float)__builtin_amdgcn_frexp_expf(low_half(__builtin_bit_cast(unsigned, most_s)));
+            for (int e = 1; e < 8; e++) m = __builtin_elementwise_max(m, halves(vs[e >> 2][g][e & 3]));
+            return m;
+        };
+        auto exponent = [](s2 m) { return (float)__builtin_amdgcn_frexp_expf(low_half(__builtin_bit_cast(unsigned, m))); };
+        s2 most_s = scale_of(0);
+#pragma unroll
+        for (int g = 1; g < SETS; g++) most_s = __builtin_elementwise_max(most_s, scale_of(g));
+        const float most_e = exponent(most_s);
         float most_y = y[0];
 #pragma unroll
         for (int e = 1; e < 8; e++) most_y = fmaxf(most_y, y[e]);
         const float reach = most_y + most_e;
-        if (__any(reach > ref + 15.0f)) {
-            const float next = fmaxf(ref, rows_max(reach) - 11.0f);
-            const float f = __builtin_amdgcn_exp2f(ref - next);
-            ref = next;
-            l *= f;
-            float fr[4];
+        // (computed anew wherever it is used: there are no registers to keep what the compiler would like to)
+        auto group_exponent = [&](int g) {
+            unsigned first = vs[0][g][0];
+            asm("" : "+v"(first));
+            vs[0][g][0] = first;
+            return exponent(scale_of(g));
+        };
+        const bool moves = __any(reach > ref + 15.0f);
+        if (moves || lifted) {
+            bool choose = false;
+            if (moves) {
+                float least_e = most_e;
 #pragma unroll
-            for (int r = 0; r < 4; r++) fr[r] = __shfl(f, 4 * j + r);
+                for (int g = 0; g < SETS; g++) least_e = fminf(least_e, group_exponent(g));
+                choose = __any(most_e - least_e > kLeastLift);
+                const float next = fmaxf(ref, rows_max(reach) - 11.0f);
+                const float f = __builtin_amdgcn_exp2f(ref - next);
+                ref = next;
+                l *= f;
+                float fr[4];
 #pragma unroll
-            for (int g = 0; g < SETS; g++) {
-                z[g] *= f;
+                for (int r = 0; r < 4; r++) fr[r] = __shfl(f, 4 * j + r);
 #pragma unroll
-                for (int k = 0; k < PRODUCTS; k++)
+                for (int g = 0; g < SETS; g++) {
+                    z[g] *= f;
 #pragma unroll
-                    for (int r = 0; r < 4; r++) acc[g][k][r] *= fr[r];
+                    for (int k = 0; k < PRODUCTS; k++)
+#pragma unroll
+                        for (int r = 0; r < 4; r++) acc[g][k][r] *= fr[r];
+                }
+            }
+            if (choose || lifted) {
+                // the scales themselves are lifted, where times 2^lift they stay binary16 numbers
+                unsigned lifts = 0;
+#pragma unroll
+                for (int g = 0; g < SETS; g++) {
+                    const float e = group_exponent(g);
+                    lifts |= (unsigned)next_lift((float)lift_of(lift, g), rows_max(most_y - ref + e), kMostLift - fmaxf(rows_max(e), 0.0f), choose) << (4 * g);
+                }
+                int was[4], now[4];  // of rows 4 j .. 4 j + 3 of the products
+#pragma unroll
+                for (int r = 0; r < 4; r++) was[r] = __shfl((int)lift, 4 * j + r), now[r] = __shfl((int)lifts, 4 * j + r);
+                lift = lifts;
+                lifted = __any(lift != 0);
+#pragma unroll
+                for (int g = 0; g < SETS; g++) {
+#pragma unroll
+                    for (int r = 0; r < 4; r++)
+#pragma unroll
+                        for (int k = 0; k < PRODUCTS; k++) acc[g][k][r] = __builtin_ldexpf(acc[g][k][r], lift_of(now[r], g) - lift_of(was[r], g));
+                    const h2 m = {(_Float16)__builtin_ldexpf(1.0f, lift_of(lift, g)), (_Float16)1.0f};
+#pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        const unsigned sl = vs[e >> 2][g][e & 3];
+                        vs[e >> 2][g][e & 3] = __builtin_bit_cast(unsigned, h2(__builtin_bit_cast(h2, sl) * m));
+                    }
+                }
             }
         }
         float p[8];
@@ -685,7 +753,7 @@ template <int BITS, int HD, int NW, int P> __global__ __launch_bounds__(NW * 64,
             for (int e = 0; e < 8; e++) {
                 const unsigned sl = vs[e >> 2][g][e & 3];
                 _Float16 we, re;
-                weight_of(we, re, p[e], sl, zero);
+                weight_of<true>(we, re, p[e], sl, zero);
                 w[e] = we, rest[e] = re;
                 z[g] = __builtin_fmaf(p[e], high_half(sl), z[g]);
             }
@@ -702,6 +770,17 @@ template <int BITS, int HD, int NW, int P> __global__ __launch_bounds__(NW * 64,
                 acc[g][k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w, codes, acc[g][k], 0, 0, 0);
                 acc[g][k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(rest, codes, acc[g][k], 0, 0, 0);
             }
+        }
+    }
+
+    if (lifted) {
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+            const unsigned of_row = (unsigned)__shfl((int)lift, 4 * j + r);
+#pragma unroll
+            for (int g = 0; g < SETS; g++)
+#pragma unroll
+                for (int k = 0; k < PRODUCTS; k++) acc[g][k][r] = __builtin_ldexpf(acc[g][k][r], -lift_of(of_row, g));
         }
     }
 
@@ -841,6 +920,8 @@ template <int BITS, int HD, int R, int NW> __global__ __launch_bounds__(NW * 64,
 #pragma unroll
     for (int i = 0; i < S::kAcc; i++) acc[i] = f4{0.f, 0.f, 0.f, 0.f};
     float ref[R], l[R], z[R][G];
+    unsigned lift = 0;  // of rows and groups, four bits each: what acc is times 2^ of
+    auto lift_of = [](unsigned lifts, int h, int g) { return (int)(lifts >> (4 * (h * G + g)) & 15u); };
 #pragma unroll
     for (int h = 0; h < R; h++) {
         ref[h] = kNothing, l[h] = 0.0f;
@@ -929,16 +1010,38 @@ template <int BITS, int HD, int R, int NW> __global__ __launch_bounds__(NW * 64,
             y = seen ? y : kNothing;
             // a weight is at most 2^15: p * scale < 2^(y - ref + exponent of the scale)
             const float reach = y + most_e;
-            if (__any(reach > ref[h] + 15.0f)) {
-                const float next = fmaxf(ref[h], wave_max(reach) - 11.0f);
-                const float f = __builtin_amdgcn_exp2f(ref[h] - next);
-                ref[h] = next;
-                l[h] *= f;
+            const bool moves = __any(reach > ref[h] + 15.0f);
+            if (moves || (G > 1 && lift != 0)) {
+                bool choose = false;
+                if (moves) {
+                    if constexpr (G > 1) {
+                        int least_e = __builtin_amdgcn_frexp_expf(low_half(vs[0]));
 #pragma unroll
-                for (int g = 0; g < G; g++) {
-                    z[h][g] *= f;
+                        for (int g = 1; g < G; g++) least_e = min(least_e, __builtin_amdgcn_frexp_expf(low_half(vs[g])));
+                        choose = __any(most_e - (float)least_e > kLeastLift);
+                    }
+                    const float next = fmaxf(ref[h], wave_max(reach) - 11.0f);
+                    const float f = __builtin_amdgcn_exp2f(ref[h] - next);
+                    ref[h] = next;
+                    l[h] *= f;
 #pragma unroll
-                    for (int i = 0; i < S::kAcc; i++) acc[i][h * GP + g] *= f;
+                    for (int g = 0; g < G; g++) {
+                        z[h][g] *= f;
+#pragma unroll
+                        for (int i = 0; i < S::kAcc; i++) acc[i][h * GP + g] *= f;
+                    }
+                }
+                if (G > 1 && (choose || lift != 0)) {
+                    unsigned lifts = lift;
+#pragma unroll
+                    for (int g = 0; g < G; g++) {
+                        const int was = lift_of(lift, h, g), at = 4 * (h * G + g);
+                        const int now = (int)next_lift((float)was, wave_max(y - ref[h] + (float)__builtin_amdgcn_frexp_expf(low_half(vs[g]))), kMostLift, choose);
+                        lifts = (lifts & ~(15u << at)) | (unsigned)now << at;
+#pragma unroll
+                        for (int i = 0; i < S::kAcc; i++) acc[i][h * GP + g] = __builtin_ldexpf(acc[i][h * GP + g], now - was);
+                    }
+                    lift = __builtin_amdgcn_readfirstlane(lifts);
                 }
             }
             const float p = seen ? __builtin_amdgcn_exp2f(y - ref[h]) : 0.0f;
@@ -947,7 +1050,7 @@ template <int BITS, int HD, int R, int NW> __global__ __launch_bounds__(NW * 64,
             for (int g = 0; g < G; g++) {
                 z[h][g] = __builtin_fmaf(p, R == 1 || seen ? high_half(vs[g]) : 0.0f, z[h][g]);  // (what others see may be NaN, and 0 * NaN is)
                 _Float16 w, rest;
-                weight_of(w, rest, p, vs[g], zero);
+                weight_of(w, rest, G == 1 ? p : __builtin_ldexpf(p, lift_of(lift, h, g)), vs[g], zero);
                 weights[(h * GP + g) * F::kLdsRow + key_place] = w;
                 weights[(4 + h * GP + g) * F::kLdsRow + key_place] = rest;
             }
@@ -959,6 +1062,15 @@ template <int BITS, int HD, int R, int NW> __global__ __launch_bounds__(NW * 64,
             weigh_values<BITS, HD>(acc, w, rest, vw[2 * u], vw[2 * u + 1], c);
         }
         wave_lds_order();
+    }
+
+    if (G > 1 && lift != 0) {
+#pragma unroll
+        for (int h = 0; h < R; h++)
+#pragma unroll
+            for (int g = 0; g < G; g++)
+#pragma unroll
+                for (int i = 0; i < S::kAcc; i++) acc[i][h * GP + g] = __builtin_ldexpf(acc[i][h * GP + g], -lift_of(lift, h, g));
     }
 
     // what the waves have, side by side

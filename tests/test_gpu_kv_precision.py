@@ -50,6 +50,12 @@ def attended(et, bits, form, seed, qscale=1.0, **kw):
     return got.astype(np.float64).reshape(-1, nh, hd), Z.reshape(-1, nh, hd)
 
 
+def off(got, Z):
+    """The 2-norm of the error over that of the result, by channel group."""
+    by_group = lambda a: a.reshape(-1, a.shape[-1] // 32, 32).transpose(1, 0, 2).reshape(a.shape[-1] // 32, -1)  # noqa: E731
+    return np.linalg.norm(by_group(got - Z), axis=1) / np.linalg.norm(by_group(Z), axis=1)
+
+
 @pytest.mark.parametrize("bits", [4, 8])
 @pytest.mark.parametrize("qscale", [1.0, 2.0 ** -13])
 @pytest.mark.parametrize("form", FORMS, ids=str)
@@ -70,6 +76,41 @@ def test_values_of_single_tokens_far_larger(et, bits, form, every, qscale):
     got, Z = attended(et, bits, form, 17, qscale, values=lambda r, tokens, width: r.standard_normal((tokens, width)) * np.where(np.arange(tokens) % every == every - 1, 128.0, 0.5)[:, None])
     e = np.linalg.norm(got - Z) / np.linalg.norm(Z)
     assert e <= NEAR, e
+
+
+def alternate(large, small):
+    return lambda r, tokens, width: np.clip(r.standard_normal((tokens, width // 32, 32)) * np.where(np.arange(width // 32) % 2, small, large)[:, None], -65504, 65504).reshape(tokens, width)
+
+
+def turning(large, small):
+    """Groups whose values are large in every other stretch of 150 tokens, each in its turn."""
+    def values(r, tokens, width):
+        size = np.where((np.arange(tokens)[:, None] // 150 + np.arange(width // 32)) % 2, small, large)
+        return np.clip(r.standard_normal((tokens, width // 32, 32)) * size[..., None], -65504, 65504).reshape(tokens, width)
+    return values
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("qscale", [1.0, 2.0 ** -13])
+@pytest.mark.parametrize("form", [f for f in FORMS if f[0] > 32], ids=str)
+@pytest.mark.parametrize("values", [alternate(2.0 ** 13, 2.0 ** -7), alternate(2.0 ** -7, 2.0 ** 13), turning(2.0 ** 13, 2.0 ** -7)], ids=["alternate", "alternate2", "turning"])
+def test_groups_of_very_different_size(et, bits, form, qscale, values):
+    """Channel groups whose values are 2^20 apart are each as near as if they were alone."""
+    got, Z = attended(et, bits, form, 12, qscale, values=values)
+    e = off(got, Z)
+    assert (e <= NEAR).all(), e
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("qscale", [1.0, 2.0 ** -13])
+@pytest.mark.parametrize("form", [f for f in FORMS if f[0] > 32], ids=str)
+@pytest.mark.parametrize("values", [alternate(2.0 ** 13, 2.0 ** -9), alternate(2.0 ** -9, 2.0 ** 13), turning(2.0 ** -9, 2.0 ** 13)], ids=["alternate", "alternate2", "turning"])
+def test_groups_of_very_different_size_further_apart(et, bits, form, qscale, values):
+    """2^22: the small ones' results come to where binary16 has subnormal numbers, each off by up to 2^-25, evenly spread."""
+    got, Z = attended(et, bits, form, 15, qscale, values=values)
+    by_group = lambda a: np.linalg.norm(a.reshape(-1, a.shape[-1] // 32, 32).transpose(1, 0, 2).reshape(a.shape[-1] // 32, -1), axis=1)  # noqa: E731
+    e, lim = by_group(got - Z), NEAR * by_group(Z) + 2.0 ** -25 / math.sqrt(3) * math.sqrt(Z.size / (Z.shape[-1] // 32))
+    assert (e <= lim).all(), e / lim
 
 
 @pytest.mark.parametrize("bits", [4, 8])
