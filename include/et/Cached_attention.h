@@ -10,6 +10,7 @@
 #pragma once
 #include <cmath>
 #include <memory>
+#include <utility>
 
 #include "Linear.h"
 
@@ -79,8 +80,14 @@ inline void Multihead_attention_cached(const KvCache &cache, const KvStep &s, co
                         scale != 0.0f ? scale : 1.0f / std::sqrt((float)cache.hd), s.causal ? ET_MHA_CAUSAL : 0, workspace, workspace_bytes, stream));
 }
 
+// What a Linear's rows have to be a multiple of.
+template <typename WEIGHT> constexpr int kLinearRows = 16;
+template <> inline constexpr int kLinearRows<w4_mat> = 1;
+template <> inline constexpr int kLinearRows<csr_mat> = 1;
+
 // The attention block of a step.  WQKV projects to nhead * hd queries, then nkv * hd keys and
-// values; both Linears are made for batch * n rows.  max_pages: as the steps will give it.
+// values; both Linears are made for batch * n rows, a multiple of 16 unless their weights are
+// w4_mat or csr_mat.  max_pages: the most that the steps will give.
 template <typename WQKV_t, typename WO_t> class CachedAttention {
     std::unique_ptr<Linear<WQKV_t>> linearQKV;
     std::unique_ptr<Linear<WO_t>> linearO;
@@ -92,7 +99,7 @@ template <typename WQKV_t, typename WO_t> class CachedAttention {
   public:
     CachedAttention(std::unique_ptr<Linear<WQKV_t>> qkv_, std::unique_ptr<Linear<WO_t>> o_, std::shared_ptr<KvCache> cache, int _nhead, int _max_pages, int _batch,
                     int _n = 1)
-        : linearQKV(std::move(qkv_)), linearO(std::move(o_)), cache_(std::move(cache)), nhead(_nhead), batch(_batch), n(_n), max_pages(_max_pages),
+        : linearQKV(std::move(qkv_)), linearO(std::move(o_)), cache_(checked(std::move(cache), linearQKV && linearO, _batch, _n)), nhead(_nhead), batch(_batch), n(_n), max_pages(_max_pages),
           qkv((std::size_t)_batch * _n * width()), z((std::size_t)_batch * _n * nhead * cache_->hd),
           workspace(cached_attention_workspace(*cache_, _max_pages, _batch, _n, _nhead) + 16) {
         require((int)linearQKV->out_size == width() && (int)linearO->in_size == nhead * cache_->hd && (int)linearQKV->size == batch * n && (int)linearO->size == batch * n,
@@ -107,6 +114,15 @@ template <typename WQKV_t, typename WO_t> class CachedAttention {
         cache_->write(s, qkv.get() + nhead * hd, qkv.get() + (nhead + cache_->nkv) * hd, ld, ld, stream);
         Multihead_attention_cached(*cache_, s, qkv.get(), ld, z.get(), nhead * hd, nhead, workspace.get(), workspace.size, 0.0f, stream);
         linearO->forward(out, z.get(), stream);
+    }
+
+  private:
+    static std::shared_ptr<KvCache> checked(std::shared_ptr<KvCache> cache, bool projections, int batch, int n) {
+        require(cache && projections, "CachedAttention: a cache and two projections are needed");
+        require(batch > 0 && n > 0, "CachedAttention: batch and n must be at least 1");
+        require(batch * n % kLinearRows<WQKV_t> == 0 && batch * n % kLinearRows<WO_t> == 0,
+                "CachedAttention: batch * n must be a multiple of 16 for projections other than w4_mat and csr_mat");
+        return cache;
     }
 };
 

@@ -158,3 +158,11 @@ def test_class_layer_runs_the_same_calls(et, tmp_path):
     for i in range(steps):
         want = dev.attention(up(et, tokens[i]), [c + i for c in counts], None, 1).numpy()
         assert np.array_equal(np.load(tmp_path / f"out_{i}.npy"), f32(want)), i
+
+
+def test_class_layer_sizes():
+    """CachedAttention with tile-sparse projections, with fewer pages than it was made for, and what it refuses when it is made."""
+    exe = EXE.with_name("cached_attention_sizes")
+    assert exe.exists(), f"{exe} is missing: build it with `python scpaper-2021_amd/build.py`"
+    res = subprocess.run([str(exe)], capture_output=True, text=True, timeout=120)
+    assert res.returncode == 0 and "ok" in res.stdout, res.stdout + res.stderr
