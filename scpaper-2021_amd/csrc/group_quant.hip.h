@@ -9,8 +9,6 @@
 
 namespace et {
 
-constexpr int kRowRor4 = 0x124, kRowRor8 = 0x128;
-
 __device__ __forceinline__ float f16_bits_value(unsigned bits) { return (float)__builtin_bit_cast(_Float16, (unsigned short)bits); }
 
 // Bits of the smallest binary16 number s with levels * s >= high - low.  The difference of two binary16 numbers has up to 41 bits: it is
