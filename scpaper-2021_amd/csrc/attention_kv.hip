@@ -432,8 +432,8 @@ template <int BITS, int HD, int NW> __global__ __launch_bounds__(NW * 64, (kv_ro
 // Values: the 16 columns of a product are channels of one group, whose scale is in the rows' weights.
 //
 // Bound by its vector instructions, some 500 a tile of 16 rows and 32 keys of 128 channels (five a score and group, the rest the codes), next to 24 products: 64 sequences of
-// 1000 tokens, 16 heads of 128, 16 rows 50.7 us (88 in blocks of 4), 8 of 4000, 4 heads, 256 rows 117 (178).  A spilled register a lane costs more than a wave a SIMD: at three
-// of those, with spills, 109 us.
+// 1000 tokens, 16 heads of 128, 16 rows 59 us (128 in blocks of 4), 8 of 4000, 4 heads, 256 rows 106 (195).  A spilled register a lane costs more than a wave a SIMD: at three
+// of those, with spills, twice the time.
 template <int BITS> struct KvWords {
     // Groups in fours, a two and a one: lane j loads what lies at j of a four's (two's, one's) bytes, group j of the four.
     static constexpr int W = BITS / 4;  // words of eight channels
@@ -1184,9 +1184,14 @@ struct KvForm {
 };
 
 // Rows: of a key/value head in the call.  fills: one block of rows for each (sequence, key/value head) is enough work for the chip, there being many, or keys to share out.
-// Blocks of 16 / kCols rows or of 16, measured in us with 16 sequences of 4096 tokens, 8 heads (of 128: 8 rows 34.3 | 37.7, 9 rows
-// 50.4 | 40.4, 16 rows 82 | 46; of 64, 10 rows 27.3 | 24.6, 8 rows 22.5 | 26.9) and 4 sequences (of 192: 5 rows 32.3 | 22.0; of 256: 6 rows 34.7 | 27.2, 32 rows 91 | 45).  Heads of 128, 5 to 8 rows, blocks of 4 and of 8 over pairs of groups: 8 rows 32.7 | 27.8 (8 bits 45.4 | 30.6), one sequence of
-// 100000 47.6 | 38.7, but 16 sequences of 1500, 7 rows, 15.1 | 18.1.  Wider heads: pairs are no better than 16 rows.
+// Blocks of 16 / kCols rows or of 16, us, 8 heads, 16 sequences of 4096 tokens with heads up to 128 and 4 with wider ones, 4 bits (8 bits):
+//    64: 8 rows 18.5 | 21.7 (20.1 | 21.8)   9 rows 26.6 | 21.9 (28.2 | 22.2)      96: 5 rows 30.6 | 29.7 (38.6 | 30.2)   8 rows 30.8 | 30.4 (38.8 | 31.0)   9 rows 42.5 | 30.6 (53.4 | 31.3)
+//   160: 4 rows 16.7 | 17.7 (19.3 | 18.9)   5 rows 27.6 | 18.1 (31.3 | 19.0)     192: 4 rows 18.7 | 20.1 (20.4 | 20.7)   5 rows 30.8 | 20.3 (34.1 | 20.9)
+//   224: 4 rows 20.0 | 23.0 (22.3 | 24.1)   5 rows 33.2 | 23.4 (37.1 | 24.3)     256: 4 rows 21.1 | 25.3 (27.8 | 26.3)   5 rows 35.1 | 25.5 (47.2 | 26.5)
+// So 5 to 8 rows of heads of 96 in 8 bits are on the slower side.  Heads of 128, 5 to 8 rows: blocks of 4, of 8 over pairs of groups or of 16, us, 8 rows:
+//   16 x 4096 35.0 | 31.1 | 38.5 (50.4 | 34.4 | 40.5)   16 x 2112 23.6 | 19.1 | 23.3 (30.2 | 20.3 | 24.3)   16 x 1984 19.6 | 21.9 | 27.3 (23.7 | 23.4 | 28.9)   40 x 1000 28.5 | 26.4 | 32.3 (36.1 | 27.9 | 33.4)
+//   4 x 2112 14.2 | 15.7 | 15.9 (16.9 | 16.7 | 16.3)    4 x 1984 16.3 | 19.2 | 24.6 (20.8 | 21.2 | 25.9)    1 x 8000 15.5 | 17.3 | 16.1 (18.6 | 18.4 | 16.5)
+// so from 2048 positions on a few sequences in 4 bits are up to 12 % on the slower side.  Wider heads: pairs are no better than 16 rows.
 template <int BITS, int HD> KvForm form_of(long long rows, bool fills) {
     if constexpr (HD <= 128) {
         constexpr int cols = KvShape<BITS, HD>::kCols, heads = 4 / cols;
@@ -1221,8 +1226,8 @@ struct KvPlan {
 
 // Waves of a workgroup and workgroups that share the keys of a (sequence, key/value head): 4096 waves, which fill the chip, but at least four tiles a wave if every
 // sequence were as long as its table; a second launch, which joins the parts, costs 3 to 6 us.  Eight waves a workgroup where there are few: 16 rows, 8 heads of 128, 1000
-// tokens, 16 sequences 25.0 us with four, 16.3 with eight, 32 sequences 34.2 and 17.7; but only two of them a SIMD fit so (of 96 three with four waves): where keys are shared
-// out anyway, four (16 x 10937 tokens, 5 heads of 96, 80 rows 147 and 170 us).
+// tokens, 32 sequences 25.1 us with four, 19.9 with eight (16 sequences 17.0 and 17.7), one row, 8 x 2048, 12 heads of 64 9.8 and 8.2; but only two of them a SIMD fit of 16 rows of
+// heads of 96 and 128 (of 96 three with four waves): where keys are shared out anyway, four (16 x 10937 tokens, 5 heads of 96, 80 rows 170 and 204 us, 64 x 1000, 16 heads of 128 59 and 73).
 int kv_plan(const char *fn, KvPlan &p, const et_kv_cache *c, int max_pages, int B, int n, int nh) {
     ET_REQUIRE(nh > 0 && nh % c->nkv == 0, ET_ERR_INVALID_ARG, "%s: nh=%d must be a multiple of nkv=%d", fn, nh, c->nkv);
     const int per = nh / c->nkv;

@@ -3,8 +3,9 @@
 // Eight lanes take one group of 32 channels of four tokens whose positions are 4q .. 4q + 3, bits of the lane: 0 and 1 the token, 3 the eights of channels 0 and 2 or 1 and
 // 3 (bit 2: the next group).  A group's extremes are then one rotation inside the 16 lanes, and the four tokens' codes of V, which the cache holds side by side, change places
 // inside four neighbouring lanes.  Where a call does not hold all four tokens, the units of 16 bits of those it holds are stored one by one: the bytes of the others are not
-// touched.  Writing is bound by its arithmetic next to memory, 19 vector instructions a value: 16 channels a lane share a group's scale (8 did not: 27 us for 16 x 1000 tokens of
-// 8 heads of 128, of which it writes and reads 86 MB in 22.2 us; reading back is memory, 86 MB in 17.0).  8 bits, 4 x 8192 tokens of 16 heads of 64, 209 MB: 54.6 and 37.6 us.
+// touched.  16 x 1000 tokens of 8 heads of 128, 4 bits, 86 MB read and written: written in 21.3 us, next to memory bound by 19 vector instructions a
+// value (16 channels a lane share a group's scale; 8 did not, and took a tenth more), read back in 20.1; 8 bits, 4 x 8192 tokens of 16 heads of 64, 210 MB: 54.7, and 37.8, which is memory's.
+// Rows from counts[b] on cost what the others do, all but their stores: with 12256 of the 16000 tokens there, 66 MB, 22.5 and 17.1 us.
 #include "group_quant.hip.h"
 
 namespace et {

@@ -417,6 +417,15 @@ class Bench:
         us = self.time_us(lambda: et.mha_kv(cache, table, pages, starts, None, q, width, z, width, B, n, nh, hd ** -0.5, et.MHA_CAUSAL, ws, need, self.stream), launches)
         self.record("mha_kv", f"{bits} bits B{B} L{length} n{n} {nh}/{nkv} heads of {hd}", us, 2 * B * length * (nkv * hd * bits // 8 + nkv * hd // 32 * 4), "hbm")
 
+    def weight_to_w4(self, n_in, n_out, group, launches):
+        """A weight to 4 bits, and what those stand for."""
+        et = self.et
+        w, back = self.dev(self.rnd((n_out, n_in), 0.02)), self.empty((n_out, n_in))
+        codes, scales = et.DeviceBuffer(n_out * n_in // 2), et.DeviceBuffer(n_in // group * n_out * 4)
+        shape, work = f"in{n_in} out{n_out} groups of {group}", n_out * n_in * 2 + n_out * n_in // 2 + n_in // group * n_out * 4
+        self.record("dense_to_w4", shape, self.time_us(lambda: et.dense_to_w4(w, codes, scales, n_in, n_out, group, self.stream), launches), work, "hbm")
+        self.record("w4_to_dense", shape, self.time_us(lambda: et.w4_to_dense(codes, scales, back, n_in, n_out, group, self.stream), launches), work, "hbm")
+
     def linear_w4(self, T, n_in, n_out, group, launches, nset=4):
         et = self.et
         w = self.dev(self.rnd((n_out, n_in), 0.02))
@@ -714,12 +723,15 @@ def main():
         print("# generating token by token: a cache of keys and values in 4 and 8 bits, attention over it, 4-bit Linears")
         for bits, B, length, nkv, hd, n in ((4, 8, 512, 12, 64, 1), (4, 16, 1000, 8, 128, 1000), (8, 4, 8192, 16, 64, 8192)):
             b.decode_cache(bits, B, length, nkv, hd, 64, n, 20)
-        for bits, B, length, nh, nkv, hd, n in ((4, 1, 128, 12, 12, 64, 1), (4, 8, 2048, 12, 12, 64, 1), (4, 64, 4096, 16, 16, 64, 1), (4, 16, 4096, 32, 8, 128, 1),
+        for bits, B, length, nh, nkv, hd, n in ((4, 1, 128, 12, 12, 64, 1), (4, 8, 2048, 12, 12, 64, 1), (4, 64, 4096, 16, 16, 64, 1), (8, 8, 2048, 12, 12, 64, 1), (8, 64, 2048, 16, 16, 64, 1),
+                                                (4, 16, 4096, 32, 8, 128, 1), (4, 16, 4096, 64, 8, 128, 1), (8, 16, 4096, 64, 8, 128, 1),
                                                 (4, 1, 131071, 32, 8, 128, 1), (8, 16, 1500, 8, 8, 96, 7), (4, 64, 1000, 16, 16, 128, 16), (4, 8, 4000, 64, 4, 128, 16)):
             b.decode_attention(bits, B, length, nh, nkv, hd, 64, n, 10)
         for T, n_in, n_out, group in ((1, 1024, 4096, 64), (1, 800, 28800, 32), (1, 8192, 28672, 128), (4, 8192, 28672, 128), (16, 8192, 28672, 128), (45, 4096, 4096, 32),
                                       (64, 4096, 16384, 64), (256, 4096, 4096, 128)):
             b.linear_w4(T, n_in, n_out, group, 10)
+        for n_in, n_out, group in ((1024, 4096, 64), (4096, 4096, 32), (8192, 28672, 128)):
+            b.weight_to_w4(n_in, n_out, group, 10)
     if args.set == "machine":
         print("# machine probes")
         b.machine()
