@@ -722,7 +722,8 @@ int et_kv_read_f16(const et_kv_cache *cache, const int32_t *table, int max_pages
  * behind a sequence's end may be anything, NaN included.  n = 1 is a decoding
  * step, n > 1 several tokens at once (a piece of a prompt, guessed tokens).
  * The codes enter the matrix products as they are; scores, softmax and sums are
- * binary32, a probability times its value's scale is two binary16 numbers, the
+ * binary32 (a score's terms keep what is 2^-17, with 8 bits 2^-14, of the row's
+ * largest |Q| times the scale of the key's group, and more), a probability times its value's scale is two binary16 numbers, the
  * rounded one and what it leaves.  |scale| is at most 1e15.
  * workspace: et_mha_kv_workspace bytes of device memory, 16-byte aligned (may be NULL where that
  * says 0); launches that can overlap in time need one each.  The sums are

@@ -113,11 +113,14 @@ template <int COLS> __device__ __forceinline__ float cols_sum(float v) {
     return v;
 }
 
-// Eight channels of a key as subnormal numbers, code * 2^-24, every other one * 16 for 4 bits: channels 0 4 1 5 2 6 3 7, or 0 2 1 3 4 6 5 7.
+// Eight channels of a key as subnormal numbers, code / key_unit, every other one * 16 for 4 bits: channels 0 4 1 5 2 6 3 7, or 0 2 1 3 4 6 5 7.  As in values, codes in the lowest bits
+// would cost the smaller terms of a score theirs: 4-bit codes are in bits 3 to 6 and 7 to 10 (at 0 to 3 and 4 to 7, one instruction less in six, a query's channel 100 times the others, and small in the
+// keys, made 2.1e-4 of the result's 2-norm 2.6e-4 to 3.7e-4).
+template <int BITS> constexpr int key_unit_log2() { return BITS == 4 ? 21 : 24; }
 template <int BITS> __device__ __forceinline__ h8 key_codes(const unsigned *w) {
     if constexpr (BITS == 4) {
-        const unsigned x = w[0] >> 8;
-        return as_h8(w[0] & 0x000f000fu, w[0] & 0x00f000f0u, x & 0x000f000fu, x & 0x00f000f0u);
+        const unsigned x = w[0] << 3, y = w[0] >> 5;
+        return as_h8(x & 0x00780078u, x & 0x07800780u, y & 0x00780078u, y & 0x07800780u);
     } else {
         return as_h8(w[0] & 0x00ff00ffu, (w[0] >> 8) & 0x00ff00ffu, w[1] & 0x00ff00ffu, (w[1] >> 8) & 0x00ff00ffu);
     }
@@ -275,10 +278,10 @@ template <int BITS, int HD, int NW> __global__ __launch_bounds__(NW * 64, (kv_ro
     top = rows_max(top);
     const int up = top > 0.0f ? 15 - __builtin_amdgcn_frexp_expf(top) : 0;
     const float grow = query_growth(top, up, a.scale_log2e);
-    const float key_scale = __builtin_ldexpf(fabsf(a.scale_log2e), 24 - up);
+    const float key_scale = __builtin_ldexpf(fabsf(a.scale_log2e), key_unit_log2<BITS>() - up);
 #pragma unroll
     for (int i = 0; i < S::kPieces; i++) q[i] = query_order<BITS>(q[i], (j * (HD / 4) + 8 * i) / 32 == gg ? grow : 0.0f, sum);
-    const float qsum = rows_sum(sum) * 0x1p-24f;
+    const float qsum = __builtin_ldexpf(rows_sum(sum), -key_unit_log2<BITS>());
 
     float ref = kNothing, l = 0.0f, z = 0.0f;
     f4 acc[S::kAcc];
@@ -537,13 +540,13 @@ template <int BITS, int HD, int NW, int P> __global__ __launch_bounds__(NW * 64,
     top = rows_max(top);
     const int up = top > 0.0f ? 15 - __builtin_amdgcn_frexp_expf(top) : 0;
     const float grow = query_growth(top, up, a.scale_log2e);
-    const float key_scale = __builtin_ldexpf(fabsf(a.scale_log2e), 24 - up);
+    const float key_scale = __builtin_ldexpf(fabsf(a.scale_log2e), key_unit_log2<BITS>() - up);
 #pragma unroll
     for (int g = 0; g < SETS; g++) {
         float sum = 0.0f;
 #pragma unroll
         for (int i = 0; i < P; i++) q[P * g + i] = query_order<BITS>(q[P * g + i], P == 1 || (j & 1) == side ? grow : 0.0f, sum);
-        qsum[g] = rows_sum(sum) * 0x1p-24f;
+        qsum[g] = __builtin_ldexpf(rows_sum(sum), -key_unit_log2<BITS>());
     }
 
     float ref = kNothing, l = 0.0f, z[SETS];
@@ -903,11 +906,11 @@ template <int BITS, int HD, int R, int NW> __global__ __launch_bounds__(NW * 64,
         top = rows_max(top);
         const int up = top > 0.0f ? 15 - __builtin_amdgcn_frexp_expf(top) : 0;
         const float grow = query_growth(top, up, a.scale_log2e);
-        const float back = __builtin_ldexpf(fabsf(a.scale_log2e), 24 - up);
+        const float back = __builtin_ldexpf(fabsf(a.scale_log2e), key_unit_log2<BITS>() - up);
         float sum = 0.0f;
 #pragma unroll
         for (int i = 0; i < S::kPieces; i++) q[i] = query_order<BITS>(q[i], (j * (HD / 4) + 8 * i) / 32 == g_own ? grow : 0.0f, sum);
-        sum = rows_sum(sum) * 0x1p-24f;
+        sum = __builtin_ldexpf(rows_sum(sum), -key_unit_log2<BITS>());
 #pragma unroll
         for (int h = 0; h < R; h++) {
             key_scale[h] = lane_value(back, h * GP);

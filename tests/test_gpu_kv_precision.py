@@ -78,6 +78,26 @@ def test_values_of_single_tokens_far_larger(et, bits, form, every, qscale):
     assert e <= NEAR, e
 
 
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("form", FORMS, ids=str)
+def test_a_channel_far_larger_in_queries(et, bits, form):
+    """One channel of each group is 200 times the others in the queries and small in the keys, whose codes there are about half of the largest: the other channels' terms are 2^-10 of its own
+    and less.  What the products drop, 2^-24 of the largest one's place, is 2^-17 of a step times that query, some 1e-4 of a score."""
+    hd, nkv, per, n, lengths = form
+    K, V, Q, starts, counts = rows_of(form, 18)
+    K[:, 2::32] = (K[:, 2::32] * 0.01).astype(np.float16)
+    Q[:, 2::32] *= 200
+    Q, nh, B = Q.astype(np.float16), nkv * per, len(lengths)
+    max_pages = -(-max(lengths) // 64)
+    table = tables(18, B, max_pages, B * max_pages)
+    host = D.Cache(bits, nkv, hd, 64, B * max_pages, fill=0xFF)
+    host.write(table, [0] * B, lengths, K, V, max(lengths))
+    got = run_attention(et, DeviceCache(et, host), table, starts, counts, Q, B, n, nh, 1 / math.sqrt(hd), True)
+    Z = D.attention(host, table, starts, counts, Q, n, nh, 1 / math.sqrt(hd), True)[0]
+    e = np.linalg.norm(got - Z) / np.linalg.norm(Z)
+    assert e <= NEAR, e
+
+
 def alternate(large, small):
     return lambda r, tokens, width: np.clip(r.standard_normal((tokens, width // 32, 32)) * np.where(np.arange(width // 32) % 2, small, large)[:, None], -65504, 65504).reshape(tokens, width)
 
