@@ -21,6 +21,8 @@ FORMS = [(32, 4, 1, 1, [300, 290]), (64, 4, 1, 1, [300, 290]), (96, 4, 1, 1, [30
          (64, 4, 4, 1, [300, 290]), (128, 2, 4, 1, [300, 290]), (160, 2, 4, 1, [300, 290]), (256, 2, 2, 1, [300, 290]), (64, 2, 5, 2, [300, 290]), (96, 2, 16, 1, [300, 290]),
          (128, 2, 3, 4, [300, 290]), (192, 2, 8, 1, [300, 290]), (224, 2, 5, 1, [300, 290]), (256, 2, 8, 1, [300, 290]), (128, 2, 8, 1, [2100, 700]), (64, 2, 1, 1, [5000, 4000]),
          (128, 1, 4, 1, [5000]), (128, 1, 8, 1, [5000]), (128, 1, 16, 1, [5000])]
+# without the longest ones but for the last, where there are many cases of each
+FEWER = [f for f in FORMS if max(f[4]) < 4000] + FORMS[-1:]
 
 
 def rows_of(form, seed, values=lambda r, tokens, width: r.standard_normal((tokens, width)) * 0.5):
@@ -70,7 +72,7 @@ def test_attention_is_as_near_as_its_result_is_rounded(et, bits, form, qscale):
 @pytest.mark.parametrize("bits", [4, 8])
 @pytest.mark.parametrize("qscale", [1.0, 2.0 ** -13])
 @pytest.mark.parametrize("every", [2, 4, 7])
-@pytest.mark.parametrize("form", FORMS, ids=str)
+@pytest.mark.parametrize("form", FEWER, ids=str)
 def test_values_of_single_tokens_far_larger(et, bits, form, every, qscale):
     """Tokens of ordinary values beside tokens whose values are 256 times as large, at any place of four: weights are kept in range by the largest scale of all."""
     got, Z = attended(et, bits, form, 17, qscale, values=lambda r, tokens, width: r.standard_normal((tokens, width)) * np.where(np.arange(tokens) % every == every - 1, 128.0, 0.5)[:, None])
@@ -112,7 +114,7 @@ def turning(large, small):
 
 @pytest.mark.parametrize("bits", [4, 8])
 @pytest.mark.parametrize("qscale", [1.0, 2.0 ** -13])
-@pytest.mark.parametrize("form", [f for f in FORMS if f[0] > 32], ids=str)
+@pytest.mark.parametrize("form", [f for f in FEWER if f[0] > 32], ids=str)
 @pytest.mark.parametrize("values", [alternate(2.0 ** 13, 2.0 ** -7), alternate(2.0 ** -7, 2.0 ** 13), turning(2.0 ** 13, 2.0 ** -7)], ids=["alternate", "alternate2", "turning"])
 def test_groups_of_very_different_size(et, bits, form, qscale, values):
     """Channel groups whose values are 2^20 apart are each as near as if they were alone."""
@@ -123,7 +125,7 @@ def test_groups_of_very_different_size(et, bits, form, qscale, values):
 
 @pytest.mark.parametrize("bits", [4, 8])
 @pytest.mark.parametrize("qscale", [1.0, 2.0 ** -13])
-@pytest.mark.parametrize("form", [f for f in FORMS if f[0] > 32], ids=str)
+@pytest.mark.parametrize("form", [f for f in FEWER if f[0] > 32], ids=str)
 @pytest.mark.parametrize("values", [alternate(2.0 ** 13, 2.0 ** -9), alternate(2.0 ** -9, 2.0 ** 13), turning(2.0 ** -9, 2.0 ** 13)], ids=["alternate", "alternate2", "turning"])
 def test_groups_of_very_different_size_further_apart(et, bits, form, qscale, values):
     """2^22: the small ones' results come to where binary16 has subnormal numbers, each off by up to 2^-25, evenly spread."""
