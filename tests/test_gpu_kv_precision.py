@@ -185,3 +185,28 @@ def test_infinite_queries_over_keys_of_one_sign(et, form, bad):
     Q[0, 5] = bad
     got = run_attention(et, DeviceCache(et, host), table, starts, counts, Q, 2, n, nh, 0.1, True).reshape(-1, nh, hd)
     assert np.isnan(got[0, 0]).all() and np.isnan(got).sum() == hd
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("hd,per,n", [(64, 1, 2), (64, 3, 5), (128, 3, 4), (256, 2, 4)])
+def test_not_a_number_of_a_later_token_beside_groups_of_very_different_size(et, bits, hd, per, n):
+    """What the rows in front of a token that is NaN give, which do not see it, is the same to the bit whatever it holds; a page without a place in between.  (Against binary64: a result to half a
+    step, 2^-11, its group's largest as much again for what cancels, each four times over.)"""
+    nkv, lengths = 2, [330, 70]
+    r = np.random.default_rng(19)
+    K = r.standard_normal((2 * 330, nkv * hd)).astype(np.float16)
+    V = alternate(2.0 ** 13, 2.0 ** -9)(r, 2 * 330, nkv * hd).astype(np.float16)
+    table = tables(19, 2, 6, 12)
+    table[0, 2] = -1
+    host = D.Cache(bits, nkv, hd, 64, 12, fill=0xFF)
+    host.write(table, [0, 0], lengths, K, V, 330)
+    starts = [l - n for l in lengths]
+    Q = r.standard_normal((2 * n, nkv * per * hd)).astype(np.float16)
+    got = run_attention(et, DeviceCache(et, host), table, starts, None, Q, 2, n, nkv * per, 1 / math.sqrt(hd), True)
+    Z = D.attention(host, table, starts, [n, n], Q, n, nkv * per, 1 / math.sqrt(hd), True)[0]
+    assert (np.abs(got - Z) <= 2.0 ** -9 * np.abs(Z) + 2.0 ** -9 * np.abs(Z).reshape(2 * n, -1, 32).max(-1).repeat(32, -1)).all()
+    row = np.full((2, nkv * hd), np.nan, np.float16)
+    host.write(table, [l - 1 for l in lengths], [1, 1], row, row, 1)
+    again = run_attention(et, DeviceCache(et, host), table, starts, None, Q, 2, n, nkv * per, 1 / math.sqrt(hd), True)
+    last = np.arange(2 * n) % n == n - 1
+    assert np.array_equal(got[~last], again[~last]) and np.isnan(again[last]).all()
