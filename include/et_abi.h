@@ -718,13 +718,14 @@ int et_kv_read_f16(const et_kv_cache *cache, const int32_t *table, int max_pages
  * aligned).  A row that sees nothing becomes zero; a result that rounding a
  * scale up carries beyond binary16's largest number becomes that number, as in
  * et_kv_read_f16.  A NaN or an infinity in a head's row of Q makes its result
- * NaN, if it sees anything.  What lies in the cache
- * behind a sequence's end may be anything, NaN included.  n = 1 is a decoding
- * step, n > 1 several tokens at once (a piece of a prompt, guessed tokens).
+ * NaN, if it sees anything.  What lies in the cache behind a sequence's end may
+ * be anything, NaN included.  n = 1 is a decoding step, n > 1 several tokens at
+ * once (a piece of a prompt, guessed tokens).
  * The codes enter the matrix products as they are; scores, softmax and sums are
  * binary32 (a score's terms keep what is 2^-17, with 8 bits 2^-14, of the row's
- * largest |Q| times the scale of the key's group, and more), a probability times its value's scale is two binary16 numbers, the
- * rounded one and what it leaves.  |scale| is at most 1e15.
+ * largest |Q| times the scale of the key's group, and more), a probability times
+ * its value's scale is two binary16 numbers, the rounded one and what it leaves.
+ * |scale| is at most 1e15.
  * workspace: et_mha_kv_workspace bytes of device memory, 16-byte aligned (may be NULL where that
  * says 0); launches that can overlap in time need one each.  The sums are
  * taken in an order that only the sizes given to the call decide. */

@@ -113,7 +113,7 @@ template <int COLS> __device__ __forceinline__ float cols_sum(float v) {
     return v;
 }
 
-// Eight channels of a key as subnormal numbers, code / key_unit, every other one * 16 for 4 bits: channels 0 4 1 5 2 6 3 7, or 0 2 1 3 4 6 5 7.  As in values, codes in the lowest bits
+// Eight channels of a key as subnormal numbers, code * 2^-key_unit_log2, every other one * 16 for 4 bits: channels 0 4 1 5 2 6 3 7, or 0 2 1 3 4 6 5 7.  As in values, codes in the lowest bits
 // would cost the smaller terms of a score theirs: 4-bit codes are in bits 3 to 6 and 7 to 10 (at 0 to 3 and 4 to 7, one instruction less in six, a query's channel 100 times the others, and small in the
 // keys, made 2.1e-4 of the result's 2-norm 2.6e-4 to 3.7e-4).
 template <int BITS> constexpr int key_unit_log2() { return BITS == 4 ? 21 : 24; }
