@@ -737,6 +737,103 @@ int et_mha_kv_f16(const et_kv_cache *cache, const int32_t *table, int max_pages,
                   int flags, void *workspace, size_t workspace_bytes,
                   et_stream stream);
 
+/* The same over what a sliding window leaves, and the first tokens, which stay
+ * visible: row i of sequence b, at position p = starts[b] + i, sees a position k
+ * below starts[b] + counts[b] (with ET_MHA_CAUSAL up to p) if k > p - window or
+ * k < sinks.  window >= 1, sinks >= 0.  Pages that no row of the call sees are
+ * not looked up: their entries may be any number, and the pages another
+ * sequence's (et_kv_tables gives them back).  Everything else as
+ * et_mha_kv_f16. */
+int et_mha_kv_window_workspace(const et_kv_cache *cache, int max_pages, int B,
+                               int n, int nh, int window, int sinks,
+                               size_t *bytes);
+int et_mha_kv_window_f16(const et_kv_cache *cache, const int32_t *table,
+                         int max_pages, const int32_t *starts,
+                         const int32_t *counts, const et_f16 *Q, int ldq,
+                         et_f16 *Z, int ldz, int B, int n, int nh, int window,
+                         int sinks, float scale, int flags, void *workspace,
+                         size_t workspace_bytes, et_stream stream);
+
+/* ------------------------------------------------------------------------
+ * Several tokens guessed at once, as a tree (no reference counterpart).  Row i
+ * of sequence b, the token at position starts[b] + i of the cache, is node i,
+ * for i < counts[b] (starts, counts and rows as above): its key and value lie
+ * there whatever its depth.  parents [B][n]: the node's parent, a smaller
+ * number than its own; one that is not has none.  n is at most 256.
+ * ------------------------------------------------------------------------ */
+/* seen [B][n][(n + 31) / 32]: bit j % 32 of word j / 32 is set if node j is on
+ * node i's way up, itself included.  Rows from counts[b] on stay as they were. */
+int et_tree_seen(const int32_t *parents, const int32_t *counts, uint32_t *seen,
+                 int B, int n, et_stream stream);
+/* Attention of the nodes: node i sees all positions below starts[b], and
+ * position starts[b] + j if bit j of its row of `seen` is set and j < counts[b]
+ * (the bits may be any; et_tree_seen makes those of a tree).  window: 0, or at
+ * least n: of the positions below starts[b] node i then sees those above
+ * starts[b] + depth - window and those below sinks, depth the number of its
+ * bits less one: what it would see if its way up were the sequence.  Everything
+ * else as et_mha_kv_f16. */
+int et_mha_kv_tree_workspace(const et_kv_cache *cache, int max_pages, int B,
+                             int n, int nh, int window, int sinks,
+                             size_t *bytes);
+int et_mha_kv_tree_f16(const et_kv_cache *cache, const int32_t *table,
+                       int max_pages, const int32_t *starts,
+                       const int32_t *counts, const uint32_t *seen,
+                       const et_f16 *Q, int ldq, et_f16 *Z, int ldz, int B,
+                       int n, int nh, int window, int sinks, float scale,
+                       void *workspace, size_t workspace_bytes,
+                       et_stream stream);
+/* The path that stands.  tokens [B][n]: each node's token, choices [B][n]: the
+ * token that the model chose after it.  From node 0, which always stands, on to
+ * the first child whose token is the choice after the current node, as long as
+ * there is one.  path [B][n]: the nodes, then -1; kept [B]: how many;
+ * next_tokens [B]: the choice after the last; next_starts [B]: starts[b] + kept.
+ * counts[b] = 0: no node stands, next_tokens[b] = -1.  No output may be an
+ * input, but next_starts may be starts. */
+int et_tree_follow(const int32_t *parents, const int32_t *tokens,
+                   const int32_t *choices, const int32_t *starts,
+                   const int32_t *counts, int32_t *path, int32_t *kept,
+                   int32_t *next_tokens, int32_t *next_starts, int B, int n,
+                   et_stream stream);
+/* Keys and values of position starts[b] + path[b][r] to position starts[b] + r,
+ * for r < kept[b] (at most n), in ncaches caches of the same sizes (the layers
+ * of a model; host array) that share the table: all are read before any is
+ * written, so paths may be in any order.  A row whose path is not in [0, n), or
+ * either of whose positions has no place, is left out. */
+int et_kv_keep(const et_kv_cache *caches, int ncaches, const int32_t *table,
+               int max_pages, const int32_t *starts, const int32_t *path,
+               const int32_t *kept, int B, int n, et_stream stream);
+
+/* ------------------------------------------------------------------------
+ * Block tables and slot maps on the device, so that a step whose lengths only
+ * the device knows needs no host.  Sequence b brings counts[b] rows (at most n)
+ * from position starts[b] on; after the call its table holds pages for what
+ * these rows see, and no others: entry i is needed if i * page is below
+ * starts[b] + counts[b] and, where there is a window, i * page < sinks or
+ * (i + 1) * page > starts[b] - window + 1.  A sequence that is over has start
+ * and count 0.  before, table [B][max_pages] (may be the same): an entry
+ * outside [0, npages) holds none.
+ *   held and needed: stays;   held, not needed: -1, its page is given back;
+ *   needed, not held: a page that was free before the call, -1 if none is left
+ * shared (or NULL): the first shared[b] entries belong to others, too: they stay
+ * as they are.  A page must not be held twice otherwise.
+ * free_pages [npages] is a ring, free_state {head, count, ..}: pages are taken
+ * from free_pages[head], [head + 1], .. (modulo npages) in the order of
+ * (b, i) and given back behind the last in that order (those that the ring
+ * has no room for, which pages held twice can cause, are dropped);
+ * next_state [3] (may be free_state): head and count after the call, and how
+ * many pages were missing.
+ * slots (or NULL) [B][n]: page number * page + place in it of each row, -1 for
+ * rows from counts[b] on and for positions without a place; 8-byte aligned.
+ * workspace: et_kv_tables_workspace bytes, 8-byte aligned (NULL where 0).
+ * B = 0 passes the state on. */
+int et_kv_tables_workspace(int max_pages, int B, size_t *bytes);
+int et_kv_tables(const int32_t *before, int32_t *table, int max_pages, int page,
+                 int npages, const int32_t *starts, const int32_t *counts,
+                 const int32_t *shared, int B, int n, int window, int sinks,
+                 int32_t *free_pages, const int32_t *free_state,
+                 int32_t *next_state, int64_t *slots, void *workspace,
+                 size_t workspace_bytes, et_stream stream);
+
 /* Attention-aware pruning: W_V is row-pruned, so V arrives compact,
  * Vc[T x nnz_col] (row stride ldvc), holding only the surviving V columns.
  * v_col_id[nnz_col] (ascending) are their full-width positions and

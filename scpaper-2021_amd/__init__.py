@@ -130,6 +130,15 @@ _SIGNATURES = {
     "et_kv_read_f16": (_vp, _vp, _i, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _vp),
     "et_mha_kv_workspace": (_vp, _i, _i, _i, _i, C.POINTER(_sz)),
     "et_mha_kv_f16": (_vp, _vp, _i, _vp, _vp, _vp, _i, _vp, _i, _i, _i, _i, _f, _i, _vp, _sz, _vp),
+    "et_mha_kv_window_workspace": (_vp, _i, _i, _i, _i, _i, _i, C.POINTER(_sz)),
+    "et_mha_kv_window_f16": (_vp, _vp, _i, _vp, _vp, _vp, _i, _vp, _i, _i, _i, _i, _i, _i, _f, _i, _vp, _sz, _vp),
+    "et_tree_seen": (_vp, _vp, _vp, _i, _i, _vp),
+    "et_mha_kv_tree_workspace": (_vp, _i, _i, _i, _i, _i, _i, C.POINTER(_sz)),
+    "et_mha_kv_tree_f16": (_vp, _vp, _i, _vp, _vp, _vp, _vp, _i, _vp, _i, _i, _i, _i, _i, _i, _f, _vp, _sz, _vp),
+    "et_tree_follow": (_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _vp),
+    "et_kv_keep": (_vp, _i, _vp, _i, _vp, _vp, _vp, _i, _i, _vp),
+    "et_kv_tables_workspace": (_i, _i, C.POINTER(_sz)),
+    "et_kv_tables": (_vp, _vp, _i, _i, _i, _vp, _vp, _vp, _i, _i, _i, _i, _vp, _vp, _vp, _vp, _vp, _sz, _vp),
     "et_dense_to_w4_f16": (_vp, _vp, _vp, _i, _i, _i, _vp),
     "et_w4_to_dense_f16": (_vp, _vp, _vp, _i, _i, _i, _vp),
     "et_linear_w4_f16": (_vp, _vp, _i, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _vp),
@@ -439,6 +448,58 @@ def mha_kv_workspace(cache, max_pages, B, n, nh) -> int:
 def mha_kv(cache, table, max_pages, starts, counts, Q, ldq, Z, ldz, B, n, nh, scale, flags=0, workspace=None, workspace_bytes=0, stream=None):
     check(lib().et_mha_kv_f16(C.byref(cache), table, max_pages, starts, counts, Q, ldq, Z, ldz, B, n, nh, scale, flags,
                               workspace, workspace_bytes, stream))
+
+
+def mha_kv_window_workspace(cache, max_pages, B, n, nh, window, sinks) -> int:
+    """Bytes of device memory that mha_kv_window needs for these sizes."""
+    need = _sz()
+    check(lib().et_mha_kv_window_workspace(C.byref(cache), max_pages, B, n, nh, window, sinks, C.byref(need)))
+    return need.value
+
+
+def mha_kv_window(cache, table, max_pages, starts, counts, Q, ldq, Z, ldz, B, n, nh, window, sinks, scale, flags=0, workspace=None, workspace_bytes=0, stream=None):
+    check(lib().et_mha_kv_window_f16(C.byref(cache), table, max_pages, starts, counts, Q, ldq, Z, ldz, B, n, nh, window, sinks, scale, flags,
+                                     workspace, workspace_bytes, stream))
+
+
+def tree_seen(parents, counts, seen, B, n, stream=None):
+    check(lib().et_tree_seen(parents, counts, seen, B, n, stream))
+
+
+def mha_kv_tree_workspace(cache, max_pages, B, n, nh, window=0, sinks=0) -> int:
+    """Bytes of device memory that mha_kv_tree needs for these sizes."""
+    need = _sz()
+    check(lib().et_mha_kv_tree_workspace(C.byref(cache), max_pages, B, n, nh, window, sinks, C.byref(need)))
+    return need.value
+
+
+def mha_kv_tree(cache, table, max_pages, starts, counts, seen, Q, ldq, Z, ldz, B, n, nh, window, sinks, scale, workspace=None, workspace_bytes=0, stream=None):
+    check(lib().et_mha_kv_tree_f16(C.byref(cache), table, max_pages, starts, counts, seen, Q, ldq, Z, ldz, B, n, nh, window, sinks, scale,
+                                   workspace, workspace_bytes, stream))
+
+
+def tree_follow(parents, tokens, choices, starts, counts, path, kept, next_tokens, next_starts, B, n, stream=None):
+    check(lib().et_tree_follow(parents, tokens, choices, starts, counts, path, kept, next_tokens, next_starts, B, n, stream))
+
+
+def kv_keep(caches, table, max_pages, starts, path, kept, B, n, stream=None):
+    """caches: KvCaches of the same sizes, as a list or as a ctypes array (which costs the host less)."""
+    if not isinstance(caches, C.Array):
+        caches = (KvCache * len(caches))(*caches)
+    check(lib().et_kv_keep(caches, len(caches), table, max_pages, starts, path, kept, B, n, stream))
+
+
+def kv_tables_workspace(max_pages, B) -> int:
+    """Bytes of device memory that kv_tables needs for these sizes."""
+    need = _sz()
+    check(lib().et_kv_tables_workspace(max_pages, B, C.byref(need)))
+    return need.value
+
+
+def kv_tables(before, table, max_pages, page, npages, starts, counts, shared, B, n, window, sinks, free_pages, free_state, next_state, slots=None,
+              workspace=None, workspace_bytes=0, stream=None):
+    check(lib().et_kv_tables(before, table, max_pages, page, npages, starts, counts, shared, B, n, window, sinks, free_pages, free_state, next_state, slots,
+                             workspace, workspace_bytes, stream))
 
 
 def dense_to_w4(W, codes, scales, n_in, n_out, group, stream=None):
