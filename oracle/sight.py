@@ -58,24 +58,35 @@ def attention(cache, table, starts, counts, Q, n, nh, scale, sees):
     for b in range(B):
         count = min(max(int(counts[b]), 0), n)
         pos, k, v = cache.rows(table, b, int(starts[b]) + count)
-        for i in range(count):
-            r = b * n + i
-            seen = sees(b, i, pos)
-            if not seen.any():
-                Z[r] = stepped[r] = lows[r] = reach[r] = 0
-                continue
-            kc, ks, kl = (a[seen] for a in k)
-            key, size = stands_for(kc, ks, kl), rep(np.abs(ks)) * kc + rep(np.abs(kl))
-            step, low = rep(v[1][seen]) * v[0][seen], rep(v[2][seen])
-            q = Q[r].astype(np.float64).reshape(nh, hd)
-            for h in range(nh):
-                g, cols = h // per, slice(h * hd, (h + 1) * hd)
-                score = scale * (key[:, g] @ q[h])
-                p = np.exp(score - score.max())
-                p /= p.sum()
-                Z[r, cols] = p @ (step[:, g] + low[:, g])
-                stepped[r, cols], lows[r, cols] = p @ step[:, g], p @ np.abs(low[:, g])
-                reach[r, cols] = abs(scale) * (size[:, g] @ np.abs(q[h])).max()
+        rows = slice(b * n, b * n + count)
+        Z[rows] = stepped[rows] = lows[rows] = reach[rows] = 0
+        if not len(pos):
+            continue
+        seen = np.array([sees(b, i, pos) for i in range(count)], bool).reshape(count, len(pos))
+        key, size = stands_for(*k), rep(np.abs(k[1])) * k[0] + rep(np.abs(k[2]))
+        step, low = rep(v[1]) * v[0], rep(v[2])
+        for g in range(cache.nkv):
+            ok = np.isfinite(key[:, g]).all(1) & np.isfinite(step[:, g] + low[:, g]).all(1)
+            for h in range(g * per, (g + 1) * per):
+                cols = slice(h * hd, (h + 1) * hd)
+                q = Q[rows, cols].astype(np.float64)
+                # rows that see only numbers, all at once; of others what they see is picked out
+                whole = np.flatnonzero(seen.any(1) & ~(seen & ~ok).any(1) & np.isfinite(q).all(1))
+                at, r = seen[np.ix_(whole, ok)], b * n + whole
+                score = np.where(at, scale * (q[whole] @ key[ok, g].T), -np.inf)
+                p = np.exp(score - score.max(1, keepdims=True, initial=-np.inf))
+                p /= p.sum(1, keepdims=True)
+                Z[r, cols] = p @ (step[ok, g] + low[ok, g])
+                stepped[r, cols], lows[r, cols] = p @ step[ok, g], p @ np.abs(low[ok, g])
+                reach[r, cols] = abs(scale) * np.where(at, np.abs(q[whole]) @ size[ok, g].T, 0).max(1, keepdims=True, initial=0)
+                for i in np.setdiff1d(np.flatnonzero(seen.any(1)), whole):
+                    at, r = seen[i], b * n + i
+                    score = scale * (key[at, g] @ q[i])
+                    p = np.exp(score - score.max())
+                    p /= p.sum()
+                    Z[r, cols] = p @ (step[at, g] + low[at, g])
+                    stepped[r, cols], lows[r, cols] = p @ step[at, g], p @ np.abs(low[at, g])
+                    reach[r, cols] = abs(scale) * (size[at, g] @ np.abs(q[i])).max()
     return Z, stepped, lows, reach
 
 

@@ -91,7 +91,7 @@ int et_mha_kv_f16(const et_kv_cache *cache, const int32_t *table, int max_pages,
     ET_REQUIRE((flags & ~ET_MHA_CAUSAL) == 0, ET_ERR_INVALID_ARG, "et_mha_kv_f16: flags=%d", flags);
     KvMhaArgs a;
     a.causal = flags & ET_MHA_CAUSAL;
-    return kv_run<false>("et_mha_kv_f16", {cache, table, max_pages, starts, counts, Q, ldq, Z, ldz, B, n, nh, scale, workspace, workspace_bytes}, (long long)max_pages * cache->page, a, stream);
+    return kv_run<false>("et_mha_kv_f16", {cache, table, max_pages, starts, counts, Q, ldq, Z, ldz, B, n, nh, scale, workspace, workspace_bytes}, (long long)max_pages * cache->page, 0, a, stream);
 }
 
 }  // extern "C"

@@ -83,6 +83,7 @@ template <int BITS, int HD> struct KvShape {
 };
 
 constexpr float kNothing = -1e30f;
+constexpr float kNoReference = -1e29f;  // of rows that have seen nothing yet: a key that is not seen has no weight by it either
 
 // Weights of channel groups that share a reference: a group whose scales are far smaller than another's would have its weights among the subnormal binary16
 // numbers, where the second number of a weight holds nothing (300 keys, scales 2^20 apart: 3.5e-4 of the group's 2-norm instead of 2.1e-4, 2^22: 9e-4).  Where scales are more than 2^kLeastLift
@@ -640,7 +641,7 @@ template <int BITS, int HD, int NW, int P, bool SIGHT> __global__ __launch_bound
         qsum[g] = __builtin_ldexpf(rows_sum(sum), -key_unit_log2<BITS>());
     }
 
-    float ref = kNothing, l = 0.0f, z[SETS];
+    float ref = SIGHT ? kNoReference : kNothing, l = 0.0f, z[SETS];
     f4 acc[SETS][PRODUCTS];
     unsigned lift = 0;    // of the sets, four bits each: what acc is times 2^ of
     bool lifted = false;  // any of any row
@@ -751,11 +752,19 @@ template <int BITS, int HD, int NW, int P, bool SIGHT> __global__ __launch_bound
                 seen[e] = is ? ~0u : 0u;
                 y[e] = is ? y[e] : kNothing;
             }
+            if constexpr (SIGHT && HD <= 64) {
+#pragma unroll
+                for (int g = 0; g < SETS; g++)
+#pragma unroll
+                    for (int e = 0; e < 8; e++) vs[e >> 2][g][e & 3] &= seen[e];
+            }
         }
+        if constexpr (!SIGHT || HD > 64) {
 #pragma unroll
-        for (int g = 0; g < SETS; g++)
+            for (int g = 0; g < SETS; g++)
 #pragma unroll
-            for (int e = 0; e < 8; e++) vs[e >> 2][g][e & 3] &= seen[e];
+                for (int e = 0; e < 8; e++) vs[e >> 2][g][e & 3] &= seen[e];
+        }
         // the largest scale: they are not negative, and their bits in the low halves of the words go up with them
         typedef unsigned short s2 __attribute__((ext_vector_type(2)));
         auto halves = [](unsigned w) { return __builtin_bit_cast(s2, w); };  // (of an element of a vector, __builtin_bit_cast takes the vector's first)
@@ -836,7 +845,7 @@ template <int BITS, int HD, int NW, int P, bool SIGHT> __global__ __launch_bound
         float p[8];
 #pragma unroll
         for (int e = 0; e < 8; e++) {
-            p[e] = y[e] == kNothing ? 0.0f : __builtin_amdgcn_exp2f(y[e] - ref);
+            p[e] = !SIGHT && y[e] == kNothing ? 0.0f : __builtin_amdgcn_exp2f(y[e] - ref);
             l += p[e];
         }
 #pragma unroll
@@ -1315,22 +1324,27 @@ struct KvMhaCall {
     size_t workspace_bytes;
 };
 
-// a: what the form of attention adds.
-template <bool SIGHT> int kv_run(const char *fn, const KvMhaCall &call, long long positions, KvArgsOf<SIGHT> &a, et_stream stream) {
-    const et_kv_cache *cache = call.cache;
+// need: bytes of workspace.
+inline int kv_check_call(const char *fn, const KvMhaCall &call, size_t need) {
     // (scores stay below 1e30 in magnitude, which stands for minus infinity; 256 products of binary16 numbers reach 1.1e12)
     ET_REQUIRE(fabsf(call.scale) <= 1e15f, ET_ERR_INVALID_ARG, "%s: scale=%g", fn, (double)call.scale);
-    KvPlan<SIGHT> p;
-    const int sp = kv_plan<SIGHT>(fn, p, cache, positions, call.B, call.n, call.nh);
-    if (sp != ET_OK) return sp;
-    const long long width = (long long)call.nh * cache->hd;
+    const long long width = (long long)call.nh * call.cache->hd;
     ET_REQUIRE(call.ldq >= width && call.ldz >= width, ET_ERR_INVALID_ARG, "%s: row strides %d, %d below nh * hd = %lld", fn, call.ldq, call.ldz, width);
     ET_REQUIRE(call.ldq % 8 == 0 && call.ldz % 8 == 0, ET_ERR_UNSUPPORTED, "%s: row strides must be multiples of 8", fn);
     ET_REQUIRE(((reinterpret_cast<uintptr_t>(call.Q) | reinterpret_cast<uintptr_t>(call.Z)) & 15) == 0, ET_ERR_UNSUPPORTED, "%s: Q and Z must be 16-byte aligned", fn);
-    ET_REQUIRE(call.workspace_bytes >= p.bytes && (call.workspace || p.bytes == 0), ET_ERR_INVALID_ARG, "%s: a workspace of %zu bytes, %zu are needed", fn,
-               call.workspace ? call.workspace_bytes : 0, p.bytes);
-    ET_REQUIRE(p.bytes == 0 || (reinterpret_cast<uintptr_t>(call.workspace) & 15) == 0, ET_ERR_UNSUPPORTED, "%s: the workspace must be 16-byte aligned", fn);
-    if (call.B == 0 || call.n == 0) return ET_OK;
+    ET_REQUIRE(call.workspace_bytes >= need && (call.workspace || need == 0), ET_ERR_INVALID_ARG, "%s: a workspace of %zu bytes, %zu are needed", fn,
+               call.workspace ? call.workspace_bytes : 0, need);
+    ET_REQUIRE(need == 0 || (reinterpret_cast<uintptr_t>(call.workspace) & 15) == 0, ET_ERR_UNSUPPORTED, "%s: the workspace must be 16-byte aligned", fn);
+    return ET_OK;
+}
+
+// All of a kernel's arguments but what the form of attention, and of the kernel, adds; and how pieces of 16 keys come to pages.
+struct KvPieces {
+    unsigned magic, shift;
+    int of_page;
+};
+inline KvPieces kv_fill(const KvMhaCall &call, KvMhaArgs &a) {
+    const et_kv_cache *cache = call.cache;
     a.k_codes = static_cast<const char *>(cache->k_codes);
     a.v_codes = static_cast<const char *>(cache->v_codes);
     a.k_scales = reinterpret_cast<const unsigned *>(cache->k_scales);
@@ -1347,19 +1361,28 @@ template <bool SIGHT> int kv_run(const char *fn, const KvMhaCall &call, long lon
     a.npages = cache->npages;
     a.n = call.n;
     a.hd = cache->hd;
-    a.cols = p.form.cols;
-    a.block_rows = p.form.rows;
     a.units = call.B * cache->nkv;
-    a.splits = p.splits;
+    a.scale_log2e = call.scale * 1.4426950408889634f;
     // pieces below 2^27 (and a few tiles on): piece / d = piece * ceil(2^s / d) >> s with s = 28 + ceil(log2 d)
     const unsigned d = (unsigned)cache->page / 16;
     unsigned shift = 28;
     while ((1ull << (shift - 28)) < d) shift++;
-    const unsigned magic = (unsigned)(((1ull << shift) + d - 1) / d);
-    a.scale_log2e = call.scale * 1.4426950408889634f;
-    const int sl = launch_kernel("mha_kv_kernel", p.waves == 4 ? p.form.four : p.form.eight, dim3((unsigned)cache->nkv, (unsigned)call.B, (unsigned)(p.blocks * p.splits)), p.waves * 64, 0,
-                                 as_stream(stream), call.table, call.starts, call.counts, call.max_pages, a.units, a.splits, a.per, magic, shift, (int)d, call.n, a);
-    return sl != ET_OK || p.splits == 1 ? sl : kv_join(a, p.blocks, as_stream(stream));
+    return {(unsigned)(((1ull << shift) + d - 1) / d), shift, (int)d};
+}
+
+// need: bytes of workspace, as many as the plan's or more; a: what the form of attention adds.
+template <bool SIGHT> int kv_run(const char *fn, const KvMhaCall &call, long long positions, size_t need, KvArgsOf<SIGHT> &a, et_stream stream) {
+    KvPlan<SIGHT> p;
+    int st = kv_plan<SIGHT>(fn, p, call.cache, positions, call.B, call.n, call.nh);
+    if (st == ET_OK) st = kv_check_call(fn, call, std::max(need, p.bytes));
+    if (st != ET_OK || call.B == 0 || call.n == 0) return st;
+    const KvPieces pieces = kv_fill(call, a);
+    a.cols = p.form.cols;
+    a.block_rows = p.form.rows;
+    a.splits = p.splits;
+    st = launch_kernel("mha_kv_kernel", p.waves == 4 ? p.form.four : p.form.eight, dim3((unsigned)a.nkv, (unsigned)call.B, (unsigned)(p.blocks * p.splits)), p.waves * 64, 0, as_stream(stream),
+                       call.table, call.starts, call.counts, call.max_pages, a.units, a.splits, a.per, pieces.magic, pieces.shift, pieces.of_page, call.n, a);
+    return st != ET_OK || p.splits == 1 ? st : kv_join(a, p.blocks, as_stream(stream));
 }
 
 }  // namespace et

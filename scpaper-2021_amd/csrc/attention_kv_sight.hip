@@ -2,16 +2,16 @@
 //
 // A block of rows walks over the tiles that some of its rows see, those of the first tokens and from the earliest window on: pages in between are neither read nor looked up.  Keys are masked
 // one by one only in tiles that are not seen whole: at a window's beginning, at the end, and where the tree's own tokens lie, whose 32 bits a row and tile are two words of it.
-#include "attention_kv.hip.h"
+#include "attention_kv_tile.h"
 
 namespace et {
 namespace {
 
 // Positions that the rows of a block see at most, rounded up by a tile at either end.  (Rows that see what stands behind them see up to n more: their keys are shared out as those of rows
 // that do not, so that a workspace needs no flags.)
-long long sight_positions(const et_kv_cache *cache, int max_pages, int n, int window, int sinks) {
-    const long long all = (long long)max_pages * cache->page;
-    return window == 0 ? all : std::min(all, (long long)window + sinks + std::min(n, 16) + 128);
+long long sight_positions(const et_kv_cache *cache, int max_pages, int n, int nh, int window, int sinks) {
+    const long long all = (long long)max_pages * cache->page, apart = std::max(16, 256 / std::max(1, nh / cache->nkv));
+    return window == 0 ? all : std::min(all, (long long)window + sinks + std::min((long long)n, apart) + 128);
 }
 
 int check_window(const char *fn, int window, int sinks, int least) {
@@ -27,11 +27,29 @@ int check_tree(const char *fn, int n, int window, int sinks) {
     return check_window(fn, window, sinks, window == 0 ? 0 : n);
 }
 
+// Rows of a key/value head in the call.
+long long rows_of(const et_kv_cache *cache, int n, int nh) { return (long long)n * std::max(0, nh / cache->nkv); }
+
+// (The larger of what both kinds of kernel need where the rows are many: which of them runs depends on the positions, and a workspace is to do for fewer pages, too.)
 int sight_workspace(const char *fn, const et_kv_cache *cache, int max_pages, int B, int n, int nh, int window, int sinks, size_t *bytes) {
+    const long long positions = sight_positions(cache, max_pages, n, nh, window, sinks);
     KvPlan<true> p;
-    const int st = kv_plan<true>(fn, p, cache, sight_positions(cache, max_pages, n, window, sinks), B, n, nh);
-    if (st == ET_OK) *bytes = p.bytes;
+    int st = kv_plan<true>(fn, p, cache, positions, B, n, nh);
+    if (st != ET_OK) return st;
+    KvTilePlan tile;
+    tile.bytes = 0;
+    if (kv_tile_rows(cache->hd, rows_of(cache, n, nh))) st = kv_tile_plan(fn, tile, cache, positions, B, n, nh);
+    if (st == ET_OK) *bytes = std::max(p.bytes, tile.bytes);
     return st;
+}
+
+int sight_run(const char *fn, const KvMhaCall &call, KvSightArgs &a, et_stream stream) {
+    const long long positions = sight_positions(call.cache, call.max_pages, call.n, call.nh, a.window, a.sinks), rows = rows_of(call.cache, call.n, call.nh);
+    size_t need = 0;
+    const int st = sight_workspace(fn, call.cache, call.max_pages, call.B, call.n, call.nh, a.window, a.sinks, &need);
+    if (st != ET_OK) return st;
+    if (kv_tile_rows(call.cache->hd, rows) && kv_tile_work(call.cache, positions, call.B, rows)) return kv_tile_run(fn, call, positions, need, a, stream);
+    return kv_run<true>(fn, call, positions, need, a, stream);
 }
 
 }  // namespace
@@ -65,8 +83,7 @@ int et_mha_kv_window_f16(const et_kv_cache *cache, const int32_t *table, int max
     a.sinks = sinks;
     a.seen = nullptr;
     a.words = 0;
-    return kv_run<true>(fn, {cache, table, max_pages, starts, counts, Q, ldq, Z, ldz, B, n, nh, scale, workspace, workspace_bytes},
-                        sight_positions(cache, max_pages, n, window, sinks), a, stream);
+    return sight_run(fn, {cache, table, max_pages, starts, counts, Q, ldq, Z, ldz, B, n, nh, scale, workspace, workspace_bytes}, a, stream);
 }
 
 int et_mha_kv_tree_workspace(const et_kv_cache *cache, int max_pages, int B, int n, int nh, int window, int sinks, size_t *bytes) {
@@ -93,8 +110,7 @@ int et_mha_kv_tree_f16(const et_kv_cache *cache, const int32_t *table, int max_p
     a.sinks = sinks;
     a.seen = seen;
     a.words = (n + 31) / 32;
-    return kv_run<true>(fn, {cache, table, max_pages, starts, counts, Q, ldq, Z, ldz, B, n, nh, scale, workspace, workspace_bytes},
-                        sight_positions(cache, max_pages, n, window, sinks), a, stream);
+    return sight_run(fn, {cache, table, max_pages, starts, counts, Q, ldq, Z, ldz, B, n, nh, scale, workspace, workspace_bytes}, a, stream);
 }
 
 }  // extern "C"

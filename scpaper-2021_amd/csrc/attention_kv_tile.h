@@ -1,0 +1,23 @@
+// Attention over a cache for many rows a key/value head (attention_kv_tile.hip): what its callers need.
+#pragma once
+#include "attention_kv.hip.h"
+
+namespace et {
+
+struct KvTilePlan {
+    int blocks, splits;
+    size_t bytes;
+};
+template <int HD> constexpr int kTilePart = (2 + HD / 2) * 64;  // floats that a wave of a shared-out block leaves: references, sums, values, a lane's side by side with the others'
+
+// Whether the rows of a key/value head are many enough, and whether there is work enough: workgroups times 32 keys.  Against 16 rows a wave (attention_kv.hip.h), us, 4 bits (8 bits):
+//   heads of 128, 16 sequences of 2000, 8 heads: 64 rows 63.7 | 60.7 (60.5 | 63.7)   96 rows 64.0 | 83.5 (60.2 | 87.3)   256 rows 84.5 | 167 (86.0 | 176)   400 rows 131 | 266 (132 | 280)
+//   of 96, the same: 96 rows 63.9 | 63.6, 128 rows 65.1 | 68.1, 256 rows 82.7 | 123;   of 64, 16 heads: 64 rows 67.4 | 53.6, 96 rows 64.7 | 73.0, 256 rows 92.4 | 171;   of 32: 128 rows 61.1 | 58.2, 160 rows 66.4 | 70.5
+//   one sequence of 30000, 4 heads: of 128 96 rows 52.1 | 51.5, 256 rows 60.9 | 85.4;   of 64 128 rows 40.2 | 31.8, 256 rows 48.4 | 47.3, 400 rows 55.3 | 81.1
+//   8 heads of 128: 1 x 1000, 400 rows (496 of those units) 25.3 | 19.7;   2 x 4000, 128 rows (2000) 32.2 | 41.8;   4 x 3000, 128 rows (3000) 34.6 | 46.9
+bool kv_tile_rows(int hd, long long rows);
+bool kv_tile_work(const et_kv_cache *c, long long positions, int B, long long rows);
+int kv_tile_plan(const char *fn, KvTilePlan &p, const et_kv_cache *c, long long positions, int B, int n, int nh);
+int kv_tile_run(const char *fn, const KvMhaCall &call, long long positions, size_t need, KvSightArgs &a, et_stream stream);  // need: bytes of workspace; a: the rows' sight
+
+}  // namespace et

@@ -1,0 +1,592 @@
+// Attention over a cache of keys and values in 4 or 8 bits for many rows a key/value head: pieces of prompts and large trees (rows' sight: attention_kv_sight.hip).
+//
+// The other kernels multiply the codes themselves and apply a group's scale to every score and every weight, five vector instructions a score and group: with many rows that is what bounds
+// them.  Here a workgroup turns 32 keys and values at a time into binary16 numbers in LDS, each in two, high and low (rounded to one, results were off by 1.7 times their own rounding), and
+// its waves, 32 rows each, multiply those: the codes are taken apart once for all rows, and the rest is matrix products and the softmax.
+//
+//   S^T = K Q^T: rows of the product are keys, columns the wave's rows, so a lane ends with 16 of the 32 scores of one row, and the other half of the row is in the lane 32 away.
+//   Z^T = V^T P^T: rows are channels, columns the same rows again: what a lane scored are the very keys that it weighs, and a row's factors are a number of its lane.
+//
+// v / 2 = high + low: halved, since the rounding up of a scale may carry a group's last steps beyond binary16's range.  High is binary16, low, at most half its step, 8 bits (e5m2: products of
+// 8 bits take half the time).  S = high q + low q8; Z = high w + low w8 + high8 rest, w a weight in binary16, rest what that leaves, q8, w8, high8 the same in 8 bits; low times rest, 2^-22, is
+// left out.  With the low parts in binary16 as well, 4096 rows of 32 heads over 8 of 128, two sequences of 6000, took 370 us, this 336.
+//
+// One product a pair would be 104 us of those 336 at the 1352 TFLOP/s that a large binary16 product reaches; with the corrections it is 182.  The rest is vector work (the softmax, taking codes
+// apart) that the other half of the waves' products hide only in part.  Eight waves share a stage, since with four each stage served half as many rows; with 16 rows a wave LDS was read twice as
+// often.
+#include "attention_kv.hip.h"
+#include "attention_kv_tile.h"
+
+namespace et {
+
+namespace {
+
+constexpr float kLowUnit = 0x1p-11f;  // of low parts, and of what weights leave, in 8 bits: at most 16, half a step behind 2^15, which 2^-12 would take beyond their range
+constexpr int kLowUnitE8 = 127 - 11, kUnitE8 = 127;
+
+// LDS of a stage, in pieces of 16 bytes, for each 32 keys.  Keys: high parts [channel / 8, the even ones first][33 places of 32 keys], low parts in 8 bits [channel / 8 odd][channel / 32][33].
+// Values: high parts [keys / 8 of them][channel], low parts and high parts in 8 bits [keys of the lower or upper lanes][channel].
+template <int HD> struct TileShape {
+    static constexpr int kSets = HD <= 64 ? 2 : 1;  // of 32 keys
+    static constexpr int kTokens = 32 * kSets, kPieces = 2 * kSets;
+    static constexpr int kRow = 33;                 // 32 keys, and one on to other banks
+    static constexpr int kKeyLow = HD / 8 * kRow, kValue = kKeyLow + HD / 16 * kRow, kValueLow = kValue + 4 * HD, kValueHigh = kValueLow + 2 * HD, kSet = kValueHigh + 2 * HD;
+    static constexpr int kStage = kSets * kSet;
+    static constexpr int kShares = kTokens * HD / 16;  // of 16 numbers: of the keys, and as many of the values
+};
+constexpr int kWaves = 8;
+template <int HD> constexpr int tile_lds() {  // two stages; at the end a wave's rows lie there
+    constexpr int stages = 2 * TileShape<HD>::kStage, rows = (kWaves * 32 * (HD + 2) * 2 + 15) / 16;
+    return stages > rows ? stages : rows;
+}
+
+// The channel that place p of the values' channels holds: so that lanes with neighbouring units of 16 bits store neighbouring pieces.
+template <int BITS, int HD> __device__ __forceinline__ int place_channel(int p) {
+    constexpr int C = 16 / BITS, N = HD / C;
+    return p % N * C + p / N;
+}
+
+// Two codes, in the low bits of a word's halves, as halves of numbers: 512 + code / 2 has the code in its lowest bits.  (mask, base: in registers, so that both are put to use in one instruction.)
+__device__ __forceinline__ h2 half_codes(unsigned word, unsigned mask, unsigned base) { return __builtin_bit_cast(h2, (word & mask) | base) - h2{512, 512}; }
+// code / 2 * scale + low / 2 as high parts, and what they leave, times 2^11, in 8 bits: the lower or upper half of a word.  (minus: -1 that the compiler does not know, with which widening and
+// subtracting are one instruction.)
+typedef short s2 __attribute__((ext_vector_type(2)));
+template <bool UPPER> __device__ __forceinline__ void parted(h2 &high, unsigned &low, h2 code, h2 scale, h2 lowest, float minus) {
+    high = __builtin_elementwise_fma(code, scale, lowest);
+    float rest[2];
+#pragma unroll
+    for (int e = 0; e < 2; e++) rest[e] = __builtin_fmaf((float)high[e], minus, __builtin_fmaf((float)code[e], (float)scale[e], (float)lowest[e]));
+    low = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf8_f32(__builtin_bit_cast(s2, low), rest[0], rest[1], kLowUnit, UPPER));
+}
+// Of two tokens' words of a scale and a lowest value: both scales, and half of both lowest values.
+__device__ __forceinline__ h2 scales_of(unsigned a, unsigned b) { return __builtin_bit_cast(h2, __builtin_amdgcn_perm(b, a, 0x05040100u)); }
+__device__ __forceinline__ h2 half_lows_of(unsigned a, unsigned b) { return __builtin_bit_cast(h2, __builtin_amdgcn_perm(b, a, 0x07060302u)) * h2{0.5f, 0.5f}; }
+
+__device__ __forceinline__ unsigned word_of(h2 x) { return __builtin_bit_cast(unsigned, x); }
+
+// Every wave's LDS accesses are done.  (__syncthreads would wait for loads from memory, too, which are on their way for the next turn.)
+__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+__device__ __forceinline__ float across_max(float v) {
+    const unsigned u = __builtin_bit_cast(unsigned, v);
+    auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    return fmaxf(__builtin_bit_cast(float, (unsigned)r[0]), __builtin_bit_cast(float, (unsigned)r[1]));
+}
+__device__ __forceinline__ float across_sum(float v) {
+    const unsigned u = __builtin_bit_cast(unsigned, v);
+    auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    return __builtin_bit_cast(float, (unsigned)r[0]) + __builtin_bit_cast(float, (unsigned)r[1]);
+}
+
+// A wave's results [32 rows][HD], of lane l row l % 32, through LDS (rows of HD + 2 numbers) to Z.
+template <int BITS, int HD, int BLOCKS>
+__device__ __forceinline__ void rows_to_lds(_Float16 *lds, const f16v *acc, int first_block, float factor, bool none, int lane) {
+    _Float16 *row = lds + (lane & 31) * (HD + 2);
+#pragma unroll
+    for (int k = 0; k < BLOCKS; k++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) {
+            const float v = none ? 0.0f : acc[k][r] * factor;
+            row[place_channel<BITS, HD>(32 * (first_block + k) + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3))] = (_Float16)(v > 65504.0f ? 65504.0f : v);  // (as result_value)
+        }
+}
+template <int HD> __device__ __forceinline__ void rows_to_memory(const _Float16 *lds, const KvSightArgs &a, int b, int kv, int row0, int rows, int first, int step) {
+    for (int e = first; e < rows * (HD / 2); e += step) {
+        const int h = e / (HD / 2), w = e - h * (HD / 2), row = row0 + h, i = a.n == 1 ? 0 : row / a.per, r = row - i * a.per;
+        *reinterpret_cast<unsigned *>(a.Z + ((size_t)b * a.n + i) * a.ldz + (size_t)(kv * a.per + r) * HD + 2 * w) = *reinterpret_cast<const unsigned *>(lds + h * (HD + 2) + 2 * w);
+    }
+}
+
+// sums + (first, second) * x * 2^-11, 64 numbers of 8 bits.
+typedef int i8 __attribute__((ext_vector_type(8)));
+__device__ __forceinline__ f16v low_products(uint4 first, uint4 second, i8 x, f16v sums) {
+    const i8 y = {(int)first.x, (int)first.y, (int)first.z, (int)first.w, (int)second.x, (int)second.y, (int)second.z, (int)second.w};
+    return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(y, x, sums, 1, 1, 0, kLowUnitE8, 0, kUnitE8);
+}
+
+// Eight waves of 32 rows each.
+template <int BITS, int HD> __global__ __launch_bounds__(kWaves * 64, 2) void mha_kv_tile_kernel(KV_LEADING, const KvSightArgs a) {
+    using T = TileShape<HD>;
+    constexpr int TB = HD * BITS / 8, G = HD / 32, CHUNKS = HD / 16, BLOCKS = HD / 32, LOWS = (HD + 63) / 64, SETS = T::kSets, PIECES = T::kPieces, SHARES = T::kShares;
+    constexpr int TURNS = (2 * SHARES + kWaves * 64 - 1) / (kWaves * 64);  // a thread's shares of a stage
+    constexpr int AHEAD = HD == 128 ? 6 : 8;                      // pieces of a stage that are asked for ahead of the products that they are for, as far as there are registers
+    constexpr bool ALIKE = HD == 64 || HD == 128;                // a wave's shares are of one piece of 16 keys
+    __shared__ uint4 lds[tile_lds<HD>()];
+    __shared__ unsigned bad[3][SETS][G + 1];  // keys whose values are no numbers, of each group and of any; of this tile, the next, and one to clear
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int c = lane & 31, half = lane >> 5;
+    const int kv = blockIdx.x, b = blockIdx.y, nkv = gridDim.x;
+    const int block = splits == 1 ? blockIdx.z : blockIdx.z / splits, split = blockIdx.z - block * splits;
+
+    const int32_t *table = table_at + (size_t)b * max_pages;
+    // the rows of this block and of this wave, and what they see
+    const int start = starts_at ? ET_KV_CONST(int32_t, starts_at)[b] : 0;
+    const int count = counts_at ? min(max(ET_KV_CONST(int32_t, counts_at)[b], 0), n) : n;
+    const int first_row = block * (32 * kWaves), rows = min(32 * kWaves, count * per - first_row);
+    if (rows <= 0) return;
+    const long long most = (long long)max_pages * a.page;
+    const int end = (int)min(max((long long)start + count, 0LL), most);
+    auto row_of = [&](int row) { return n == 1 ? 0 : row / per; };  // of the call's rows
+    auto limit = [&](int i) { return a.causal ? (int)min((long long)end, max((long long)start + i + 1, 0LL)) : end; };
+    KvTiles<true, T::kTokens> tiles;
+    const int last_i = row_of(first_row + rows - 1);
+    tiles.around(a, start, count, row_of(first_row), last_i, limit(last_i));
+    const int v_end = tiles.end(limit(last_i));
+    const int row0 = first_row + 32 * wave, mine = min(32, rows - 32 * wave);  // (of the last block's waves some may have none: they fill the stages only)
+    const int wave_first = row_of(row0), wave_last = row_of(row0 + max(mine, 1) - 1);
+    const int lim_least = limit(wave_first), lim_most = mine > 0 ? limit(wave_last) : 0;
+    // positions of tiles that this wave's rows see some of, and all of
+    KvTiles<true, T::kTokens> near;
+    near.around(a, start, count, wave_first, wave_last, lim_most);
+    const int sees_first = near.head * T::kTokens, sees_from = (near.head + near.gap) * T::kTokens, sees_to = lim_most, whole_from = near.whole_from, whole_to = min(lim_least, near.whole_to);
+
+    // Pages of the pieces of the next tiles, a lane each, asked for 64 at a time: where they lie and which of them have one.  (Asked for tile by tile through the scalar cache, every wait for
+    // LDS in between waited for them as well.)
+    constexpr int TURNS_ASKED = 64 / PIECES;
+    int pages, offs, next_pages, next_offs;
+    auto ask = [&](int v) {
+        const int piece = PIECES * tiles.tile(v + lane / PIECES * splits) + lane % PIECES;
+        const int pidx = (int)(((unsigned long long)(unsigned)piece * magic) >> shift);
+        next_offs = (piece - pidx * page_pieces) << 4;
+        next_pages = pidx < max_pages ? table[pidx] : -1;
+    };
+    ask(split);
+
+    h8 q[CHUNKS];
+    const int row = min(row0 + min(c, max(mine, 1) - 1), first_row + rows - 1), i_row = row_of(row), r_row = row - i_row * per;
+    const int lim = limit(i_row);
+    KvSight<true> sight;
+    sight.of(a, b, n, i_row, start, count);
+    const _Float16 *qrow = a.Q + ((size_t)b * n + i_row) * a.ldq + (size_t)(kv * per + r_row) * HD + half * 8;
+    float top = 0.0f;
+#pragma unroll
+    for (int i = 0; i < CHUNKS; i++) {
+        q[i] = *reinterpret_cast<const h8 *>(qrow + 16 * i);
+#pragma unroll
+        for (int e = 0; e < 8; e++) top = fmaxf(top, fabsf((float)q[i][e]));
+    }
+    top = across_max(top);
+    const int up = top > 0.0f ? 15 - __builtin_amdgcn_frexp_expf(top) : 0;
+    const float grow = query_growth(top, up, a.scale_log2e);
+    const float key_scale = __builtin_ldexpf(fabsf(a.scale_log2e), 1 - up);
+#pragma unroll
+    for (int i = 0; i < CHUNKS; i++) {
+        // in the order that the keys' codes come out of their words
+        constexpr int order[2][8] = {{0, 4, 1, 5, 2, 6, 3, 7}, {0, 2, 1, 3, 4, 6, 5, 7}};
+        const h8 x = q[i];
+#pragma unroll
+        for (int e = 0; e < 8; e++) q[i][e] = (_Float16)((float)x[order[BITS == 8][e]] * grow);
+    }
+
+    // the same in 8 bits, for 64 channels at a time (none behind the last: zero)
+    i8 q8[LOWS];
+#pragma unroll
+    for (int i = 0; i < 4 * LOWS; i++)
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+            s2 w = {0, 0};
+            if (i < CHUNKS) {
+                const h8 x = q[i < CHUNKS ? i : 0];
+                w = __builtin_amdgcn_cvt_scalef32_pk_bf8_f32(w, (float)x[4 * e], (float)x[4 * e + 1], 1.0f, false);
+                w = __builtin_amdgcn_cvt_scalef32_pk_bf8_f32(w, (float)x[4 * e + 2], (float)x[4 * e + 3], 1.0f, true);
+            }
+            q8[i / 4][2 * (i % 4) + e] = __builtin_bit_cast(int, w);
+        }
+
+    const char *k_codes = a.k_codes + (size_t)kv * a.page * TB, *v_codes = a.v_codes + (size_t)kv * a.page * TB;
+    const unsigned *k_scales = a.k_scales + (size_t)kv * (G * a.page), *v_scales = a.v_scales + (size_t)kv * (G * a.page);
+    const unsigned page_bytes = (unsigned)nkv * a.page * TB, page_scales = (unsigned)nkv * G * a.page;
+
+    float minus = -1.0f;
+    unsigned mask = BITS == 4 ? 0x000f000fu : 0x00ff00ffu, base = 0x60006000u;
+    asm("" : "+s"(minus));
+    asm("" : "+v"(mask));
+    asm("" : "+v"(base));
+    // a tile's codes and scales, on their way
+    unsigned codes[TURNS][4], scales[TURNS][8];
+    unsigned code_at[TURNS], scale_at[TURNS];  // of a lane's shares, in their pieces
+#pragma unroll
+    for (int k = 0; k < TURNS; k++) {
+        const int s0 = (wave + k * kWaves) * 64, s = s0 + lane;
+        if (s0 < SHARES) {
+            const int key = s / (HD / 16), u = s - key * (HD / 16);
+            code_at[k] = (key & 15) * TB + u * (2 * BITS), scale_at[k] = (u >> 1) * a.page + (key & 15);
+        } else {
+            const int of = (s - SHARES) / (HD / 2), rest = s - SHARES - of * (HD / 2), unit = BITS == 4 ? rest % (HD / 4) : rest;
+            code_at[k] = (of & 1) * 4 * TB + unit * 8, scale_at[k] = (BITS == 4 ? unit >> 3 : unit >> 4) * a.page + (of & 1) * 4;
+        }
+    }
+    unsigned long long have = 0;  // pieces asked for that have pages
+    int turn = TURNS_ASKED;       // of those asked for, the next to fetch
+    unsigned ok = 0;              // of the tile that was fetched last: its pieces that have pages
+    auto fetch = [&](int v) {     // tile v of those counted without the gap
+        if (turn == TURNS_ASKED) {
+            const bool is = next_pages >= 0 && next_pages < a.npages;
+            have = __ballot(is);
+            pages = is ? next_pages : 0, offs = is ? next_offs : 0;
+            turn = 0;
+            ask(v + TURNS_ASKED * splits);
+        }
+        const int first = PIECES * turn++;
+        ok = (unsigned)(have >> first) & ((1u << PIECES) - 1);
+        auto pick = [&](int of, int piece) { return (unsigned)(ALIKE ? __builtin_amdgcn_readlane(of, first + piece) : __shfl(of, first + piece)); };
+#pragma unroll
+        for (int k = 0; k < TURNS; k++) {
+            const int s0 = (wave + k * kWaves) * 64, s = s0 + lane;
+            if (s0 < SHARES) {  // 16 channels of a key
+                const int piece = ALIKE ? s0 / (HD / 16) >> 4 : s / (HD / 16) >> 4;
+                const unsigned of_page = pick(pages, piece), at = pick(offs, piece);
+                unsigned w[BITS / 2];
+                load_words<BITS / 2>(w, k_codes + ((size_t)of_page * page_bytes + at * TB) + code_at[k]);
+#pragma unroll
+                for (int i = 0; i < BITS / 2; i++) codes[k][i] = w[i];
+                scales[k][0] = (k_scales + ((size_t)of_page * page_scales + at))[scale_at[k]];
+            } else if (s0 < 2 * SHARES) {  // two channels of the values of eight keys: 4 half .. and 8 + 4 half .. of a piece
+                const int piece = ALIKE ? (s0 - SHARES) / HD : (s - SHARES) / HD;
+                const unsigned of_page = pick(pages, piece), at = pick(offs, piece);
+                const char *p = v_codes + ((size_t)of_page * page_bytes + at * TB) + code_at[k];
+                const u2 x = *reinterpret_cast<const u2 *>(p), y = *reinterpret_cast<const u2 *>(p + 8 * TB);
+                codes[k][0] = x[0], codes[k][1] = x[1], codes[k][2] = y[0], codes[k][3] = y[1];
+                const unsigned *sc = v_scales + ((size_t)of_page * page_scales + at) + scale_at[k];
+                const u4 m = *reinterpret_cast<const u4 *>(sc), o = *reinterpret_cast<const u4 *>(sc + 8);
+#pragma unroll
+                for (int i = 0; i < 4; i++) scales[k][i] = m[i], scales[k][4 + i] = o[i];
+            }
+        }
+    };
+    // .. as numbers, in a stage
+    auto fill = [&](uint4 *stage, unsigned (*flags)[G + 1]) {
+#pragma unroll
+        for (int k = 0; k < TURNS; k++) {
+            __builtin_amdgcn_sched_barrier(0);  // (one after the other: two at once take more registers than there are)
+            const int s0 = (wave + k * kWaves) * 64, s = s0 + lane;
+            if (s0 < SHARES) {
+                const int key = s / (HD / 16), u = s - key * (HD / 16);
+                const h2 sc = scales_of(scales[k][0], scales[k][0]), lo = half_lows_of(scales[k][0], scales[k][0]);
+                uint4 *set = stage + (key >> 5) * T::kSet + (key & 31);
+#pragma unroll
+                for (int p = 0; p < 2; p++) {
+                    h2 high[4];
+                    unsigned low[2] = {0, 0};
+                    auto word = [&](int e) { return BITS == 4 ? codes[k][p] >> (4 * e) : codes[k][2 * p + (e >> 1)] >> (8 * (e & 1)); };
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
+                        parted<false>(high[2 * e], low[e], half_codes(word(2 * e), mask, base), sc, lo, minus);
+                        parted<true>(high[2 * e + 1], low[e], half_codes(word(2 * e + 1), mask, base), sc, lo, minus);
+                    }
+                    set[(p * (HD / 16) + u) * T::kRow] = uint4{word_of(high[0]), word_of(high[1]), word_of(high[2]), word_of(high[3])};
+                    reinterpret_cast<uint2 *>(set + T::kKeyLow + (p * (HD / 32) + (u >> 1)) * T::kRow)[u & 1] = uint2{low[0], low[1]};
+                }
+            } else if (s0 < 2 * SHARES) {
+                const int of = (s - SHARES) / (HD / 2), rest = s - SHARES - of * (HD / 2), unit = BITS == 4 ? rest % (HD / 4) : rest, pair = BITS == 4 ? rest / (HD / 4) : 0;
+                h2 high[2][4], sum = {0, 0};
+                unsigned low[2][2] = {};
+#pragma unroll
+                for (int x = 0; x < 4; x++) {  // tokens 2 x and the next
+                    const h2 sc = scales_of(scales[k][2 * x], scales[k][2 * x + 1]), lo = half_lows_of(scales[k][2 * x], scales[k][2 * x + 1]);
+                    const unsigned w = BITS == 4 ? codes[k][x] >> (8 * pair) : codes[k][x];
+#pragma unroll
+                    for (int i = 0; i < 2; i++) {
+                        const h2 code = half_codes(w >> (BITS * i), mask, base);
+                        if (x & 1) parted<true>(high[i][x], low[i][x >> 1], code, sc, lo, minus);
+                        else parted<false>(high[i][x], low[i][x >> 1], code, sc, lo, minus);
+                        sum = __builtin_elementwise_fma(high[i][x], h2{0, 0}, sum);
+                    }
+                }
+                // What is not a number, or infinite, must not meet the zero weight of a row that does not see it: it leaves the stage, and the rows that do see it are marked.
+                if (word_of(sum) != 0) {
+                    unsigned keys = 0;
+#pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        const bool is = (word_of(high[0][e >> 1]) >> (16 * (e & 1)) & 0x7c00u) == 0x7c00u || (word_of(high[1][e >> 1]) >> (16 * (e & 1)) & 0x7c00u) == 0x7c00u;
+                        if (is) {
+                            keys |= 1u << (16 * (of >> 1 & 1) + 4 * (of & 1) + (e & 3) + (e >> 2) * 8);
+#pragma unroll
+                            for (int i = 0; i < 2; i++) high[i][e >> 1][e & 1] = (_Float16)0.0f, low[i][e >> 2] &= ~(255u << (8 * (e & 3)));
+                        }
+                    }
+                    atomicOr(&flags[of >> 2][BITS == 4 ? unit >> 3 : unit >> 4], keys);
+                    atomicOr(&flags[of >> 2][G], keys);
+                }
+                uint4 *set = stage + (of >> 2) * T::kSet;
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    const int place = (BITS == 4 ? 2 * pair + i : i) * (HD / (16 / BITS)) + unit, keys = of & 1, part = of >> 1 & 1;
+                    set[T::kValue + (of & 3) * HD + place] = uint4{word_of(high[i][0]), word_of(high[i][1]), word_of(high[i][2]), word_of(high[i][3])};
+                    reinterpret_cast<uint2 *>(set + T::kValueLow + keys * HD + place)[part] = uint2{low[i][0], low[i][1]};
+                    // (the upper bytes of binary16 numbers are such numbers in 8 bits)
+                    reinterpret_cast<uint2 *>(set + T::kValueHigh + keys * HD + place)[part] =
+                        uint2{__builtin_amdgcn_perm(word_of(high[i][1]), word_of(high[i][0]), 0x07050301u), __builtin_amdgcn_perm(word_of(high[i][3]), word_of(high[i][2]), 0x07050301u)};
+                }
+            }
+        }
+    };
+
+    float ref = kNothing, l = 0.0f;
+    unsigned not_numbers = 0;  // groups of whose values this row sees some
+    f16v acc[BLOCKS];
+#pragma unroll
+    for (int k = 0; k < BLOCKS; k++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) acc[k][r] = 0.0f;
+
+    if (threadIdx.x < 3 * SETS * (G + 1)) (&bad[0][0][0])[threadIdx.x] = 0;
+    // Each turn computes a tile and fills in the next one: into the other stage, half of the waves before they compute and half behind, so that a SIMD has vector work beside matrix products.
+    // The first turn only fills in.
+    const bool early = wave < kWaves / 2;
+    int slot = 2, buffer = 1;
+    unsigned now = 0;  // pieces of the tile to compute that have pages
+    if (split < v_end) fetch(split);
+    for (int v = split - splits; v < v_end; v += splits) {
+        lds_barrier();
+        const int tile = tiles.tile(v) * T::kTokens, next_slot = slot == 2 ? 0 : slot + 1, clear_slot = next_slot == 2 ? 0 : next_slot + 1;
+        const bool more = v + splits < v_end;
+        const unsigned then = ok;
+        const uint4 *stage = lds + buffer * T::kStage;
+        if (threadIdx.x < SETS * (G + 1)) (&bad[clear_slot][0][0])[threadIdx.x] = 0;
+        auto go_on = [&]() {
+            fill(lds + (buffer ^ 1) * T::kStage, bad[next_slot]);
+            if (v + 2 * splits < v_end) fetch(v + 2 * splits);
+        };
+        if (early && more) go_on();
+        if (v >= split && tile < sees_to && (tile < sees_first || tile >= sees_from)) {
+            // (products go first: one takes one of eight turns to issue, and leaves the others to vector work of the SIMD's other wave, which would leave it none)
+            __builtin_amdgcn_s_setprio(1);
+            unsigned marked[SETS];
+            f16v s[SETS];
+#pragma unroll
+            for (int x = 0; x < SETS; x++) {
+                marked[x] = bad[slot][x][G];
+                s[x] = f16v{};
+                const uint4 *keys = stage + x * T::kSet + c;
+#pragma unroll
+                for (int i = 0; i < CHUNKS; i++) s[x] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, keys[(half * CHUNKS + i) * T::kRow]), q[i], s[x], 0, 0, 0);
+#pragma unroll
+                for (int i = 0; i < LOWS; i++) {
+                    const uint4 one = keys[T::kKeyLow + (half * (HD / 32) + 2 * i) * T::kRow], two = 2 * i + 1 < HD / 32 ? keys[T::kKeyLow + (half * (HD / 32) + 2 * i + 1) * T::kRow] : one;
+                    s[x] = low_products(one, two, q8[i], s[x]);
+                }
+            }
+            constexpr int READS = (CHUNKS + HD / 32) * SETS, EARLY = READS < AHEAD ? READS : AHEAD;
+            __builtin_amdgcn_sched_group_barrier(0x100, EARLY, 0);
+#pragma unroll
+            for (int i = 0; i < READS - EARLY; i++) {
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+            }
+            __builtin_amdgcn_sched_group_barrier(0x008, (CHUNKS + LOWS) * SETS - (READS - EARLY), 0);
+            __builtin_amdgcn_s_setprio(0);
+            const bool whole = tile + T::kTokens <= whole_to && (tile >= whole_from || tile + T::kTokens <= a.sinks) && now == (1u << PIECES) - 1;
+            unsigned seen[SETS];
+#pragma unroll
+            for (int x = 0; x < SETS; x++) seen[x] = ~0u;
+            if (!whole) {
+#pragma unroll
+                for (int x = 0; x < SETS; x++) {
+                    // (from the lane's first key on: what a register is compared with or shifted by is a constant then, and needs none itself)
+                    const int at = tile + 32 * x, first = at + 4 * half, to = lim - first, low = sight.low - first, sinks = a.sinks - first;
+                    const unsigned tree = sight.tree(a, at) >> (4 * half);
+                    unsigned keep = 0;
+#pragma unroll
+                    for (int r = 0; r < 16; r++) {
+                        const int key = 8 * (r >> 2) + (r & 3);
+                        const bool is = (now >> (2 * x + (r >> 3)) & 1u) && key < to && (key >= low || key < sinks) && (tree & 1u << key);
+                        keep |= is ? 1u << key : 0u;
+                        s[x][r] = is ? s[x][r] : kNothing;
+                    }
+                    seen[x] = keep;
+                }
+            }
+            float top = s[0][0];
+#pragma unroll
+            for (int e = 1; e < 16 * SETS; e++) top = fmaxf(top, s[e >> 4][e & 15]);
+            const float reach = across_max(top) * key_scale;
+            // a weight is at most 2^15; a row's reference moves by its own scores alone, so that its bits do not depend on the rows beside it
+            const bool moves = reach > ref + 15.0f;
+            if (__any(moves)) {
+                const float next = moves ? reach - 11.0f : ref, f = __builtin_amdgcn_exp2f(ref - next);
+                ref = next;
+                l *= f;
+#pragma unroll
+                for (int k = 0; k < BLOCKS; k++)
+#pragma unroll
+                    for (int r = 0; r < 16; r++) acc[k][r] *= f;
+            }
+#pragma unroll
+            for (int x = 0; x < SETS; x++)
+#pragma unroll
+                for (int r = 0; r < 16; r++) s[x][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x][r], key_scale, -ref));
+            if (!whole) {
+#pragma unroll
+                for (int e = 0; e < 16 * SETS; e++) s[e >> 4][e & 15] = seen[e >> 4] & 1u << (8 * (e >> 2 & 3) + (e & 3)) ? s[e >> 4][e & 15] : 0.0f;
+            }
+#pragma unroll
+            for (int x = 0; x < SETS; x++)
+                if (__builtin_amdgcn_readfirstlane(marked[x]) != 0) {
+#pragma unroll
+                    for (int g = 0; g < G; g++) not_numbers |= (bad[slot][x][g] >> (4 * half) & seen[x] & 0x0f0f0f0fu) != 0 ? 1u << g : 0u;
+                }
+            __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+            for (int x = 0; x < SETS; x++) {
+                h8 weights[2];
+                s2 eight[8];  // weights in 8 bits, and what the 16 leave
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    const float p0 = s[x][2 * e], p1 = s[x][2 * e + 1];
+                    unsigned w = word_of(h2{(_Float16)p0, (_Float16)p1});
+                    asm("" : "+v"(w));  // (or each half is rounded once more, on its own)
+                    const h2 wide = __builtin_bit_cast(h2, w);
+                    weights[e >> 2][2 * (e & 3)] = wide[0], weights[e >> 2][2 * (e & 3) + 1] = wide[1];
+                    const float r0 = __builtin_fmaf((float)wide[0], minus, p0), r1 = __builtin_fmaf((float)wide[1], minus, p1);
+                    s2 &whole = eight[e >> 1], &left = eight[4 + (e >> 1)];
+                    whole = e & 1 ? __builtin_amdgcn_cvt_scalef32_pk_bf8_f32(whole, p0, p1, 1.0f, true) : __builtin_amdgcn_cvt_scalef32_pk_bf8_f32(s2{0, 0}, p0, p1, 1.0f, false);
+                    left = e & 1 ? __builtin_amdgcn_cvt_scalef32_pk_bf8_f32(left, r0, r1, kLowUnit, true) : __builtin_amdgcn_cvt_scalef32_pk_bf8_f32(s2{0, 0}, r0, r1, kLowUnit, false);
+                    l += p0;
+                    l += p1;
+                }
+                i8 small;
+#pragma unroll
+                for (int e = 0; e < 8; e++) small[e] = __builtin_bit_cast(int, eight[e]);
+                const uint4 *values = stage + x * T::kSet + c;
+#pragma unroll
+                for (int m = 0; m < BLOCKS; m++) {
+                    acc[m] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, values[T::kValue + half * HD + 32 * m]), weights[0], acc[m], 0, 0, 0);
+                    acc[m] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, values[T::kValue + (2 + half) * HD + 32 * m]), weights[1], acc[m], 0, 0, 0);
+                    acc[m] = low_products(values[T::kValueLow + half * HD + 32 * m], values[T::kValueHigh + half * HD + 32 * m], small, acc[m]);
+                }
+            }
+            constexpr int VALUES = 4 * BLOCKS * SETS;
+            __builtin_amdgcn_sched_group_barrier(0x100, AHEAD < VALUES ? AHEAD : VALUES, 0);
+#pragma unroll
+            for (int i = 0; i < (VALUES - AHEAD) / 4; i++) {
+                __builtin_amdgcn_sched_group_barrier(0x008, 3, 0);
+                __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+            }
+        }
+        __builtin_amdgcn_s_setprio(0);
+        if (!early && more) go_on();
+        now = then;
+        slot = next_slot;
+        buffer ^= 1;
+    }
+
+    const float sum = across_sum(l);
+    not_numbers |= (unsigned)__shfl_xor((int)not_numbers, 32);
+    if (__any(not_numbers != 0)) {
+#pragma unroll
+        for (int m = 0; m < BLOCKS; m++)
+#pragma unroll
+            for (int r = 0; r < 16; r++)
+                if (not_numbers >> (place_channel<BITS, HD>(32 * m + 8 * (r >> 2) + 4 * half + (r & 3)) >> 5) & 1u) acc[m][r] = __builtin_nanf("");
+    }
+    if (splits > 1) {
+        if (mine <= 0) return;
+        float *part = a.parts + (((size_t)blockIdx.z * units + (unsigned)(b * nkv + kv)) * kWaves + wave) * kTilePart<HD> + lane;
+        part[0] = ref;
+        part[64] = sum;
+#pragma unroll
+        for (int m = 0; m < BLOCKS; m++)
+#pragma unroll
+            for (int r = 0; r < 16; r++) part[(2 + 16 * m + r) * 64] = acc[m][r];
+        return;
+    }
+    __syncthreads();  // the stages are read
+    if (mine <= 0) return;
+    _Float16 *mem = reinterpret_cast<_Float16 *>(lds) + wave * (32 * (HD + 2));
+    rows_to_lds<BITS, HD, BLOCKS>(mem, acc, 0, 2.0f / sum, sum == 0.0f, lane);
+    wave_lds_order();
+    rows_to_memory<HD>(mem, a, b, kv, row0, mine, lane, 64);
+}
+
+// The parts of 32 rows: a wave for each 32 channels.
+template <int BITS, int HD> __global__ __launch_bounds__(HD * 2) void mha_kv_tile_join_kernel(const KvSightArgs a) {
+    __shared__ _Float16 lds[32 * (HD + 2)];
+    const int lane = threadIdx.x & 63, m = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int unit = blockIdx.x, block = blockIdx.y, wave = blockIdx.z;
+    const int b = unit / a.nkv, kv = unit - b * a.nkv;
+    const int row0 = (block * kWaves + wave) * 32, rows = min(32, (a.counts ? min(max(a.counts[b], 0), a.n) : a.n) * a.per - row0);
+    if (rows <= 0) return;
+    const float *part = a.parts + (((size_t)block * a.splits * a.units + unit) * kWaves + wave) * kTilePart<HD> + lane;
+    const size_t next = (size_t)a.units * kWaves * kTilePart<HD>;
+    float ref = kNothing, l = 0.0f;
+    f16v acc = {};
+    for (int s0 = 0; s0 < a.splits; s0 += 4) {  // four parts asked for at once
+        float r[4], ls[4];
+        f16v vs[4];
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const float *p = part + (s0 + k < a.splits ? s0 + k : s0) * next;
+            r[k] = s0 + k < a.splits ? p[0] : kNothing;
+            ls[k] = p[64];
+#pragma unroll
+            for (int e = 0; e < 16; e++) vs[k][e] = p[(2 + 16 * m + e) * 64];
+        }
+        const float most = fmaxf(fmaxf(fmaxf(r[0], r[1]), fmaxf(r[2], r[3])), ref), was = __builtin_amdgcn_exp2f(ref - most);
+        ref = most;
+        l *= was;
+        acc *= was;
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const float f = s0 + k < a.splits ? __builtin_amdgcn_exp2f(r[k] - most) : 0.0f;
+            l = __builtin_fmaf(ls[k], f, l);
+#pragma unroll
+            for (int e = 0; e < 16; e++) acc[e] = __builtin_fmaf(f, vs[k][e], acc[e]);
+        }
+    }
+    rows_to_lds<BITS, HD, 1>(lds, &acc, m, 2.0f / l, l == 0.0f, lane);
+    __syncthreads();
+    rows_to_memory<HD>(lds, a, b, kv, row0, rows, threadIdx.x, HD * 2);
+}
+
+struct TileForm {
+    void (*kernel)(KV_LEADING, const KvSightArgs);
+    void (*join)(const KvSightArgs);
+};
+template <int BITS> TileForm tile_form(int hd) {
+    switch (hd) {
+        case 32: return {mha_kv_tile_kernel<BITS, 32>, mha_kv_tile_join_kernel<BITS, 32>};
+        case 64: return {mha_kv_tile_kernel<BITS, 64>, mha_kv_tile_join_kernel<BITS, 64>};
+        case 96: return {mha_kv_tile_kernel<BITS, 96>, mha_kv_tile_join_kernel<BITS, 96>};
+        default: return {mha_kv_tile_kernel<BITS, 128>, mha_kv_tile_join_kernel<BITS, 128>};
+    }
+}
+
+}  // namespace
+
+bool kv_tile_rows(int hd, long long rows) { return hd <= 128 && rows > (hd == 128 ? 64 : hd == 32 ? 128 : 96); }
+bool kv_tile_work(const et_kv_cache *c, long long positions, int B, long long rows) {
+    return (long long)B * c->nkv * ((rows + 32 * kWaves - 1) / (32 * kWaves)) * ((positions + 31) / 32) >= 1024;
+}
+
+int kv_tile_plan(const char *fn, KvTilePlan &p, const et_kv_cache *c, long long positions, int B, int n, int nh) {
+    ET_REQUIRE(nh > 0 && nh % c->nkv == 0, ET_ERR_INVALID_ARG, "%s: nh=%d must be a multiple of nkv=%d", fn, nh, c->nkv);
+    const long long rows = (long long)n * (nh / c->nkv), units = (long long)B * c->nkv;
+    const long long blocks = (rows + 32 * kWaves - 1) / (32 * kWaves), groups = units * blocks;
+    ET_REQUIRE(rows <= 0x7fffffffLL && B <= 65535 && blocks <= 65535 && groups <= (1LL << 24), ET_ERR_UNSUPPORTED, "%s: B=%d n=%d nh=%d", fn, B, n, nh);
+    p.blocks = (int)blocks;
+    const int tokens = c->hd <= 64 ? 64 : 32;
+    const long long tiles = (positions + tokens - 1) / tokens;
+    p.splits = groups == 0 ? 1 : (int)std::max(1LL, std::min({2048 / (groups * kWaves), tiles / 4, 256LL}));
+    p.splits = std::min(p.splits, (int)(65535 / std::max(1LL, blocks)));
+    p.bytes = p.splits > 1 ? (size_t)(groups * p.splits * kWaves) * (2 + c->hd / 2) * 64 * sizeof(float) : 0;
+    return ET_OK;
+}
+
+int kv_tile_run(const char *fn, const KvMhaCall &call, long long positions, size_t need, KvSightArgs &a, et_stream stream) {
+    KvTilePlan p;
+    int st = kv_tile_plan(fn, p, call.cache, positions, call.B, call.n, call.nh);
+    if (st == ET_OK) st = kv_check_call(fn, call, need);
+    if (st != ET_OK || call.B == 0 || call.n == 0) return st;
+    const KvPieces pieces = kv_fill(call, a);
+    a.cols = 1;
+    a.block_rows = 32 * kWaves;
+    a.splits = p.splits;
+    const TileForm f = call.cache->bits == 4 ? tile_form<4>(a.hd) : tile_form<8>(a.hd);
+    st = launch_kernel("mha_kv_tile_kernel", f.kernel, dim3((unsigned)a.nkv, (unsigned)call.B, (unsigned)(p.blocks * p.splits)), (unsigned)kWaves * 64, 0, as_stream(stream), call.table,
+                       call.starts, call.counts, call.max_pages, a.units, a.splits, a.per, pieces.magic, pieces.shift, pieces.of_page, call.n, a);
+    if (st != ET_OK || p.splits == 1) return st;
+    return launch_kernel("mha_kv_tile_join_kernel", f.join, dim3((unsigned)a.units, (unsigned)p.blocks, (unsigned)kWaves), (unsigned)a.hd * 2, 0, as_stream(stream), a);
+}
+
+}  // namespace et

@@ -59,16 +59,28 @@ def gone(table, page, starts, window, sinks):
     return table
 
 
-def near(got, Z, stepped, lows, reach, hd, keys, ldz_rest=None):
+def near(got, Z, stepped, lows, reach, hd, keys, rows):
+    """rows: of a key/value head.  Of more than 64, keys and values may enter the products as a binary16 number and what it leaves, at most half a step, 2^-11 of it, in 8 bits (e5m2, half a step
+    is 2^-3), times a factor in 8 bits: off by 2^-11 (2^-3 + 2^-3 + 2^-6) = 1.3e-4 of a score's terms.  Of a value's that is as much, and what a weight leaves, in 8 bits, times the upper
+    byte of the value (cut off: 2^-2): 2^-11 (2^-2 + 2^-3 + 2^-5) = 2.0e-4, in all 3.3e-4 of the sum of p |value|."""
     there = ~np.isnan(Z[:, 0])
     width = Z.shape[1]
     assert (got[:, width:] == -77).all() and (got[~there] == -77).all()
     d = np.abs(got[there, :width].astype(np.float64) - Z[there])
     lim = allowed(Z, stepped, lows, reach, hd, keys)[there]
+    if rows > 64:
+        lim += ((np.expm1(2 * 1.3e-4 * reach) + 3.3e-4) * (stepped + lows))[there]
     assert (d <= lim).all(), (np.nanmax(d / lim), np.argwhere(~(d <= lim))[:4])
 
 
-def check_window(et, bits, nkv, per, hd, page, lengths, n, window, sinks, causal, seed=0, qscale=1.0, starts=None, ldq=None, ldz=None, more_pages=0):
+def first(copies, got):
+    """The rows of the first of several batches that are alike, each of which gives the same bits."""
+    got = got.reshape(copies, -1, got.shape[-1])
+    assert np.array_equal(got, np.broadcast_to(got[0], got.shape), equal_nan=True)
+    return got[0]
+
+
+def check_window(et, bits, nkv, per, hd, page, lengths, n, window, sinks, causal, seed=0, qscale=1.0, starts=None, ldq=None, ldz=None, more_pages=0, copies=1):
     B, nh = len(lengths), nkv * per
     max_pages = max(1, -(-max(lengths) // page)) + more_pages
     npages = B * max_pages + 1
@@ -78,16 +90,17 @@ def check_window(et, bits, nkv, per, hd, page, lengths, n, window, sinks, causal
     counts = [l - s for l, s in zip(lengths, starts)]
     Q = (np.random.default_rng(seed + 3).standard_normal((B * n, nh * hd)) * qscale).astype(np.float16)
     scale = 1 / math.sqrt(hd)
-    got = run_window(et, DeviceCache(et, host), gone(table, page, starts, window, sinks), starts, counts, Q, B, n, nh, window, sinks, scale, causal, ldq, ldz)
+    got = first(copies, run_window(et, DeviceCache(et, host), np.tile(gone(table, page, starts, window, sinks), (copies, 1)), starts * copies, counts * copies, np.tile(Q, (copies, 1)), B * copies, n, nh,
+                                   window, sinks, scale, causal, ldq, ldz))
     want = S.attention(host, table, starts, counts, Q, n, nh, scale, S.window_sight(starts, counts, n, window, sinks, causal))
-    near(got, *want, hd, min(max(lengths), window + sinks + n))
+    near(got, *want, hd, min(max(lengths), window + sinks + n), n * per)
     return got, want[0]
 
 
-def check_tree(et, bits, nkv, per, hd, page, lengths, counts, n, window=0, sinks=0, seed=0, words=None, ldq=None, ldz=None):
+def check_tree(et, bits, nkv, per, hd, page, lengths, counts, n, window=0, sinks=0, seed=0, words=None, ldq=None, ldz=None, more_pages=0, copies=1):
     B, nh = len(lengths), nkv * per
     ends = [l + c for l, c in zip(lengths, counts)]
-    max_pages = max(1, -(-max(ends) // page))
+    max_pages = max(1, -(-max(ends) // page)) + more_pages
     npages = B * max_pages + 1
     table = tables(seed + 1, B, max_pages, npages)
     host = filled(bits, nkv, hd, page, table, ends, seed + 2, npages)
@@ -96,9 +109,10 @@ def check_tree(et, bits, nkv, per, hd, page, lengths, counts, n, window=0, sinks
     Q = np.random.default_rng(seed + 3).standard_normal((B * n, nh * hd)).astype(np.float16)
     scale = 1 / math.sqrt(hd)
     used = gone(table, page, lengths, window, sinks) if window else table
-    got = run_tree(et, DeviceCache(et, host), used, lengths, counts, words, Q, B, n, nh, window, sinks, scale, ldq, ldz)
+    got = first(copies, run_tree(et, DeviceCache(et, host), np.tile(used, (copies, 1)), lengths * copies, counts * copies, np.tile(words, (copies, 1, 1)), np.tile(Q, (copies, 1)), B * copies, n, nh, window,
+                                 sinks, scale, ldq, ldz))
     want = S.attention(host, table, lengths, counts, Q, n, nh, scale, S.tree_sight(lengths, counts, n, words, window, sinks))
-    near(got, *want, hd, max(ends))
+    near(got, *want, hd, max(ends), n * per)
     return got, want[0]
 
 
@@ -111,6 +125,47 @@ ROWS = [(1, 1), (4, 1), (2, 1), (3, 5), (1, 33), (4, 40)]
 @pytest.mark.parametrize("per,n", ROWS)
 def test_window_head_sizes(et, bits, hd, per, n):
     check_window(et, bits, 2, per, hd, 16, [197, 1, 70], n, 50, 3, n > 1, seed=hd)
+
+
+# many rows over a key/value head, and work for many workgroups
+MANY = [(4, 40), (1, 130), (8, 33), (3, 100), (1, 256)]
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("hd", [32, 64, 96, 128])
+@pytest.mark.parametrize("per,n", MANY)
+def test_window_many_rows(et, bits, hd, per, n):
+    check_window(et, bits, 2, per, hd, 16, [497, 1, 70], n, 50, 3, True, seed=hd, copies=64)
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("hd", [32, 64, 96, 128])
+@pytest.mark.parametrize("per,n", MANY)
+def test_tree_many_rows(et, bits, hd, per, n):
+    check_tree(et, bits, 2, per, hd, 16, [97, 0, 70], [n, n, max(1, n // 2)], n, seed=hd, copies=64)
+
+
+@pytest.mark.parametrize("page", [16, 48, 64])
+@pytest.mark.parametrize("window,sinks", [(1, 0), (2, 16), (31, 1), (32, 33), (33, 0), (64, 100), (65, 5), (1 << 30, 0)])
+def test_window_sizes_many_rows(et, page, window, sinks):
+    for bits, hd, per, n, causal in ((4, 128, 8, 9, True), (8, 64, 1, 100, False), (4, 96, 2, 77, True), (8, 32, 3, 50, True)):
+        check_window(et, bits, 1, per, hd, page, [300, 33, 64], n, window, sinks, causal, seed=page, copies=192)
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+def test_many_rows_shared_out(et, bits):
+    """Keys of many rows that several workgroups share: long contexts, and short ones beside tables for long ones."""
+    check_tree(et, bits, 2, 4, 128, 64, [18000, 9], [30, 17], 30, seed=5)
+    check_tree(et, bits, 1, 1, 64, 48, [70, 0, 600], [130, 99, 1], 130, seed=6, more_pages=400)
+    check_tree(et, bits, 2, 2, 96, 16, [9000, 30], [64, 64], 64, 8500, 20, seed=7, more_pages=3)
+    check_window(et, bits, 4, 2, 128, 64, [9000, 200], 50, 8600, 70, True, seed=8)
+    check_window(et, bits, 4, 3, 32, 16, [9000, 200], 50, 8600, 3, True, seed=9)
+    check_window(et, bits, 4, 1, 64, 64, [9000, 200], 200, 8600, 3, True, seed=10, starts=[8800, 0])
+
+
+def test_many_rows_strides(et):
+    check_window(et, 4, 2, 2, 96, 16, [140, 85], 70, 60, 2, True, seed=8, ldq=3 * 384 + 8, ldz=384 + 8, copies=192)
+    check_tree(et, 8, 2, 2, 128, 16, [140, 85], [70, 33], 70, seed=8, ldq=3 * 512 + 8, ldz=512 + 8, copies=64)
 
 
 @pytest.mark.parametrize("page", [16, 48, 64])
@@ -155,7 +210,7 @@ def test_window_behind_the_table(et):
     for start in (30, 40, 2 ** 31 - 3):
         got = run_window(et, dev, table, [start], [2], Q, 1, 2, 1, 12, 3, 0.1, True)
         want = S.attention(host, table, [min(start, 60)], [2], Q, 2, 1, 0.1, S.window_sight([min(start, 60)], [2], 2, 12, 3, True))
-        near(got, *want, 64, 32)
+        near(got, *want, 64, 32, 2)
 
 
 @pytest.mark.parametrize("bits", [4, 8])
@@ -171,11 +226,11 @@ def test_tree_sizes(et, n, page, lengths):
     check_tree(et, 4, 1, 1, 64, page, lengths, [n, max(0, n - 1), n // 2], n, seed=page + n)
 
 
-@pytest.mark.parametrize("hd,per,n", [(64, 1, 1), (64, 2, 1), (64, 1, 20), (128, 4, 9), (256, 1, 3), (32, 3, 40), (128, 8, 33)])
-def test_tree_with_a_window(et, hd, per, n):
+@pytest.mark.parametrize("hd,per,n,copies", [(64, 1, 1, 1), (64, 2, 1, 1), (64, 1, 20, 1), (128, 4, 9, 1), (256, 1, 3, 1), (32, 3, 40, 1), (128, 8, 33, 1), (128, 8, 33, 100), (64, 1, 100, 200), (32, 4, 40, 200)])
+def test_tree_with_a_window(et, hd, per, n, copies):
     """Measured from a node's depth: the oldest keys that a node sees depend on how deep it is."""
     for window in (n, n + 1, 60, 300):
-        check_tree(et, 4, 1, per, hd, 32, [280, 40, 0], [n, n, n], n, max(n, window), 5, seed=window)
+        check_tree(et, 4, 1, per, hd, 32, [280, 40, 0], [n, n, n], n, max(n, window), 5, seed=window, copies=copies)
 
 
 @pytest.mark.parametrize("bits", [4, 8])
@@ -191,9 +246,9 @@ def test_tree_of_any_bits(et):
     r = np.random.default_rng(1)
     words = r.integers(0, 2 ** 32, (2, 40, 2), dtype=np.uint32)
     words[0, 3] = 0
-    for per, hd in ((1, 64), (4, 128), (1, 32)):
-        check_tree(et, 4, 1, per, hd, 16, [70, 0], [40, 23], 40, seed=2, words=words)
-        check_tree(et, 4, 1, per, hd, 16, [70, 0], [40, 23], 40, 50, 3, seed=2, words=words)
+    for per, hd, copies in ((1, 64, 1), (4, 128, 1), (1, 32, 1), (4, 128, 256), (4, 32, 256), (3, 64, 256), (3, 96, 256)):
+        check_tree(et, 4, 1, per, hd, 16, [70, 0], [40, 23], 40, seed=2, words=words, copies=copies)
+        check_tree(et, 4, 1, per, hd, 16, [70, 0], [40, 23], 40, 50, 3, seed=2, words=words, copies=copies)
     words[1, 0] = 0
     got, Z = check_tree(et, 4, 1, 1, 64, 16, [70, 0], [40, 23], 40, seed=2, words=words)
     assert (Z[40] == 0).all() and (got[40] == 0).all()
@@ -213,14 +268,15 @@ def test_tree_that_is_a_chain_is_causal_attention(et):
 
 
 @pytest.mark.parametrize("bits", [4, 8])
-@pytest.mark.parametrize("hd,per,n", [(64, 1, 2), (32, 1, 4), (64, 3, 5), (128, 1, 2), (256, 2, 3), (128, 4, 40), (64, 1, 40), (96, 2, 40), (256, 1, 70)])
+@pytest.mark.parametrize("hd,per,n,copies", [(64, 1, 2, 1), (32, 1, 4, 1), (64, 3, 5, 1), (128, 1, 2, 1), (256, 2, 3, 1), (128, 4, 40, 1), (64, 1, 40, 1), (96, 2, 40, 1), (256, 1, 70, 1), (128, 4, 40, 64),
+                                             (64, 1, 130, 64), (96, 2, 70, 64), (32, 4, 40, 128)])
 @pytest.mark.parametrize("bad", [np.nan, np.inf])
-def test_not_a_number_where_others_look(et, bits, hd, per, n, bad):
+def test_not_a_number_where_others_look(et, bits, hd, per, n, copies, bad):
     """A node on nobody's way is NaN, and so are a token before the window and one between the first tokens and it: everyone else's rows are what they are without."""
     nkv, lengths = 2, [140, 64]
-    B, nh = len(lengths), nkv * per
-    table = tables(1, B, 20, 40)
-    host = filled(bits, nkv, hd, 16, table, [l + n for l in lengths], 4, 40)
+    nh, one = nkv * per, tables(1, 2, 20, 40)
+    host = filled(bits, nkv, hd, 16, one, [l + n for l in lengths], 4, 40)
+    table, B, lengths = np.tile(one, (copies, 1)), 2 * copies, lengths * copies
     Q = Hn.randn((B * n, nh * hd), 5)
     parents = np.tile(np.maximum(np.arange(n) - 1, 0), (B, 1)).astype(np.int32)
     parents[:, 0], parents[:, -1] = -1, max(0, n - 3)  # the last two are siblings, or the last is the root's child
@@ -229,26 +285,47 @@ def test_not_a_number_where_others_look(et, bits, hd, per, n, bad):
     tree = lambda: run_tree(et, DeviceCache(et, host), table, lengths, [n] * B, words, Q, B, n, nh, window, sinks, 0.1).reshape(B, n, -1)  # noqa: E731
     slide = lambda: run_window(et, DeviceCache(et, host), table, lengths, [n] * B, Q, B, n, nh, window, sinks, 0.1, True).reshape(B, n, -1)  # noqa: E731
     want, wide = tree(), slide()
-    row = np.full((B, nkv * hd), bad, np.float16)
+    row = np.full((2, nkv * hd), bad, np.float16)
     for pos in ([sinks] * B, [sinks + 9] * B, [l - window for l in lengths]):
-        host.write(table, pos, [int(sinks <= p <= l - window) for p, l in zip(pos, lengths)], row, row, 1)  # (a short sequence's window reaches to its beginning)
+        host.write(one, pos[:2], [int(sinks <= p <= l - window) for p, l in zip(pos[:2], lengths)], row, row, 1)  # (a short sequence's window reaches to its beginning)
     assert np.array_equal(tree(), want) and np.array_equal(slide(), wide)
     if n > 1:
-        host.write(table, [l + n - 1 for l in lengths], [1] * B, row, row, 1)
+        host.write(one, [l + n - 1 for l in lengths[:2]], [1, 1], row, row, 1)
         got, last = tree(), slide()
         assert np.array_equal(got[:, :-1], want[:, :-1]) and np.isnan(got[:, -1]).all()
         assert np.array_equal(last[:, :-1], wide[:, :-1]) and np.isnan(last[:, -1]).all()
 
 
-# (hd, key/value heads, query heads to each, rows, length)
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("hd", [32, 64, 96, 128])
+def test_each_key_has_its_own_weight(et, bits, hd):
+    """Of a sequence's values only one is not zero, 1, at another key for each sequence: the result is that key's weight, nothing at all for a row that does not see it."""
+    B, n, page, length = 128, 130, 16, 272
+    table = tables(1, B, 17, B * 17)
+    host = D.Cache(bits, 1, hd, page, B * 17)
+    r = np.random.default_rng(1)
+    K, V = r.standard_normal((length, hd)).astype(np.float16), np.zeros((B, length, hd), np.float16)
+    V[np.arange(B), length - B + np.arange(B)] = 1
+    host.write(table, [0] * B, [length] * B, np.tile(K, (B, 1)), V.reshape(-1, hd), length)
+    Q = r.standard_normal((n, hd)).astype(np.float16)
+    got = run_window(et, DeviceCache(et, host), table, [length - n] * B, [n] * B, np.tile(Q, (B, 1)), B, n, 1, 1 << 20, 0, 0.1, True).reshape(B, n, hd).astype(np.float64)
+    score = np.where(np.arange(length) <= length - n + np.arange(n)[:, None], 0.1 * Q.astype(np.float64) @ D.stands_for(*D.quantise(K, 2 ** bits - 1)).T, -np.inf)
+    p = np.exp(score - score.max(1, keepdims=True))
+    p = (p / p.sum(1, keepdims=True))[:, length - B:].T[:, :, None]
+    # a weight: half a step of the result; scores as for near(), their terms add up to less than 12 here
+    assert (got[np.broadcast_to(p, got.shape) == 0] == 0).all() and (np.abs(got - p) <= (2.0 ** -11 + np.expm1(2 * 1.3e-4 * 12) + 2.0 ** -13) * p + 2.0 ** -25).all()
+
+
+# (hd, key/value heads, query heads to each, rows, length, how many alike)
 FORMS = [(32, 2, 1, 1, 300), (64, 2, 1, 1, 300), (128, 2, 1, 1, 300), (64, 2, 2, 1, 300), (128, 2, 4, 1, 300), (256, 2, 2, 1, 300), (64, 2, 5, 2, 300), (96, 2, 16, 1, 300), (128, 2, 3, 4, 300),
          (192, 2, 8, 1, 300), (256, 2, 8, 1, 300), (128, 2, 8, 1, 2100), (64, 2, 1, 40, 300), (128, 1, 8, 20, 300), (32, 1, 4, 40, 300), (64, 1, 1, 70, 5000), (96, 1, 3, 70, 700),
-         (256, 1, 2, 70, 400), (160, 1, 4, 40, 300), (128, 1, 4, 64, 3500)]
+         (256, 1, 2, 70, 400), (160, 1, 4, 40, 300), (128, 1, 4, 64, 3500), (32, 1, 4, 40, 300, 160), (64, 1, 1, 130, 300, 160), (96, 1, 3, 70, 700, 100), (128, 1, 8, 20, 300, 160),
+         (128, 4, 1, 70, 20000)]
 
 
 def attended(et, bits, form, seed, qscale=1.0, values=lambda r, tokens, width: r.standard_normal((tokens, width)) * 0.5, keys=None):
     """(result, the same in binary64), [rows][heads][hd]: a window for odd seeds, a tree for even ones."""
-    hd, nkv, per, n, length = form
+    hd, nkv, per, n, length, copies = (*form, 1)[:6]
     r = np.random.default_rng(seed)
     width, nh = nkv * hd, nkv * per
     K = (r.standard_normal((length, width)) + 1.5 * r.standard_normal(width)).astype(np.float16)
@@ -263,15 +340,16 @@ def attended(et, bits, form, seed, qscale=1.0, values=lambda r, tokens, width: r
     host = D.Cache(bits, nkv, hd, page, max_pages, fill=0xFF)
     host.write(table, [0], [length], K, V, length)
     starts, counts, dev, scale = [length - n], [n], DeviceCache(et, host), 1 / math.sqrt(hd)
+    alike = lambda x: np.tile(x, (copies,) + (1,) * (np.ndim(x) - 1))  # noqa: E731
     if seed % 2:
         window, sinks = length // 2 + 11, 5
-        got = run_window(et, dev, table, starts, counts, Q, 1, n, nh, window, sinks, scale, True)
+        got = run_window(et, dev, alike(table), alike(starts), alike(counts), alike(Q), copies, n, nh, window, sinks, scale, True)
         Z = S.attention(host, table, starts, counts, Q, n, nh, scale, S.window_sight(starts, counts, n, window, sinks, True))[0]
     else:
         words = S.seen_words(trees(seed, 1, n), counts, n)
-        got = run_tree(et, dev, table, starts, counts, words, Q, 1, n, nh, 0, 0, scale)
+        got = run_tree(et, dev, alike(table), alike(starts), alike(counts), alike(words), alike(Q), copies, n, nh, 0, 0, scale)
         Z = S.attention(host, table, starts, counts, Q, n, nh, scale, S.tree_sight(starts, counts, n, words, 0, 0))[0]
-    return got.astype(np.float64).reshape(-1, nh, hd), Z.reshape(-1, nh, hd)
+    return first(copies, got).astype(np.float64).reshape(-1, nh, hd), Z.reshape(-1, nh, hd)
 
 
 def distance(got, Z):
@@ -357,7 +435,7 @@ def test_large_offsets(et):
         need = et.mha_kv_window_workspace(c, 2, 1, n, nkv, 90, 4)
         et.mha_kv_window(c, d_table, 2, up(et, np.array([length - n], np.int32)), None, up(et, Q), nkv * hd, z, nkv * hd, 1, n, nkv, 90, 4, 1 / 16, et.MHA_CAUSAL,
                          up(et, np.zeros(max(need, 16), np.uint8)), need)
-        near(z.numpy(), *S.attention(host, table, [length - n], [n], Q, n, nkv, 1 / 16, S.window_sight([length - n], [n], n, 90, 4, True)), hd, length)
+        near(z.numpy(), *S.attention(host, table, [length - n], [n], Q, n, nkv, 1 / 16, S.window_sight([length - n], [n], n, 90, 4, True)), hd, length, n)
     # the path moves there, too: the last token to where the second stands
     path, kept = up(et, np.array([[0, length - 1]], np.int32)), up(et, np.array([2], np.int32))
     start = up(et, np.array([0], np.int32))
