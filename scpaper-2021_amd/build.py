@@ -109,6 +109,7 @@ def build_all(jobs: int | None = None, verbose: bool = True) -> Path:
 # C++ programs written against the class layer (include/et/*.h) and linked with the library.
 PROGRAMS = {ROOT / "tests" / "cpp" / "class_layer_cases.cpp": ROOT / "tests" / "cpp" / "bin" / "class_layer_cases",
             ROOT / "tests" / "cpp" / "decode_cases.cpp": ROOT / "tests" / "cpp" / "bin" / "decode_cases",
+            ROOT / "tests" / "cpp" / "guess_cases.cpp": ROOT / "tests" / "cpp" / "bin" / "guess_cases",
             ROOT / "tests" / "cpp" / "cached_attention_sizes.cpp": ROOT / "tests" / "cpp" / "bin" / "cached_attention_sizes",
             PKG / "programs" / "et_sweeps.cpp": PKG / "bin" / "et_sweeps"}
 
