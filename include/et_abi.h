@@ -802,7 +802,8 @@ int et_tree_follow(const int32_t *parents, const int32_t *tokens,
  * for r < kept[b] (at most n), in ncaches caches of the same sizes (the layers
  * of a model; host array) that share the table: all are read before any is
  * written, so paths may be in any order.  A row whose path is not in [0, n), or
- * either of whose positions has no place, is left out. */
+ * either of whose positions has no place, is left out.  No cache may be given
+ * twice. */
 int et_kv_keep(const et_kv_cache *caches, int ncaches, const int32_t *table,
                int max_pages, const int32_t *starts, const int32_t *path,
                const int32_t *kept, int B, int n, et_stream stream);

@@ -2,7 +2,8 @@
 // they need and do not have come from its front, both in the order of (sequence, page), so that the result depends on nothing but the arguments.
 //
 // A wave takes a stretch of entries; what it gives and takes is placed by counting those of the waves before it.  Small tables are one workgroup's, in one launch; larger ones take two, since
-// no workgroup waits for another: the first counts, the second places.  Bound by launches and dependent accesses, and by the table's bytes where it is large.
+// no workgroup waits for another: the first counts, the second places.  Bound by a launch and dependent accesses (8 sequences of 64 pages: 4.4 us), and by the table's bytes where it is large:
+// 512 sequences of 8192 pages are read in 4.9 us (3.4 TB/s) and read and written in 10.9 (3.1 TB/s).  Sixteen entries at once for a lane rather than four changed neither.
 #include "common.hip.h"
 
 namespace et {

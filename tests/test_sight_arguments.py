@@ -80,6 +80,7 @@ def test_trees_and_paths(et):
                          ((two, 2, None, 4, None, P, P, 1, 4), -1), ((two, 2, P, 4, None, P, P, 1, 257), -2), ((two, 2, P, 4, None, P, P, 65536, 4), -2), ((two, 2, P, 4, None, P, P, 0, 4), 0),
                          ((two, 2, P, 4, None, P, P, 1, 0), 0)):
         assert lib.et_kv_keep(*args, None) == status, args
+    assert lib.et_kv_keep(two, 2, P, 4, None, P, P, 1, 4, None) == -1 and b"are the same" in lib.et_last_error()
 
 
 def test_block_tables(et):
