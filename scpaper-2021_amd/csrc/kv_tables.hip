@@ -22,7 +22,8 @@ struct TablesArgs {
 };
 
 constexpr int kOneWaves = 16, kManyWaves = 8;
-constexpr int kOneEntries = 16384, kOneSequences = 512;  // of tables that one workgroup takes
+// of tables that one workgroup takes (one launch|two, us: 512 entries 4.4|6.2, 2048 5.5|6.1, 4096 6.6|6.3, of 512 sequences 7.7|9.2, 8192 9.8|6.3, 16384 16.1|6.4)
+constexpr int kOneEntries = 4096, kOneSequences = 512;
 
 // The pages that a sequence needs: i < end, and i < first or i >= near.  Those before `own` are not its own to give or take.
 struct Needs {

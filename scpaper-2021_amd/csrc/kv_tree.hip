@@ -22,9 +22,9 @@ template <int W> __global__ __launch_bounds__(32 * W < 64 ? 64 : 32 * W) void tr
     __shared__ int up[2][32 * W];
     const int b = blockIdx.x, i = threadIdx.x, words = (n + 31) / 32;
     const int count = tree_count(counts, b, n);
+    const int p = parents[(size_t)b * n + min(i, n - 1)];  // (asked for without waiting for the count)
     const bool there = i < count;
-    const int p = there ? parents[(size_t)b * n + i] : -1;
-    int at = p >= 0 && p < i ? p : -1;
+    int at = there && p >= 0 && p < i ? p : -1;
     unsigned own[W];
 #pragma unroll
     for (int w = 0; w < W; w++) own[w] = i >> 5 == w ? 1u << (i & 31) : 0u;

@@ -1,7 +1,7 @@
 #!/usr/bin/env python3
 """Per-kernel throughput against the roofline that bounds it, through the C ABI.
 
-    python scpaper-2021_amd/kernel_bench.py [--set configs|scale|vo|mha|qkv|fuseo|plan|machine|decode|all] [--json FILE]
+    python scpaper-2021_amd/kernel_bench.py [--set configs|scale|vo|mha|qkv|fuseo|plan|machine|decode|guess|all] [--json FILE]
 
 `configs` are the shapes of the benchmark configurations (attention block at batch
 1/4/16, the tile/row/column-pruned Linears at 2048 token rows, the BERT-large-shaped
@@ -417,6 +417,64 @@ class Bench:
         us = self.time_us(lambda: et.mha_kv(cache, table, pages, starts, None, q, width, z, width, B, n, nh, hd ** -0.5, et.MHA_CAUSAL, ws, need, self.stream), launches)
         self.record("mha_kv", f"{bits} bits B{B} L{length} n{n} {nh}/{nkv} heads of {hd}", us, 2 * B * length * (nkv * hd * bits // 8 + nkv * hd // 32 * 4), "hbm")
 
+    def guess_attention(self, bits, B, length, n, nh, nkv, hd, page, window, sinks, tree, launches):
+        """Attention of a window's rows, or of a tree's nodes, which hang on one of the few before them."""
+        et = self.et
+        cache, table, pages, bufs = self.decode_cache(bits, B, length, nkv, hd, page, 0, 1)
+        starts, width = self.dev(np.full(B, length - n, np.int32)), nh * hd
+        q, z = self.dev(self.rnd((B * n, width))), self.empty((B * n, width))
+        where, shape = (cache, table, pages, starts, None), f"{bits} bits B{B} L{length} n{n} {nh}/{nkv} heads of {hd}" + (f" window {window} + {sinks}" if window else "")
+        seen = min(length, window + sinks + n) if window else length
+        bytes_, flops = 2 * B * seen * (nkv * hd * bits // 8 + nkv * hd // 32 * 4) + 4 * B * n * width, 4 * B * n * nh * hd * (min(length, window + sinks) if window else length)
+        work = (flops, "mfma") if flops / 1.35e15 > bytes_ / 5.1e12 else (bytes_, "hbm")
+        if not tree:
+            need = et.mha_kv_window_workspace(cache, pages, B, n, nh, window, sinks)
+            ws = et.DeviceBuffer(max(need, 16))
+            us = self.time_us(lambda: et.mha_kv_window(*where, q, width, z, width, B, n, nh, window, sinks, hd ** -0.5, et.MHA_CAUSAL, ws, need, self.stream), launches)
+            return self.record("mha_kv_window", shape, us, *work)
+        parents = np.arange(n) - 1 - self.rng.integers(0, 4, (B, n))
+        parents = self.dev(np.where(np.arange(n) == 0, -1, np.maximum(parents, 0)).astype(np.int32))
+        words = et.DeviceBuffer(B * n * -(-n // 32) * 4)
+        self.record("tree_seen", f"B{B} n{n}", self.time_us(lambda: et.tree_seen(parents, None, words, B, n, self.stream), launches), 4 * B * n * (1 + -(-n // 32)), "hbm")
+        need = et.mha_kv_tree_workspace(cache, pages, B, n, nh, window, sinks)
+        ws = et.DeviceBuffer(max(need, 16))
+        us = self.time_us(lambda: et.mha_kv_tree(*where, words, q, width, z, width, B, n, nh, window, sinks, hd ** -0.5, ws, need, self.stream), launches)
+        return self.record("mha_kv_tree", shape, us, *work)
+
+    def guess_accept(self, bits, B, n, depth, layers, nkv, hd, page, launches):
+        """The path that stands, `depth` nodes of a tree of n, and its tokens moved together in the layers' caches."""
+        et, pages = self.et, -(-n // page) + 1
+        caches = [self.decode_cache(bits, B, pages * page, nkv, hd, page, 0, 1) for _ in range(layers)]
+        table = caches[0][1]
+        path = np.sort(np.stack([self.rng.permutation(n)[:depth] for _ in range(B)]), 1)
+        path[:, 0] = 0
+        parents, tokens, choices = np.zeros((B, n), np.int32), np.full((B, n), -2, np.int32), np.full((B, n), -1, np.int32)
+        parents[:, 0] = -1
+        for b in range(B):
+            for at, to in zip(path[b][:-1], path[b][1:]):
+                parents[b, to], tokens[b, to], choices[b, at] = at, 7, 7
+        parents, tokens, choices = (self.dev(a) for a in (parents, tokens, choices))
+        starts, kept, following, moved = (self.dev(np.zeros(B, np.int32)) for _ in range(4))
+        out = self.dev(np.zeros((B, n), np.int32))
+        us = self.time_us(lambda: et.tree_follow(parents, tokens, choices, starts, None, out, kept, following, moved, B, n, self.stream), launches)
+        self.record("tree_follow", f"B{B} n{n} path of {depth}", us, 16 * B * n, "hbm")
+        token = 2 * (nkv * hd * bits // 8 + nkv * hd // 32 * 4)
+        us = self.time_us(lambda: et.kv_keep([c[0] for c in caches], table, pages, starts, out, kept, B, n, self.stream), launches)
+        self.record("kv_keep", f"{bits} bits B{B} n{n} path of {depth} {layers} x {nkv} heads of {hd}", us, 2 * B * (depth - 1) * layers * token, "hbm")
+
+    def guess_tables(self, B, max_pages, page, n, window, sinks, launches):
+        """Block tables of sequences that fill their tables."""
+        et, npages = self.et, B * max_pages
+        tables = [self.dev(np.full((B, max_pages), -1, np.int32)) for _ in range(2)]
+        ring, states = self.dev(np.arange(npages, dtype=np.int32)), [self.dev(np.array([0, npages, 0], np.int32)) for _ in range(2)]
+        starts, slots = self.dev(np.full(B, max_pages * page - n, np.int32)), et.DeviceBuffer(8 * B * n)
+        need = et.kv_tables_workspace(max_pages, B)
+        ws = et.DeviceBuffer(max(need, 16))
+        step = lambda a, b: et.kv_tables(tables[a], tables[b], max_pages, page, npages, starts, None, None, B, n, window, sinks, ring, states[a], states[b], slots, ws, need, self.stream)  # noqa: E731
+        step(0, 0)
+        us = self.time_us(lambda: step(0, 1), launches)
+        self.record("kv_tables", f"B{B} {max_pages} pages n{n} window {window} + {sinks}", us, 8 * B * max_pages + 8 * B * n, "hbm")
+
     def weight_to_w4(self, n_in, n_out, group, launches):
         """A weight to 4 bits, and what those stand for."""
         et = self.et
@@ -659,7 +717,7 @@ def run_scale(b: Bench):
 
 def main():
     ap = argparse.ArgumentParser()
-    ap.add_argument("--set", choices=("configs", "scale", "vo", "mha", "qkv", "fuseo", "local", "depth", "plan", "machine", "decode", "all"), default="all")
+    ap.add_argument("--set", choices=("configs", "scale", "vo", "mha", "qkv", "fuseo", "local", "depth", "plan", "machine", "decode", "guess", "all"), default="all")
     ap.add_argument("--json", default=None, help="also write the rows as JSON to this file")
     args = ap.parse_args()
     b = Bench()
@@ -732,6 +790,18 @@ def main():
             b.linear_w4(T, n_in, n_out, group, 10)
         for n_in, n_out, group in ((1024, 4096, 64), (4096, 4096, 32), (8192, 28672, 128)):
             b.weight_to_w4(n_in, n_out, group, 10)
+    if args.set == "guess":
+        print("# long contexts and guessed tokens over the cache: windows with first tokens, trees, the path that stands, block tables")
+        for bits, B, length, n, nh, nkv, hd, page, window, sinks, tree in (
+                (4, 8, 600, 1, 12, 12, 64, 16, 256, 4, False), (4, 64, 16000, 1, 16, 16, 64, 64, 4096, 4, False), (4, 2, 6000, 4096, 32, 8, 128, 128, 1024, 16, False),
+                (4, 1, 16384, 4096, 16, 16, 64, 64, 4096, 0, False), (8, 16, 1500, 13, 16, 8, 96, 48, 333, 5, False), (4, 1, 300, 8, 12, 12, 64, 16, 0, 0, True),
+                (4, 16, 2000, 27, 32, 8, 128, 64, 0, 0, True), (4, 64, 4096, 64, 16, 16, 64, 64, 0, 0, True), (8, 8, 16000, 16, 32, 8, 128, 128, 4096, 16, True),
+                (4, 1, 30000, 64, 32, 8, 128, 64, 0, 0, True)):
+            b.guess_attention(bits, B, length, n, nh, nkv, hd, page, window, sinks, tree, 10)
+        for bits, B, n, depth, layers, nkv, hd, page in ((4, 8, 16, 4, 1, 12, 64, 16), (8, 64, 64, 12, 6, 16, 64, 64), (4, 64, 64, 12, 12, 8, 128, 64)):
+            b.guess_accept(bits, B, n, depth, layers, nkv, hd, page, 20)
+        for B, max_pages, n, window, sinks in ((8, 64, 1, 0, 0), (64, 256, 16, 0, 0), (64, 2048, 16, 4096, 16), (512, 8192, 512, 4096, 16)):
+            b.guess_tables(B, max_pages, 16, n, window, sinks, 20)
     if args.set == "machine":
         print("# machine probes")
         b.machine()
