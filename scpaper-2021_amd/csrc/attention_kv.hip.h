@@ -240,7 +240,7 @@ template <bool SIGHT, int TILE> struct KvTiles {
             const int t_end = (lim_most + TILE - 1) / TILE;
             head = (min(a.sinks, lim_most) + TILE - 1) / TILE;
             gap = max(min((int)(max(low, 0LL) / TILE), t_end) - head, 0);
-            whole_from = (int)max(high, 0LL);
+            whole_from = (int)min(max(high, 0LL), 0x7fffffffLL);
         }
     }
     __device__ __forceinline__ int end(int lim_most) const { return ((lim_most + TILE - 1) >> (TILE == 64 ? 6 : 5)) - gap; }  // of the tiles counted without the gap
@@ -269,7 +269,7 @@ template <bool SIGHT> struct KvSight {
                     for (int w = 0; w < a.words; w++) own += __builtin_popcount(bits[w] & (count >= 32 * w + 32 ? ~0u : count <= 32 * w ? 0u : (1u << (count & 31)) - 1));
                 }
             }
-            if (a.window) low = (int)max((long long)start + own - a.window + 1, 0LL);
+            if (a.window) low = (int)min(max((long long)start + own - a.window + 1, 0LL), 0x7fffffffLL);
         }
     }
     // Bit e: position at + e, unless a window or a limit hides it (at is a multiple of 32).

@@ -15,6 +15,8 @@ template <int HD> constexpr int kTilePart = (2 + HD / 2) * 64;  // floats that a
 //   of 96, the same: 96 rows 63.9 | 63.6, 128 rows 65.1 | 68.1, 256 rows 82.7 | 123;   of 64, 16 heads: 64 rows 67.4 | 53.6, 96 rows 64.7 | 73.0, 256 rows 92.4 | 171;   of 32: 128 rows 61.1 | 58.2, 160 rows 66.4 | 70.5
 //   one sequence of 30000, 4 heads: of 128 96 rows 52.1 | 51.5, 256 rows 60.9 | 85.4;   of 64 128 rows 40.2 | 31.8, 256 rows 48.4 | 47.3, 400 rows 55.3 | 81.1
 //   8 heads of 128: 1 x 1000, 400 rows (496 of those units) 25.3 | 19.7;   2 x 4000, 128 rows (2000) 32.2 | 41.8;   4 x 3000, 128 rows (3000) 34.6 | 46.9
+//   8 sequences of 512 rows, 8 heads of 64, a window of 1 (1536 units) 25.3 | 17.0, 128 (2048) 27.1 | 23.4, 256 (2560) 30.2 | 28.3, 512 (3584) 35.5 | 37.3;   2 of 2048, 4 heads, 512 (1792) 27.8 | 20.8;   8 of 512, 8 heads of 96, 256 (2560) 38.2 | 37.8,
+//   512 (3584) 46.3 | 50.5;   of 128, a window of 1 (1536) 30.6 | 34.0, 512 48.4 | 69.2;   1 of 4096, 2 heads of 128 with four each, a window of 1 (1536) 34.9 | 33.9, 64 (1792) 29.6 | 36.8
 bool kv_tile_rows(int hd, long long rows);
 bool kv_tile_work(const et_kv_cache *c, long long positions, int B, long long rows);
 int kv_tile_plan(const char *fn, KvTilePlan &p, const et_kv_cache *c, long long positions, int B, int n, int nh);

@@ -11,9 +11,11 @@
 // 8 bits take half the time).  S = high q + low q8; Z = high w + low w8 + high8 rest, w a weight in binary16, rest what that leaves, q8, w8, high8 the same in 8 bits; low times rest, 2^-22, is
 // left out.  With the low parts in binary16 as well, 4096 rows of 32 heads over 8 of 128, two sequences of 6000, took 370 us, this 336.
 //
-// One product a pair would be 104 us of those 336 at the 1352 TFLOP/s that a large binary16 product reaches; with the corrections it is 182.  The rest is vector work (the softmax, taking codes
-// apart) that the other half of the waves' products hide only in part.  Eight waves share a stage, since with four each stage served half as many rows; with 16 rows a wave LDS was read twice as
-// often.
+// One product a pair would be 104 us of those 336 at the 1352 TFLOP/s that a large binary16 product reaches; with the corrections it is 182.  What bounds it is the vector work (360 instructions
+// a wave and 32 keys, a third of them to take codes apart) in the shadow of products: registers allow two waves a SIMD, and while one multiplies the other issues an instruction every eight
+// clocks, where two take one every four.  Eight waves share a stage, since with four each stage served half as many rows; with 16 rows a wave LDS was read twice as often.  Dealing stages out
+// to groups of two or four of the waves for up to 64 or 128 rows, each group with its own keys, changed little: for 64 rows of heads of 128 60.7 -> 50.0 us, of 64 with sequences of unequal
+// length 187 -> 275, for 128 rows of 128 65.8 -> 75.0.
 #include "attention_kv.hip.h"
 #include "attention_kv_tile.h"
 
@@ -556,7 +558,7 @@ template <int BITS> TileForm tile_form(int hd) {
 
 bool kv_tile_rows(int hd, long long rows) { return hd <= 128 && rows > (hd == 128 ? 64 : hd == 32 ? 128 : 96); }
 bool kv_tile_work(const et_kv_cache *c, long long positions, int B, long long rows) {
-    return (long long)B * c->nkv * ((rows + 32 * kWaves - 1) / (32 * kWaves)) * ((positions + 31) / 32) >= 1024;
+    return (long long)B * c->nkv * ((rows + 32 * kWaves - 1) / (32 * kWaves)) * ((positions + 31) / 32) >= (c->hd == 128 ? 1024 : 3072);
 }
 
 int kv_tile_plan(const char *fn, KvTilePlan &p, const et_kv_cache *c, long long positions, int B, int n, int nh) {

@@ -135,14 +135,14 @@ MANY = [(4, 40), (1, 130), (8, 33), (3, 100), (1, 256)]
 @pytest.mark.parametrize("hd", [32, 64, 96, 128])
 @pytest.mark.parametrize("per,n", MANY)
 def test_window_many_rows(et, bits, hd, per, n):
-    check_window(et, bits, 2, per, hd, 16, [497, 1, 70], n, 50, 3, True, seed=hd, copies=64)
+    check_window(et, bits, 2, per, hd, 16, [497, 1, 70], n, 50, 3, True, seed=hd, copies=128)
 
 
 @pytest.mark.parametrize("bits", [4, 8])
 @pytest.mark.parametrize("hd", [32, 64, 96, 128])
 @pytest.mark.parametrize("per,n", MANY)
 def test_tree_many_rows(et, bits, hd, per, n):
-    check_tree(et, bits, 2, per, hd, 16, [97, 0, 70], [n, n, max(1, n // 2)], n, seed=hd, copies=64)
+    check_tree(et, bits, 2, per, hd, 16, [97, 0, 70], [n, n, max(1, n // 2)], n, seed=hd, copies=128)
 
 
 @pytest.mark.parametrize("page", [16, 48, 64])
@@ -156,11 +156,11 @@ def test_window_sizes_many_rows(et, page, window, sinks):
 def test_many_rows_shared_out(et, bits):
     """Keys of many rows that several workgroups share: long contexts, and short ones beside tables for long ones."""
     check_tree(et, bits, 2, 4, 128, 64, [18000, 9], [30, 17], 30, seed=5)
-    check_tree(et, bits, 1, 1, 64, 48, [70, 0, 600], [130, 99, 1], 130, seed=6, more_pages=400)
-    check_tree(et, bits, 2, 2, 96, 16, [9000, 30], [64, 64], 64, 8500, 20, seed=7, more_pages=3)
+    check_tree(et, bits, 1, 1, 64, 48, [70, 0, 600], [130, 99, 1], 130, seed=6, more_pages=800)
+    check_tree(et, bits, 6, 2, 96, 16, [9000, 30], [64, 64], 64, 8500, 20, seed=7, more_pages=3)
     check_window(et, bits, 4, 2, 128, 64, [9000, 200], 50, 8600, 70, True, seed=8)
-    check_window(et, bits, 4, 3, 32, 16, [9000, 200], 50, 8600, 3, True, seed=9)
-    check_window(et, bits, 4, 1, 64, 64, [9000, 200], 200, 8600, 3, True, seed=10, starts=[8800, 0])
+    check_window(et, bits, 6, 3, 32, 16, [9000, 200], 50, 8600, 3, True, seed=9)
+    check_window(et, bits, 6, 1, 64, 64, [9000, 200], 200, 8600, 3, True, seed=10, starts=[8800, 0])
 
 
 def test_many_rows_strides(et):
@@ -213,6 +213,29 @@ def test_window_behind_the_table(et):
         near(got, *want, 64, 32, 2)
 
 
+@pytest.mark.parametrize("hd,per,n,copies", [(64, 1, 1, 1), (64, 1, 6, 1), (128, 2, 20, 1), (128, 1, 130, 512), (64, 1, 130, 1024)])
+def test_positions_beyond_32_bits(et, hd, per, n, copies):
+    """Rows whose positions, and windows' beginnings, lie behind 2^31 see the first tokens alone; so do the nodes of a tree there."""
+    host = filled(4, 1, hd, 16, np.array([[0, 1]], np.int32), [32], 1, 2)
+    dev, table, Q = DeviceCache(et, host), np.tile(np.array([[0, 1]], np.int32), (copies, 1)), np.tile(Hn.randn((n, per * hd), 1), (copies, 1))
+    words = np.tile(S.seen_words(np.arange(n, dtype=np.int32)[None] - 1, [n], n), (copies, 1, 1))
+    for start in (2 ** 31 - 1, 2 ** 31 - 3):
+        for window in (max(n, 2), 300):
+            got = [run_window(et, dev, table, [start] * copies, [n] * copies, Q, copies, n, per, window, 3, 0.1, True),
+                   run_tree(et, dev, table, [start] * copies, [n] * copies, words, Q, copies, n, per, window, 3, 0.1)]
+            want = S.attention(host, table[:1], [1000], [n], Q[:n], n, per, 0.1, S.window_sight([1000], [n], n, window, 3, True))
+            for z in got:
+                near(first(copies, z), *want, hd, 32, n * per)
+
+
+@pytest.mark.parametrize("hd,per,n", [(64, 1, 70), (128, 2, 60), (32, 3, 50)])
+def test_starts_in_front_of_the_sequence(et, hd, per, n):
+    """Rows in front of position 0 see nothing and become zero."""
+    for copies in (1, 256):
+        got, Z = check_window(et, 4, 1, per, hd, 16, [n - 30, 0, 14 + n], n, 20, 2, True, seed=3, starts=[-30, 0, 14], copies=copies)
+        assert (Z[:30] == 0).all() and (got[:30] == 0).all()
+
+
 @pytest.mark.parametrize("bits", [4, 8])
 @pytest.mark.parametrize("hd", [32, 64, 96, 128, 160, 192, 224, 256])
 @pytest.mark.parametrize("per,n", ROWS)
@@ -246,7 +269,7 @@ def test_tree_of_any_bits(et):
     r = np.random.default_rng(1)
     words = r.integers(0, 2 ** 32, (2, 40, 2), dtype=np.uint32)
     words[0, 3] = 0
-    for per, hd, copies in ((1, 64, 1), (4, 128, 1), (1, 32, 1), (4, 128, 256), (4, 32, 256), (3, 64, 256), (3, 96, 256)):
+    for per, hd, copies in ((1, 64, 1), (4, 128, 1), (1, 32, 1), (4, 128, 512), (4, 32, 512), (3, 64, 512), (3, 96, 512)):
         check_tree(et, 4, 1, per, hd, 16, [70, 0], [40, 23], 40, seed=2, words=words, copies=copies)
         check_tree(et, 4, 1, per, hd, 16, [70, 0], [40, 23], 40, 50, 3, seed=2, words=words, copies=copies)
     words[1, 0] = 0
@@ -269,7 +292,7 @@ def test_tree_that_is_a_chain_is_causal_attention(et):
 
 @pytest.mark.parametrize("bits", [4, 8])
 @pytest.mark.parametrize("hd,per,n,copies", [(64, 1, 2, 1), (32, 1, 4, 1), (64, 3, 5, 1), (128, 1, 2, 1), (256, 2, 3, 1), (128, 4, 40, 1), (64, 1, 40, 1), (96, 2, 40, 1), (256, 1, 70, 1), (128, 4, 40, 64),
-                                             (64, 1, 130, 64), (96, 2, 70, 64), (32, 4, 40, 128)])
+                                             (64, 1, 130, 128), (96, 2, 70, 128), (32, 4, 40, 128)])
 @pytest.mark.parametrize("bad", [np.nan, np.inf])
 def test_not_a_number_where_others_look(et, bits, hd, per, n, copies, bad):
     """A node on nobody's way is NaN, and so are a token before the window and one between the first tokens and it: everyone else's rows are what they are without."""
@@ -301,7 +324,7 @@ def test_not_a_number_where_others_look(et, bits, hd, per, n, copies, bad):
 def test_each_key_has_its_own_weight(et, bits, hd):
     """Of a sequence's values only one is not zero, 1, at another key for each sequence: the result is that key's weight, nothing at all for a row that does not see it."""
     B, n, page, length = 128, 130, 16, 272
-    table = tables(1, B, 17, B * 17)
+    table = np.hstack([tables(1, B, 17, B * 17), np.full((B, 60), -1, np.int32)])
     host = D.Cache(bits, 1, hd, page, B * 17)
     r = np.random.default_rng(1)
     K, V = r.standard_normal((length, hd)).astype(np.float16), np.zeros((B, length, hd), np.float16)
@@ -319,7 +342,7 @@ def test_each_key_has_its_own_weight(et, bits, hd):
 # (hd, key/value heads, query heads to each, rows, length, how many alike)
 FORMS = [(32, 2, 1, 1, 300), (64, 2, 1, 1, 300), (128, 2, 1, 1, 300), (64, 2, 2, 1, 300), (128, 2, 4, 1, 300), (256, 2, 2, 1, 300), (64, 2, 5, 2, 300), (96, 2, 16, 1, 300), (128, 2, 3, 4, 300),
          (192, 2, 8, 1, 300), (256, 2, 8, 1, 300), (128, 2, 8, 1, 2100), (64, 2, 1, 40, 300), (128, 1, 8, 20, 300), (32, 1, 4, 40, 300), (64, 1, 1, 70, 5000), (96, 1, 3, 70, 700),
-         (256, 1, 2, 70, 400), (160, 1, 4, 40, 300), (128, 1, 4, 64, 3500), (32, 1, 4, 40, 300, 160), (64, 1, 1, 130, 300, 160), (96, 1, 3, 70, 700, 100), (128, 1, 8, 20, 300, 160),
+         (256, 1, 2, 70, 400), (160, 1, 4, 40, 300), (128, 1, 4, 64, 3500), (32, 1, 4, 40, 300, 320), (64, 1, 1, 130, 300, 320), (96, 1, 3, 70, 700, 200), (128, 1, 8, 20, 300, 160),
          (128, 4, 1, 70, 20000)]
 
 
