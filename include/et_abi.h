@@ -743,7 +743,7 @@ int et_mha_kv_f16(const et_kv_cache *cache, const int32_t *table, int max_pages,
  * k < sinks.  window >= 1, sinks >= 0.  Pages that no row of the call sees are
  * not looked up: their entries may be any number, and the pages another
  * sequence's (et_kv_tables gives them back).  Everything else as
- * et_mha_kv_f16, but that with more than 64 rows to a key/value head (n * nh /
+ * et_mha_kv_f16, but that with more than 32 rows to a key/value head (n * nh /
  * nkv) keys, values and probabilities may enter the products as a binary16
  * number and 8 bits of what it leaves: a score's terms are then off by up to
  * 1.3e-4 of themselves, a result by up to 3.3e-4 of the sum of its

@@ -38,7 +38,8 @@ int sight_workspace(const char *fn, const et_kv_cache *cache, int max_pages, int
     if (st != ET_OK) return st;
     KvTilePlan tile;
     tile.bytes = 0;
-    if (kv_tile_rows(cache->hd, rows_of(cache, n, nh))) st = kv_tile_plan(fn, tile, cache, positions, B, n, nh);
+    const int waves = kv_tile_most_waves(cache->hd, rows_of(cache, n, nh));
+    if (waves) st = kv_tile_plan(fn, tile, cache, positions, B, n, nh, waves);
     if (st == ET_OK) *bytes = std::max(p.bytes, tile.bytes);
     return st;
 }
@@ -48,7 +49,8 @@ int sight_run(const char *fn, const KvMhaCall &call, KvSightArgs &a, et_stream s
     size_t need = 0;
     const int st = sight_workspace(fn, call.cache, call.max_pages, call.B, call.n, call.nh, a.window, a.sinks, &need);
     if (st != ET_OK) return st;
-    if (kv_tile_rows(call.cache->hd, rows) && kv_tile_work(call.cache, positions, call.B, rows)) return kv_tile_run(fn, call, positions, need, a, stream);
+    const int waves = kv_tile_waves(call.cache, positions, call.B, rows);
+    if (waves) return kv_tile_run(fn, call, positions, waves, need, a, stream);
     return kv_run<true>(fn, call, positions, need, a, stream);
 }
 

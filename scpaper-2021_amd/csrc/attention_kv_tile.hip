@@ -13,9 +13,11 @@
 //
 // One product a pair would be 104 us of those 336 at the 1352 TFLOP/s that a large binary16 product reaches; with the corrections it is 182.  What bounds it is the vector work (360 instructions
 // a wave and 32 keys, a third of them to take codes apart) in the shadow of products: registers allow two waves a SIMD, and while one multiplies the other issues an instruction every eight
-// clocks, where two take one every four.  Eight waves share a stage, since with four each stage served half as many rows; with 16 rows a wave LDS was read twice as often.  Dealing stages out
-// to groups of two or four of the waves for up to 64 or 128 rows, each group with its own keys, changed little: for 64 rows of heads of 128 60.7 -> 50.0 us, of 64 with sequences of unequal
-// length 187 -> 275, for 128 rows of 128 65.8 -> 75.0.
+// clocks, where two take one every four.  Eight waves share a stage, since with four each stage served half as many rows; with 16 rows a wave LDS was read twice as often.
+//
+// Up to 64 rows of heads of 128 two waves share a stage, and a workgroup is two such pairs, each with every other tile of its keys (16 nodes of 32 heads over 8, 8 bits, 8 sequences that see 4112
+// tokens: 60.9 -> 46.8 us).  The same for heads of 64 took 272 us where blocks of 16 rows took 371, 64 sequences of 4096 and 16 heads, but 209 where those took 180 with sequences and trees of
+// unequal size; four waves for up to 128 rows were within a tenth of eight, on either side.
 #include "attention_kv.hip.h"
 #include "attention_kv_tile.h"
 
@@ -28,6 +30,7 @@ constexpr int kLowUnitE8 = 127 - 11, kUnitE8 = 127;
 
 // LDS of a stage, in pieces of 16 bytes, for each 32 keys.  Keys: high parts [channel / 8, the even ones first][33 places of 32 keys], low parts in 8 bits [channel / 8 odd][channel / 32][33].
 // Values: high parts [keys / 8 of them][channel], low parts and high parts in 8 bits [keys of the lower or upper lanes][channel].
+constexpr int kWaves = 8;
 template <int HD> struct TileShape {
     static constexpr int kSets = HD <= 64 ? 2 : 1;  // of 32 keys
     static constexpr int kTokens = 32 * kSets, kPieces = 2 * kSets;
@@ -36,10 +39,12 @@ template <int HD> struct TileShape {
     static constexpr int kStage = kSets * kSet;
     static constexpr int kShares = kTokens * HD / 16;  // of 16 numbers: of the keys, and as many of the values
 };
-constexpr int kWaves = 8;
-template <int HD> constexpr int tile_lds() {  // two stages; at the end a wave's rows lie there
-    constexpr int stages = 2 * TileShape<HD>::kStage, rows = (kWaves * 32 * (HD + 2) * 2 + 15) / 16;
-    return stages > rows ? stages : rows;
+// W waves share a stage, each with 32 rows; GROUPS of them are a workgroup, each with its own keys.  A group of eight has two stages, others one.  At the end half of the groups' sums, then a
+// wave's rows, lie there.
+template <int HD, int W, int GROUPS> constexpr int tile_lds() {
+    constexpr int stages = (W == kWaves ? 2 : GROUPS) * TileShape<HD>::kStage, rows = (W * 32 * (HD + 2) * 2 + 15) / 16;
+    constexpr int sums = GROUPS == 1 ? 0 : GROUPS / 2 * W * kTilePart<HD> / 4;
+    return stages > rows ? (stages > sums ? stages : sums) : (rows > sums ? rows : sums);
 }
 
 // The channel that place p of the values' channels holds: so that lanes with neighbouring units of 16 bits store neighbouring pieces.
@@ -106,25 +111,46 @@ __device__ __forceinline__ f16v low_products(uint4 first, uint4 second, i8 x, f1
     return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(y, x, sums, 1, 1, 0, kLowUnitE8, 0, kUnitE8);
 }
 
-// Eight waves of 32 rows each.
-template <int BITS, int HD> __global__ __launch_bounds__(kWaves * 64, 2) void mha_kv_tile_kernel(KV_LEADING, const KvSightArgs a) {
+// GROUPS times W waves of 32 rows each.
+template <int BITS, int HD, int W, int GROUPS> __global__ __launch_bounds__(W * GROUPS * 64, 2) void mha_kv_tile_kernel(KV_LEADING, const KvSightArgs a) {
     using T = TileShape<HD>;
     constexpr int TB = HD * BITS / 8, G = HD / 32, CHUNKS = HD / 16, BLOCKS = HD / 32, LOWS = (HD + 63) / 64, SETS = T::kSets, PIECES = T::kPieces, SHARES = T::kShares;
-    constexpr int TURNS = (2 * SHARES + kWaves * 64 - 1) / (kWaves * 64);  // a thread's shares of a stage
-    constexpr int AHEAD = HD == 128 ? 6 : 8;                      // pieces of a stage that are asked for ahead of the products that they are for, as far as there are registers
-    constexpr bool ALIKE = HD == 64 || HD == 128;                // a wave's shares are of one piece of 16 keys
-    __shared__ uint4 lds[tile_lds<HD>()];
-    __shared__ unsigned bad[3][SETS][G + 1];  // keys whose values are no numbers, of each group and of any; of this tile, the next, and one to clear
+    constexpr int SLOTS = W == kWaves ? 3 : 2;
+    // What a thread takes apart of a stage.  Of eight waves some take a share of the keys, 16 channels of one, and as many a share of the values, two channels of eight tokens.  Of two each
+    // takes two shares of the keys, and a wide one of the values, four channels.
+    constexpr bool WIDE = W == 2;
+    static_assert(W == kWaves || (WIDE && HD == 128), "two waves have 2 * 128 and 128 shares");
+    constexpr int KEY_TURNS = WIDE ? 2 : 1, KEY_WORDS = BITS / 2 + 1, PAIRS = WIDE ? 2 : 1, VALUE_CODES = WIDE ? BITS : 4, UNITS = HD / 2 / PAIRS;
+    constexpr int KEYS_AT = WIDE ? VALUE_CODES + 8 : 0, WORDS = WIDE ? KEYS_AT + KEY_TURNS * KEY_WORDS : VALUE_CODES + 8;
+    constexpr int AHEAD = WIDE ? 4 : HD == 128 ? 6 : 8;  // pieces of a stage that are asked for ahead of the products that they are for, as far as there are registers
+    constexpr bool ALIKE = HD == 64 || HD == 128, VALUES_ALIKE = WIDE || ALIKE;  // a wave's shares are of one piece of 16 keys
+    __shared__ uint4 lds[tile_lds<HD, W, GROUPS>()];
+    constexpr bool Q8_APART = WIDE;  // queries in 8 bits are read from LDS: there are no registers for them
+    __shared__ uint4 q8_apart[Q8_APART ? W * LOWS * 2 : 1][64];
+    __shared__ unsigned all_marks[GROUPS == 1 ? 1 : W * GROUPS][64];
+    __shared__ unsigned all_bad[GROUPS][SLOTS][SETS][G + 1];  // keys whose values are no numbers, of each group of channels and of any; of this tile, the next, and one to clear
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int c = lane & 31, half = lane >> 5;
-    const int kv = blockIdx.x, b = blockIdx.y, nkv = gridDim.x;
+    const int c = lane & 31, half = lane >> 5, team = wave / W, member = wave % W;
+    auto &bad = all_bad[team];
+    const int kv = blockIdx.x, nkv = gridDim.x;
+    int b = blockIdx.y;
+    if (WIDE && starts_at && nkv * gridDim.y > 256 && gridDim.y <= 64) {
+        // the longest sequences first: of 64 of 0 to 2000 tokens and 8 heads, 64 rows, 107.6 us rather than 115.9 (of 2000 each 129.9 rather than 127.5)
+        const int B = gridDim.y, key = lane < B ? (int)((unsigned)starts_at[lane] + (counts_at ? (unsigned)counts_at[lane] : 0u)) : 0;
+        int rank = 0;
+        for (int j = 0; j < B; j++) {
+            const int other = __builtin_amdgcn_readlane(key, j);
+            rank += other > key || (other == key && j < lane) ? 1 : 0;
+        }
+        b = __builtin_ctzll(__ballot(lane < B && rank == b));
+    }
     const int block = splits == 1 ? blockIdx.z : blockIdx.z / splits, split = blockIdx.z - block * splits;
 
     const int32_t *table = table_at + (size_t)b * max_pages;
     // the rows of this block and of this wave, and what they see
     const int start = starts_at ? ET_KV_CONST(int32_t, starts_at)[b] : 0;
     const int count = counts_at ? min(max(ET_KV_CONST(int32_t, counts_at)[b], 0), n) : n;
-    const int first_row = block * (32 * kWaves), rows = min(32 * kWaves, count * per - first_row);
+    const int first_row = block * (32 * W), rows = min(32 * W, count * per - first_row);
     if (rows <= 0) return;
     const long long most = (long long)max_pages * a.page;
     const int end = (int)min(max((long long)start + count, 0LL), most);
@@ -134,7 +160,7 @@ template <int BITS, int HD> __global__ __launch_bounds__(kWaves * 64, 2) void mh
     const int last_i = row_of(first_row + rows - 1);
     tiles.around(a, start, count, row_of(first_row), last_i, limit(last_i));
     const int v_end = tiles.end(limit(last_i));
-    const int row0 = first_row + 32 * wave, mine = min(32, rows - 32 * wave);  // (of the last block's waves some may have none: they fill the stages only)
+    const int row0 = first_row + 32 * member, mine = min(32, rows - 32 * member);  // (of the last block's waves some may have none: they fill the stages only)
     const int wave_first = row_of(row0), wave_last = row_of(row0 + max(mine, 1) - 1);
     const int lim_least = limit(wave_first), lim_most = mine > 0 ? limit(wave_last) : 0;
     // positions of tiles that this wave's rows see some of, and all of
@@ -142,17 +168,20 @@ template <int BITS, int HD> __global__ __launch_bounds__(kWaves * 64, 2) void mh
     near.around(a, start, count, wave_first, wave_last, lim_most);
     const int sees_first = near.head * T::kTokens, sees_from = (near.head + near.gap) * T::kTokens, sees_to = lim_most, whole_from = near.whole_from, whole_to = min(lim_least, near.whole_to);
 
+    // tiles of this group: from `own` on, `step` apart
+    const int own = split * GROUPS + team, step = splits * GROUPS;
+
     // Pages of the pieces of the next tiles, a lane each, asked for 64 at a time: where they lie and which of them have one.  (Asked for tile by tile through the scalar cache, every wait for
     // LDS in between waited for them as well.)
     constexpr int TURNS_ASKED = 64 / PIECES;
     int pages, offs, next_pages, next_offs;
     auto ask = [&](int v) {
-        const int piece = PIECES * tiles.tile(v + lane / PIECES * splits) + lane % PIECES;
+        const int piece = PIECES * tiles.tile(v + lane / PIECES * step) + lane % PIECES;
         const int pidx = (int)(((unsigned long long)(unsigned)piece * magic) >> shift);
         next_offs = (piece - pidx * page_pieces) << 4;
         next_pages = pidx < max_pages ? table[pidx] : -1;
     };
-    ask(split);
+    ask(own);
 
     h8 q[CHUNKS];
     const int row = min(row0 + min(c, max(mine, 1) - 1), first_row + rows - 1), i_row = row_of(row), r_row = row - i_row * per;
@@ -195,6 +224,17 @@ template <int BITS, int HD> __global__ __launch_bounds__(kWaves * 64, 2) void mh
             q8[i / 4][2 * (i % 4) + e] = __builtin_bit_cast(int, w);
         }
 
+    if (Q8_APART && team == 0) {
+#pragma unroll
+        for (int i = 0; i < 2 * LOWS; i++) {
+            uint4 x;
+            unsigned *to = reinterpret_cast<unsigned *>(&x);
+#pragma unroll
+            for (int e = 0; e < 4; e++) to[e] = (unsigned)q8[i / 2][4 * (i % 2) + e];
+            q8_apart[member * LOWS * 2 + i][lane] = x;
+        }
+    }
+
     const char *k_codes = a.k_codes + (size_t)kv * a.page * TB, *v_codes = a.v_codes + (size_t)kv * a.page * TB;
     const unsigned *k_scales = a.k_scales + (size_t)kv * (G * a.page), *v_scales = a.v_scales + (size_t)kv * (G * a.page);
     const unsigned page_bytes = (unsigned)nkv * a.page * TB, page_scales = (unsigned)nkv * G * a.page;
@@ -204,20 +244,19 @@ template <int BITS, int HD> __global__ __launch_bounds__(kWaves * 64, 2) void mh
     asm("" : "+s"(minus));
     asm("" : "+v"(mask));
     asm("" : "+v"(base));
-    // a tile's codes and scales, on their way
-    unsigned codes[TURNS][4], scales[TURNS][8];
-    unsigned code_at[TURNS], scale_at[TURNS];  // of a lane's shares, in their pieces
-#pragma unroll
-    for (int k = 0; k < TURNS; k++) {
-        const int s0 = (wave + k * kWaves) * 64, s = s0 + lane;
-        if (s0 < SHARES) {
-            const int key = s / (HD / 16), u = s - key * (HD / 16);
-            code_at[k] = (key & 15) * TB + u * (2 * BITS), scale_at[k] = (u >> 1) * a.page + (key & 15);
-        } else {
-            const int of = (s - SHARES) / (HD / 2), rest = s - SHARES - of * (HD / 2), unit = BITS == 4 ? rest % (HD / 4) : rest;
-            code_at[k] = (of & 1) * 4 * TB + unit * 8, scale_at[k] = (BITS == 4 ? unit >> 3 : unit >> 4) * a.page + (of & 1) * 4;
-        }
-    }
+    // a tile's codes and scales, on their way: of values, then of keys
+    const bool takes_keys = WIDE || 64 * member < SHARES, takes_values = WIDE || (!takes_keys && 64 * member < 2 * SHARES);
+    const int key_share0 = 64 * member, value_share0 = WIDE ? key_share0 : 64 * member - SHARES;
+    unsigned words[WORDS];
+    // (a wide share of 8-bit values is two units of 16 bits a token side by side; of 4-bit values one, whose upper half narrow shares leave to another thread)
+    struct ValueShare {
+        int of, unit, pair, group;
+    };
+    auto value_share = [&](int lane) {
+        const int of = (value_share0 + lane) / UNITS, rest = value_share0 + lane - of * UNITS;
+        const int unit = WIDE ? BITS / 4 * rest : BITS == 4 ? rest % (HD / 4) : rest;
+        return ValueShare{of, unit, WIDE || BITS == 8 ? 0 : rest / (HD / 4), BITS == 4 ? unit >> 3 : unit >> 4};
+    };
     unsigned long long have = 0;  // pieces asked for that have pages
     int turn = TURNS_ASKED;       // of those asked for, the next to fetch
     unsigned ok = 0;              // of the tile that was fetched last: its pieces that have pages
@@ -227,50 +266,60 @@ template <int BITS, int HD> __global__ __launch_bounds__(kWaves * 64, 2) void mh
             have = __ballot(is);
             pages = is ? next_pages : 0, offs = is ? next_offs : 0;
             turn = 0;
-            ask(v + TURNS_ASKED * splits);
+            ask(v + TURNS_ASKED * step);
         }
+        int lane_now = lane;
+        if (WIDE) asm("" : "+v"(lane_now));  // (what follows from it is worked out anew each time: kept, it takes registers that there are not)
         const int first = PIECES * turn++;
         ok = (unsigned)(have >> first) & ((1u << PIECES) - 1);
-        auto pick = [&](int of, int piece) { return (unsigned)(ALIKE ? __builtin_amdgcn_readlane(of, first + piece) : __shfl(of, first + piece)); };
+        auto pick = [&](int of, int piece, bool alike) { return (unsigned)(alike ? __builtin_amdgcn_readlane(of, first + piece) : __shfl(of, first + piece)); };
+        if (takes_keys) {
 #pragma unroll
-        for (int k = 0; k < TURNS; k++) {
-            const int s0 = (wave + k * kWaves) * 64, s = s0 + lane;
-            if (s0 < SHARES) {  // 16 channels of a key
-                const int piece = ALIKE ? s0 / (HD / 16) >> 4 : s / (HD / 16) >> 4;
-                const unsigned of_page = pick(pages, piece), at = pick(offs, piece);
+            for (int k = 0; k < KEY_TURNS; k++) {
+                const int s0 = key_share0 + 128 * k;
+                const int s = s0 + lane_now, key = s / (HD / 16), u = s - key * (HD / 16), piece = (ALIKE ? s0 : s) / (HD / 16) >> 4;
+                const unsigned of_page = pick(pages, piece, ALIKE), at = pick(offs, piece, ALIKE);
                 unsigned w[BITS / 2];
-                load_words<BITS / 2>(w, k_codes + ((size_t)of_page * page_bytes + at * TB) + code_at[k]);
+                load_words<BITS / 2>(w, k_codes + ((size_t)of_page * page_bytes + at * TB) + (unsigned)((key & 15) * TB + u * (2 * BITS)));
 #pragma unroll
-                for (int i = 0; i < BITS / 2; i++) codes[k][i] = w[i];
-                scales[k][0] = (k_scales + ((size_t)of_page * page_scales + at))[scale_at[k]];
-            } else if (s0 < 2 * SHARES) {  // two channels of the values of eight keys: 4 half .. and 8 + 4 half .. of a piece
-                const int piece = ALIKE ? (s0 - SHARES) / HD : (s - SHARES) / HD;
-                const unsigned of_page = pick(pages, piece), at = pick(offs, piece);
-                const char *p = v_codes + ((size_t)of_page * page_bytes + at * TB) + code_at[k];
-                const u2 x = *reinterpret_cast<const u2 *>(p), y = *reinterpret_cast<const u2 *>(p + 8 * TB);
-                codes[k][0] = x[0], codes[k][1] = x[1], codes[k][2] = y[0], codes[k][3] = y[1];
-                const unsigned *sc = v_scales + ((size_t)of_page * page_scales + at) + scale_at[k];
-                const u4 m = *reinterpret_cast<const u4 *>(sc), o = *reinterpret_cast<const u4 *>(sc + 8);
-#pragma unroll
-                for (int i = 0; i < 4; i++) scales[k][i] = m[i], scales[k][4 + i] = o[i];
+                for (int i = 0; i < BITS / 2; i++) words[KEYS_AT + KEY_WORDS * k + i] = w[i];
+                words[KEYS_AT + KEY_WORDS * k + BITS / 2] = (k_scales + ((size_t)of_page * page_scales + at))[(unsigned)((u >> 1) * a.page + (key & 15))];
             }
+        }
+        if (takes_values) {  // of the values of eight keys: 4 half .. and 8 + 4 half .. of a piece
+            const ValueShare from = value_share(lane_now);
+            const int piece = (VALUES_ALIKE ? value_share0 / UNITS : from.of) >> 1;
+            const unsigned of_page = pick(pages, piece, VALUES_ALIKE), at = pick(offs, piece, VALUES_ALIKE);
+            const char *p = v_codes + ((size_t)of_page * page_bytes + at * TB) + (unsigned)((from.of & 1) * 4 * TB + from.unit * 8);
+#pragma unroll
+            for (int i = 0; i < VALUE_CODES / 4; i++) {
+                const u2 x = *reinterpret_cast<const u2 *>(p + 8 * i), y = *reinterpret_cast<const u2 *>(p + 8 * TB + 8 * i);
+                words[4 * i] = x[0], words[4 * i + 1] = x[1], words[4 * i + 2] = y[0], words[4 * i + 3] = y[1];
+            }
+            const unsigned *sc = v_scales + ((size_t)of_page * page_scales + at) + (unsigned)(from.group * a.page + (from.of & 1) * 4);
+            const u4 m = *reinterpret_cast<const u4 *>(sc), o = *reinterpret_cast<const u4 *>(sc + 8);
+#pragma unroll
+            for (int i = 0; i < 4; i++) words[VALUE_CODES + i] = m[i], words[VALUE_CODES + 4 + i] = o[i];
         }
     };
     // .. as numbers, in a stage
     auto fill = [&](uint4 *stage, unsigned (*flags)[G + 1]) {
+        int lane_now = lane;
+        if (WIDE) asm("" : "+v"(lane_now));  // (as above)
+        if (takes_keys) {
 #pragma unroll
-        for (int k = 0; k < TURNS; k++) {
-            __builtin_amdgcn_sched_barrier(0);  // (one after the other: two at once take more registers than there are)
-            const int s0 = (wave + k * kWaves) * 64, s = s0 + lane;
-            if (s0 < SHARES) {
+            for (int k = 0; k < KEY_TURNS; k++) {
+                __builtin_amdgcn_sched_barrier(0);  // (one after the other: two at once take more registers than there are)
+                const int s0 = key_share0 + 128 * k, s = s0 + lane_now;
                 const int key = s / (HD / 16), u = s - key * (HD / 16);
-                const h2 sc = scales_of(scales[k][0], scales[k][0]), lo = half_lows_of(scales[k][0], scales[k][0]);
+                const unsigned *codes = words + KEYS_AT + KEY_WORDS * k, scale = codes[BITS / 2];
+                const h2 sc = scales_of(scale, scale), lo = half_lows_of(scale, scale);
                 uint4 *set = stage + (key >> 5) * T::kSet + (key & 31);
 #pragma unroll
                 for (int p = 0; p < 2; p++) {
                     h2 high[4];
                     unsigned low[2] = {0, 0};
-                    auto word = [&](int e) { return BITS == 4 ? codes[k][p] >> (4 * e) : codes[k][2 * p + (e >> 1)] >> (8 * (e & 1)); };
+                    auto word = [&](int e) { return BITS == 4 ? codes[p] >> (4 * e) : codes[2 * p + (e >> 1)] >> (8 * (e & 1)); };
 #pragma unroll
                     for (int e = 0; e < 2; e++) {
                         parted<false>(high[2 * e], low[e], half_codes(word(2 * e), mask, base), sc, lo, minus);
@@ -279,14 +328,21 @@ template <int BITS, int HD> __global__ __launch_bounds__(kWaves * 64, 2) void mh
                     set[(p * (HD / 16) + u) * T::kRow] = uint4{word_of(high[0]), word_of(high[1]), word_of(high[2]), word_of(high[3])};
                     reinterpret_cast<uint2 *>(set + T::kKeyLow + (p * (HD / 32) + (u >> 1)) * T::kRow)[u & 1] = uint2{low[0], low[1]};
                 }
-            } else if (s0 < 2 * SHARES) {
-                const int of = (s - SHARES) / (HD / 2), rest = s - SHARES - of * (HD / 2), unit = BITS == 4 ? rest % (HD / 4) : rest, pair = BITS == 4 ? rest / (HD / 4) : 0;
+            }
+        }
+        if (takes_values) {
+            const unsigned *scales = words + VALUE_CODES;
+            const ValueShare to = value_share(lane_now);
+#pragma unroll
+            for (int p = 0; p < PAIRS; p++) {
+                __builtin_amdgcn_sched_barrier(0);
+                const int of = to.of, unit = to.unit + (BITS == 8 ? p : 0), pair = BITS == 4 ? to.pair + p : 0;
                 h2 high[2][4], sum = {0, 0};
                 unsigned low[2][2] = {};
 #pragma unroll
                 for (int x = 0; x < 4; x++) {  // tokens 2 x and the next
-                    const h2 sc = scales_of(scales[k][2 * x], scales[k][2 * x + 1]), lo = half_lows_of(scales[k][2 * x], scales[k][2 * x + 1]);
-                    const unsigned w = BITS == 4 ? codes[k][x] >> (8 * pair) : codes[k][x];
+                    const h2 sc = scales_of(scales[2 * x], scales[2 * x + 1]), lo = half_lows_of(scales[2 * x], scales[2 * x + 1]);
+                    const unsigned w = BITS == 4 ? words[x] >> (8 * pair) : words[4 * p + x];
 #pragma unroll
                     for (int i = 0; i < 2; i++) {
                         const h2 code = half_codes(w >> (BITS * i), mask, base);
@@ -307,7 +363,7 @@ template <int BITS, int HD> __global__ __launch_bounds__(kWaves * 64, 2) void mh
                             for (int i = 0; i < 2; i++) high[i][e >> 1][e & 1] = (_Float16)0.0f, low[i][e >> 2] &= ~(255u << (8 * (e & 3)));
                         }
                     }
-                    atomicOr(&flags[of >> 2][BITS == 4 ? unit >> 3 : unit >> 4], keys);
+                    atomicOr(&flags[of >> 2][to.group], keys);
                     atomicOr(&flags[of >> 2][G], keys);
                 }
                 uint4 *set = stage + (of >> 2) * T::kSet;
@@ -332,33 +388,17 @@ template <int BITS, int HD> __global__ __launch_bounds__(kWaves * 64, 2) void mh
 #pragma unroll
         for (int r = 0; r < 16; r++) acc[k][r] = 0.0f;
 
-    if (threadIdx.x < 3 * SETS * (G + 1)) (&bad[0][0][0])[threadIdx.x] = 0;
-    // Each turn computes a tile and fills in the next one: into the other stage, half of the waves before they compute and half behind, so that a SIMD has vector work beside matrix products.
-    // The first turn only fills in.
-    const bool early = wave < kWaves / 2;
-    int slot = 2, buffer = 1;
-    unsigned now = 0;  // pieces of the tile to compute that have pages
-    if (split < v_end) fetch(split);
-    for (int v = split - splits; v < v_end; v += splits) {
-        lds_barrier();
-        const int tile = tiles.tile(v) * T::kTokens, next_slot = slot == 2 ? 0 : slot + 1, clear_slot = next_slot == 2 ? 0 : next_slot + 1;
-        const bool more = v + splits < v_end;
-        const unsigned then = ok;
-        const uint4 *stage = lds + buffer * T::kStage;
-        if (threadIdx.x < SETS * (G + 1)) (&bad[clear_slot][0][0])[threadIdx.x] = 0;
-        auto go_on = [&]() {
-            fill(lds + (buffer ^ 1) * T::kStage, bad[next_slot]);
-            if (v + 2 * splits < v_end) fetch(v + 2 * splits);
-        };
-        if (early && more) go_on();
-        if (v >= split && tile < sees_to && (tile < sees_first || tile >= sees_from)) {
+    if (threadIdx.x < GROUPS * SLOTS * SETS * (G + 1)) (&all_bad[0][0][0][0])[threadIdx.x] = 0;
+    // a tile in a stage, with its marks and its pieces that have pages
+    auto compute = [&](const int tile, const uint4 *stage, const unsigned (*marks)[G + 1], const unsigned now) {
+        if (tile < sees_to && (tile < sees_first || tile >= sees_from)) {
             // (products go first: one takes one of eight turns to issue, and leaves the others to vector work of the SIMD's other wave, which would leave it none)
             __builtin_amdgcn_s_setprio(1);
             unsigned marked[SETS];
             f16v s[SETS];
 #pragma unroll
             for (int x = 0; x < SETS; x++) {
-                marked[x] = bad[slot][x][G];
+                marked[x] = marks[x][G];
                 s[x] = f16v{};
                 const uint4 *keys = stage + x * T::kSet + c;
 #pragma unroll
@@ -366,17 +406,22 @@ template <int BITS, int HD> __global__ __launch_bounds__(kWaves * 64, 2) void mh
 #pragma unroll
                 for (int i = 0; i < LOWS; i++) {
                     const uint4 one = keys[T::kKeyLow + (half * (HD / 32) + 2 * i) * T::kRow], two = 2 * i + 1 < HD / 32 ? keys[T::kKeyLow + (half * (HD / 32) + 2 * i + 1) * T::kRow] : one;
-                    s[x] = low_products(one, two, q8[i], s[x]);
+                    i8 small = q8[i];
+                    if (Q8_APART) {
+                        const uint4 a0 = q8_apart[(member * LOWS + i) * 2][lane], a1 = q8_apart[(member * LOWS + i) * 2 + 1][lane];
+                        small = i8{(int)a0.x, (int)a0.y, (int)a0.z, (int)a0.w, (int)a1.x, (int)a1.y, (int)a1.z, (int)a1.w};
+                    }
+                    s[x] = low_products(one, two, small, s[x]);
                 }
             }
-            constexpr int READS = (CHUNKS + HD / 32) * SETS, EARLY = READS < AHEAD ? READS : AHEAD;
+            constexpr int READS = (CHUNKS + HD / 32) * SETS + (Q8_APART ? 2 * LOWS : 0), EARLY = READS < AHEAD ? READS : AHEAD;
             __builtin_amdgcn_sched_group_barrier(0x100, EARLY, 0);
 #pragma unroll
             for (int i = 0; i < READS - EARLY; i++) {
                 __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
                 __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
             }
-            __builtin_amdgcn_sched_group_barrier(0x008, (CHUNKS + LOWS) * SETS - (READS - EARLY), 0);
+            __builtin_amdgcn_sched_group_barrier(0x008, CHUNKS + LOWS > (READS - EARLY) / SETS ? (CHUNKS + LOWS) * SETS - (READS - EARLY) : 1, 0);
             __builtin_amdgcn_s_setprio(0);
             const bool whole = tile + T::kTokens <= whole_to && (tile >= whole_from || tile + T::kTokens <= a.sinks) && now == (1u << PIECES) - 1;
             unsigned seen[SETS];
@@ -426,7 +471,7 @@ template <int BITS, int HD> __global__ __launch_bounds__(kWaves * 64, 2) void mh
             for (int x = 0; x < SETS; x++)
                 if (__builtin_amdgcn_readfirstlane(marked[x]) != 0) {
 #pragma unroll
-                    for (int g = 0; g < G; g++) not_numbers |= (bad[slot][x][g] >> (4 * half) & seen[x] & 0x0f0f0f0fu) != 0 ? 1u << g : 0u;
+                    for (int g = 0; g < G; g++) not_numbers |= (marks[x][g] >> (4 * half) & seen[x] & 0x0f0f0f0fu) != 0 ? 1u << g : 0u;
                 }
             __builtin_amdgcn_s_setprio(1);
 #pragma unroll
@@ -467,10 +512,81 @@ template <int BITS, int HD> __global__ __launch_bounds__(kWaves * 64, 2) void mh
             }
         }
         __builtin_amdgcn_s_setprio(0);
-        if (!early && more) go_on();
-        now = then;
-        slot = next_slot;
-        buffer ^= 1;
+    };
+
+    if (own < v_end) fetch(own);
+    if (W == kWaves) {
+        // Each turn computes a tile and fills in the next one, into the other stage; the first only fills in.  Half of the waves, one of every SIMD, fill in before they compute, the others behind,
+        // so that a SIMD has vector work beside matrix products.
+        const bool early = wave < kWaves / 2;
+        int slot = 2, buffer = 1;
+        unsigned now = 0;
+        for (int v = own - step; v < v_end; v += step) {
+            lds_barrier();
+            const int next_slot = slot == 2 ? 0 : slot + 1, clear_slot = next_slot == 2 ? 0 : next_slot + 1;
+            const bool more = v + step < v_end;
+            const unsigned then = ok;
+            if (threadIdx.x < SETS * (G + 1)) (&bad[clear_slot][0][0])[threadIdx.x] = 0;
+            auto go_on = [&]() {
+                fill(lds + (buffer ^ 1) * T::kStage, bad[next_slot]);
+                if (v + 2 * step < v_end) fetch(v + 2 * step);
+            };
+            if (early && more) go_on();
+            if (v >= own) compute(tiles.tile(v) * T::kTokens, lds + buffer * T::kStage, bad[slot], now);
+            if (!early && more) go_on();
+            now = then;
+            slot = next_slot;
+            buffer ^= 1;
+        }
+    } else {
+        // Each turn fills in a tile and computes it: a second workgroup of the compute unit has vector work beside the products.
+        const int first = split * GROUPS;
+        uint4 *stage = lds + team * T::kStage;
+        int slot = 0, v = own;
+        for (int u = first; u < v_end; u += step) {
+            lds_barrier();
+            const unsigned now = ok;
+            if (v < v_end) {
+                fill(stage, bad[slot]);
+                if (v + step < v_end) fetch(v + step);
+            }
+            lds_barrier();
+            if (v < v_end) {
+                const int by = threadIdx.x - team * (W * 64);
+                if (by < SETS * (G + 1)) (&bad[slot ^ 1][0][0])[by] = 0;
+                compute(tiles.tile(v) * T::kTokens, stage, bad[slot], now);
+            }
+            slot ^= 1;
+            v += step;
+        }
+        // the groups' sums to the first
+        float *sums = reinterpret_cast<float *>(lds);
+#pragma unroll
+        for (int some = GROUPS / 2; some > 0; some /= 2) {
+            __syncthreads();
+            if (team >= some && team < 2 * some) {
+                float *to = sums + (wave - some * W) * kTilePart<HD> + lane;
+                to[0] = ref, to[64] = l;
+#pragma unroll
+                for (int k = 0; k < BLOCKS; k++)
+#pragma unroll
+                    for (int r = 0; r < 16; r++) to[(2 + 16 * k + r) * 64] = acc[k][r];
+                all_marks[wave][lane] = not_numbers;
+            }
+            __syncthreads();
+            if (team < some) {
+                const float *from = sums + wave * kTilePart<HD> + lane;
+                const float other = from[0], most = fmaxf(ref, other), f = __builtin_amdgcn_exp2f(ref - most), fo = __builtin_amdgcn_exp2f(other - most);
+                ref = most;
+                l = l * f + from[64] * fo;
+#pragma unroll
+                for (int k = 0; k < BLOCKS; k++)
+#pragma unroll
+                    for (int r = 0; r < 16; r++) acc[k][r] = acc[k][r] * f + from[(2 + 16 * k + r) * 64] * fo;
+                not_numbers |= all_marks[wave + some * W][lane];
+            }
+        }
+        if (team > 0) return;
     }
 
     const float sum = across_sum(l);
@@ -484,7 +600,7 @@ template <int BITS, int HD> __global__ __launch_bounds__(kWaves * 64, 2) void mh
     }
     if (splits > 1) {
         if (mine <= 0) return;
-        float *part = a.parts + (((size_t)blockIdx.z * units + (unsigned)(b * nkv + kv)) * kWaves + wave) * kTilePart<HD> + lane;
+        float *part = a.parts + (((size_t)blockIdx.z * units + (unsigned)(b * nkv + kv)) * W + member) * kTilePart<HD> + lane;
         part[0] = ref;
         part[64] = sum;
 #pragma unroll
@@ -493,9 +609,12 @@ template <int BITS, int HD> __global__ __launch_bounds__(kWaves * 64, 2) void mh
             for (int r = 0; r < 16; r++) part[(2 + 16 * m + r) * 64] = acc[m][r];
         return;
     }
-    __syncthreads();  // the stages are read
+    if (GROUPS == 1) __syncthreads();  // the stages are read
     if (mine <= 0) return;
-    _Float16 *mem = reinterpret_cast<_Float16 *>(lds) + wave * (32 * (HD + 2));
+    // (where groups' sums were, a wave has read its own alone)
+    constexpr int APART = GROUPS == 1 ? 32 * (HD + 2) : 2 * kTilePart<HD>;
+    static_assert(W * APART * 2 <= sizeof(lds), "a wave's rows");
+    _Float16 *mem = reinterpret_cast<_Float16 *>(lds) + member * APART;
     rows_to_lds<BITS, HD, BLOCKS>(mem, acc, 0, 2.0f / sum, sum == 0.0f, lane);
     wave_lds_order();
     rows_to_memory<HD>(mem, a, b, kv, row0, mine, lane, 64);
@@ -505,12 +624,12 @@ template <int BITS, int HD> __global__ __launch_bounds__(kWaves * 64, 2) void mh
 template <int BITS, int HD> __global__ __launch_bounds__(HD * 2) void mha_kv_tile_join_kernel(const KvSightArgs a) {
     __shared__ _Float16 lds[32 * (HD + 2)];
     const int lane = threadIdx.x & 63, m = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int unit = blockIdx.x, block = blockIdx.y, wave = blockIdx.z;
+    const int unit = blockIdx.x, block = blockIdx.y, wave = blockIdx.z, waves = gridDim.z;
     const int b = unit / a.nkv, kv = unit - b * a.nkv;
-    const int row0 = (block * kWaves + wave) * 32, rows = min(32, (a.counts ? min(max(a.counts[b], 0), a.n) : a.n) * a.per - row0);
+    const int row0 = (block * waves + wave) * 32, rows = min(32, (a.counts ? min(max(a.counts[b], 0), a.n) : a.n) * a.per - row0);
     if (rows <= 0) return;
-    const float *part = a.parts + (((size_t)block * a.splits * a.units + unit) * kWaves + wave) * kTilePart<HD> + lane;
-    const size_t next = (size_t)a.units * kWaves * kTilePart<HD>;
+    const float *part = a.parts + (((size_t)block * a.splits * a.units + unit) * waves + wave) * kTilePart<HD> + lane;
+    const size_t next = (size_t)a.units * waves * kTilePart<HD>;
     float ref = kNothing, l = 0.0f;
     f16v acc = {};
     for (int s0 = 0; s0 < a.splits; s0 += 4) {  // four parts asked for at once
@@ -545,50 +664,59 @@ struct TileForm {
     void (*kernel)(KV_LEADING, const KvSightArgs);
     void (*join)(const KvSightArgs);
 };
-template <int BITS> TileForm tile_form(int hd) {
+template <int BITS, int HD> TileForm tile_form(int waves) {
+    if constexpr (HD == 128) {
+        if (waves == 2) return {mha_kv_tile_kernel<BITS, HD, 2, 2>, mha_kv_tile_join_kernel<BITS, HD>};
+    }
+    return {mha_kv_tile_kernel<BITS, HD, kWaves, 1>, mha_kv_tile_join_kernel<BITS, HD>};
+}
+template <int BITS> TileForm tile_form(int hd, int waves) {
     switch (hd) {
-        case 32: return {mha_kv_tile_kernel<BITS, 32>, mha_kv_tile_join_kernel<BITS, 32>};
-        case 64: return {mha_kv_tile_kernel<BITS, 64>, mha_kv_tile_join_kernel<BITS, 64>};
-        case 96: return {mha_kv_tile_kernel<BITS, 96>, mha_kv_tile_join_kernel<BITS, 96>};
-        default: return {mha_kv_tile_kernel<BITS, 128>, mha_kv_tile_join_kernel<BITS, 128>};
+        case 32: return tile_form<BITS, 32>(waves);
+        case 64: return tile_form<BITS, 64>(waves);
+        case 96: return tile_form<BITS, 96>(waves);
+        default: return tile_form<BITS, 128>(waves);
     }
 }
 
 }  // namespace
 
-bool kv_tile_rows(int hd, long long rows) { return hd <= 128 && rows > (hd == 128 ? 64 : hd == 32 ? 128 : 96); }
-bool kv_tile_work(const et_kv_cache *c, long long positions, int B, long long rows) {
-    return (long long)B * c->nkv * ((rows + 32 * kWaves - 1) / (32 * kWaves)) * ((positions + 31) / 32) >= (c->hd == 128 ? 1024 : 3072);
+int kv_tile_most_waves(int hd, long long rows) { return hd > 128 ? 0 : rows > (hd == 128 ? 64 : hd == 32 ? 128 : 96) ? kWaves : hd == 128 && rows > 32 ? 2 : 0; }
+int kv_tile_waves(const et_kv_cache *c, long long positions, int B, long long rows) {
+    const int waves = kv_tile_most_waves(c->hd, rows);
+    const long long work = (long long)B * c->nkv * ((rows + 32 * kWaves - 1) / (32 * kWaves)) * ((positions + 31) / 32);
+    return work >= (waves == 2 ? 4000 : c->hd == 128 ? 1024 : 3072) ? waves : 0;
 }
 
-int kv_tile_plan(const char *fn, KvTilePlan &p, const et_kv_cache *c, long long positions, int B, int n, int nh) {
+int kv_tile_plan(const char *fn, KvTilePlan &p, const et_kv_cache *c, long long positions, int B, int n, int nh, int waves) {
     ET_REQUIRE(nh > 0 && nh % c->nkv == 0, ET_ERR_INVALID_ARG, "%s: nh=%d must be a multiple of nkv=%d", fn, nh, c->nkv);
     const long long rows = (long long)n * (nh / c->nkv), units = (long long)B * c->nkv;
-    const long long blocks = (rows + 32 * kWaves - 1) / (32 * kWaves), groups = units * blocks;
+    const long long blocks = (rows + 32 * waves - 1) / (32 * waves), groups = units * blocks;
     ET_REQUIRE(rows <= 0x7fffffffLL && B <= 65535 && blocks <= 65535 && groups <= (1LL << 24), ET_ERR_UNSUPPORTED, "%s: B=%d n=%d nh=%d", fn, B, n, nh);
     p.blocks = (int)blocks;
+    p.waves = waves;
     const int tokens = c->hd <= 64 ? 64 : 32;
-    const long long tiles = (positions + tokens - 1) / tokens;
-    p.splits = groups == 0 ? 1 : (int)std::max(1LL, std::min({2048 / (groups * kWaves), tiles / 4, 256LL}));
+    const long long tiles = (positions + tokens - 1) / tokens, at_once = waves == 2 ? 512 : 256;
+    p.splits = groups == 0 ? 1 : (int)std::max(1LL, std::min({at_once / groups, tiles / (waves == 2 ? 8 : 4), waves == 2 ? 64LL : 256LL}));
     p.splits = std::min(p.splits, (int)(65535 / std::max(1LL, blocks)));
-    p.bytes = p.splits > 1 ? (size_t)(groups * p.splits * kWaves) * (2 + c->hd / 2) * 64 * sizeof(float) : 0;
+    p.bytes = p.splits > 1 ? (size_t)(groups * p.splits * waves) * (2 + c->hd / 2) * 64 * sizeof(float) : 0;
     return ET_OK;
 }
 
-int kv_tile_run(const char *fn, const KvMhaCall &call, long long positions, size_t need, KvSightArgs &a, et_stream stream) {
+int kv_tile_run(const char *fn, const KvMhaCall &call, long long positions, int waves, size_t need, KvSightArgs &a, et_stream stream) {
     KvTilePlan p;
-    int st = kv_tile_plan(fn, p, call.cache, positions, call.B, call.n, call.nh);
+    int st = kv_tile_plan(fn, p, call.cache, positions, call.B, call.n, call.nh, waves);
     if (st == ET_OK) st = kv_check_call(fn, call, need);
     if (st != ET_OK || call.B == 0 || call.n == 0) return st;
     const KvPieces pieces = kv_fill(call, a);
     a.cols = 1;
-    a.block_rows = 32 * kWaves;
+    a.block_rows = 32 * p.waves;
     a.splits = p.splits;
-    const TileForm f = call.cache->bits == 4 ? tile_form<4>(a.hd) : tile_form<8>(a.hd);
-    st = launch_kernel("mha_kv_tile_kernel", f.kernel, dim3((unsigned)a.nkv, (unsigned)call.B, (unsigned)(p.blocks * p.splits)), (unsigned)kWaves * 64, 0, as_stream(stream), call.table,
+    const TileForm f = call.cache->bits == 4 ? tile_form<4>(a.hd, p.waves) : tile_form<8>(a.hd, p.waves);
+    st = launch_kernel("mha_kv_tile_kernel", f.kernel, dim3((unsigned)a.nkv, (unsigned)call.B, (unsigned)(p.blocks * p.splits)), (unsigned)(p.waves == 2 ? 4 : p.waves) * 64, 0, as_stream(stream), call.table,
                        call.starts, call.counts, call.max_pages, a.units, a.splits, a.per, pieces.magic, pieces.shift, pieces.of_page, call.n, a);
     if (st != ET_OK || p.splits == 1) return st;
-    return launch_kernel("mha_kv_tile_join_kernel", f.join, dim3((unsigned)a.units, (unsigned)p.blocks, (unsigned)kWaves), (unsigned)a.hd * 2, 0, as_stream(stream), a);
+    return launch_kernel("mha_kv_tile_join_kernel", f.join, dim3((unsigned)a.units, (unsigned)p.blocks, (unsigned)p.waves), (unsigned)a.hd * 2, 0, as_stream(stream), a);
 }
 
 }  // namespace et
