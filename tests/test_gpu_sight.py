@@ -508,3 +508,57 @@ def test_on_two_streams_at_once_and_again(et):
         et.check(lib.et_stream_sync(s))
         assert (z[k].numpy() == want[k]).all()
         et.check(lib.et_stream_destroy(s))
+
+
+@pytest.mark.parametrize("hd,per,n,length", [(128, 2, 60, 3000), (128, 4, 16, 8200), (64, 2, 100, 6500), (128, 1, 16, 3000)])
+def test_many_rows_recorded_on_two_streams(et, hd, per, n, length):
+    """Keys shared out over workgroups, without starts or counts: two graphs of a window's and a tree's attention, each with its workspace, replayed side by side, and the bits of eager calls each time."""
+    lib, nkv, B, page = et.lib(), 8, 2, 64
+    pages = -(-length // page)
+    table = tables(2, B, pages, B * pages)
+    host = filled(4, nkv, hd, page, table, [length] * B, 7, B * pages)
+    dev, width, dt = DeviceCache(et, host), nkv * per * hd, up(et, table)
+    starts = up(et, np.full(B, length - n, np.int32))
+    words = up(et, S.seen_words(trees(3, B, n), [n] * B, n))
+    q = [up(et, Hn.randn((B * n, width), 5 + k)) for k in range(2)]
+    need = [et.mha_kv_tree_workspace(dev.c, pages, B, n, nkv * per, 0, 0), et.mha_kv_window_workspace(dev.c, pages, B, n, nkv * per, length - 200, 7)]
+    assert min(need) > 0 or n * per <= 32
+
+    def run(k, z, ws, stream):
+        if k == 0:
+            et.mha_kv_tree(dev.c, dt, pages, starts, None, words, q[0], width, z, width, B, n, nkv * per, 0, 0, 0.1, ws, need[0], stream)
+        else:
+            et.mha_kv_window(dev.c, dt, pages, starts, None, q[1], width, z, width, B, n, nkv * per, length - 200, 7, 0.1, et.MHA_CAUSAL, ws, need[1], stream)
+
+    new = lambda k: (up(et, np.zeros((B * n, width), np.float16)), up(et, np.full(max(need[k], 16), 0xFF, np.uint8)))  # noqa: E731
+    want, streams, graphs, out = [], [], [], []
+    for k in range(2):
+        z, ws = new(k)
+        run(k, z, ws, None)
+        et.check(lib.et_device_sync())
+        want.append(z.numpy())
+        out.append(new(k))
+        s, g = C.c_void_p(), C.c_void_p()
+        et.check(lib.et_stream_create(C.byref(s)))
+        et.check(lib.et_graph_begin_capture(s))
+        run(k, *out[k], s)
+        et.check(lib.et_graph_end_capture(s, C.byref(g)))
+        streams.append(s)
+        graphs.append(g)
+    for _ in range(6):
+        for k in range(2):
+            zero = np.zeros((B * n, width), np.float16)
+            et.check(lib.et_memcpy_h2d(out[k][0].ptr, zero.ctypes.data, zero.nbytes))
+            et.check(lib.et_graph_launch(graphs[k], streams[k]))
+        run(0, *(eager := new(0)), None)
+        et.check(lib.et_device_sync())
+        assert np.array_equal(eager[0].numpy(), want[0])
+        for k in range(2):
+            assert np.array_equal(out[k][0].numpy(), want[k])
+    for g, s in zip(graphs, streams):
+        et.check(lib.et_graph_destroy(g))
+        et.check(lib.et_stream_destroy(s))
+    # from position 0 on, and n rows of each sequence
+    z, ws = new(1)
+    et.mha_kv_window(dev.c, dt, pages, None, None, q[1], width, z, width, B, n, nkv * per, 40, 3, 0.1, et.MHA_CAUSAL, ws, need[1], None)
+    near(z.numpy(), *S.attention(host, table, [0] * B, [n] * B, q[1].numpy(), n, nkv * per, 0.1, S.window_sight([0] * B, [n] * B, n, 40, 3, True)), hd, n, n * per)
