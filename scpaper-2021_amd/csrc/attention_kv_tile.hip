@@ -685,7 +685,7 @@ int kv_tile_most_waves(int hd, long long rows) { return hd > 128 ? 0 : rows > (h
 int kv_tile_waves(const et_kv_cache *c, long long positions, int B, long long rows) {
     const int waves = kv_tile_most_waves(c->hd, rows);
     const long long work = (long long)B * c->nkv * ((rows + 32 * kWaves - 1) / (32 * kWaves)) * ((positions + 31) / 32);
-    return work >= (waves == 2 ? 4000 : c->hd == 128 ? 1024 : 3072) ? waves : 0;
+    return work >= (waves == 2 ? 4000 : c->hd == 128 ? 1024 : 3000) ? waves : 0;
 }
 
 int kv_tile_plan(const char *fn, KvTilePlan &p, const et_kv_cache *c, long long positions, int B, int n, int nh, int waves) {
