@@ -55,19 +55,26 @@ template <int BITS, int HD> __device__ __forceinline__ int place_channel(int p) 
 
 // Two codes, in the low bits of a word's halves, as halves of numbers: 512 + code / 2 has the code in its lowest bits.  (mask, base: in registers, so that both are put to use in one instruction.)
 __device__ __forceinline__ h2 half_codes(unsigned word, unsigned mask, unsigned base) { return __builtin_bit_cast(h2, (word & mask) | base) - h2{512, 512}; }
-// code / 2 * scale + low / 2 as high parts, and what they leave, times 2^11, in 8 bits: the lower or upper half of a word.  (minus: -1 that the compiler does not know, with which widening and
-// subtracting are one instruction.)
+// code / 2 * scale + low / 2 as high parts, and what they leave, times 2^11, in 8 bits: the lower or upper half of a word.  (Half of a lowest value that is an odd multiple of 2^-24 is no binary16
+// number: what is left is that of the half in binary32.  minus: -1 that the compiler does not know, with which widening and subtracting are one instruction.)
 typedef short s2 __attribute__((ext_vector_type(2)));
-template <bool UPPER> __device__ __forceinline__ void parted(h2 &high, unsigned &low, h2 code, h2 scale, h2 lowest, float minus) {
-    high = __builtin_elementwise_fma(code, scale, lowest);
+struct HalfLows {
+    h2 rounded;
+    float whole[2];
+};
+template <bool UPPER> __device__ __forceinline__ void parted(h2 &high, unsigned &low, h2 code, h2 scale, const HalfLows &lowest, float minus) {
+    high = __builtin_elementwise_fma(code, scale, lowest.rounded);
     float rest[2];
 #pragma unroll
-    for (int e = 0; e < 2; e++) rest[e] = __builtin_fmaf((float)high[e], minus, __builtin_fmaf((float)code[e], (float)scale[e], (float)lowest[e]));
+    for (int e = 0; e < 2; e++) rest[e] = __builtin_fmaf((float)high[e], minus, __builtin_fmaf((float)code[e], (float)scale[e], lowest.whole[e]));
     low = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf8_f32(__builtin_bit_cast(s2, low), rest[0], rest[1], kLowUnit, UPPER));
 }
 // Of two tokens' words of a scale and a lowest value: both scales, and half of both lowest values.
 __device__ __forceinline__ h2 scales_of(unsigned a, unsigned b) { return __builtin_bit_cast(h2, __builtin_amdgcn_perm(b, a, 0x05040100u)); }
-__device__ __forceinline__ h2 half_lows_of(unsigned a, unsigned b) { return __builtin_bit_cast(h2, __builtin_amdgcn_perm(b, a, 0x07060302u)) * h2{0.5f, 0.5f}; }
+__device__ __forceinline__ HalfLows half_lows_of(unsigned a, unsigned b) {
+    const h2 lows = __builtin_bit_cast(h2, __builtin_amdgcn_perm(b, a, 0x07060302u));
+    return {lows * h2{0.5f, 0.5f}, {0.5f * (float)lows[0], 0.5f * (float)lows[1]}};
+}
 
 __device__ __forceinline__ unsigned word_of(h2 x) { return __builtin_bit_cast(unsigned, x); }
 
@@ -313,7 +320,8 @@ template <int BITS, int HD, int W, int GROUPS> __global__ __launch_bounds__(W * 
                 const int s0 = key_share0 + 128 * k, s = s0 + lane_now;
                 const int key = s / (HD / 16), u = s - key * (HD / 16);
                 const unsigned *codes = words + KEYS_AT + KEY_WORDS * k, scale = codes[BITS / 2];
-                const h2 sc = scales_of(scale, scale), lo = half_lows_of(scale, scale);
+                const h2 sc = scales_of(scale, scale);
+                const HalfLows lo = half_lows_of(scale, scale);
                 uint4 *set = stage + (key >> 5) * T::kSet + (key & 31);
 #pragma unroll
                 for (int p = 0; p < 2; p++) {
@@ -341,7 +349,8 @@ template <int BITS, int HD, int W, int GROUPS> __global__ __launch_bounds__(W * 
                 unsigned low[2][2] = {};
 #pragma unroll
                 for (int x = 0; x < 4; x++) {  // tokens 2 x and the next
-                    const h2 sc = scales_of(scales[2 * x], scales[2 * x + 1]), lo = half_lows_of(scales[2 * x], scales[2 * x + 1]);
+                    const h2 sc = scales_of(scales[2 * x], scales[2 * x + 1]);
+                    const HalfLows lo = half_lows_of(scales[2 * x], scales[2 * x + 1]);
                     const unsigned w = BITS == 4 ? words[x] >> (8 * pair) : words[4 * p + x];
 #pragma unroll
                     for (int i = 0; i < 2; i++) {

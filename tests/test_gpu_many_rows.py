@@ -1,0 +1,68 @@
+"""Attention over a window or a tree with many rows a key/value head, by the kernels that turn codes into numbers before they multiply them, where numbers are hard to keep: values of a
+few of binary16's smallest steps.  Against binary64."""
+import math
+
+import numpy as np
+import pytest
+
+from oracle import decode as D
+from oracle import sight as S
+from tests.test_gpu_kv_cache import DeviceCache
+from tests.test_gpu_sight import first, near, run_window
+
+pytestmark = pytest.mark.gpu
+
+# (hd, query heads, rows, batches alike or apart): one key/value head, eight waves a workgroup, and two of them a block of 64 rows
+MANY = [(32, 4, 40, 320), (64, 1, 130, 320), (96, 3, 70, 320), (128, 8, 20, 220), (128, 4, 16, 480)]
+PAGE, PAGES = 64, 5
+
+
+def attended(et, bits, form, K, V, Q, scale):
+    """Rows that all see every token, K and V [sequences][tokens][hd], Q [sequences][rows][heads * hd]; (result, then what S.attention gives), a table of PAGES pages for each sequence.
+    One sequence stands for as many as the form has."""
+    hd, nh, n, copies = form
+    B, tokens = K.shape[:2]
+    table = np.full((B, PAGES), -1, np.int32)
+    used = -(-tokens // PAGE)
+    table[:, :used] = np.arange(B * used).reshape(B, used)
+    host = D.Cache(bits, 1, hd, PAGE, B * used, fill=0xFF)
+    host.write(table, [0] * B, [tokens] * B, K.reshape(-1, hd), V.reshape(-1, hd), tokens)
+    starts, counts, times = [tokens - n] * B, [n] * B, copies // B
+    got = run_window(et, DeviceCache(et, host), np.tile(table, (times, 1)), starts * times, counts * times, np.tile(Q.reshape(B * n, -1), (times, 1)), B * times, n, nh, 1 << 20, 0, scale, False)
+    return first(times, got), S.attention(host, table, starts, counts, Q.reshape(B * n, -1), n, nh, scale, S.window_sight(starts, counts, n, 1 << 20, 0, False))
+
+
+def small(r, *shape):
+    """Multiples of 2^-24 up to 40 of them, groups that are all 1, 3 and 17, and numbers about 2^-14 and 2^-13."""
+    x = r.integers(1, 41, shape)
+    kind = r.integers(0, 8, shape[:-1] + (shape[-1] // 32,)).repeat(32, -1)
+    for k, whole in ((0, 1), (1, 3), (2, 17)):
+        x = np.where(kind == k, whole, x)
+    x = np.where(kind == 3, x + 1024, np.where(kind == 4, x + 2047, x))
+    return (x * 2.0 ** -24).astype(np.float16)
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("form", MANY, ids=str)
+def test_values_of_the_smallest_steps(et, bits, form):
+    hd, nh, n, _ = form
+    r = np.random.default_rng(hd)
+    K, Q = r.standard_normal((1, 300, hd)).astype(np.float16), r.standard_normal((1, n, nh * hd)).astype(np.float16)
+    got, want = attended(et, bits, form, K, small(r, 1, 300, hd), Q, 1 / math.sqrt(hd))
+    near(got, *want, hd, 300, nh * n)
+    # one number alone comes out as it is
+    for whole in (1, 3, 5, 17, 1025, 2047):
+        got, _ = attended(et, bits, form, K, np.full((1, 300, hd), whole * 2.0 ** -24, np.float16), Q, 1 / math.sqrt(hd))
+        assert (got == np.float16(whole * 2.0 ** -24)).all(), (whole, np.unique(got.astype(np.float64) * 2.0 ** 24))
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("form", MANY, ids=str)
+def test_keys_of_the_smallest_steps(et, bits, form):
+    """Against queries near the largest numbers, so that a step of a key is some tenths of a score."""
+    hd, nh, n, _ = form
+    r = np.random.default_rng(hd)
+    K = (r.integers(1, 41, (1, 300, 1)) + r.integers(0, 2, (1, 300, hd))).astype(np.float64) * 2.0 ** -24
+    V, Q = r.standard_normal((1, 300, hd)).astype(np.float16), (5e4 + 1e4 * r.random((1, n, nh * hd))).astype(np.float16)
+    got, want = attended(et, bits, form, K.astype(np.float16), V, Q, 64 / hd)
+    near(got, *want, hd, 300, nh * n)
