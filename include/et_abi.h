@@ -744,10 +744,9 @@ int et_mha_kv_f16(const et_kv_cache *cache, const int32_t *table, int max_pages,
  * not looked up: their entries may be any number, and the pages another
  * sequence's (et_kv_tables gives them back).  Everything else as
  * et_mha_kv_f16, but that with more than 32 rows to a key/value head (n * nh /
- * nkv) keys, values and probabilities may enter the products as a binary16
- * number and 8 bits of what it leaves: a score's terms are then off by up to
- * 1.3e-4 of themselves, a result by up to 3.3e-4 of the sum of its
- * probabilities times |values|, and by far less where such errors differ. */
+ * nkv) keys, values and probabilities may enter the products as two binary16
+ * numbers each, which keep 2^-20 of a score's terms and of a probability times
+ * its value. */
 int et_mha_kv_window_workspace(const et_kv_cache *cache, int max_pages, int B,
                                int n, int nh, int window, int sinks,
                                size_t *bytes);

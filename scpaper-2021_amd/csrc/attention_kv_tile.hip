@@ -7,13 +7,14 @@
 //   S^T = K Q^T: rows of the product are keys, columns the wave's rows, so a lane ends with 16 of the 32 scores of one row, and the other half of the row is in the lane 32 away.
 //   Z^T = V^T P^T: rows are channels, columns the same rows again: what a lane scored are the very keys that it weighs, and a row's factors are a number of its lane.
 //
-// v / 2 = high + low: halved, since the rounding up of a scale may carry a group's last steps beyond binary16's range.  High is binary16, low, at most half its step, 8 bits (e5m2: products of
-// 8 bits take half the time).  S = high q + low q8; Z = high w + low w8 + high8 rest, w a weight in binary16, rest what that leaves, q8, w8, high8 the same in 8 bits; low times rest, 2^-22, is
-// left out.  With the low parts in binary16 as well, 4096 rows of 32 heads over 8 of 128, two sequences of 6000, took 370 us, this 336.
+// v = high + low, high cut off to binary16, low, less than a step of it, rounded: off by 2^-21 of v at most.  S = high q + low q; Z = high w + low w + high rest, w a weight in binary16, rest what
+// that leaves; low times rest, 2^-21, is left out.  With low, q, w and rest of the corrections in 8 bits, whose products take half the time, 4096 rows of 32 heads over 8 of 128, two sequences of 6000,
+// took 327 us where this takes 369 (16 nodes of 32 heads over 8, 8 bits, 8 sequences that see 4112 tokens: 46.4 and 44.7), but a score's terms were off by up to 1.3e-4 of themselves, and a result
+// by up to 3.3e-4 of the sum of its probabilities times |values|.
 //
-// One product a pair would be 104 us of those 336 at the 1352 TFLOP/s that a large binary16 product reaches; with the corrections it is 182.  What bounds it is the vector work (360 instructions
-// a wave and 32 keys, a third of them to take codes apart) in the shadow of products: registers allow two waves a SIMD, and while one multiplies the other issues an instruction every eight
-// clocks, where two take one every four.  Eight waves share a stage, since with four each stage served half as many rows; with 16 rows a wave LDS was read twice as often.
+// One product a pair would be 104 us of those 369 at the 1352 TFLOP/s that a large binary16 product reaches; with the corrections, 2.5 of them, it is 260.  The rest is vector work (some 360
+// instructions a wave and 32 keys, a third of them to take codes apart) that the products do not hide: registers allow two waves a SIMD, and while one multiplies the other issues an instruction every
+// eight clocks, where two take one every four.  Eight waves share a stage, since with four each stage served half as many rows; with 16 rows a wave LDS was read twice as often.
 //
 // Up to 64 rows of heads of 128 two waves share a stage, and a workgroup is two such pairs, each with every other tile of its keys (16 nodes of 32 heads over 8, 8 bits, 8 sequences that see 4112
 // tokens: 60.9 -> 46.8 us).  The same for heads of 64 took 272 us where blocks of 16 rows took 371, 64 sequences of 4096 and 16 heads, but 209 where those took 180 with sequences and trees of
@@ -25,17 +26,14 @@ namespace et {
 
 namespace {
 
-constexpr float kLowUnit = 0x1p-11f;  // of low parts, and of what weights leave, in 8 bits: at most 16, half a step behind 2^15, which 2^-12 would take beyond their range
-constexpr int kLowUnitE8 = 127 - 11, kUnitE8 = 127;
-
-// LDS of a stage, in pieces of 16 bytes, for each 32 keys.  Keys: high parts [channel / 8, the even ones first][33 places of 32 keys], low parts in 8 bits [channel / 8 odd][channel / 32][33].
-// Values: high parts [keys / 8 of them][channel], low parts and high parts in 8 bits [keys of the lower or upper lanes][channel].
+// LDS of a stage, in pieces of 16 bytes, for each 32 keys.  Keys: high parts [channel / 8, the even ones first][33 places of 32 keys], and low parts as well.  Values: high parts [keys / 8 of
+// them][channel], and low parts as well.
 constexpr int kWaves = 8;
 template <int HD> struct TileShape {
     static constexpr int kSets = HD <= 64 ? 2 : 1;  // of 32 keys
     static constexpr int kTokens = 32 * kSets, kPieces = 2 * kSets;
     static constexpr int kRow = 33;                 // 32 keys, and one on to other banks
-    static constexpr int kKeyLow = HD / 8 * kRow, kValue = kKeyLow + HD / 16 * kRow, kValueLow = kValue + 4 * HD, kValueHigh = kValueLow + 2 * HD, kSet = kValueHigh + 2 * HD;
+    static constexpr int kKeyLow = HD / 8 * kRow, kValue = 2 * kKeyLow, kValueLow = kValue + 4 * HD, kSet = kValueLow + 4 * HD;
     static constexpr int kStage = kSets * kSet;
     static constexpr int kShares = kTokens * HD / 16;  // of 16 numbers: of the keys, and as many of the values
 };
@@ -53,28 +51,22 @@ template <int BITS, int HD> __device__ __forceinline__ int place_channel(int p) 
     return p % N * C + p / N;
 }
 
-// Two codes, in the low bits of a word's halves, as halves of numbers: 512 + code / 2 has the code in its lowest bits.  (mask, base: in registers, so that both are put to use in one instruction.)
-__device__ __forceinline__ h2 half_codes(unsigned word, unsigned mask, unsigned base) { return __builtin_bit_cast(h2, (word & mask) | base) - h2{512, 512}; }
-// code / 2 * scale + low / 2 as high parts, and what they leave, times 2^11, in 8 bits: the lower or upper half of a word.  (Half of a lowest value that is an odd multiple of 2^-24 is no binary16
-// number: what is left is that of the half in binary32.  minus: -1 that the compiler does not know, with which widening and subtracting are one instruction.)
-typedef short s2 __attribute__((ext_vector_type(2)));
-struct HalfLows {
-    h2 rounded;
-    float whole[2];
-};
-template <bool UPPER> __device__ __forceinline__ void parted(h2 &high, unsigned &low, h2 code, h2 scale, const HalfLows &lowest, float minus) {
-    high = __builtin_elementwise_fma(code, scale, lowest.rounded);
-    float rest[2];
+// Two codes, in the low bits of a word's halves: 1024 + code has the code in its lowest bits.  (mask, base: in registers, so that both are put to use in one instruction.)
+__device__ __forceinline__ h2 codes_of(unsigned word, unsigned mask, unsigned base) { return __builtin_bit_cast(h2, (word & mask) | base) - h2{1024, 1024}; }
+// code * scale + low as two binary16 numbers.  The first is cut off: rounding the scale up may carry a group's last steps beyond binary16's range, which then are its largest number and what is left.
+// (minus: -1 that the compiler does not know, with which widening and subtracting are one instruction.)
+__device__ __forceinline__ void parted(h2 &high, h2 &low, h2 code, h2 scale, h2 lowest, float minus) {
+    float v[2], rest[2];
 #pragma unroll
-    for (int e = 0; e < 2; e++) rest[e] = __builtin_fmaf((float)high[e], minus, __builtin_fmaf((float)code[e], (float)scale[e], lowest.whole[e]));
-    low = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf8_f32(__builtin_bit_cast(s2, low), rest[0], rest[1], kLowUnit, UPPER));
+    for (int e = 0; e < 2; e++) v[e] = __builtin_fmaf((float)code[e], (float)scale[e], (float)lowest[e]);
+    high = __builtin_bit_cast(h2, __builtin_amdgcn_cvt_pkrtz(v[0], v[1]));
+#pragma unroll
+    for (int e = 0; e < 2; e++) rest[e] = __builtin_fmaf((float)high[e], minus, v[e]);
+    low = h2{(_Float16)rest[0], (_Float16)rest[1]};
 }
-// Of two tokens' words of a scale and a lowest value: both scales, and half of both lowest values.
+// Of two tokens' words of a scale and a lowest value: both scales, and both lowest values.
 __device__ __forceinline__ h2 scales_of(unsigned a, unsigned b) { return __builtin_bit_cast(h2, __builtin_amdgcn_perm(b, a, 0x05040100u)); }
-__device__ __forceinline__ HalfLows half_lows_of(unsigned a, unsigned b) {
-    const h2 lows = __builtin_bit_cast(h2, __builtin_amdgcn_perm(b, a, 0x07060302u));
-    return {lows * h2{0.5f, 0.5f}, {0.5f * (float)lows[0], 0.5f * (float)lows[1]}};
-}
+__device__ __forceinline__ h2 lows_of(unsigned a, unsigned b) { return __builtin_bit_cast(h2, __builtin_amdgcn_perm(b, a, 0x07060302u)); }
 
 __device__ __forceinline__ unsigned word_of(h2 x) { return __builtin_bit_cast(unsigned, x); }
 
@@ -111,17 +103,10 @@ template <int HD> __device__ __forceinline__ void rows_to_memory(const _Float16 
     }
 }
 
-// sums + (first, second) * x * 2^-11, 64 numbers of 8 bits.
-typedef int i8 __attribute__((ext_vector_type(8)));
-__device__ __forceinline__ f16v low_products(uint4 first, uint4 second, i8 x, f16v sums) {
-    const i8 y = {(int)first.x, (int)first.y, (int)first.z, (int)first.w, (int)second.x, (int)second.y, (int)second.z, (int)second.w};
-    return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(y, x, sums, 1, 1, 0, kLowUnitE8, 0, kUnitE8);
-}
-
 // GROUPS times W waves of 32 rows each.
 template <int BITS, int HD, int W, int GROUPS> __global__ __launch_bounds__(W * GROUPS * 64, 2) void mha_kv_tile_kernel(KV_LEADING, const KvSightArgs a) {
     using T = TileShape<HD>;
-    constexpr int TB = HD * BITS / 8, G = HD / 32, CHUNKS = HD / 16, BLOCKS = HD / 32, LOWS = (HD + 63) / 64, SETS = T::kSets, PIECES = T::kPieces, SHARES = T::kShares;
+    constexpr int TB = HD * BITS / 8, G = HD / 32, CHUNKS = HD / 16, BLOCKS = HD / 32, SETS = T::kSets, PIECES = T::kPieces, SHARES = T::kShares;
     constexpr int SLOTS = W == kWaves ? 3 : 2;
     // What a thread takes apart of a stage.  Of eight waves some take a share of the keys, 16 channels of one, and as many a share of the values, two channels of eight tokens.  Of two each
     // takes two shares of the keys, and a wide one of the values, four channels.
@@ -132,8 +117,6 @@ template <int BITS, int HD, int W, int GROUPS> __global__ __launch_bounds__(W * 
     constexpr int AHEAD = WIDE ? 4 : HD == 128 ? 6 : 8;  // pieces of a stage that are asked for ahead of the products that they are for, as far as there are registers
     constexpr bool ALIKE = HD == 64 || HD == 128, VALUES_ALIKE = WIDE || ALIKE;  // a wave's shares are of one piece of 16 keys
     __shared__ uint4 lds[tile_lds<HD, W, GROUPS>()];
-    constexpr bool Q8_APART = WIDE;  // queries in 8 bits are read from LDS: there are no registers for them
-    __shared__ uint4 q8_apart[Q8_APART ? W * LOWS * 2 : 1][64];
     __shared__ unsigned all_marks[GROUPS == 1 ? 1 : W * GROUPS][64];
     __shared__ unsigned all_bad[GROUPS][SLOTS][SETS][G + 1];  // keys whose values are no numbers, of each group of channels and of any; of this tile, the next, and one to clear
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -206,7 +189,7 @@ template <int BITS, int HD, int W, int GROUPS> __global__ __launch_bounds__(W * 
     top = across_max(top);
     const int up = top > 0.0f ? 15 - __builtin_amdgcn_frexp_expf(top) : 0;
     const float grow = query_growth(top, up, a.scale_log2e);
-    const float key_scale = __builtin_ldexpf(fabsf(a.scale_log2e), 1 - up);
+    const float key_scale = __builtin_ldexpf(fabsf(a.scale_log2e), -up);
 #pragma unroll
     for (int i = 0; i < CHUNKS; i++) {
         // in the order that the keys' codes come out of their words
@@ -216,38 +199,12 @@ template <int BITS, int HD, int W, int GROUPS> __global__ __launch_bounds__(W * 
         for (int e = 0; e < 8; e++) q[i][e] = (_Float16)((float)x[order[BITS == 8][e]] * grow);
     }
 
-    // the same in 8 bits, for 64 channels at a time (none behind the last: zero)
-    i8 q8[LOWS];
-#pragma unroll
-    for (int i = 0; i < 4 * LOWS; i++)
-#pragma unroll
-        for (int e = 0; e < 2; e++) {
-            s2 w = {0, 0};
-            if (i < CHUNKS) {
-                const h8 x = q[i < CHUNKS ? i : 0];
-                w = __builtin_amdgcn_cvt_scalef32_pk_bf8_f32(w, (float)x[4 * e], (float)x[4 * e + 1], 1.0f, false);
-                w = __builtin_amdgcn_cvt_scalef32_pk_bf8_f32(w, (float)x[4 * e + 2], (float)x[4 * e + 3], 1.0f, true);
-            }
-            q8[i / 4][2 * (i % 4) + e] = __builtin_bit_cast(int, w);
-        }
-
-    if (Q8_APART && team == 0) {
-#pragma unroll
-        for (int i = 0; i < 2 * LOWS; i++) {
-            uint4 x;
-            unsigned *to = reinterpret_cast<unsigned *>(&x);
-#pragma unroll
-            for (int e = 0; e < 4; e++) to[e] = (unsigned)q8[i / 2][4 * (i % 2) + e];
-            q8_apart[member * LOWS * 2 + i][lane] = x;
-        }
-    }
-
     const char *k_codes = a.k_codes + (size_t)kv * a.page * TB, *v_codes = a.v_codes + (size_t)kv * a.page * TB;
     const unsigned *k_scales = a.k_scales + (size_t)kv * (G * a.page), *v_scales = a.v_scales + (size_t)kv * (G * a.page);
     const unsigned page_bytes = (unsigned)nkv * a.page * TB, page_scales = (unsigned)nkv * G * a.page;
 
     float minus = -1.0f;
-    unsigned mask = BITS == 4 ? 0x000f000fu : 0x00ff00ffu, base = 0x60006000u;
+    unsigned mask = BITS == 4 ? 0x000f000fu : 0x00ff00ffu, base = 0x64006400u;
     asm("" : "+s"(minus));
     asm("" : "+v"(mask));
     asm("" : "+v"(base));
@@ -320,21 +277,19 @@ template <int BITS, int HD, int W, int GROUPS> __global__ __launch_bounds__(W * 
                 const int s0 = key_share0 + 128 * k, s = s0 + lane_now;
                 const int key = s / (HD / 16), u = s - key * (HD / 16);
                 const unsigned *codes = words + KEYS_AT + KEY_WORDS * k, scale = codes[BITS / 2];
-                const h2 sc = scales_of(scale, scale);
-                const HalfLows lo = half_lows_of(scale, scale);
+                const h2 sc = scales_of(scale, scale), lo = lows_of(scale, scale);
                 uint4 *set = stage + (key >> 5) * T::kSet + (key & 31);
 #pragma unroll
                 for (int p = 0; p < 2; p++) {
-                    h2 high[4];
-                    unsigned low[2] = {0, 0};
-                    auto word = [&](int e) { return BITS == 4 ? codes[p] >> (4 * e) : codes[2 * p + (e >> 1)] >> (8 * (e & 1)); };
+                    h2 high[4], low[4];
 #pragma unroll
-                    for (int e = 0; e < 2; e++) {
-                        parted<false>(high[2 * e], low[e], half_codes(word(2 * e), mask, base), sc, lo, minus);
-                        parted<true>(high[2 * e + 1], low[e], half_codes(word(2 * e + 1), mask, base), sc, lo, minus);
+                    for (int e = 0; e < 4; e++) {
+                        const unsigned word = BITS == 4 ? codes[p] >> (4 * e) : codes[2 * p + (e >> 1)] >> (8 * (e & 1));
+                        parted(high[e], low[e], codes_of(word, mask, base), sc, lo, minus);
                     }
-                    set[(p * (HD / 16) + u) * T::kRow] = uint4{word_of(high[0]), word_of(high[1]), word_of(high[2]), word_of(high[3])};
-                    reinterpret_cast<uint2 *>(set + T::kKeyLow + (p * (HD / 32) + (u >> 1)) * T::kRow)[u & 1] = uint2{low[0], low[1]};
+                    uint4 *to = set + (p * (HD / 16) + u) * T::kRow;
+                    to[0] = uint4{word_of(high[0]), word_of(high[1]), word_of(high[2]), word_of(high[3])};
+                    to[T::kKeyLow] = uint4{word_of(low[0]), word_of(low[1]), word_of(low[2]), word_of(low[3])};
                 }
             }
         }
@@ -345,31 +300,27 @@ template <int BITS, int HD, int W, int GROUPS> __global__ __launch_bounds__(W * 
             for (int p = 0; p < PAIRS; p++) {
                 __builtin_amdgcn_sched_barrier(0);
                 const int of = to.of, unit = to.unit + (BITS == 8 ? p : 0), pair = BITS == 4 ? to.pair + p : 0;
-                h2 high[2][4], sum = {0, 0};
-                unsigned low[2][2] = {};
+                h2 high[2][4], low[2][4], sum = {0, 0};
 #pragma unroll
                 for (int x = 0; x < 4; x++) {  // tokens 2 x and the next
-                    const h2 sc = scales_of(scales[2 * x], scales[2 * x + 1]);
-                    const HalfLows lo = half_lows_of(scales[2 * x], scales[2 * x + 1]);
+                    const h2 sc = scales_of(scales[2 * x], scales[2 * x + 1]), lo = lows_of(scales[2 * x], scales[2 * x + 1]);
                     const unsigned w = BITS == 4 ? words[x] >> (8 * pair) : words[4 * p + x];
 #pragma unroll
                     for (int i = 0; i < 2; i++) {
-                        const h2 code = half_codes(w >> (BITS * i), mask, base);
-                        if (x & 1) parted<true>(high[i][x], low[i][x >> 1], code, sc, lo, minus);
-                        else parted<false>(high[i][x], low[i][x >> 1], code, sc, lo, minus);
-                        sum = __builtin_elementwise_fma(high[i][x], h2{0, 0}, sum);
+                        parted(high[i][x], low[i][x], codes_of(w >> (BITS * i), mask, base), sc, lo, minus);
+                        sum = __builtin_elementwise_fma(low[i][x], h2{0, 0}, sum);
                     }
                 }
-                // What is not a number, or infinite, must not meet the zero weight of a row that does not see it: it leaves the stage, and the rows that do see it are marked.
+                // What is not a number, or infinite, must not meet the zero weight of a row that does not see it: it leaves the stage, and the rows that do see it are marked.  (The low part of such a value is no number either.)
                 if (word_of(sum) != 0) {
                     unsigned keys = 0;
 #pragma unroll
                     for (int e = 0; e < 8; e++) {
-                        const bool is = (word_of(high[0][e >> 1]) >> (16 * (e & 1)) & 0x7c00u) == 0x7c00u || (word_of(high[1][e >> 1]) >> (16 * (e & 1)) & 0x7c00u) == 0x7c00u;
+                        const bool is = (word_of(low[0][e >> 1]) >> (16 * (e & 1)) & 0x7c00u) == 0x7c00u || (word_of(low[1][e >> 1]) >> (16 * (e & 1)) & 0x7c00u) == 0x7c00u;
                         if (is) {
                             keys |= 1u << (16 * (of >> 1 & 1) + 4 * (of & 1) + (e & 3) + (e >> 2) * 8);
 #pragma unroll
-                            for (int i = 0; i < 2; i++) high[i][e >> 1][e & 1] = (_Float16)0.0f, low[i][e >> 2] &= ~(255u << (8 * (e & 3)));
+                            for (int i = 0; i < 2; i++) high[i][e >> 1][e & 1] = low[i][e >> 1][e & 1] = (_Float16)0.0f;
                         }
                     }
                     atomicOr(&flags[of >> 2][to.group], keys);
@@ -378,12 +329,10 @@ template <int BITS, int HD, int W, int GROUPS> __global__ __launch_bounds__(W * 
                 uint4 *set = stage + (of >> 2) * T::kSet;
 #pragma unroll
                 for (int i = 0; i < 2; i++) {
-                    const int place = (BITS == 4 ? 2 * pair + i : i) * (HD / (16 / BITS)) + unit, keys = of & 1, part = of >> 1 & 1;
-                    set[T::kValue + (of & 3) * HD + place] = uint4{word_of(high[i][0]), word_of(high[i][1]), word_of(high[i][2]), word_of(high[i][3])};
-                    reinterpret_cast<uint2 *>(set + T::kValueLow + keys * HD + place)[part] = uint2{low[i][0], low[i][1]};
-                    // (the upper bytes of binary16 numbers are such numbers in 8 bits)
-                    reinterpret_cast<uint2 *>(set + T::kValueHigh + keys * HD + place)[part] =
-                        uint2{__builtin_amdgcn_perm(word_of(high[i][1]), word_of(high[i][0]), 0x07050301u), __builtin_amdgcn_perm(word_of(high[i][3]), word_of(high[i][2]), 0x07050301u)};
+                    const int place = (BITS == 4 ? 2 * pair + i : i) * (HD / (16 / BITS)) + unit;
+                    uint4 *at = set + T::kValue + (of & 3) * HD + place;
+                    at[0] = uint4{word_of(high[i][0]), word_of(high[i][1]), word_of(high[i][2]), word_of(high[i][3])};
+                    at[T::kValueLow - T::kValue] = uint4{word_of(low[i][0]), word_of(low[i][1]), word_of(low[i][2]), word_of(low[i][3])};
                 }
             }
         }
@@ -411,26 +360,19 @@ template <int BITS, int HD, int W, int GROUPS> __global__ __launch_bounds__(W * 
                 s[x] = f16v{};
                 const uint4 *keys = stage + x * T::kSet + c;
 #pragma unroll
-                for (int i = 0; i < CHUNKS; i++) s[x] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, keys[(half * CHUNKS + i) * T::kRow]), q[i], s[x], 0, 0, 0);
+                for (int part = 0; part < 2; part++)
 #pragma unroll
-                for (int i = 0; i < LOWS; i++) {
-                    const uint4 one = keys[T::kKeyLow + (half * (HD / 32) + 2 * i) * T::kRow], two = 2 * i + 1 < HD / 32 ? keys[T::kKeyLow + (half * (HD / 32) + 2 * i + 1) * T::kRow] : one;
-                    i8 small = q8[i];
-                    if (Q8_APART) {
-                        const uint4 a0 = q8_apart[(member * LOWS + i) * 2][lane], a1 = q8_apart[(member * LOWS + i) * 2 + 1][lane];
-                        small = i8{(int)a0.x, (int)a0.y, (int)a0.z, (int)a0.w, (int)a1.x, (int)a1.y, (int)a1.z, (int)a1.w};
-                    }
-                    s[x] = low_products(one, two, small, s[x]);
-                }
+                    for (int i = 0; i < CHUNKS; i++)
+                        s[x] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, keys[part * T::kKeyLow + (half * CHUNKS + i) * T::kRow]), q[i], s[x], 0, 0, 0);
             }
-            constexpr int READS = (CHUNKS + HD / 32) * SETS + (Q8_APART ? 2 * LOWS : 0), EARLY = READS < AHEAD ? READS : AHEAD;
+            constexpr int READS = 2 * CHUNKS * SETS, EARLY = READS < AHEAD ? READS : AHEAD;
             __builtin_amdgcn_sched_group_barrier(0x100, EARLY, 0);
 #pragma unroll
             for (int i = 0; i < READS - EARLY; i++) {
                 __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
                 __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
             }
-            __builtin_amdgcn_sched_group_barrier(0x008, CHUNKS + LOWS > (READS - EARLY) / SETS ? (CHUNKS + LOWS) * SETS - (READS - EARLY) : 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x008, EARLY, 0);
             __builtin_amdgcn_s_setprio(0);
             const bool whole = tile + T::kTokens <= whole_to && (tile >= whole_from || tile + T::kTokens <= a.sinks) && now == (1u << PIECES) - 1;
             unsigned seen[SETS];
@@ -485,8 +427,7 @@ template <int BITS, int HD, int W, int GROUPS> __global__ __launch_bounds__(W * 
             __builtin_amdgcn_s_setprio(1);
 #pragma unroll
             for (int x = 0; x < SETS; x++) {
-                h8 weights[2];
-                s2 eight[8];  // weights in 8 bits, and what the 16 leave
+                h8 weights[2], rests[2];
 #pragma unroll
                 for (int e = 0; e < 8; e++) {
                     const float p0 = s[x][2 * e], p1 = s[x][2 * e + 1];
@@ -494,29 +435,26 @@ template <int BITS, int HD, int W, int GROUPS> __global__ __launch_bounds__(W * 
                     asm("" : "+v"(w));  // (or each half is rounded once more, on its own)
                     const h2 wide = __builtin_bit_cast(h2, w);
                     weights[e >> 2][2 * (e & 3)] = wide[0], weights[e >> 2][2 * (e & 3) + 1] = wide[1];
-                    const float r0 = __builtin_fmaf((float)wide[0], minus, p0), r1 = __builtin_fmaf((float)wide[1], minus, p1);
-                    s2 &whole = eight[e >> 1], &left = eight[4 + (e >> 1)];
-                    whole = e & 1 ? __builtin_amdgcn_cvt_scalef32_pk_bf8_f32(whole, p0, p1, 1.0f, true) : __builtin_amdgcn_cvt_scalef32_pk_bf8_f32(s2{0, 0}, p0, p1, 1.0f, false);
-                    left = e & 1 ? __builtin_amdgcn_cvt_scalef32_pk_bf8_f32(left, r0, r1, kLowUnit, true) : __builtin_amdgcn_cvt_scalef32_pk_bf8_f32(s2{0, 0}, r0, r1, kLowUnit, false);
+                    rests[e >> 2][2 * (e & 3)] = (_Float16)__builtin_fmaf((float)wide[0], minus, p0), rests[e >> 2][2 * (e & 3) + 1] = (_Float16)__builtin_fmaf((float)wide[1], minus, p1);
                     l += p0;
                     l += p1;
                 }
-                i8 small;
+                const uint4 *values = stage + x * T::kSet + T::kValue + half * HD + c;
 #pragma unroll
-                for (int e = 0; e < 8; e++) small[e] = __builtin_bit_cast(int, eight[e]);
-                const uint4 *values = stage + x * T::kSet + c;
+                for (int m = 0; m < BLOCKS; m++)
 #pragma unroll
-                for (int m = 0; m < BLOCKS; m++) {
-                    acc[m] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, values[T::kValue + half * HD + 32 * m]), weights[0], acc[m], 0, 0, 0);
-                    acc[m] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, values[T::kValue + (2 + half) * HD + 32 * m]), weights[1], acc[m], 0, 0, 0);
-                    acc[m] = low_products(values[T::kValueLow + half * HD + 32 * m], values[T::kValueHigh + half * HD + 32 * m], small, acc[m]);
-                }
+                    for (int k = 0; k < 2; k++) {
+                        const h8 high = __builtin_bit_cast(h8, values[2 * k * HD + 32 * m]), low = __builtin_bit_cast(h8, values[T::kValueLow - T::kValue + 2 * k * HD + 32 * m]);
+                        acc[m] = __builtin_amdgcn_mfma_f32_32x32x16_f16(high, weights[k], acc[m], 0, 0, 0);
+                        acc[m] = __builtin_amdgcn_mfma_f32_32x32x16_f16(high, rests[k], acc[m], 0, 0, 0);
+                        acc[m] = __builtin_amdgcn_mfma_f32_32x32x16_f16(low, weights[k], acc[m], 0, 0, 0);
+                    }
             }
             constexpr int VALUES = 4 * BLOCKS * SETS;
             __builtin_amdgcn_sched_group_barrier(0x100, AHEAD < VALUES ? AHEAD : VALUES, 0);
 #pragma unroll
             for (int i = 0; i < (VALUES - AHEAD) / 4; i++) {
-                __builtin_amdgcn_sched_group_barrier(0x008, 3, 0);
+                __builtin_amdgcn_sched_group_barrier(0x008, 6, 0);
                 __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
             }
         }
@@ -624,7 +562,7 @@ template <int BITS, int HD, int W, int GROUPS> __global__ __launch_bounds__(W * 
     constexpr int APART = GROUPS == 1 ? 32 * (HD + 2) : 2 * kTilePart<HD>;
     static_assert(W * APART * 2 <= sizeof(lds), "a wave's rows");
     _Float16 *mem = reinterpret_cast<_Float16 *>(lds) + member * APART;
-    rows_to_lds<BITS, HD, BLOCKS>(mem, acc, 0, 2.0f / sum, sum == 0.0f, lane);
+    rows_to_lds<BITS, HD, BLOCKS>(mem, acc, 0, 1.0f / sum, sum == 0.0f, lane);
     wave_lds_order();
     rows_to_memory<HD>(mem, a, b, kv, row0, mine, lane, 64);
 }
@@ -664,7 +602,7 @@ template <int BITS, int HD> __global__ __launch_bounds__(HD * 2) void mha_kv_til
             for (int e = 0; e < 16; e++) acc[e] = __builtin_fmaf(f, vs[k][e], acc[e]);
         }
     }
-    rows_to_lds<BITS, HD, 1>(lds, &acc, m, 2.0f / l, l == 0.0f, lane);
+    rows_to_lds<BITS, HD, 1>(lds, &acc, m, 1.0f / l, l == 0.0f, lane);
     __syncthreads();
     rows_to_memory<HD>(lds, a, b, kv, row0, rows, threadIdx.x, HD * 2);
 }

@@ -1,5 +1,5 @@
 """Attention over a window or a tree with many rows a key/value head, by the kernels that turn codes into numbers before they multiply them, where numbers are hard to keep: values of a
-few of binary16's smallest steps.  Against binary64."""
+few of binary16's smallest steps, and results of which nearly everything cancels, so that what numbers lose is not behind the result's own rounding.  Against binary64."""
 import math
 
 import numpy as np
@@ -66,3 +66,65 @@ def test_keys_of_the_smallest_steps(et, bits, form):
     V, Q = r.standard_normal((1, 300, hd)).astype(np.float16), (5e4 + 1e4 * r.random((1, n, nh * hd))).astype(np.float16)
     got, want = attended(et, bits, form, K.astype(np.float16), V, Q, 64 / hd)
     near(got, *want, hd, 300, nh * n)
+
+
+def kept(got, want, hd, keys):
+    """Held to what a key's and a value's number in two binary16 numbers leaves (the first cut off: 2^-10 of it, the second rounded: 2^-11 of that), as a weight's two do (2^-22), the product of
+    second parts that is left out (2^-10 times 2^-11), and binary32: scores off by d, from 2^-21 of their terms, hd + 16 roundings of 2^-24 in sums of magnitude `reach` and
+    2^-20 for exp2, move every p by 2 d; a sum over the keys has keys + 16 roundings.  The result is rounded once: 2^-11, or 2^-25 where it is subnormal."""
+    Z, stepped, lows, reach = want
+    d = ((hd + 16) * 2.0 ** -24 + 2.0 ** -21) * reach + 2.0 ** -20
+    lim = 2.0 ** -11 * np.abs(Z) + 2.0 ** -25 + (np.expm1(2 * d) + (keys + 16) * 2.0 ** -24 + 3 * 2.0 ** -21) * (stepped + lows)
+    off = np.abs(got.astype(np.float64) - Z)
+    assert (off <= lim).all(), np.nanmax(off / lim)
+
+
+def groups(r, bits, B, hd):
+    """For each sequence a row whose channels, but for two of every 32, are one number, a step between 1 and 2 that takes more than binary16's bits."""
+    x = np.empty((B, 1, hd))
+    for b in range(B):
+        low, high = np.float64(np.float16(1 + 0.4 * r.random())), np.float64(np.float16(1.5 + 0.49 * r.random()))
+        x[b] = low + (high - low) * r.integers(1, 2 ** bits - 1) / (2 ** bits - 1)
+        x[b, 0, 0::32], x[b, 0, 1::32] = low, high
+    return x.astype(np.float16)
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("form", MANY, ids=str)
+def test_values_that_nearly_cancel(et, bits, form):
+    """Every other token has the opposite values of the others, but for what its codes make of them: what a value loses stays."""
+    hd, nh, n, copies = form
+    r, B, tokens = np.random.default_rng(hd), copies // 2, 32
+    V = np.repeat((1 + r.random((B, 1, hd))).astype(np.float16), tokens, 1)
+    V[:, 1::2] *= -1
+    got, want = attended(et, bits, form, np.zeros((B, tokens, hd), np.float16), V, r.standard_normal((B, n, nh * hd)).astype(np.float16), 0.1)
+    kept(got, want, hd, tokens)
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("form", MANY, ids=str)
+def test_weights_that_nearly_cancel(et, bits, form):
+    """One token is weighed more and has no values; four times 1.249 and five times -1 are what the others have, all with one weight, which takes more than binary16's bits."""
+    hd, nh, n, copies = form
+    r, B = np.random.default_rng(hd + 1), copies // 2
+    K, V = np.zeros((B, 10, hd)), np.zeros((B, 10, hd))
+    K[:, 0] = 1
+    V[:, 1:5], V[:, 5:] = 1.249, -1
+    Q = np.repeat((0.5 + r.random((B, 1, 1))), nh * hd, 2).repeat(n, 1)
+    got, want = attended(et, bits, form, K.astype(np.float16), V.astype(np.float16), Q.astype(np.float16), 2 / hd)
+    kept(got, want, hd, 10)
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("form", MANY, ids=str)
+def test_scores_that_nearly_agree(et, bits, form):
+    """Two kinds of tokens with scores of about 10 to 20 and values of 1 and -1: the result is half of the difference of their scores."""
+    hd, nh, n, copies = form
+    r, B, tokens = np.random.default_rng(hd + 2), copies // 2, 32
+    K = np.repeat(groups(r, bits, B, hd), tokens, 1)
+    K[:, 1::2] = groups(r, bits, B, hd)
+    Q = np.repeat((1 + 0.25 * r.random((B, 1, 1))), nh * hd, 2).repeat(n, 1)
+    V = np.ones((B, tokens, hd))
+    V[:, 1::2] = -1
+    got, want = attended(et, bits, form, K, V.astype(np.float16), Q.astype(np.float16), 8 / hd)
+    kept(got, want, hd, tokens)
