@@ -773,8 +773,8 @@ int et_tree_seen(const int32_t *parents, const int32_t *counts, uint32_t *seen,
  * (the bits may be any; et_tree_seen makes those of a tree).  window: 0, or at
  * least n: of the positions below starts[b] node i then sees those above
  * starts[b] + depth - window and those below sinks, depth the number of its
- * bits less one: what it would see if its way up were the sequence.  Everything
- * else as et_mha_kv_window_f16. */
+ * bits less one (0 where there are none): what it would see if its way up were
+ * the sequence.  Everything else as et_mha_kv_window_f16. */
 int et_mha_kv_tree_workspace(const et_kv_cache *cache, int max_pages, int B,
                              int n, int nh, int window, int sinks,
                              size_t *bytes);

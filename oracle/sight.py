@@ -41,7 +41,7 @@ def tree_sight(starts, counts, n, words, window, sinks):
     def sees(b, i, pos):
         start, count = int(starts[b]), min(max(int(counts[b]), 0), n)
         bits = np.array([bool(words[b, i, j // 32] >> np.uint32(j % 32) & np.uint32(1)) for j in range(count)], bool)
-        own = start + int(bits.sum()) - 1
+        own = start + max(int(bits.sum()) - 1, 0)
         node = pos - start
         tree = (node >= 0) & (node < count) & bits[np.clip(node, 0, max(count - 1, 0))]
         near = (pos > own - window) | (pos < sinks) if window else np.ones(len(pos), bool)

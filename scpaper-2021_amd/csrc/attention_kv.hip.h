@@ -267,6 +267,7 @@ template <bool SIGHT> struct KvSight {
                 if (a.window) {
                     own = -1;
                     for (int w = 0; w < a.words; w++) own += __builtin_popcount(bits[w] & (count >= 32 * w + 32 ? ~0u : count <= 32 * w ? 0u : (1u << (count & 31)) - 1));
+                    own = max(own, 0);  // (of no bits as of one: what lies before the window of the first node is not walked, and its pages may be others')
                 }
             }
             if (a.window) low = (int)min(max((long long)start + own - a.window + 1, 0LL), 0x7fffffffLL);
