@@ -823,7 +823,8 @@ int et_kv_keep(const et_kv_cache *caches, int ncaches, const int32_t *table,
  * free_pages [npages] is a ring, free_state {head, count, ..}: pages are taken
  * from free_pages[head], [head + 1], .. (modulo npages) in the order of
  * (b, i) and given back behind the last in that order (those that the ring
- * has no room for, which pages held twice can cause, are dropped);
+ * had no room for before the call, which pages held twice can cause, are
+ * dropped, and not counted);
  * next_state [3] (may be free_state): head and count after the call, and how
  * many pages were missing.
  * slots (or NULL) [B][n]: page number * page + place in it of each row, -1 for

@@ -147,4 +147,4 @@ def tables(before, page, npages, starts, counts, shared, n, window, sinks, ring,
             p = start + i
             if 0 <= p < M * page and 0 <= table[b, p // page] < npages:
                 slots[b, i] = int(table[b, p // page]) * page + p % page
-    return table, ring, np.array([(head + taken) % npages, min(free - taken + given, npages), missing], np.int32), slots
+    return table, ring, np.array([(head + taken) % npages, min(free + given, npages) - taken, missing], np.int32), slots

@@ -119,7 +119,7 @@ template <bool ONE> __device__ __forceinline__ void place_stretch(const TablesAr
 __device__ __forceinline__ void store_state(const TablesArgs &a, Counted total, int2 ring) {
     const int taken = min(total.needed, ring.y);
     a.next_state[0] = (int)(((long long)ring.x + taken) % a.npages);
-    a.next_state[1] = (int)min((long long)ring.y - taken + total.given, (long long)a.npages);
+    a.next_state[1] = (int)min((long long)ring.y + total.given, (long long)a.npages) - taken;  // (what was dropped has no place: places of pages that were taken are not free ones)
     a.next_state[2] = total.needed - taken;
 }
 
