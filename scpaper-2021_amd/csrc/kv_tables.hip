@@ -213,7 +213,8 @@ bool one_workgroup(int max_pages, int B) { return B <= kOneSequences && (long lo
 
 int check_sizes(const char *fn, int max_pages, int B) {
     ET_REQUIRE(max_pages > 0 && B >= 0, ET_ERR_INVALID_ARG, "%s: max_pages=%d B=%d", fn, max_pages, B);
-    ET_REQUIRE(B <= 65535 && (long long)B * max_pages <= 0x7fffffffLL, ET_ERR_UNSUPPORTED, "%s: B=%d max_pages=%d", fn, B, max_pages);
+    // (max_pages: entries rounded up to those of all waves, and the last step behind them, stay below 2^31)
+    ET_REQUIRE(B <= 65535 && max_pages <= 0x7ffffe00 && (long long)B * max_pages <= 0x7fffffffLL, ET_ERR_UNSUPPORTED, "%s: B=%d max_pages=%d", fn, B, max_pages);
     return ET_OK;
 }
 
