@@ -2,9 +2,10 @@
 // they need and do not have come from its front, both in the order of (sequence, page), so that the result depends on nothing but the arguments.
 //
 // A wave takes a stretch of entries; what it gives and takes is placed by counting those of the waves before it.  Small tables are one workgroup's, in one launch; larger ones take two, since
-// no workgroup waits for another: the first counts, the second places.  Bound by a launch and dependent accesses (8 sequences of 64 pages: 4.4 us), and by the table's bytes where it is large:
+// no workgroup waits for another: the first counts, the second places.  Slots of many rows are written by a launch of their own (kv_tables_forms.h).  Bound by a launch and dependent accesses (8 sequences of 64 pages: 4.4 us), and by the table's bytes where it is large:
 // 512 sequences of 8192 pages are read in 4.9 us (3.4 TB/s) and read and written in 10.9 (3.1 TB/s).  Sixteen entries at once for a lane rather than four changed neither.
 #include "common.hip.h"
+#include "kv_tables_forms.h"
 
 namespace et {
 namespace {
@@ -22,8 +23,6 @@ struct TablesArgs {
 };
 
 constexpr int kOneWaves = 16, kManyWaves = 8;
-// of tables that one workgroup takes (one launch|two, us: 512 entries 4.4|6.2, 2048 5.5|6.1, 4096 6.6|6.3, of 512 sequences 7.7|9.2, 8192 9.8|6.3, 16384 16.1|6.4)
-constexpr int kOneEntries = 4096, kOneSequences = 512;
 
 // The pages that a sequence needs: i < end, and i < first or i >= near.  Those before `own` are not its own to give or take.
 struct Needs {
@@ -123,20 +122,22 @@ __device__ __forceinline__ void store_state(const TablesArgs &a, Counted total, 
     a.next_state[2] = total.needed - taken;
 }
 
-// Slots of the rows [0, rows) of sequences from b0 on, whose tables the workgroup has written.
+// Where row i of sequence b lies in a table that is written: page number * page + place, or -1.
+__device__ __forceinline__ long long slot_of(const TablesArgs &a, int b, int i) {
+    const int count = a.counts ? min(max(a.counts[b], 0), a.n) : a.n;
+    const long long pos = (long long)(a.starts ? a.starts[b] : 0) + i;
+    if (i >= count || pos < 0 || pos >= (long long)a.max_pages * a.page) return -1;
+    const int at = (int)pos / a.page, page = a.table[(size_t)b * a.max_pages + at];
+    return page >= 0 && page < a.npages ? (long long)page * a.page + ((int)pos - at * a.page) : -1;
+}
+
+// Slots of the rows of sequences from b0 on, whose tables the workgroup has written.
 __device__ __forceinline__ void store_slots(const TablesArgs &a, int b0, int sequences, int threads) {
     if (!a.slots) return;
-    const long long rows = (long long)sequences * a.n;
-    for (long long r = threadIdx.x; r < rows; r += threads) {
-        const int of = (int)(r / a.n), b = b0 + of, i = (int)(r - (long long)of * a.n);
-        const int count = a.counts ? min(max(a.counts[b], 0), a.n) : a.n;
-        const long long pos = (long long)(a.starts ? a.starts[b] : 0) + i;
-        long long slot = -1;
-        if (i < count && pos >= 0 && pos < (long long)a.max_pages * a.page) {
-            const int at = (int)pos / a.page, page = a.table[(size_t)b * a.max_pages + at];
-            if (page >= 0 && page < a.npages) slot = (long long)page * a.page + ((int)pos - at * a.page);
-        }
-        a.slots[(size_t)b0 * a.n + r] = slot;
+    const unsigned rows = (unsigned)sequences * (unsigned)a.n;
+    for (unsigned r = threadIdx.x; r < rows; r += threads) {
+        const unsigned of = r / (unsigned)a.n;
+        a.slots[(size_t)b0 * a.n + r] = slot_of(a, b0 + (int)of, (int)(r - of * (unsigned)a.n));
     }
 }
 
@@ -209,7 +210,11 @@ __global__ __launch_bounds__(kManyWaves * 64) void kv_tables_place_kernel(const 
     store_slots(a, blockIdx.x, 1, kManyWaves * 64);
 }
 
-bool one_workgroup(int max_pages, int B) { return B <= kOneSequences && (long long)B * max_pages <= kOneEntries; }
+// Slots of many rows, behind the launch that writes the tables.
+__global__ __launch_bounds__(256) void kv_slots_kernel(const TablesArgs a) {
+    const int i = (int)(blockIdx.x * 256 + threadIdx.x);
+    if (i < a.n) a.slots[(size_t)blockIdx.y * a.n + i] = slot_of(a, blockIdx.y, i);
+}
 
 int check_sizes(const char *fn, int max_pages, int B) {
     ET_REQUIRE(max_pages > 0 && B >= 0, ET_ERR_INVALID_ARG, "%s: max_pages=%d B=%d", fn, max_pages, B);
@@ -218,7 +223,7 @@ int check_sizes(const char *fn, int max_pages, int B) {
     return ET_OK;
 }
 
-size_t tables_bytes(int max_pages, int B) { return one_workgroup(max_pages, B) ? 0 : ((size_t)B * kManyWaves + 1) * sizeof(int2); }
+size_t tables_bytes(int max_pages, int B) { return tables_of_one_workgroup(max_pages, B) ? 0 : ((size_t)B * kManyWaves + 1) * sizeof(int2); }
 
 }  // namespace
 }  // namespace et
@@ -264,10 +269,18 @@ int et_kv_tables(const int32_t *before, int32_t *table, int max_pages, int page,
     a.n = n;
     a.window = window;
     a.sinks = sinks;
-    if (one_workgroup(max_pages, B)) return launch_kernel("kv_tables_one_kernel", kv_tables_one_kernel, dim3(1), kOneWaves * 64, 0, as_stream(stream), a);
-    const int sl = launch_kernel("kv_tables_count_kernel", kv_tables_count_kernel, dim3((unsigned)B), kManyWaves * 64, 0, as_stream(stream), a);
-    if (sl != ET_OK) return sl;
-    return launch_kernel("kv_tables_place_kernel", kv_tables_place_kernel, dim3((unsigned)B), kManyWaves * 64, 0, as_stream(stream), a);
+    const bool one = tables_of_one_workgroup(max_pages, B), apart = slots && slots_apart(max_pages, B, n);
+    if (apart) a.slots = nullptr;
+    int sl;
+    if (one) {
+        sl = launch_kernel("kv_tables_one_kernel", kv_tables_one_kernel, dim3(1), kOneWaves * 64, 0, as_stream(stream), a);
+    } else {
+        sl = launch_kernel("kv_tables_count_kernel", kv_tables_count_kernel, dim3((unsigned)B), kManyWaves * 64, 0, as_stream(stream), a);
+        if (sl == ET_OK) sl = launch_kernel("kv_tables_place_kernel", kv_tables_place_kernel, dim3((unsigned)B), kManyWaves * 64, 0, as_stream(stream), a);
+    }
+    if (sl != ET_OK || !apart) return sl;
+    a.slots = reinterpret_cast<long long *>(slots);
+    return launch_kernel("kv_slots_kernel", kv_slots_kernel, dim3((unsigned)((n + 255LL) / 256), (unsigned)B), 256, 0, as_stream(stream), a);
 }
 
 }  // extern "C"
