@@ -8,7 +8,8 @@ import pytest
 from oracle import decode as D
 from oracle import sight as S
 from tests.test_gpu_kv_cache import DeviceCache
-from tests.test_gpu_sight import first, near, run_window
+from tests.test_gpu_kv_precision import NEAR, alternate, off, turning
+from tests.test_gpu_sight import distance, first, large_channel, near, run_window
 
 pytestmark = pytest.mark.gpu
 
@@ -17,12 +18,12 @@ MANY = [(32, 4, 40, 320), (64, 1, 130, 320), (96, 3, 70, 320), (128, 8, 20, 220)
 PAGE, PAGES = 64, 5
 
 
-def attended(et, bits, form, K, V, Q, scale):
-    """Rows that all see every token, K and V [sequences][tokens][hd], Q [sequences][rows][heads * hd]; (result, then what S.attention gives), a table of PAGES pages for each sequence.
+def attended(et, bits, form, K, V, Q, scale, pages=PAGES):
+    """Rows that all see every token, K and V [sequences][tokens][hd], Q [sequences][rows][heads * hd]; (result, then what S.attention gives), a table of so many pages for each sequence.
     One sequence stands for as many as the form has."""
     hd, nh, n, copies = form
     B, tokens = K.shape[:2]
-    table = np.full((B, PAGES), -1, np.int32)
+    table = np.full((B, pages), -1, np.int32)
     used = -(-tokens // PAGE)
     table[:, :used] = np.arange(B * used).reshape(B, used)
     host = D.Cache(bits, 1, hd, PAGE, B * used, fill=0xFF)
@@ -128,3 +129,59 @@ def test_scores_that_nearly_agree(et, bits, form):
     V[:, 1::2] = -1
     got, want = attended(et, bits, form, K, V.astype(np.float16), Q.astype(np.float16), 8 / hd)
     kept(got, want, hd, tokens)
+
+
+# keys shared out over workgroups, eight waves of each and two pairs of two, and joined: (form, pages of the table, tokens)
+SHARED = [((128, 1, 70, 16), 32, 2000), ((128, 2, 128, 8), 64, 1500), ((64, 1, 130, 16), 94, 2000), ((128, 4, 10, 32), 63, 2000), ((128, 1, 64, 1), 2000, 700)]
+
+
+def spread(et, bits, form, pages, tokens, seed, values=lambda r, tokens, width: r.standard_normal((tokens, width)) * 0.5, qscale=1.0, keys=None):
+    """(result, the same in binary64), [rows][heads][hd]."""
+    hd, nh, n, _ = form
+    r = np.random.default_rng(seed)
+    K = (r.standard_normal((tokens, hd)) + 1.5 * r.standard_normal(hd)).astype(np.float16)
+    V, Q = values(r, tokens, hd).astype(np.float16), r.standard_normal((n, nh * hd)) * qscale
+    if keys:
+        K, Q = keys(K, Q)
+    got, want = attended(et, bits, form, K[None], V[None], Q.astype(np.float16)[None], 1 / math.sqrt(hd), pages)
+    return got.astype(np.float64).reshape(n, nh, hd), want[0].reshape(n, nh, hd)
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("form,pages,tokens", SHARED, ids=str)
+def test_shared_out(et, bits, form, pages, tokens):
+    """Ordinary values, single tokens whose values are far larger, a channel far larger in queries, even probabilities."""
+    far = lambda every: lambda r, t, width: r.standard_normal((t, width)) * np.where(np.arange(t) % every == every - 1, 128.0, 0.5)[:, None]  # noqa: E731
+    for more in ({}, dict(values=far(2)), dict(values=far(7)), dict(keys=large_channel), dict(qscale=2.0 ** -13)):
+        assert distance(*spread(et, bits, form, pages, tokens, 17, **more)) <= NEAR, more
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("form,pages,tokens", SHARED, ids=str)
+def test_shared_out_groups_of_very_different_size(et, bits, form, pages, tokens):
+    for qscale in (1.0, 2.0 ** -13):
+        for values in (alternate(2.0 ** 13, 2.0 ** -7), turning(2.0 ** 13, 2.0 ** -7)):
+            assert (off(*spread(et, bits, form, pages, tokens, 21, values, qscale)) <= NEAR).all()
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("form,pages,tokens", SHARED, ids=str)
+def test_shared_out_at_the_end_of_the_range(et, bits, form, pages, tokens):
+    got, Z = spread(et, bits, form, pages, tokens, 13, lambda r, t, width: np.tile(np.where(np.arange(width) % 3, 65504.0, -65504.0), (t, 1)), 2.0 ** -17,
+                    lambda K, Q: (np.where(K > 0, np.float16(65504), np.float16(-65504)), Q))
+    want = np.clip(Z, -65504, 65504)
+    assert np.isfinite(got).all() and (np.abs(got - want) <= 2.0 ** -10 * np.abs(want)).all()
+
+
+@pytest.mark.parametrize("form,pages,tokens", SHARED, ids=str)
+def test_shared_out_infinite_queries_make_their_row_not_a_number(et, form, pages, tokens):
+    want, _ = spread(et, 4, form, pages, tokens, 14, keys=lambda K, Q: (np.abs(K) + np.float16(1), Q))
+    for bad in (np.inf, -np.inf, np.nan):
+        def put(K, Q):
+            Q[0, 5] = bad
+            return np.abs(K) + np.float16(1), Q
+        with np.errstate(invalid="ignore"):
+            got, _ = spread(et, 4, form, pages, tokens, 14, keys=put)
+        assert np.isnan(got[0, 0]).all()
+        got[0, 0] = want[0, 0]
+        assert np.array_equal(got, want)
