@@ -17,8 +17,8 @@
 // eight clocks, where two take one every four.  Eight waves share a stage, since with four each stage served half as many rows; with 16 rows a wave LDS was read twice as often.
 //
 // Up to 64 rows of heads of 128 two waves share a stage, and a workgroup is two such pairs, each with every other tile of its keys (16 nodes of 32 heads over 8, 8 bits, 8 sequences that see 4112
-// tokens: 60.9 -> 46.8 us).  The same for heads of 64 took 272 us where blocks of 16 rows took 371, 64 sequences of 4096 and 16 heads, but 209 where those took 180 with sequences and trees of
-// unequal size; four waves for up to 128 rows were within a tenth of eight, on either side.
+// tokens, with what the nodes see: 44.8 us; eight waves 65.5, blocks of 16 rows 60.4).  With corrections in 8 bits the same for heads of 64 took 272 us where blocks of 16 rows took 371, 64 sequences of
+// 4096 and 16 heads, but 209 where those took 180 with sequences and trees of unequal size; four waves for up to 128 rows were within a tenth of eight, on either side.
 #include "attention_kv.hip.h"
 #include "attention_kv_tile.h"
 
@@ -125,7 +125,7 @@ template <int BITS, int HD, int W, int GROUPS> __global__ __launch_bounds__(W * 
     const int kv = blockIdx.x, nkv = gridDim.x;
     int b = blockIdx.y;
     if (WIDE && starts_at && nkv * gridDim.y > 256 && gridDim.y <= 64) {
-        // the longest sequences first: of 64 of 0 to 2000 tokens and 8 heads, 64 rows, 107.6 us rather than 115.9 (of 2000 each 129.9 rather than 127.5)
+        // the longest sequences first: of 64 of 0 to 2000 tokens and 8 heads, 64 rows, 104 us rather than 117 (of 2000 each 137 either way)
         const int B = gridDim.y, key = lane < B ? (int)((unsigned)starts_at[lane] + (counts_at ? (unsigned)counts_at[lane] : 0u)) : 0;
         int rank = 0;
         for (int j = 0; j < B; j++) {
