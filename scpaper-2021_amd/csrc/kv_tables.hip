@@ -3,7 +3,8 @@
 //
 // A wave takes a stretch of entries; what it gives and takes is placed by counting those of the waves before it.  Small tables are one workgroup's, in one launch; larger ones take two, since
 // no workgroup waits for another: the first counts, the second places.  Slots of many rows are written by a launch of their own (kv_tables_forms.h).  Bound by a launch and dependent accesses (8 sequences of 64 pages: 4.4 us), and by the table's bytes where it is large:
-// 512 sequences of 8192 pages are read in 4.9 us (3.4 TB/s) and read and written in 10.9 (3.1 TB/s).  Sixteen entries at once for a lane rather than four changed neither.
+// 512 sequences of 8192 pages are read in 6.0 us (2.8 TB/s) and read and written in 12.5 (2.7 TB/s).  Sixteen entries at once for a lane rather than four changed neither.  With thousands of
+// sequences bound by adding up the counts of all workgroups before one's own, which grows with the square: 4096 sequences of 8 pages 59 us, 65535 7400.
 #include "common.hip.h"
 #include "kv_tables_forms.h"
 

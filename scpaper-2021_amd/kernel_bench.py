@@ -796,11 +796,13 @@ def main():
                 (4, 8, 600, 1, 12, 12, 64, 16, 256, 4, False), (4, 64, 16000, 1, 16, 16, 64, 64, 4096, 4, False), (4, 2, 6000, 4096, 32, 8, 128, 128, 1024, 16, False),
                 (4, 1, 16384, 4096, 16, 16, 64, 64, 4096, 0, False), (8, 16, 1500, 13, 16, 8, 96, 48, 333, 5, False), (4, 1, 300, 8, 12, 12, 64, 16, 0, 0, True),
                 (4, 16, 2000, 27, 32, 8, 128, 64, 0, 0, True), (4, 64, 4096, 64, 16, 16, 64, 64, 0, 0, True), (8, 8, 16000, 16, 32, 8, 128, 128, 4096, 16, True),
-                (4, 1, 30000, 64, 32, 8, 128, 64, 0, 0, True)):
+                (4, 1, 30000, 64, 32, 8, 128, 64, 0, 0, True), (8, 64, 16000, 1, 16, 16, 64, 64, 4096, 4, False), (8, 2, 6000, 4096, 32, 8, 128, 128, 1024, 16, False),
+                (4, 2, 6000, 1024, 16, 4, 256, 64, 1024, 16, False), (8, 16, 2000, 27, 16, 4, 256, 64, 0, 0, True)):
             b.guess_attention(bits, B, length, n, nh, nkv, hd, page, window, sinks, tree, 10)
         for bits, B, n, depth, layers, nkv, hd, page in ((4, 8, 16, 4, 1, 12, 64, 16), (8, 64, 64, 12, 6, 16, 64, 64), (4, 64, 64, 12, 12, 8, 128, 64)):
             b.guess_accept(bits, B, n, depth, layers, nkv, hd, page, 20)
-        for B, max_pages, n, window, sinks in ((8, 64, 1, 0, 0), (64, 256, 16, 0, 0), (64, 2048, 16, 4096, 16), (512, 8192, 512, 4096, 16)):
+        for B, max_pages, n, window, sinks in ((8, 64, 1, 0, 0), (64, 256, 16, 0, 0), (64, 2048, 16, 4096, 16), (512, 8192, 512, 4096, 16), (512, 8, 128, 0, 0), (8, 512, 4096, 0, 0),
+                                               (4096, 8, 1, 0, 0)):
             b.guess_tables(B, max_pages, 16, n, window, sinks, 20)
     if args.set == "machine":
         print("# machine probes")
